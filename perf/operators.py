@@ -229,7 +229,8 @@ def _quantise(x):
     """Codes (uint8), scales and minima (bf16 values in fp32) of groups of 64: [..., G, 64], [..., G]."""
     x = x.float().unflatten(-1, (-1, 64))
     low = x.amin(-1)
-    scale = ((x.amax(-1) - low) / 15).bfloat16().float()
+    # A quotient of tensors: torch multiplies by 1 / 15 where the divisor is a number.
+    scale = ((x.amax(-1) - low) / torch.full_like(low, 15)).bfloat16().float()
     low = low.bfloat16().float()
     codes = ((x - low[..., None]) / scale[..., None]).round().nan_to_num(0).clamp(0, 15)
     return codes.to(torch.uint8), scale, low
