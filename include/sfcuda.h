@@ -244,6 +244,70 @@ SF_API int sf_mamba2_chunk_scan(const void* x, const void* dt, const void* dA_cu
                const void* Dskip, const void* states, void* y, int64_t B, int64_t L, int64_t H, int64_t P, int64_t N,
                int64_t chunk, int32_t dtype, void* stream, char* err, uint64_t cap);
 
+/* ---------------------------------------------------------------------------------------
+ * Serving operators: no reference counterpart (its tasks have neither grouped heads, a cache nor
+ * windows); they stand beside rmsnorm, rope and flash_attention.  Tensors are [tokens, heads, D] with
+ * unit stride along D; `strides` holds the token and head strides in elements, tensor after tensor,
+ * NULL for contiguous tensors.  Index tensors are int32.  F16 / BF16, fp32 arithmetic.
+ * ------------------------------------------------------------------------------------- */
+
+/*
+ * qk_norm_rope: per-head RMS norm of q [T, Hq, D] and k [T, Hk, D] (weights wq, wk [D]) and, in the
+ * same pass, the rotate-half rotary embedding of the first `rotary` elements at position[t]:
+ *   y = x * rsqrt(mean(x^2) + eps) * w,  r = rotary / 2,  angle = position[t] * base^(-i / r)
+ *   out[i] = y[i] cos - y[i+r] sin,  out[i+r] = y[i] sin + y[i+r] cos,  i < r;  out = y behind rotary.
+ * strides: q, k, q_out, k_out.  The outputs may be the inputs.  rotary even, 0..D.
+ */
+SF_API int sf_qk_norm_rope(const void* q, const void* k, const void* wq, const void* wk, const void* positions, void* q_out,
+               void* k_out, int64_t T, int64_t Hq, int64_t Hk, int64_t D, const int64_t* strides, int64_t rotary, double base,
+               float eps, int32_t dtype, void* stream, char* err, uint64_t cap);
+
+/*
+ * The 4-bit paged key/value cache: [pages, H, page_size / 16, 18 D] bytes (16-byte aligned, page_size a
+ * multiple of 16, D 64 or 128), one record for 16 tokens of a head (csrc/kv4.cuh gives its layout).
+ * Token slot s is row s % page_size of page s / page_size.  Every 64 elements of a token's head hold a
+ * bf16 minimum and scale = (max - min) / 15 and codes clamp(rint((x - minimum) / scale), 0, 15); a code
+ * q stands for minimum + scale q.  A group with a value or a range that is not finite is stored as NaN.
+ *
+ * kv4_store writes tokens k, v [T, H, D] at slots[T]; kv4_load reads them back.  A negative slot is
+ * padding (nothing written; zeros read); one past the cache is treated the same and reported through
+ * sf_kernel_status (code 3).  The slots of one store must differ: of two tokens at one slot a mixture may stay.
+ * strides: k, v (multiples of 8 elements).
+ */
+SF_API int sf_kv4_store(const void* k, const void* v, const void* slots, void* cache, int64_t T, int64_t H, int64_t D,
+               int64_t pages, int64_t page_size, const int64_t* strides, int32_t dtype, void* stream, char* err, uint64_t cap);
+SF_API int sf_kv4_load(const void* cache, const void* slots, void* k, void* v, int64_t T, int64_t H, int64_t D, int64_t pages,
+               int64_t page_size, const int64_t* strides, int32_t dtype, void* stream, char* err, uint64_t cap);
+
+/*
+ * kv4_attention: one query token a request over the 4-bit cache, o[b] = softmax(scale q[b] . K^T) V, q and
+ * o [B, Hq, D], Hq a multiple of the cache's Hk (query head h reads head h / (Hq / Hk)).  Request b has
+ * lens[b] tokens (the query's own last); token j sits at row j % page_size of page table[b, j / page_size],
+ * table [B, width].  Seen are j >= lens[b] - window or j < sinks (window 0: all).  lens[b] <= 0 gives
+ * zeros; a length past the table is cut to it, a page id outside the cache hides its tokens, both
+ * reported through sf_kernel_status (code 3).  strides: q, o, then the table's row stride (5 numbers).
+ * workspace: 16-byte aligned, sf_kv4_attention_workspace_bytes bytes (variant 0; 0 bytes: may be NULL), no
+ * initial content; two calls that overlap on the GPU need one each.  variant: see SF_OP_KV4_ATTENTION.
+ */
+SF_API uint64_t sf_kv4_attention_workspace_bytes(int64_t B, int64_t Hq, int64_t Hk, int64_t D, int64_t page_size, int64_t width,
+               int64_t window, int64_t sinks, int32_t variant);
+SF_API int sf_kv4_attention(const void* q, const void* cache, const void* table, const void* lens, void* o, void* workspace,
+               uint64_t workspace_bytes, int64_t B, int64_t Hq, int64_t Hk, int64_t D, int64_t pages, int64_t page_size,
+               int64_t width, const int64_t* strides, float scale, int64_t window, int64_t sinks, int32_t dtype, int32_t variant, void* stream,
+               char* err, uint64_t cap);
+
+/*
+ * window_attention: attention of packed prompts, q, o [Tq, Hq, D], k, v [Tk, Hk, D], Hq a multiple of Hk.
+ * Sequence s has queries cu_q[s]..cu_q[s+1] and keys cu_k[s]..cu_k[s+1] (both [seqs + 1], not decreasing);
+ * its query i sits at position p = i + nk - nq and sees keys j <= p with j > p - window or j < sinks
+ * (window 0: all j <= p).  A query that sees nothing gives zeros; rows of no sequence are left as they
+ * were.  strides: q, k, v, o.  D <= 256; tcgen05 kernel for D in {64, 128}, 16-byte aligned tensors and
+ * strides and at most 128 query heads a key head, general kernel otherwise.  variant as in sf_op_desc.
+ */
+SF_API int sf_window_attention(const void* q, const void* k, const void* v, const void* cu_q, const void* cu_k, void* o,
+               int64_t Tq, int64_t Tk, int64_t seqs, int64_t Hq, int64_t Hk, int64_t D, const int64_t* strides, float scale,
+               int64_t window, int64_t sinks, int32_t dtype, int32_t variant, void* stream, char* err, uint64_t cap);
+
 /*
  * gemm_nt: C[M,N] = A[M,K] . B[N,K]^T, fp16 or bf16 in, fp32 accumulation, one rounding
  * (the dense-gemm workload; the oracle is tasks/gemm/reference.py:110-114 applied to B^T).
@@ -340,6 +404,11 @@ SF_API int sf_launch_kernel(void* function, uint32_t gx, uint32_t gy, uint32_t g
 #define SF_OP_GEMV 19
 #define SF_OP_GEMM_SILU 20
 #define SF_OP_KDA_FIXED 21
+#define SF_OP_QK_NORM_ROPE 22
+#define SF_OP_KV4_STORE 23
+#define SF_OP_KV4_LOAD 24
+#define SF_OP_KV4_ATTENTION 25
+#define SF_OP_WINDOW_ATTENTION 26
 
 typedef struct sf_op_desc {
     int32_t op;       /* SF_OP_* */
@@ -384,6 +453,16 @@ SF_API int32_t sf_op_nargs(int32_t op);
  *   SF_OP_KDA_FIXED dims = {N, H, D}  attrs = {lower_bound}
  *                   args = {q, k, v, g, beta, A_log, dt_bias, initial_state, scale, output, final_state,
  *                           work_items, item_counts, handoff_states}
+ *   SF_OP_QK_NORM_ROPE  dims = {T, Hq, Hk, D, rotary}  attrs = {base, eps}
+ *                   args = {q, k, wq, wk, positions, q_out, k_out}
+ *   SF_OP_KV4_STORE dims = {T, H, D, pages, page_size}                 args = {k, v, slots, cache}
+ *   SF_OP_KV4_LOAD  dims = {T, H, D, pages, page_size}                 args = {cache, slots, k, v}
+ *   SF_OP_KV4_ATTENTION  dims = {B, Hq, Hk, D, pages, page_size, width, ws_bytes}  attrs = {scale, window, sinks}
+ *                   args = {q, cache, table, lens, o, workspace}
+ *                   variant 1 deals every request's keys to all CTAs, 3 keeps a (request, head) to a CTA
+ *   SF_OP_WINDOW_ATTENTION  dims = {Tq, Tk, seqs, Hq, Hk, D, window, sinks}  attrs = {scale}
+ *                   args = {q, k, v, cu_q, cu_k, o}
+ * (these five: contiguous tensors)
  * desc->variant: 0 = exact dispatch with fallback, 1 = force the specialised (tensor-core /
  * vectorised) kernel, 2 = force the general fallback kernel.
  */

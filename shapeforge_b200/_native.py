@@ -87,6 +87,11 @@ OPS = {
     "gemv": 19,
     "gemm_silu": 20,
     "kda": 21,
+    "qk_norm_rope": 22,
+    "kv4_store": 23,
+    "kv4_load": 24,
+    "kv4_attention": 25,
+    "window_attention": 26,
 }
 
 _P = ctypes.c_void_p
@@ -125,6 +130,12 @@ SIGNATURES: dict[str, tuple[object, tuple]] = {
     "sf_varlen_kda_gated_workspace_bytes": (_U64, (_I64, _I64, _I64, _I64)),
     "sf_varlen_kda_gated_ws": (ctypes.c_int, (_P,) * 9 + (_I64, _I64, _I64, _I64, _F32, _I32, _P, _U64, _P, *_ERR)),
     "sf_mamba2_chunk_scan": (ctypes.c_int, (_P,) * 8 + (_I64,) * 6 + (_I32, _P, *_ERR)),
+    "sf_qk_norm_rope": (ctypes.c_int, (_P,) * 7 + (_I64,) * 4 + (_P, _I64, ctypes.c_double, _F32, _I32, _P, *_ERR)),
+    "sf_kv4_store": (ctypes.c_int, (_P,) * 4 + (_I64,) * 5 + (_P, _I32, _P, *_ERR)),
+    "sf_kv4_load": (ctypes.c_int, (_P,) * 4 + (_I64,) * 5 + (_P, _I32, _P, *_ERR)),
+    "sf_kv4_attention_workspace_bytes": (_U64, (_I64,) * 8 + (_I32,)),
+    "sf_kv4_attention": (ctypes.c_int, (_P,) * 6 + (_U64,) + (_I64,) * 7 + (_P, _F32, _I64, _I64, _I32, _I32, _P, *_ERR)),
+    "sf_window_attention": (ctypes.c_int, (_P,) * 6 + (_I64,) * 6 + (_P, _F32, _I64, _I64, _I32, _I32, _P, *_ERR)),
     "sf_gemm_nt": (ctypes.c_int, (_P, _P, _P, _I64, _I64, _I64, _I32, _P, *_ERR)),
     "sf_gemm_nn_workspace_bytes": (_U64, (_I64, _I64, _I64, _I32)),
     "sf_gemm_nn": (ctypes.c_int, (_P, _P, _P, _I64, _I64, _I64, _I32, _P, _U64, _P, *_ERR)),

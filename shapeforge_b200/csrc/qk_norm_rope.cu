@@ -1,0 +1,284 @@
+// Per-head RMS norm of queries and keys with the rotary embedding in the same pass, sm_100a:
+//
+//   y = x * rsqrt(mean(x^2) + eps) * w                        over one head's D elements
+//   angle_i = position[t] * base^(-i / r),  r = rotary / 2,  i < r
+//   out_i     = y_i cos(angle_i) - y_{i+r} sin(angle_i)
+//   out_{i+r} = y_i sin(angle_i) + y_{i+r} cos(angle_i)        the other D - 2r elements: out = y
+//
+// q [T, Hq, D] and k [T, Hk, D] with any token and head strides (views of a packed projection),
+// w_q, w_k [D], position [T] int32, fp16 / bf16 in and out, fp32 arithmetic, one rounding.  The
+// outputs may be the inputs' own buffers: the lanes that write a row have read all of it.
+//
+// HBM-bound: T (Hq + Hk) D elements in and out, each moved once.
+//  * A row of D elements is held by D/16 lanes, two 8-element chunks a lane; a lane's chunks are c
+//    and c + r/8, so both members of a rotated pair sit in one lane and only the sum of squares
+//    crosses lanes (2-4 shuffles).
+//  * The angle depends on (t, i) alone, so a warp stays with one token, takes sine and cosine of
+//    its 8 angles a lane once, and walks the token's heads, two row groups in flight.  Tokens are
+//    split over heads only when there are too few of them to fill the GPU.
+//  * The angle is reduced in double precision (a position near 2^20 times a frequency leaves no
+//    fraction bits in fp32), in turns: frac(position * base^(-i/r) / 2 pi), |.| <= 1/2, then the
+//    special-function sine and cosine of at most pi (absolute error ~2^-21, far below half a step
+//    of a 16-bit output).
+#include "sf_common.cuh"
+
+#include <cmath>
+
+namespace {
+
+struct Side {
+    const void* x;
+    void* y;
+    const void* w;
+    int64_t xt, xh, yt, yh;  // token and head strides in elements
+};
+
+// Sine and cosine of 2 pi * turns.
+__device__ __forceinline__ void sincos_turns(double turns, float* s, float* c) {
+    const float f = (float)(turns - rint(turns));
+    __sincosf(f * 6.283185307f, s, c);
+}
+
+template <typename T>
+struct Row {
+    uint4 a, b;  // the lane's two chunks
+};
+
+template <typename T>
+__device__ __forceinline__ void unpack8(const uint4& u, float (&v)[8]) {
+    const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const float2 f = sf::Pair<T>::to_f2(w[i]);
+        v[2 * i] = f.x;
+        v[2 * i + 1] = f.y;
+    }
+}
+
+template <typename T>
+__device__ __forceinline__ uint4 pack8(const float (&v)[8]) {
+    uint32_t w[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) w[i] = sf::Pair<T>::from_f2(make_float2(v[2 * i], v[2 * i + 1]));
+    return make_uint4(w[0], w[1], w[2], w[3]);
+}
+
+// LPR lanes a row (a power of two >= D / 16); `items` = tokens x head parts, one warp an item.
+template <typename T, int LPR>
+__global__ void __launch_bounds__(256) qk_norm_rope_kernel(const Side q, const Side k, const int32_t* __restrict__ position, int64_t tokens,
+                                                           int hq, int hk, int D, int r, double ratio, float eps, int parts) {
+    constexpr int RPW = 32 / LPR;  // rows a warp holds at once
+    const int lane = threadIdx.x & 31;
+    const int p = lane % LPR, sub = lane / LPR;
+    const bool live = p < D / 16;
+    const bool turned = p < r / 8;
+    // Element offsets of the lane's chunks.
+    const int e0 = turned ? 8 * p : 2 * r + 16 * (p - r / 8);
+    const int e1 = turned ? e0 + r : e0 + 8;
+    // base^(-i/r) / 2 pi of the lane's 8 angles: the first by repeated squaring, then by `ratio`.
+    double turn0 = 0.15915494309189533577;
+    if (turned) {
+        double sq = ratio;
+        for (int e = 8 * p; e > 0; e >>= 1) {
+            if (e & 1) turn0 *= sq;
+            sq *= sq;
+        }
+    }
+    uint4 wq0 = {}, wq1 = {}, wk0 = {}, wk1 = {};
+    if (live) {
+        if (hq) {
+            wq0 = *reinterpret_cast<const uint4*>((const T*)q.w + e0);
+            wq1 = *reinterpret_cast<const uint4*>((const T*)q.w + e1);
+        }
+        if (hk) {
+            wk0 = *reinterpret_cast<const uint4*>((const T*)k.w + e0);
+            wk1 = *reinterpret_cast<const uint4*>((const T*)k.w + e1);
+        }
+    }
+    const float inv_d = 1.0f / (float)D;
+    const int rows = hq + hk;
+    const int groups = (rows + RPW - 1) / RPW;
+    const int per = (groups + parts - 1) / parts;
+    const int64_t items = tokens * parts;
+    const int64_t step = (int64_t)gridDim.x * (blockDim.x >> 5);
+    for (int64_t item = (int64_t)blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5); item < items; item += step) {
+        const int64_t t = item / parts;
+        const int g0 = (int)(item - t * parts) * per, g1 = min(groups, g0 + per);
+        const int32_t pos = __ldg(position + t);
+        float sn[8], cs[8];
+        bool have = false;
+        for (int g = g0; g < g1; g += 2) {
+            uint4 a[2], b[2];
+            int row[2];
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+                row[u] = (g + u) * RPW + sub;
+                const bool ok = live && g + u < g1 && row[u] < rows;
+                if (!ok) row[u] = -1;
+                a[u] = b[u] = make_uint4(0, 0, 0, 0);
+                if (ok) {
+                    const bool isq = row[u] < hq;
+                    const T* x = isq ? (const T*)q.x + t * q.xt + (int64_t)row[u] * q.xh : (const T*)k.x + t * k.xt + (int64_t)(row[u] - hq) * k.xh;
+                    a[u] = *reinterpret_cast<const uint4*>(x + e0);
+                    b[u] = *reinterpret_cast<const uint4*>(x + e1);
+                }
+            }
+            if (!have) {  // while the first rows are on their way
+                have = true;
+                double f = turn0;
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    sn[j] = 0.f;
+                    cs[j] = 1.f;
+                    if (turned) sincos_turns((double)pos * f, &sn[j], &cs[j]);
+                    f *= ratio;
+                }
+            }
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+                float va[8], vb[8];
+                unpack8<T>(a[u], va);
+                unpack8<T>(b[u], vb);
+                float2 ss = make_float2(0.f, 0.f);
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    const float2 x2 = make_float2(va[j], vb[j]);
+                    ss = sf::f2_fma(x2, x2, ss);
+                }
+                float sum = ss.x + ss.y;
+#pragma unroll
+                for (int o = LPR / 2; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+                if (row[u] < 0) continue;
+                const float rs = rsqrtf(fmaf(sum, inv_d, eps));
+                const bool isq = row[u] < hq;
+                float w0[8], w1[8], o0[8], o1[8];
+                unpack8<T>(isq ? wq0 : wk0, w0);
+                unpack8<T>(isq ? wq1 : wk1, w1);
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    const float y0 = va[j] * rs * w0[j], y1 = vb[j] * rs * w1[j];
+                    // Plain products and sums where nothing turns keep an infinite partner out.
+                    o0[j] = turned ? y0 * cs[j] - y1 * sn[j] : y0;
+                    o1[j] = turned ? y0 * sn[j] + y1 * cs[j] : y1;
+                }
+                T* y = isq ? (T*)q.y + t * q.yt + (int64_t)row[u] * q.yh : (T*)k.y + t * k.yt + (int64_t)(row[u] - hq) * k.yh;
+                *reinterpret_cast<uint4*>(y + e0) = pack8<T>(o0);
+                *reinterpret_cast<uint4*>(y + e1) = pack8<T>(o1);
+            }
+        }
+    }
+}
+
+// Any D, rotary size and 2-byte alignment: a warp a row, element by element.  A lane reads and
+// writes both members of its pairs, so in-place calls stay right here too.
+template <typename T>
+__global__ void __launch_bounds__(256) qk_norm_rope_general_kernel(const Side q, const Side k, const int32_t* __restrict__ position,
+                                                                   int64_t tokens, int hq, int hk, int D, int r, double base, float eps) {
+    const int lane = threadIdx.x & 31;
+    const int64_t rows = tokens * (hq + hk);
+    const int64_t step = (int64_t)gridDim.x * (blockDim.x >> 5);
+    for (int64_t i = (int64_t)blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5); i < rows; i += step) {
+        const int64_t t = i / (hq + hk);
+        const int row = (int)(i - t * (hq + hk));
+        const Side& s = row < hq ? q : k;
+        const int64_t h = row < hq ? row : row - hq;
+        const T* x = (const T*)s.x + t * s.xt + h * s.xh;
+        T* y = (T*)s.y + t * s.yt + h * s.yh;
+        const T* w = (const T*)s.w;
+        float sum = 0.f;
+        for (int d = lane; d < D; d += 32) {
+            const float v = sf::Dt<T>::to_f(x[d]);
+            sum = fmaf(v, v, sum);
+        }
+        const float rs = rsqrtf(sf::warp_sum(sum) / (float)D + eps);
+        const double pos = (double)position[t];
+        for (int d = lane; d < r; d += 32) {
+            const float y0 = sf::Dt<T>::to_f(x[d]) * rs * sf::Dt<T>::to_f(w[d]);
+            const float y1 = sf::Dt<T>::to_f(x[d + r]) * rs * sf::Dt<T>::to_f(w[d + r]);
+            float sn, cs;
+            sincos_turns(pos * (pow(base, -(double)d / (double)r) * 0.15915494309189533577), &sn, &cs);
+            y[d] = sf::Dt<T>::from_f(y0 * cs - y1 * sn);
+            y[d + r] = sf::Dt<T>::from_f(y0 * sn + y1 * cs);
+        }
+        for (int d = 2 * r + lane; d < D; d += 32) y[d] = sf::Dt<T>::from_f(sf::Dt<T>::to_f(x[d]) * rs * sf::Dt<T>::to_f(w[d]));
+    }
+}
+
+template <typename T, int LPR>
+int launch_vec(const Side& q, const Side& k, const int32_t* pos, int64_t T_, int hq, int hk, int D, int r, double base, float eps,
+               cudaStream_t st, char* err, uint64_t cap) {
+    constexpr int RPW = 32 / LPR;
+    static const int resident = sf::resident_ctas(qk_norm_rope_kernel<T, LPR>, 256, 0);
+    const int64_t ctas = (int64_t)sf::sm_count() * resident;
+    const int64_t groups = (hq + hk + RPW - 1) / RPW;
+    // A warp takes a whole token (its angles once) while the tokens fill the GPU's warps; fewer
+    // tokens are split over their heads so that every warp has work.
+    int64_t parts = ctas * 8 / T_;
+    parts = parts < 1 ? 1 : (parts > groups ? groups : parts);
+    const int64_t items = T_ * parts;
+    // Small problems: two-warp CTAs spread over all SMs.
+    const int threads = items <= (int64_t)sf::sm_count() * 8 ? 64 : 256;
+    int64_t blocks = (items + threads / 32 - 1) / (threads / 32);
+    if (blocks > ctas * (256 / threads)) blocks = ctas * (256 / threads);
+    qk_norm_rope_kernel<T, LPR><<<(unsigned)blocks, threads, 0, st>>>(q, k, pos, T_, hq, hk, D, r, r ? std::pow(base, -1.0 / (double)r) : 1.0, eps,
+                                                                      (int)parts);
+    return sf::check_launch("qk_norm_rope launch", err, cap);
+}
+
+bool vec_side(const Side& s, int64_t T_, int64_t h) {
+    if (h == 0) return true;
+    return sf::aligned16(s.x) && sf::aligned16(s.y) && sf::aligned16(s.w) && (T_ == 1 || (s.xt % 8 == 0 && s.yt % 8 == 0)) &&
+           (h == 1 || (s.xh % 8 == 0 && s.yh % 8 == 0));
+}
+
+template <typename T>
+int launch_t(const Side& q, const Side& k, const int32_t* pos, int64_t T_, int hq, int hk, int D, int rotary, double base, float eps,
+             int32_t variant, cudaStream_t st, char* err, uint64_t cap) {
+    const int r = rotary / 2;
+    const bool vec = D % 16 == 0 && D <= 512 && r % 8 == 0 && vec_side(q, T_, hq) && vec_side(k, T_, hk);
+    if (variant == 1 && !vec)
+        return sf::fail(SF_EINVAL, err, cap, "qk_norm_rope: the vectorised variant needs D %% 16 == 0, D <= 512, rotary %% 16 == 0 and 16-byte aligned rows");
+    if (vec && variant != 2) {
+        if (D <= 64) return launch_vec<T, 4>(q, k, pos, T_, hq, hk, D, r, base, eps, st, err, cap);
+        if (D <= 128) return launch_vec<T, 8>(q, k, pos, T_, hq, hk, D, r, base, eps, st, err, cap);
+        if (D <= 256) return launch_vec<T, 16>(q, k, pos, T_, hq, hk, D, r, base, eps, st, err, cap);
+        return launch_vec<T, 32>(q, k, pos, T_, hq, hk, D, r, base, eps, st, err, cap);
+    }
+    const int64_t rows = T_ * (hq + hk);
+    int64_t blocks = (rows + 7) / 8;
+    const int64_t most = (int64_t)sf::sm_count() * 8;
+    if (blocks > most) blocks = most;
+    qk_norm_rope_general_kernel<T><<<(unsigned)blocks, 256, 0, st>>>(q, k, pos, T_, hq, hk, D, r, base, eps);
+    return sf::check_launch("qk_norm_rope general launch", err, cap);
+}
+
+}  // namespace
+
+int sf_qk_norm_rope_launch(const void* q, const void* k, const void* wq, const void* wk, const void* positions, void* q_out, void* k_out,
+                           int64_t T, int64_t Hq, int64_t Hk, int64_t D, const int64_t* strides, int64_t rotary, double base, float eps,
+                           int32_t dtype, int32_t variant, cudaStream_t st, char* err, uint64_t cap) {
+    if (T < 0 || Hq < 0 || Hk < 0 || Hq + Hk > (1 << 20) || D < 1 || D > (1 << 20))
+        return sf::fail(SF_EINVAL, err, cap, "qk_norm_rope: need T, Hq, Hk >= 0 and D >= 1");
+    if (rotary < 0 || rotary % 2 || rotary > D) return sf::fail(SF_EINVAL, err, cap, "qk_norm_rope: rotary must be even and at most D");
+    if (!(base > 0) || !std::isfinite(base)) return sf::fail(SF_EINVAL, err, cap, "qk_norm_rope: base must be > 0");
+    if (!(eps >= 0)) return sf::fail(SF_EINVAL, err, cap, "qk_norm_rope: eps must be >= 0");
+    if (dtype != SF_DTYPE_F16 && dtype != SF_DTYPE_BF16) return sf::fail(SF_EINVAL, err, cap, "qk_norm_rope: dtype %d is not fp16/bf16", dtype);
+    if (T * (Hq + Hk) == 0) return SF_OK;
+    if (!positions || (Hq && (!q || !q_out || !wq)) || (Hk && (!k || !k_out || !wk)))
+        return sf::fail(SF_EINVAL, err, cap, "qk_norm_rope: null tensor pointer");
+    const int64_t dense[8] = {Hq * D, D, Hk * D, D, Hq * D, D, Hk * D, D};
+    const int64_t* s = strides ? strides : dense;
+    for (int i = 0; i < 8; ++i)
+        if (s[i] < 0) return sf::fail(SF_EINVAL, err, cap, "qk_norm_rope: negative stride");
+    const Side sq{q, q_out, wq, s[0], s[1], s[4], s[5]}, sk{k, k_out, wk, s[2], s[3], s[6], s[7]};
+    if (dtype == SF_DTYPE_F16)
+        return launch_t<__half>(sq, sk, (const int32_t*)positions, T, (int)Hq, (int)Hk, (int)D, (int)rotary, base, eps, variant, st, err, cap);
+    return launch_t<__nv_bfloat16>(sq, sk, (const int32_t*)positions, T, (int)Hq, (int)Hk, (int)D, (int)rotary, base, eps, variant, st, err, cap);
+}
+
+extern "C" int sf_qk_norm_rope(const void* q, const void* k, const void* wq, const void* wk, const void* positions, void* q_out, void* k_out,
+                               int64_t T, int64_t Hq, int64_t Hk, int64_t D, const int64_t* strides, int64_t rotary, double base,
+                               float eps, int32_t dtype, void* stream, char* err, uint64_t cap) {
+    return sf_qk_norm_rope_launch(q, k, wq, wk, positions, q_out, k_out, T, Hq, Hk, D, strides, rotary, base, eps, dtype, 0,
+                                  (cudaStream_t)stream, err, cap);
+}

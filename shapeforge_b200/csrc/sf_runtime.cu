@@ -127,6 +127,11 @@ extern "C" int32_t sf_op_nargs(int32_t op) {
         case SF_OP_GEMV: return 3;
         case SF_OP_GEMM_SILU: return 4;
         case SF_OP_KDA_FIXED: return 14;
+        case SF_OP_QK_NORM_ROPE: return 7;
+        case SF_OP_KV4_STORE: return 4;
+        case SF_OP_KV4_LOAD: return 4;
+        case SF_OP_KV4_ATTENTION: return 6;
+        case SF_OP_WINDOW_ATTENTION: return 6;
         default: return 0;
     }
 }
@@ -190,6 +195,23 @@ static int dispatch(const sf_op_desc* d, const void* const* a, cudaStream_t s, c
             return sf_kda_fixed_launch(a[0], a[1], a[2], a[3], a[4], a[5], a[6], a[7], a[8], (void*)a[9], (void*)a[10], (void*)a[11],
                                        (void*)a[12], d->dims[0], d->dims[1], d->dims[2], (float)d->attrs[0], d->dtype, d->variant, s,
                                        err, cap);
+        case SF_OP_QK_NORM_ROPE:
+            return sf_qk_norm_rope_launch(a[0], a[1], a[2], a[3], a[4], (void*)a[5], (void*)a[6], d->dims[0], d->dims[1], d->dims[2],
+                                          d->dims[3], nullptr, d->dims[4], d->attrs[0], (float)d->attrs[1], d->dtype, d->variant, s, err, cap);
+        case SF_OP_KV4_STORE:
+            return sf_kv4_store_launch(a[0], a[1], a[2], (void*)a[3], d->dims[0], d->dims[1], d->dims[2], d->dims[3], d->dims[4], nullptr,
+                                       d->dtype, s, err, cap);
+        case SF_OP_KV4_LOAD:
+            return sf_kv4_load_launch(a[0], a[1], (void*)a[2], (void*)a[3], d->dims[0], d->dims[1], d->dims[2], d->dims[3], d->dims[4],
+                                      nullptr, d->dtype, s, err, cap);
+        case SF_OP_KV4_ATTENTION:
+            return sf_kv4_attention_launch(a[0], a[1], a[2], a[3], (void*)a[4], (void*)a[5], (uint64_t)d->dims[7], d->dims[0], d->dims[1],
+                                           d->dims[2], d->dims[3], d->dims[4], d->dims[5], d->dims[6], nullptr, (float)d->attrs[0],
+                                           (int64_t)d->attrs[1], (int64_t)d->attrs[2], d->dtype, d->variant, s, err, cap);
+        case SF_OP_WINDOW_ATTENTION:
+            return sf_window_attention_launch(a[0], a[1], a[2], a[3], a[4], (void*)a[5], d->dims[0], d->dims[1], d->dims[2], d->dims[3],
+                                              d->dims[4], d->dims[5], nullptr, (float)d->attrs[0], d->dims[6], d->dims[7], d->dtype,
+                                              d->variant, s, err, cap);
         default:
             return sf::fail(SF_EINVAL, err, cap, "unknown op %d", d->op);
     }

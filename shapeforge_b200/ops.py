@@ -9,6 +9,7 @@ missing native library raises.
 from __future__ import annotations
 
 import functools
+import struct
 
 import torch
 
@@ -471,4 +472,220 @@ def mamba2_chunk_scan(x, dt, dA_cumsum, b_mat, c_mat, d_skip, states, out: torch
     _check(out, "out", x.dtype)
     ptrs = [t.data_ptr() for _, t in tensors] + [out.data_ptr()]
     _run("mamba2_chunk_scan", x, ptrs, dims=(bsz, seq, heads, hd, n, chunk), variant=variant)
+    return out
+
+
+# ---- serving operators: [tokens, heads, D] tensors with any token and head strides -----------------
+
+
+def _check_rows(t: torch.Tensor, name: str, dtype: torch.dtype | None = None, written: bool = False) -> tuple[int, int]:
+    """Check a [tokens, heads, D] CUDA tensor with unit stride along D; return its token and head
+    strides in elements (0 along an axis of one entry, whose stride says nothing)."""
+    if not isinstance(t, torch.Tensor):
+        raise TypeError(f"{name} must be a torch.Tensor")
+    if not t.is_cuda:
+        raise ValueError(f"{name} must be a CUDA tensor (there is no CPU path)")
+    if dtype is not None and t.dtype != dtype:
+        raise TypeError(f"{name} has dtype {t.dtype}, expected {dtype}")
+    if t.dim() != 3:
+        raise ValueError(f"{name} must have three axes (tokens, heads, D), got shape {tuple(t.shape)}")
+    n, h, d = t.shape
+    a, b, c = t.stride()
+    if d > 1 and c != 1:
+        raise ValueError(f"{name} must have unit stride along its last axis")
+    a, b = (a if n > 1 else 0), (b if h > 1 else 0)
+    if written and t.numel():
+        # Rows that share memory would be written by two threads: each axis must step over what the
+        # smaller one spans.
+        (near, many), (far, more) = sorted([(a, n), (b, h)])
+        if (many > 1 and near < d) or (more > 1 and far < (near * (many - 1) + d if many > 1 else d)):
+            raise ValueError(f"{name} has rows that overlap (strides {t.stride()})")
+    return a, b
+
+
+def _check_index(t: torch.Tensor, name: str, length: int | None = None) -> None:
+    _check(t, name, torch.int32)
+    if t.dim() != 1 or (length is not None and t.shape[0] != length):
+        raise ValueError(f"{name} must be one axis of {'int32' if length is None else length} entries, got shape {tuple(t.shape)}")
+
+
+def _on_tensors_device(name: str, tensors, *args) -> None:
+    """``_native.call`` with the tensors' GPU current (entered only when it is not), on the current
+    stream of that GPU; tensors on two GPUs are refused."""
+    dev = tensors[0].device
+    for t in tensors[1:]:
+        if t.device != dev:
+            raise ValueError(f"{name[3:]}: tensors on more than one device ({dev}, {t.device})")
+    if torch.cuda.current_device() == dev.index:
+        _native.call(name, *args, torch.cuda.current_stream().cuda_stream)
+    else:
+        with torch.cuda.device(dev):
+            _native.call(name, *args, torch.cuda.current_stream().cuda_stream)
+
+
+def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, q_weight: torch.Tensor, k_weight: torch.Tensor, positions: torch.Tensor,
+                 base: float = 10000.0, eps: float = 1e-6, rotary_dim: int | None = None, q_out: torch.Tensor | None = None,
+                 k_out: torch.Tensor | None = None) -> tuple[torch.Tensor, torch.Tensor]:
+    """Per-head RMS norm of queries ``q [T, Hq, D]`` and keys ``k [T, Hk, D]`` (weights ``[D]``) and the
+    rotate-half rotary embedding of their first ``rotary_dim`` (default D) elements at ``positions [T]``
+    (int32), in one pass; :func:`rmsnorm` then :func:`rope`, at any positions.  ``q`` and ``k`` may be
+    views of a packed projection (unit stride along D); ``q_out`` / ``k_out`` may be ``q`` / ``k``
+    themselves (in place), otherwise they must not overlap the inputs.  Returns ``(q_out, k_out)``."""
+    qs, ks = _check_rows(q, "q"), _check_rows(k, "k", q.dtype)
+    t, hq, d = q.shape
+    hk = k.shape[1]
+    if k.shape[0] != t or k.shape[2] != d:
+        raise ValueError(f"k has shape {tuple(k.shape)}, expected [{t}, heads, {d}]")
+    for name, w in (("q_weight", q_weight), ("k_weight", k_weight)):
+        _check(w, name, q.dtype)
+        if w.numel() != d:
+            raise ValueError(f"{name} has {w.numel()} elements, expected D={d}")
+    _check_index(positions, "positions", t)
+    rotary = d if rotary_dim is None else int(rotary_dim)
+    q_out = torch.empty((t, hq, d), dtype=q.dtype, device=q.device) if q_out is None else q_out
+    k_out = torch.empty((t, hk, d), dtype=q.dtype, device=q.device) if k_out is None else k_out
+    qos, kos = _check_rows(q_out, "q_out", q.dtype, written=True), _check_rows(k_out, "k_out", q.dtype, written=True)
+    if q_out.shape != q.shape or k_out.shape != k.shape:
+        raise ValueError("q_out and k_out must have the shapes of q and k")
+    _on_tensors_device("sf_qk_norm_rope", (q, k, q_weight, k_weight, positions, q_out, k_out), q.data_ptr(), k.data_ptr(),
+                       q_weight.data_ptr(), k_weight.data_ptr(), positions.data_ptr(), q_out.data_ptr(), k_out.data_ptr(), t, hq, hk, d,
+                       struct.pack("8q", *qs, *ks, *qos, *kos), rotary, float(base), float(eps), _native.DTYPE_CODES[dtype_name(q)])
+    return q_out, k_out
+
+
+def kv4_cache(num_pages: int, page_size: int, heads: int, dim: int, device: torch.device | str = "cuda") -> torch.Tensor:
+    """A zeroed 4-bit paged key/value cache for :func:`kv4_store`, :func:`kv4_load` and
+    :func:`kv4_attention`: uint8 ``[num_pages, heads, page_size / 16, 18 * dim]``, 4.5 bits a value
+    (``dim`` 64 or 128, ``page_size`` a multiple of 16).  Slot ``s`` is row ``s % page_size`` of page
+    ``s // page_size``."""
+    if page_size < 16 or page_size % 16 or dim not in (64, 128) or num_pages < 0 or heads < 1:
+        raise ValueError("kv4_cache needs a page size that is a multiple of 16, dim 64 or 128 and at least one head")
+    return torch.zeros((num_pages, heads, page_size // 16, 18 * dim), dtype=torch.uint8, device=device)
+
+
+def _check_cache(cache: torch.Tensor) -> tuple[int, int, int, int]:
+    """(pages, heads, page size, D) of a 4-bit cache."""
+    _check(cache, "cache", torch.uint8)
+    if cache.dim() != 4 or cache.shape[3] not in (18 * 64, 18 * 128) or cache.shape[2] < 1:
+        raise ValueError(f"cache must be [pages, heads, page_size / 16, 18 * D], D 64 or 128, got {tuple(cache.shape)}")
+    pages, heads, tiles, record = cache.shape
+    return pages, heads, 16 * tiles, record // 18
+
+
+def kv4_store(k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor, cache: torch.Tensor) -> torch.Tensor:
+    """Quantise the tokens ``k, v [T, H, D]`` (unit stride along D) to 4 bits and write them at ``slots
+    [T]`` (int32) of ``cache`` (:func:`kv4_cache`); returns ``cache``.  Every 64 elements of a token's
+    head get a bf16 minimum and scale = (max - min) / 15 and codes rint((x - minimum) / scale) in 0..15; a
+    group that is not finite reads back as NaN.  A negative slot is padding and skipped, one past the
+    cache is skipped and reported by :func:`kernel_status` (code 3).  The slots must differ."""
+    pages, heads, page, d = _check_cache(cache)
+    ks, vs = _check_rows(k, "k"), _check_rows(v, "v", k.dtype)
+    t = k.shape[0]
+    if k.shape != (t, heads, d) or v.shape != k.shape:
+        raise ValueError(f"k and v must be [T, {heads}, {d}] for this cache, got {tuple(k.shape)} and {tuple(v.shape)}")
+    _check_index(slots, "slots", t)
+    _on_tensors_device("sf_kv4_store", (k, v, slots, cache), k.data_ptr(), v.data_ptr(), slots.data_ptr(), cache.data_ptr(), t, heads, d,
+                       pages, page, struct.pack("4q", *ks, *vs), _native.DTYPE_CODES[dtype_name(k)])
+    return cache
+
+
+def kv4_load(cache: torch.Tensor, slots: torch.Tensor, dtype: torch.dtype = torch.bfloat16, k_out: torch.Tensor | None = None,
+             v_out: torch.Tensor | None = None) -> tuple[torch.Tensor, torch.Tensor]:
+    """Read the tokens at ``slots [T]`` (int32, in any order, repeated or not) of a 4-bit cache back as
+    ``(k, v)``, each ``[T, H, D]`` in ``dtype`` (minimum + scale * code, rounded once), e.g. as the
+    context of a prompt's next chunk for :func:`window_attention`.  Negative slots (and, reported by
+    :func:`kernel_status`, slots past the cache) read as zeros."""
+    pages, heads, page, d = _check_cache(cache)
+    _check_index(slots, "slots")
+    t = slots.shape[0]
+    dtype = dtype if k_out is None else k_out.dtype
+    k_out = torch.empty((t, heads, d), dtype=dtype, device=cache.device) if k_out is None else k_out
+    v_out = torch.empty((t, heads, d), dtype=dtype, device=cache.device) if v_out is None else v_out
+    ks, vs = _check_rows(k_out, "k_out", dtype, written=True), _check_rows(v_out, "v_out", dtype, written=True)
+    if k_out.shape != (t, heads, d) or v_out.shape != (t, heads, d):
+        raise ValueError(f"k_out and v_out must be [{t}, {heads}, {d}]")
+    _on_tensors_device("sf_kv4_load", (cache, slots, k_out, v_out), cache.data_ptr(), slots.data_ptr(), k_out.data_ptr(), v_out.data_ptr(),
+                       t, heads, d, pages, page, struct.pack("4q", *ks, *vs), _native.DTYPE_CODES[dtype_name(k_out)])
+    return k_out, v_out
+
+
+def kv4_attention_workspace_bytes(batch: int, q_heads: int, kv_heads: int, dim: int, page_size: int, table_width: int, window: int = 0,
+                                  sinks: int = 0, variant: int = 0) -> int:
+    """Workspace bytes of :func:`kv4_attention` (0 when a request's keys stay with one CTA)."""
+    return int(_native.load().sf_kv4_attention_workspace_bytes(batch, q_heads, kv_heads, dim, page_size, table_width, window, sinks, variant))
+
+
+def kv4_attention(q: torch.Tensor, cache: torch.Tensor, block_table: torch.Tensor, seq_lens: torch.Tensor, scale: float, window: int = 0,
+                  sinks: int = 0, out: torch.Tensor | None = None, workspace: torch.Tensor | None = None, variant: int = 0) -> torch.Tensor:
+    """Attention of one query token a request over the 4-bit paged cache: ``softmax(q K^T * scale) V``.
+
+    ``q [B, Hq, D]`` (unit stride along D), Hq a multiple of the cache's heads; ``block_table [B, width]``
+    (int32, rows may be strided) holds each request's pages in order, ``seq_lens [B]`` (int32) its tokens
+    in the cache, the query's own last.  Token ``j`` is seen when ``j >= seq_len - window`` or ``j <
+    sinks`` (``window`` 0: all).  A length of 0 gives zeros; a length past the table is cut to it and a
+    page id outside the cache hides its tokens, both reported by :func:`kernel_status` (code 3).
+    ``workspace`` (uint8, :func:`kv4_attention_workspace_bytes`) is allocated here when not given;
+    calls that overlap on the GPU need one each.  ``variant``: 0 = by size, 1 = all requests' keys
+    dealt evenly to all CTAs, 3 = a CTA a (request, head)."""
+    pages, heads, page, d = _check_cache(cache)
+    qs = _check_rows(q, "q")
+    b, hq = q.shape[:2]
+    if q.shape[2] != d or hq % heads:
+        raise ValueError(f"q must be [B, a multiple of {heads}, {d}] for this cache, got {tuple(q.shape)}")
+    if not isinstance(block_table, torch.Tensor) or not block_table.is_cuda or block_table.dtype != torch.int32:
+        raise TypeError("block_table must be an int32 CUDA tensor")
+    if block_table.dim() != 2 or block_table.shape[0] != b or (block_table.shape[1] > 1 and block_table.stride(1) != 1):
+        raise ValueError(f"block_table must be [{b}, width] with unit stride along a row")
+    width = block_table.shape[1]
+    _check_index(seq_lens, "seq_lens", b)
+    out = torch.empty((b, hq, d), dtype=q.dtype, device=q.device) if out is None else out
+    os_ = _check_rows(out, "out", q.dtype, written=True)
+    if out.shape != q.shape:
+        raise ValueError(f"out must be {tuple(q.shape)}")
+    if workspace is None:
+        need = kv4_attention_workspace_bytes(b, hq, heads, d, page, width, window, sinks, variant)
+        if need:
+            workspace = torch.empty(need, dtype=torch.uint8, device=q.device)
+    else:
+        _check(workspace, "workspace")
+    ws_ptr, ws_bytes = (0, 0) if workspace is None else (workspace.data_ptr(), workspace.numel() * workspace.element_size())
+    tensors = (q, cache, block_table, seq_lens, out) if workspace is None else (q, cache, block_table, seq_lens, out, workspace)
+    strides = struct.pack("5q", *qs, *os_, block_table.stride(0) if b > 1 else 0)
+    _on_tensors_device("sf_kv4_attention", tensors, q.data_ptr(), cache.data_ptr(), block_table.data_ptr(), seq_lens.data_ptr(),
+                       out.data_ptr(), ws_ptr, ws_bytes, b, hq, heads, d, pages, page, width, strides, float(scale), int(window), int(sinks),
+                       _native.DTYPE_CODES[dtype_name(q)], int(variant))
+    return out
+
+
+def window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqlens: torch.Tensor, scale: float, window: int = 0, sinks: int = 0,
+                     cu_seqlens_k: torch.Tensor | None = None, out: torch.Tensor | None = None, variant: int = 0) -> torch.Tensor:
+    """Causal attention of packed prompts with grouped heads, a sliding window and sinks.
+
+    ``q [Tq, Hq, D]``, ``k, v [Tk, Hk, D]`` (unit stride along D, Hq a multiple of Hk); sequence ``s`` has
+    the queries ``cu_seqlens[s] : cu_seqlens[s + 1]`` and the keys of ``cu_seqlens_k`` (default: the same
+    rows).  Query ``i`` of a sequence with nq queries and nk keys sits at ``p = i + nk - nq`` and sees the
+    keys ``j <= p`` with ``j > p - window`` or ``j < sinks`` (``window`` 0: all ``j <= p``), so a prompt's next
+    chunk comes with its whole context as keys.  A query that sees nothing gives zeros; rows of ``out``
+    that belong to no sequence are left as they were.  D up to 256; D 64 and 128 with 16-byte aligned
+    rows and at most 128 query heads a key head run on the tensor cores.  ``variant``: 0 = by shape, 1 =
+    tensor cores (refused where they do not apply), 2 = general kernel."""
+    qs, ks, vs = _check_rows(q, "q"), _check_rows(k, "k", q.dtype), _check_rows(v, "v", q.dtype)
+    tq, hq, d = q.shape
+    tk, hk, _ = k.shape
+    if k.shape[2] != d or v.shape != k.shape or hk == 0 or hq % hk:
+        raise ValueError(f"window_attention expects k and v of one shape [Tk, Hk, {d}] with Hk dividing {hq}, got {tuple(k.shape)} and {tuple(v.shape)}")
+    _check_index(cu_seqlens, "cu_seqlens")
+    cu_k = cu_seqlens if cu_seqlens_k is None else cu_seqlens_k
+    _check_index(cu_k, "cu_seqlens_k", cu_seqlens.shape[0])
+    seqs = cu_seqlens.shape[0] - 1
+    if seqs < 0:
+        raise ValueError("cu_seqlens must have at least one entry")
+    out = torch.empty((tq, hq, d), dtype=q.dtype, device=q.device) if out is None else out
+    os_ = _check_rows(out, "out", q.dtype, written=True)
+    if out.shape != q.shape:
+        raise ValueError(f"out must be {tuple(q.shape)}")
+    _on_tensors_device("sf_window_attention", (q, k, v, cu_seqlens, cu_k, out), q.data_ptr(), k.data_ptr(), v.data_ptr(),
+                       cu_seqlens.data_ptr(), cu_k.data_ptr(), out.data_ptr(), tq, tk, seqs, hq, hk, d,
+                       struct.pack("8q", *qs, *ks, *vs, *os_), float(scale), int(window), int(sinks), _native.DTYPE_CODES[dtype_name(q)],
+                       int(variant))
     return out
