@@ -246,21 +246,35 @@ SF_API int sf_mamba2_chunk_scan(const void* x, const void* dt, const void* dA_cu
 
 /* ---------------------------------------------------------------------------------------
  * Serving operators: no reference counterpart (its tasks have neither grouped heads, a cache nor
- * windows); they stand beside rmsnorm, rope and flash_attention.  Tensors are [tokens, heads, D] with
- * unit stride along D; `strides` holds the token and head strides in elements, tensor after tensor,
- * NULL for contiguous tensors.  Index tensors are int32.  F16 / BF16, fp32 arithmetic.
+ * windows); they stand beside rmsnorm, rope and flash_attention.  Their arguments come in a struct, read
+ * before the call returns.  Tensors are [tokens, heads, D] with unit stride along D and the token and
+ * head strides, in elements, that the struct gives; index tensors are int32 and contiguous.  F16 / BF16
+ * in and out, fp32 arithmetic.
  * ------------------------------------------------------------------------------------- */
+
+/* Token and head stride of a [tokens, heads, D] tensor, in elements. */
+typedef struct sf_rows {
+    int64_t token;
+    int64_t head;
+} sf_rows;
 
 /*
  * qk_norm_rope: per-head RMS norm of q [T, Hq, D] and k [T, Hk, D] (weights wq, wk [D]) and, in the
- * same pass, the rotate-half rotary embedding of the first `rotary` elements at position[t]:
- *   y = x * rsqrt(mean(x^2) + eps) * w,  r = rotary / 2,  angle = position[t] * base^(-i / r)
+ * same pass, the rotate-half rotary embedding of the first `rotary` elements at positions[t]:
+ *   y = x * rsqrt(mean(x^2) + eps) * w,  r = rotary / 2,  angle = positions[t] * base^(-i / r)
  *   out[i] = y[i] cos - y[i+r] sin,  out[i+r] = y[i] sin + y[i+r] cos,  i < r;  out = y behind rotary.
- * strides: q, k, q_out, k_out.  The outputs may be the inputs.  rotary even, 0..D.
+ * The outputs may be the inputs.  rotary even, 0..D.  variant 1 forces the vectorised kernel, 2 the
+ * general one.
  */
-SF_API int sf_qk_norm_rope(const void* q, const void* k, const void* wq, const void* wk, const void* positions, void* q_out,
-               void* k_out, int64_t T, int64_t Hq, int64_t Hk, int64_t D, const int64_t* strides, int64_t rotary, double base,
-               float eps, int32_t dtype, void* stream, char* err, uint64_t cap);
+typedef struct sf_qk_norm_rope_args {
+    const void *q, *k, *wq, *wk, *positions;
+    void *q_out, *k_out;
+    int64_t T, Hq, Hk, D, rotary;
+    sf_rows q_rows, k_rows, q_out_rows, k_out_rows;
+    double base, eps;
+    int32_t dtype, variant;
+} sf_qk_norm_rope_args;
+SF_API int sf_qk_norm_rope(const sf_qk_norm_rope_args* args, void* stream, char* err, uint64_t cap);
 
 /*
  * The 4-bit paged key/value cache: [pages, H, page_size / 16, 18 D] bytes (16-byte aligned, page_size a
@@ -271,42 +285,65 @@ SF_API int sf_qk_norm_rope(const void* q, const void* k, const void* wq, const v
  *
  * kv4_store writes tokens k, v [T, H, D] at slots[T]; kv4_load reads them back.  A negative slot is
  * padding (nothing written; zeros read); one past the cache is treated the same and reported through
- * sf_kernel_status (code 3).  The slots of one store must differ: of two tokens at one slot a mixture may stay.
- * strides: k, v (multiples of 8 elements).
+ * sf_kernel_status (code 3).  The slots of one store must differ: of two tokens at one slot a mixture
+ * may stay.  k and v 16-byte aligned, strides multiples of 8 elements.
  */
-SF_API int sf_kv4_store(const void* k, const void* v, const void* slots, void* cache, int64_t T, int64_t H, int64_t D,
-               int64_t pages, int64_t page_size, const int64_t* strides, int32_t dtype, void* stream, char* err, uint64_t cap);
-SF_API int sf_kv4_load(const void* cache, const void* slots, void* k, void* v, int64_t T, int64_t H, int64_t D, int64_t pages,
-               int64_t page_size, const int64_t* strides, int32_t dtype, void* stream, char* err, uint64_t cap);
+typedef struct sf_kv4_cache_args {
+    void *k, *v;
+    const void* slots;
+    void* cache;
+    int64_t T, H, D, pages, page_size;
+    sf_rows k_rows, v_rows;
+    int32_t dtype, variant;
+} sf_kv4_cache_args;
+SF_API int sf_kv4_store(const sf_kv4_cache_args* args, void* stream, char* err, uint64_t cap);
+SF_API int sf_kv4_load(const sf_kv4_cache_args* args, void* stream, char* err, uint64_t cap);
 
 /*
  * kv4_attention: one query token a request over the 4-bit cache, o[b] = softmax(scale q[b] . K^T) V, q and
  * o [B, Hq, D], Hq a multiple of the cache's Hk (query head h reads head h / (Hq / Hk)).  Request b has
  * lens[b] tokens (the query's own last); token j sits at row j % page_size of page table[b, j / page_size],
- * table [B, width].  Seen are j >= lens[b] - window or j < sinks (window 0: all).  lens[b] <= 0 gives
- * zeros; a length past the table is cut to it, a page id outside the cache hides its tokens, both
- * reported through sf_kernel_status (code 3).  strides: q, o, then the table's row stride (5 numbers).
- * workspace: 16-byte aligned, sf_kv4_attention_workspace_bytes bytes (variant 0; 0 bytes: may be NULL), no
- * initial content; two calls that overlap on the GPU need one each.  variant: see SF_OP_KV4_ATTENTION.
+ * table [B, width] with table_stride elements from row to row.  Seen are j >= lens[b] - window or
+ * j < sinks (window 0: all).  lens[b] <= 0 gives zeros; a length past the table is cut to it, a page id
+ * outside the cache hides its tokens, both reported through sf_kernel_status (code 3).  q and o 16-byte
+ * aligned, strides multiples of 8 elements.  workspace: 16-byte aligned,
+ * sf_kv4_attention_workspace_bytes bytes (0: may be NULL), no initial content; two calls that overlap
+ * on the GPU need one each.  variant 1 deals every request's keys to all CTAs, 3 keeps a (request,
+ * head) to a CTA, 0 decides by size.
  */
+typedef struct sf_kv4_attention_args {
+    const void *q, *cache, *table, *lens;
+    void *o, *workspace;
+    uint64_t workspace_bytes;
+    int64_t B, Hq, Hk, D, pages, page_size, width, table_stride;
+    sf_rows q_rows, o_rows;
+    int64_t window, sinks;
+    double scale;
+    int32_t dtype, variant;
+} sf_kv4_attention_args;
 SF_API uint64_t sf_kv4_attention_workspace_bytes(int64_t B, int64_t Hq, int64_t Hk, int64_t D, int64_t page_size, int64_t width,
                int64_t window, int64_t sinks, int32_t variant);
-SF_API int sf_kv4_attention(const void* q, const void* cache, const void* table, const void* lens, void* o, void* workspace,
-               uint64_t workspace_bytes, int64_t B, int64_t Hq, int64_t Hk, int64_t D, int64_t pages, int64_t page_size,
-               int64_t width, const int64_t* strides, float scale, int64_t window, int64_t sinks, int32_t dtype, int32_t variant, void* stream,
-               char* err, uint64_t cap);
+SF_API int sf_kv4_attention(const sf_kv4_attention_args* args, void* stream, char* err, uint64_t cap);
 
 /*
  * window_attention: attention of packed prompts, q, o [Tq, Hq, D], k, v [Tk, Hk, D], Hq a multiple of Hk.
  * Sequence s has queries cu_q[s]..cu_q[s+1] and keys cu_k[s]..cu_k[s+1] (both [seqs + 1], not decreasing);
  * its query i sits at position p = i + nk - nq and sees keys j <= p with j > p - window or j < sinks
  * (window 0: all j <= p).  A query that sees nothing gives zeros; rows of no sequence are left as they
- * were.  strides: q, k, v, o.  D <= 256; tcgen05 kernel for D in {64, 128}, 16-byte aligned tensors and
- * strides and at most 128 query heads a key head, general kernel otherwise.  variant as in sf_op_desc.
+ * were.  D <= 256; tcgen05 kernel for D in {64, 128}, 16-byte aligned tensors, strides that are
+ * multiples of 8 elements and at most 128 query heads a key head (variant 1 forces it), general kernel
+ * otherwise (variant 2).
  */
-SF_API int sf_window_attention(const void* q, const void* k, const void* v, const void* cu_q, const void* cu_k, void* o,
-               int64_t Tq, int64_t Tk, int64_t seqs, int64_t Hq, int64_t Hk, int64_t D, const int64_t* strides, float scale,
-               int64_t window, int64_t sinks, int32_t dtype, int32_t variant, void* stream, char* err, uint64_t cap);
+typedef struct sf_window_attention_args {
+    const void *q, *k, *v, *cu_q, *cu_k;
+    void* o;
+    int64_t Tq, Tk, seqs, Hq, Hk, D;
+    sf_rows q_rows, k_rows, v_rows, o_rows;
+    int64_t window, sinks;
+    double scale;
+    int32_t dtype, variant;
+} sf_window_attention_args;
+SF_API int sf_window_attention(const sf_window_attention_args* args, void* stream, char* err, uint64_t cap);
 
 /*
  * gemm_nt: C[M,N] = A[M,K] . B[N,K]^T, fp16 or bf16 in, fp32 accumulation, one rounding

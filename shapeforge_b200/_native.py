@@ -9,6 +9,7 @@ from __future__ import annotations
 
 import ctypes
 import os
+import struct
 import threading
 from pathlib import Path
 
@@ -94,6 +95,16 @@ OPS = {
     "window_attention": 26,
 }
 
+# The serving operators' argument structs (include/sfcuda.h), packed in one go: a ctypes call costs
+# ~0.25 us an argument on the host, and these have up to 30.
+ARGS = {
+    "sf_qk_norm_rope": struct.Struct("7P 5q 8q 2d 2i"),
+    "sf_kv4_store": struct.Struct("4P 5q 4q 2i"),
+    "sf_kv4_load": struct.Struct("4P 5q 4q 2i"),
+    "sf_kv4_attention": struct.Struct("6P Q 8q 4q 2q d 2i"),
+    "sf_window_attention": struct.Struct("6P 6q 8q 2q d 2i"),
+}
+
 _P = ctypes.c_void_p
 _I32 = ctypes.c_int32
 _I64 = ctypes.c_int64
@@ -130,12 +141,12 @@ SIGNATURES: dict[str, tuple[object, tuple]] = {
     "sf_varlen_kda_gated_workspace_bytes": (_U64, (_I64, _I64, _I64, _I64)),
     "sf_varlen_kda_gated_ws": (ctypes.c_int, (_P,) * 9 + (_I64, _I64, _I64, _I64, _F32, _I32, _P, _U64, _P, *_ERR)),
     "sf_mamba2_chunk_scan": (ctypes.c_int, (_P,) * 8 + (_I64,) * 6 + (_I32, _P, *_ERR)),
-    "sf_qk_norm_rope": (ctypes.c_int, (_P,) * 7 + (_I64,) * 4 + (_P, _I64, ctypes.c_double, _F32, _I32, _P, *_ERR)),
-    "sf_kv4_store": (ctypes.c_int, (_P,) * 4 + (_I64,) * 5 + (_P, _I32, _P, *_ERR)),
-    "sf_kv4_load": (ctypes.c_int, (_P,) * 4 + (_I64,) * 5 + (_P, _I32, _P, *_ERR)),
+    "sf_qk_norm_rope": (ctypes.c_int, (_P, _P, *_ERR)),
+    "sf_kv4_store": (ctypes.c_int, (_P, _P, *_ERR)),
+    "sf_kv4_load": (ctypes.c_int, (_P, _P, *_ERR)),
     "sf_kv4_attention_workspace_bytes": (_U64, (_I64,) * 8 + (_I32,)),
-    "sf_kv4_attention": (ctypes.c_int, (_P,) * 6 + (_U64,) + (_I64,) * 7 + (_P, _F32, _I64, _I64, _I32, _I32, _P, *_ERR)),
-    "sf_window_attention": (ctypes.c_int, (_P,) * 6 + (_I64,) * 6 + (_P, _F32, _I64, _I64, _I32, _I32, _P, *_ERR)),
+    "sf_kv4_attention": (ctypes.c_int, (_P, _P, *_ERR)),
+    "sf_window_attention": (ctypes.c_int, (_P, _P, *_ERR)),
     "sf_gemm_nt": (ctypes.c_int, (_P, _P, _P, _I64, _I64, _I64, _I32, _P, *_ERR)),
     "sf_gemm_nn_workspace_bytes": (_U64, (_I64, _I64, _I64, _I32)),
     "sf_gemm_nn": (ctypes.c_int, (_P, _P, _P, _I64, _I64, _I64, _I32, _P, _U64, _P, *_ERR)),
@@ -194,6 +205,20 @@ def call(name: str, *args) -> None:
     lib = load()
     buf = ctypes.create_string_buffer(ERR_CAP)
     rc = getattr(lib, name)(*args, buf, ERR_CAP)
+    if rc != SF_OK:
+        raise SfError(int(rc), buf.value.decode(errors="replace") or name)
+
+
+_err = threading.local()
+
+
+def call_args(name: str, stream: int, *fields) -> None:
+    """Call an entry point that takes an argument struct; raise on failure."""
+    try:
+        buf = _err.buf
+    except AttributeError:
+        buf = _err.buf = ctypes.create_string_buffer(ERR_CAP)
+    rc = getattr(_lib or load(), name)(ARGS[name].pack(*fields), stream, buf, ERR_CAP)
     if rc != SF_OK:
         raise SfError(int(rc), buf.value.decode(errors="replace") or name)
 

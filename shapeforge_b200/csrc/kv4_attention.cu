@@ -29,6 +29,7 @@
 #include "kv4.cuh"
 
 #include <algorithm>
+#include <initializer_list>
 #include <mutex>
 #include <type_traits>
 
@@ -712,60 +713,6 @@ int launch_t(Args a, const Plan& p, cudaStream_t st, char* err, uint64_t cap) {
 
 }  // namespace
 
-int sf_kv4_attention_launch(const void* q, const void* cache, const void* table, const void* lens, void* o, void* workspace, uint64_t workspace_bytes,
-                            int64_t B, int64_t Hq, int64_t Hk, int64_t D, int64_t pages, int64_t page_size, int64_t width, const int64_t* strides,
-                            float scale, int64_t window, int64_t sinks, int32_t dtype, int32_t variant, cudaStream_t st, char* err, uint64_t cap) {
-    if (B < 0 || Hq < 0 || Hk < 0 || pages < 0 || width < 0) return sf::fail(SF_EINVAL, err, cap, "kv4_attention: negative size");
-    if (D != 64 && D != 128) return sf::fail(SF_EINVAL, err, cap, "kv4_attention: D must be 64 or 128");
-    if (page_size < 16 || page_size % 16) return sf::fail(SF_EINVAL, err, cap, "kv4_attention: the page size must be a multiple of 16");
-    if (pages > 0x7fffffffLL / page_size || width > 0x7fffffffLL / page_size)
-        return sf::fail(SF_EINVAL, err, cap, "kv4_attention: more than 2^31 - 1 slots");
-    if (Hq && (Hk == 0 || Hq % Hk)) return sf::fail(SF_EINVAL, err, cap, "kv4_attention: the query heads must be a multiple of the cache's heads");
-    if (!(scale > 0.f) || !(scale < INFINITY)) return sf::fail(SF_EINVAL, err, cap, "kv4_attention: scale must be > 0");
-    if (window < 0 || sinks < 0) return sf::fail(SF_EINVAL, err, cap, "kv4_attention: window and sinks must be >= 0");
-    if (dtype != SF_DTYPE_F16 && dtype != SF_DTYPE_BF16) return sf::fail(SF_EINVAL, err, cap, "kv4_attention: dtype %d is not fp16/bf16", dtype);
-    if (B * Hq == 0) return SF_OK;
-    if (!q || !o || !lens || (pages && !cache) || (width && !table)) return sf::fail(SF_EINVAL, err, cap, "kv4_attention: null tensor pointer");
-    const int64_t dense[5] = {Hq * D, D, Hq * D, D, width};
-    const int64_t* s = strides ? strides : dense;
-    for (int i = 0; i < 5; ++i)
-        if (s[i] < 0 || (i < 4 && s[i] % 8)) return sf::fail(SF_EINVAL, err, cap, "kv4_attention: strides of q and out must be multiples of 8 elements");
-    if (!sf::aligned16(q) || !sf::aligned16(o) || !sf::aligned16(cache)) return sf::fail(SF_EINVAL, err, cap, "kv4_attention: q, out and the cache must be 16-byte aligned");
-    const int64_t tpp = page_size / 16;
-    if (pages * Hk > 0x7fffffffLL / tpp) return sf::fail(SF_EINVAL, err, cap, "kv4_attention: more than 2^31 - 1 records");
-    // The tiles of all requests are counted in 32 bits.
-    if (B > 0x7fffffffLL / std::max<int64_t>(1, width * tpp)) return sf::fail(SF_EINVAL, err, cap, "kv4_attention: requests x table width too large");
-    const Plan p = plan_of(B, Hq, Hk, D, width, tpp, window, sinks, variant);
-    if (B * Hk > 0x7fffffffLL / p.blocks) return sf::fail(SF_EINVAL, err, cap, "kv4_attention: grid too large");
-    if (p.split && (!workspace || workspace_bytes < workspace_of(p, D) || !sf::aligned16(workspace)))
-        return sf::fail(SF_EINVAL, err, cap, "kv4_attention: needs a 16-byte aligned workspace of %llu bytes", (unsigned long long)workspace_of(p, D));
-    Args a = {};
-    a.q = q;
-    a.o = o;
-    a.cache = (const uint8_t*)cache;
-    a.table = (const int32_t*)table;
-    a.lens = (const int32_t*)lens;
-    if (p.split) {
-        a.part = (float*)workspace;
-        a.stat = a.part + (int64_t)p.grid * 2 * 8 * p.nt * D;
-        a.chain = (int32_t*)(a.stat + (int64_t)p.grid * 2 * 8 * p.nt * 2);
-    }
-    a.qb = s[0], a.qh = s[1], a.ob = s[2], a.oh = s[3], a.tb = s[4];
-    a.window = (int)std::min<int64_t>(window, 0x7fffffff);  // lengths are below 2^31
-    a.sinks = window ? (int)std::min<int64_t>(sinks, 0x7fffffff - 15) : 0;
-    a.B = (int)B, a.Hk = (int)Hk, a.group = (int)(Hq / Hk), a.blocks = p.blocks;
-    a.pages = (int)pages, a.tpp = (int)tpp, a.width = (int)width;
-    a.scale_log2 = scale * LOG2E;
-    a.split = p.split;
-    const bool half = dtype == SF_DTYPE_F16;
-    if (D == 64) {
-        if (p.nt == 1) return half ? launch_t<__half, 1, 1>(a, p, st, err, cap) : launch_t<__nv_bfloat16, 1, 1>(a, p, st, err, cap);
-        return half ? launch_t<__half, 1, 2>(a, p, st, err, cap) : launch_t<__nv_bfloat16, 1, 2>(a, p, st, err, cap);
-    }
-    if (p.nt == 1) return half ? launch_t<__half, 2, 1>(a, p, st, err, cap) : launch_t<__nv_bfloat16, 2, 1>(a, p, st, err, cap);
-    return half ? launch_t<__half, 2, 2>(a, p, st, err, cap) : launch_t<__nv_bfloat16, 2, 2>(a, p, st, err, cap);
-}
-
 int sf_kv4_attention_status_read(uint32_t* code, uint32_t* where, cudaStream_t stream) {
     return kv4::read_status(g_kv4_attention_status, code, where, stream);
 }
@@ -776,11 +723,59 @@ extern "C" uint64_t sf_kv4_attention_workspace_bytes(int64_t B, int64_t Hq, int6
     return workspace_of(plan_of(B, Hq, Hk, D, width, page_size / 16, window, sinks, variant), D);
 }
 
-extern "C" int sf_kv4_attention(const void* q, const void* cache, const void* table, const void* lens, void* o, void* workspace,
-                                uint64_t workspace_bytes, int64_t B, int64_t Hq, int64_t Hk, int64_t D, int64_t pages, int64_t page_size,
-                                int64_t width, const int64_t* strides, float scale, int64_t window, int64_t sinks, int32_t dtype, int32_t variant,
-                                void* stream,
-                                char* err, uint64_t cap) {
-    return sf_kv4_attention_launch(q, cache, table, lens, o, workspace, workspace_bytes, B, Hq, Hk, D, pages, page_size, width, strides, scale, window,
-                                   sinks, dtype, variant, (cudaStream_t)stream, err, cap);
+extern "C" int sf_kv4_attention(const sf_kv4_attention_args* x, void* stream, char* err, uint64_t cap) {
+    if (!x) return sf::fail(SF_EINVAL, err, cap, "kv4_attention: null arguments");
+    const int64_t B = x->B, Hq = x->Hq, Hk = x->Hk, D = x->D, pages = x->pages, page_size = x->page_size, width = x->width;
+    const int64_t window = x->window, sinks = x->sinks;
+    const float scale = (float)x->scale;
+    if (B < 0 || Hq < 0 || Hk < 0 || pages < 0 || width < 0) return sf::fail(SF_EINVAL, err, cap, "kv4_attention: negative size");
+    if (D != 64 && D != 128) return sf::fail(SF_EINVAL, err, cap, "kv4_attention: D must be 64 or 128");
+    if (page_size < 16 || page_size % 16) return sf::fail(SF_EINVAL, err, cap, "kv4_attention: the page size must be a multiple of 16");
+    if (pages > 0x7fffffffLL / page_size || width > 0x7fffffffLL / page_size)
+        return sf::fail(SF_EINVAL, err, cap, "kv4_attention: more than 2^31 - 1 slots");
+    if (Hq && (Hk == 0 || Hq % Hk)) return sf::fail(SF_EINVAL, err, cap, "kv4_attention: the query heads must be a multiple of the cache's heads");
+    if (!(scale > 0.f) || !(scale < INFINITY)) return sf::fail(SF_EINVAL, err, cap, "kv4_attention: scale must be > 0");
+    if (window < 0 || sinks < 0) return sf::fail(SF_EINVAL, err, cap, "kv4_attention: window and sinks must be >= 0");
+    if (x->dtype != SF_DTYPE_F16 && x->dtype != SF_DTYPE_BF16) return sf::fail(SF_EINVAL, err, cap, "kv4_attention: dtype %d is not fp16/bf16", x->dtype);
+    for (int64_t s : {x->q_rows.token, x->q_rows.head, x->o_rows.token, x->o_rows.head})
+        if (s < 0 || s % 8) return sf::fail(SF_EINVAL, err, cap, "kv4_attention: strides of q and out must be multiples of 8 elements");
+    if (x->table_stride < 0) return sf::fail(SF_EINVAL, err, cap, "kv4_attention: negative table stride");
+    if (B * Hq == 0) return SF_OK;
+    if (!x->q || !x->o || !x->lens || (pages && !x->cache) || (width && !x->table)) return sf::fail(SF_EINVAL, err, cap, "kv4_attention: null tensor pointer");
+    if (!sf::aligned16(x->q) || !sf::aligned16(x->o) || !sf::aligned16(x->cache))
+        return sf::fail(SF_EINVAL, err, cap, "kv4_attention: q, out and the cache must be 16-byte aligned");
+    const int64_t tpp = page_size / 16;
+    if (pages * Hk > 0x7fffffffLL / tpp) return sf::fail(SF_EINVAL, err, cap, "kv4_attention: more than 2^31 - 1 records");
+    // The tiles of all requests are counted in 32 bits.
+    if (B > 0x7fffffffLL / std::max<int64_t>(1, width * tpp)) return sf::fail(SF_EINVAL, err, cap, "kv4_attention: requests x table width too large");
+    const Plan p = plan_of(B, Hq, Hk, D, width, tpp, window, sinks, x->variant);
+    if (B * Hk > 0x7fffffffLL / p.blocks) return sf::fail(SF_EINVAL, err, cap, "kv4_attention: grid too large");
+    if (p.split && (!x->workspace || x->workspace_bytes < workspace_of(p, D) || !sf::aligned16(x->workspace)))
+        return sf::fail(SF_EINVAL, err, cap, "kv4_attention: needs a 16-byte aligned workspace of %llu bytes", (unsigned long long)workspace_of(p, D));
+    Args a = {};
+    a.q = x->q;
+    a.o = x->o;
+    a.cache = (const uint8_t*)x->cache;
+    a.table = (const int32_t*)x->table;
+    a.lens = (const int32_t*)x->lens;
+    if (p.split) {
+        a.part = (float*)x->workspace;
+        a.stat = a.part + (int64_t)p.grid * 2 * 8 * p.nt * D;
+        a.chain = (int32_t*)(a.stat + (int64_t)p.grid * 2 * 8 * p.nt * 2);
+    }
+    a.qb = x->q_rows.token, a.qh = x->q_rows.head, a.ob = x->o_rows.token, a.oh = x->o_rows.head, a.tb = x->table_stride;
+    a.window = (int)std::min<int64_t>(window, 0x7fffffff);  // lengths are below 2^31
+    a.sinks = window ? (int)std::min<int64_t>(sinks, 0x7fffffff - 15) : 0;
+    a.B = (int)B, a.Hk = (int)Hk, a.group = (int)(Hq / Hk), a.blocks = p.blocks;
+    a.pages = (int)pages, a.tpp = (int)tpp, a.width = (int)width;
+    a.scale_log2 = scale * LOG2E;
+    a.split = p.split;
+    const bool half = x->dtype == SF_DTYPE_F16;
+    cudaStream_t st = (cudaStream_t)stream;
+    if (D == 64) {
+        if (p.nt == 1) return half ? launch_t<__half, 1, 1>(a, p, st, err, cap) : launch_t<__nv_bfloat16, 1, 1>(a, p, st, err, cap);
+        return half ? launch_t<__half, 1, 2>(a, p, st, err, cap) : launch_t<__nv_bfloat16, 1, 2>(a, p, st, err, cap);
+    }
+    if (p.nt == 1) return half ? launch_t<__half, 2, 1>(a, p, st, err, cap) : launch_t<__nv_bfloat16, 2, 1>(a, p, st, err, cap);
+    return half ? launch_t<__half, 2, 2>(a, p, st, err, cap) : launch_t<__nv_bfloat16, 2, 2>(a, p, st, err, cap);
 }

@@ -6,6 +6,8 @@
 // computed once.
 #include "kv4.cuh"
 
+#include <initializer_list>
+
 __device__ sm100::KernelStatus g_kv4_status[2];  // [0] an index out of range; [1] unused
 
 namespace {
@@ -171,20 +173,26 @@ __global__ void __launch_bounds__(256) kv4_load_kernel(const Args a) {
     }
 }
 
-int check(const char* what, const void* k, const void* v, const void* slots, const void* cache, int64_t T, int64_t H, int64_t D, int64_t pages,
-          int64_t page_size, const int64_t* s, int32_t dtype, char* err, uint64_t cap) {
-    if (T < 0 || H < 0 || pages < 0) return sf::fail(SF_EINVAL, err, cap, "%s: negative size", what);
-    if (D != 64 && D != 128) return sf::fail(SF_EINVAL, err, cap, "%s: D must be 64 or 128", what);
-    if (page_size < 16 || page_size % 16) return sf::fail(SF_EINVAL, err, cap, "%s: the page size must be a multiple of 16", what);
-    if (pages > 0x7fffffffLL / page_size) return sf::fail(SF_EINVAL, err, cap, "%s: the cache has more than 2^31 - 1 slots", what);
-    if (dtype != SF_DTYPE_F16 && dtype != SF_DTYPE_BF16) return sf::fail(SF_EINVAL, err, cap, "%s: dtype %d is not fp16/bf16", what, dtype);
-    if (H > 65535) return sf::fail(SF_EINVAL, err, cap, "%s: too many heads", what);
-    if (T * H == 0) return SF_OK;
-    if (!k || !v || !slots || !cache) return sf::fail(SF_EINVAL, err, cap, "%s: null tensor pointer", what);
-    if (!sf::aligned16(k) || !sf::aligned16(v) || !sf::aligned16(cache)) return sf::fail(SF_EINVAL, err, cap, "%s: k, v and the cache must be 16-byte aligned", what);
-    for (int i = 0; i < 4; ++i)
-        if (s[i] < 0 || s[i] % 8) return sf::fail(SF_EINVAL, err, cap, "%s: strides must be multiples of 8 elements", what);
+int check(const char* what, const sf_kv4_cache_args* x, char* err, uint64_t cap) {
+    if (!x) return sf::fail(SF_EINVAL, err, cap, "%s: null arguments", what);
+    if (x->T < 0 || x->H < 0 || x->pages < 0) return sf::fail(SF_EINVAL, err, cap, "%s: negative size", what);
+    if (x->D != 64 && x->D != 128) return sf::fail(SF_EINVAL, err, cap, "%s: D must be 64 or 128", what);
+    if (x->page_size < 16 || x->page_size % 16) return sf::fail(SF_EINVAL, err, cap, "%s: the page size must be a multiple of 16", what);
+    if (x->pages > 0x7fffffffLL / x->page_size) return sf::fail(SF_EINVAL, err, cap, "%s: the cache has more than 2^31 - 1 slots", what);
+    if (x->dtype != SF_DTYPE_F16 && x->dtype != SF_DTYPE_BF16) return sf::fail(SF_EINVAL, err, cap, "%s: dtype %d is not fp16/bf16", what, x->dtype);
+    if (x->H > 65535) return sf::fail(SF_EINVAL, err, cap, "%s: too many heads", what);
+    for (int64_t s : {x->k_rows.token, x->k_rows.head, x->v_rows.token, x->v_rows.head})
+        if (s < 0 || s % 8) return sf::fail(SF_EINVAL, err, cap, "%s: strides must be multiples of 8 elements", what);
+    if (x->T * x->H == 0) return SF_OK;
+    if (!x->k || !x->v || !x->slots || (x->pages && !x->cache)) return sf::fail(SF_EINVAL, err, cap, "%s: null tensor pointer", what);
+    if (!sf::aligned16(x->k) || !sf::aligned16(x->v) || !sf::aligned16(x->cache))
+        return sf::fail(SF_EINVAL, err, cap, "%s: k, v and the cache must be 16-byte aligned", what);
     return SF_OK;
+}
+
+Args args_of(const sf_kv4_cache_args& x) {
+    return Args{x.k, x.v, (const int32_t*)x.slots, (uint8_t*)x.cache, x.T, x.k_rows.token, x.k_rows.head, x.v_rows.token, x.v_rows.head,
+                x.pages * x.page_size, (int)x.H, 0, (int)(x.page_size / 16)};
 }
 
 template <typename F>
@@ -202,44 +210,28 @@ int launch(F kernel, Args a, int ng, const char* what, cudaStream_t st, char* er
 
 }  // namespace
 
-int sf_kv4_store_launch(const void* k, const void* v, const void* slots, void* cache, int64_t T, int64_t H, int64_t D, int64_t pages,
-                        int64_t page_size, const int64_t* strides, int32_t dtype, cudaStream_t st, char* err, uint64_t cap) {
-    const int64_t dense[4] = {H * D, D, H * D, D};
-    const int64_t* s = strides ? strides : dense;
-    const int rc = check("kv4_store", k, v, slots, cache, T, H, D, pages, page_size, s, dtype, err, cap);
-    if (rc || T * H == 0) return rc;
-    Args a{const_cast<void*>(k), const_cast<void*>(v), (const int32_t*)slots, (uint8_t*)cache, T, s[0], s[1], s[2], s[3], pages * page_size, (int)H, 0,
-           (int)(page_size / 16)};
-    if (dtype == SF_DTYPE_F16)
-        return D == 64 ? launch(kv4_store_kernel<__half, 1>, a, 1, "kv4_store launch", st, err, cap)
-                       : launch(kv4_store_kernel<__half, 2>, a, 2, "kv4_store launch", st, err, cap);
-    return D == 64 ? launch(kv4_store_kernel<__nv_bfloat16, 1>, a, 1, "kv4_store launch", st, err, cap)
-                   : launch(kv4_store_kernel<__nv_bfloat16, 2>, a, 2, "kv4_store launch", st, err, cap);
-}
-
-int sf_kv4_load_launch(const void* cache, const void* slots, void* k, void* v, int64_t T, int64_t H, int64_t D, int64_t pages,
-                       int64_t page_size, const int64_t* strides, int32_t dtype, cudaStream_t st, char* err, uint64_t cap) {
-    const int64_t dense[4] = {H * D, D, H * D, D};
-    const int64_t* s = strides ? strides : dense;
-    const int rc = check("kv4_load", k, v, slots, cache, T, H, D, pages, page_size, s, dtype, err, cap);
-    if (rc || T * H == 0) return rc;
-    Args a{k, v, (const int32_t*)slots, (uint8_t*)const_cast<void*>(cache), T, s[0], s[1], s[2], s[3], pages * page_size, (int)H, 0,
-           (int)(page_size / 16)};
-    if (dtype == SF_DTYPE_F16)
-        return D == 64 ? launch(kv4_load_kernel<__half, 1>, a, 1, "kv4_load launch", st, err, cap)
-                       : launch(kv4_load_kernel<__half, 2>, a, 2, "kv4_load launch", st, err, cap);
-    return D == 64 ? launch(kv4_load_kernel<__nv_bfloat16, 1>, a, 1, "kv4_load launch", st, err, cap)
-                   : launch(kv4_load_kernel<__nv_bfloat16, 2>, a, 2, "kv4_load launch", st, err, cap);
-}
-
 int sf_kv4_status_read(uint32_t* code, uint32_t* where, cudaStream_t stream) { return kv4::read_status(g_kv4_status, code, where, stream); }
 
-extern "C" int sf_kv4_store(const void* k, const void* v, const void* slots, void* cache, int64_t T, int64_t H, int64_t D, int64_t pages,
-                            int64_t page_size, const int64_t* strides, int32_t dtype, void* stream, char* err, uint64_t cap) {
-    return sf_kv4_store_launch(k, v, slots, cache, T, H, D, pages, page_size, strides, dtype, (cudaStream_t)stream, err, cap);
+extern "C" int sf_kv4_store(const sf_kv4_cache_args* x, void* stream, char* err, uint64_t cap) {
+    const int rc = check("kv4_store", x, err, cap);
+    if (rc || x->T * x->H == 0) return rc;
+    const Args a = args_of(*x);
+    cudaStream_t st = (cudaStream_t)stream;
+    if (x->dtype == SF_DTYPE_F16)
+        return x->D == 64 ? launch(kv4_store_kernel<__half, 1>, a, 1, "kv4_store launch", st, err, cap)
+                          : launch(kv4_store_kernel<__half, 2>, a, 2, "kv4_store launch", st, err, cap);
+    return x->D == 64 ? launch(kv4_store_kernel<__nv_bfloat16, 1>, a, 1, "kv4_store launch", st, err, cap)
+                      : launch(kv4_store_kernel<__nv_bfloat16, 2>, a, 2, "kv4_store launch", st, err, cap);
 }
 
-extern "C" int sf_kv4_load(const void* cache, const void* slots, void* k, void* v, int64_t T, int64_t H, int64_t D, int64_t pages,
-                           int64_t page_size, const int64_t* strides, int32_t dtype, void* stream, char* err, uint64_t cap) {
-    return sf_kv4_load_launch(cache, slots, k, v, T, H, D, pages, page_size, strides, dtype, (cudaStream_t)stream, err, cap);
+extern "C" int sf_kv4_load(const sf_kv4_cache_args* x, void* stream, char* err, uint64_t cap) {
+    const int rc = check("kv4_load", x, err, cap);
+    if (rc || x->T * x->H == 0) return rc;
+    const Args a = args_of(*x);
+    cudaStream_t st = (cudaStream_t)stream;
+    if (x->dtype == SF_DTYPE_F16)
+        return x->D == 64 ? launch(kv4_load_kernel<__half, 1>, a, 1, "kv4_load launch", st, err, cap)
+                          : launch(kv4_load_kernel<__half, 2>, a, 2, "kv4_load launch", st, err, cap);
+    return x->D == 64 ? launch(kv4_load_kernel<__nv_bfloat16, 1>, a, 1, "kv4_load launch", st, err, cap)
+                      : launch(kv4_load_kernel<__nv_bfloat16, 2>, a, 2, "kv4_load launch", st, err, cap);
 }

@@ -23,6 +23,7 @@
 #include "sf_common.cuh"
 
 #include <cmath>
+#include <initializer_list>
 
 namespace {
 
@@ -254,31 +255,26 @@ int launch_t(const Side& q, const Side& k, const int32_t* pos, int64_t T_, int h
 
 }  // namespace
 
-int sf_qk_norm_rope_launch(const void* q, const void* k, const void* wq, const void* wk, const void* positions, void* q_out, void* k_out,
-                           int64_t T, int64_t Hq, int64_t Hk, int64_t D, const int64_t* strides, int64_t rotary, double base, float eps,
-                           int32_t dtype, int32_t variant, cudaStream_t st, char* err, uint64_t cap) {
+extern "C" int sf_qk_norm_rope(const sf_qk_norm_rope_args* x, void* stream, char* err, uint64_t cap) {
+    if (!x) return sf::fail(SF_EINVAL, err, cap, "qk_norm_rope: null arguments");
+    const int64_t T = x->T, Hq = x->Hq, Hk = x->Hk, D = x->D;
     if (T < 0 || Hq < 0 || Hk < 0 || Hq + Hk > (1 << 20) || D < 1 || D > (1 << 20))
         return sf::fail(SF_EINVAL, err, cap, "qk_norm_rope: need T, Hq, Hk >= 0 and D >= 1");
-    if (rotary < 0 || rotary % 2 || rotary > D) return sf::fail(SF_EINVAL, err, cap, "qk_norm_rope: rotary must be even and at most D");
-    if (!(base > 0) || !std::isfinite(base)) return sf::fail(SF_EINVAL, err, cap, "qk_norm_rope: base must be > 0");
-    if (!(eps >= 0)) return sf::fail(SF_EINVAL, err, cap, "qk_norm_rope: eps must be >= 0");
-    if (dtype != SF_DTYPE_F16 && dtype != SF_DTYPE_BF16) return sf::fail(SF_EINVAL, err, cap, "qk_norm_rope: dtype %d is not fp16/bf16", dtype);
+    if (x->rotary < 0 || x->rotary % 2 || x->rotary > D) return sf::fail(SF_EINVAL, err, cap, "qk_norm_rope: rotary must be even and at most D");
+    if (!(x->base > 0) || !std::isfinite(x->base)) return sf::fail(SF_EINVAL, err, cap, "qk_norm_rope: base must be > 0");
+    if (!(x->eps >= 0)) return sf::fail(SF_EINVAL, err, cap, "qk_norm_rope: eps must be >= 0");
+    if (x->dtype != SF_DTYPE_F16 && x->dtype != SF_DTYPE_BF16)
+        return sf::fail(SF_EINVAL, err, cap, "qk_norm_rope: dtype %d is not fp16/bf16", x->dtype);
+    for (const sf_rows* r : {&x->q_rows, &x->k_rows, &x->q_out_rows, &x->k_out_rows})
+        if (r->token < 0 || r->head < 0) return sf::fail(SF_EINVAL, err, cap, "qk_norm_rope: negative stride");
     if (T * (Hq + Hk) == 0) return SF_OK;
-    if (!positions || (Hq && (!q || !q_out || !wq)) || (Hk && (!k || !k_out || !wk)))
+    if (!x->positions || (Hq && (!x->q || !x->q_out || !x->wq)) || (Hk && (!x->k || !x->k_out || !x->wk)))
         return sf::fail(SF_EINVAL, err, cap, "qk_norm_rope: null tensor pointer");
-    const int64_t dense[8] = {Hq * D, D, Hk * D, D, Hq * D, D, Hk * D, D};
-    const int64_t* s = strides ? strides : dense;
-    for (int i = 0; i < 8; ++i)
-        if (s[i] < 0) return sf::fail(SF_EINVAL, err, cap, "qk_norm_rope: negative stride");
-    const Side sq{q, q_out, wq, s[0], s[1], s[4], s[5]}, sk{k, k_out, wk, s[2], s[3], s[6], s[7]};
-    if (dtype == SF_DTYPE_F16)
-        return launch_t<__half>(sq, sk, (const int32_t*)positions, T, (int)Hq, (int)Hk, (int)D, (int)rotary, base, eps, variant, st, err, cap);
-    return launch_t<__nv_bfloat16>(sq, sk, (const int32_t*)positions, T, (int)Hq, (int)Hk, (int)D, (int)rotary, base, eps, variant, st, err, cap);
-}
-
-extern "C" int sf_qk_norm_rope(const void* q, const void* k, const void* wq, const void* wk, const void* positions, void* q_out, void* k_out,
-                               int64_t T, int64_t Hq, int64_t Hk, int64_t D, const int64_t* strides, int64_t rotary, double base,
-                               float eps, int32_t dtype, void* stream, char* err, uint64_t cap) {
-    return sf_qk_norm_rope_launch(q, k, wq, wk, positions, q_out, k_out, T, Hq, Hk, D, strides, rotary, base, eps, dtype, 0,
-                                  (cudaStream_t)stream, err, cap);
+    const Side q{x->q, x->q_out, x->wq, x->q_rows.token, x->q_rows.head, x->q_out_rows.token, x->q_out_rows.head};
+    const Side k{x->k, x->k_out, x->wk, x->k_rows.token, x->k_rows.head, x->k_out_rows.token, x->k_out_rows.head};
+    const int32_t* pos = (const int32_t*)x->positions;
+    if (x->dtype == SF_DTYPE_F16)
+        return launch_t<__half>(q, k, pos, T, (int)Hq, (int)Hk, (int)D, (int)x->rotary, x->base, (float)x->eps, x->variant, (cudaStream_t)stream, err, cap);
+    return launch_t<__nv_bfloat16>(q, k, pos, T, (int)Hq, (int)Hk, (int)D, (int)x->rotary, x->base, (float)x->eps, x->variant, (cudaStream_t)stream, err,
+                                   cap);
 }

@@ -252,19 +252,6 @@ int sf_mamba2_launch(const void* x, const void* dt, const void* cs, const void* 
                      void* y, int64_t B, int64_t L, int64_t H, int64_t P, int64_t N, int64_t C, int32_t dtype, int32_t variant,
                      cudaStream_t st, char* err, uint64_t cap);
 int sf_mamba2_status_read(uint32_t* code, uint32_t* where, cudaStream_t stream);
-int sf_qk_norm_rope_launch(const void* q, const void* k, const void* wq, const void* wk, const void* positions, void* q_out, void* k_out,
-                           int64_t T, int64_t Hq, int64_t Hk, int64_t D, const int64_t* strides, int64_t rotary, double base, float eps,
-                           int32_t dtype, int32_t variant, cudaStream_t st, char* err, uint64_t cap);
-int sf_kv4_store_launch(const void* k, const void* v, const void* slots, void* cache, int64_t T, int64_t H, int64_t D, int64_t pages,
-                        int64_t page_size, const int64_t* strides, int32_t dtype, cudaStream_t st, char* err, uint64_t cap);
-int sf_kv4_load_launch(const void* cache, const void* slots, void* k, void* v, int64_t T, int64_t H, int64_t D, int64_t pages,
-                       int64_t page_size, const int64_t* strides, int32_t dtype, cudaStream_t st, char* err, uint64_t cap);
 int sf_kv4_status_read(uint32_t* code, uint32_t* where, cudaStream_t stream);
-int sf_kv4_attention_launch(const void* q, const void* cache, const void* table, const void* lens, void* o, void* workspace,
-                            uint64_t workspace_bytes, int64_t B, int64_t Hq, int64_t Hk, int64_t D, int64_t pages, int64_t page_size,
-                            int64_t width, const int64_t* strides, float scale, int64_t window, int64_t sinks, int32_t dtype,
-                            int32_t variant, cudaStream_t st, char* err, uint64_t cap);
 int sf_kv4_attention_status_read(uint32_t* code, uint32_t* where, cudaStream_t stream);
-int sf_window_attention_launch(const void* q, const void* k, const void* v, const void* cu_q, const void* cu_k, void* o, int64_t Tq,
-                               int64_t Tk, int64_t seqs, int64_t Hq, int64_t Hk, int64_t D, const int64_t* strides, float scale,
-                               int64_t window, int64_t sinks, int32_t dtype, int32_t variant, cudaStream_t st, char* err, uint64_t cap);
+int sf_window_status_read(uint32_t* code, uint32_t* where, cudaStream_t stream);

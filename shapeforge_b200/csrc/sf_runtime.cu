@@ -195,23 +195,36 @@ static int dispatch(const sf_op_desc* d, const void* const* a, cudaStream_t s, c
             return sf_kda_fixed_launch(a[0], a[1], a[2], a[3], a[4], a[5], a[6], a[7], a[8], (void*)a[9], (void*)a[10], (void*)a[11],
                                        (void*)a[12], d->dims[0], d->dims[1], d->dims[2], (float)d->attrs[0], d->dtype, d->variant, s,
                                        err, cap);
-        case SF_OP_QK_NORM_ROPE:
-            return sf_qk_norm_rope_launch(a[0], a[1], a[2], a[3], a[4], (void*)a[5], (void*)a[6], d->dims[0], d->dims[1], d->dims[2],
-                                          d->dims[3], nullptr, d->dims[4], d->attrs[0], (float)d->attrs[1], d->dtype, d->variant, s, err, cap);
+        case SF_OP_QK_NORM_ROPE: {
+            const int64_t Hq = d->dims[1], Hk = d->dims[2], D = d->dims[3];
+            const sf_rows q = {Hq * D, D}, k = {Hk * D, D};
+            const sf_qk_norm_rope_args x = {a[0], a[1], a[2], a[3], a[4], (void*)a[5], (void*)a[6], d->dims[0], Hq, Hk, D, d->dims[4],
+                                            q, k, q, k, d->attrs[0], d->attrs[1], d->dtype, d->variant};
+            return sf_qk_norm_rope(&x, s, err, cap);
+        }
         case SF_OP_KV4_STORE:
-            return sf_kv4_store_launch(a[0], a[1], a[2], (void*)a[3], d->dims[0], d->dims[1], d->dims[2], d->dims[3], d->dims[4], nullptr,
-                                       d->dtype, s, err, cap);
-        case SF_OP_KV4_LOAD:
-            return sf_kv4_load_launch(a[0], a[1], (void*)a[2], (void*)a[3], d->dims[0], d->dims[1], d->dims[2], d->dims[3], d->dims[4],
-                                      nullptr, d->dtype, s, err, cap);
-        case SF_OP_KV4_ATTENTION:
-            return sf_kv4_attention_launch(a[0], a[1], a[2], a[3], (void*)a[4], (void*)a[5], (uint64_t)d->dims[7], d->dims[0], d->dims[1],
-                                           d->dims[2], d->dims[3], d->dims[4], d->dims[5], d->dims[6], nullptr, (float)d->attrs[0],
-                                           (int64_t)d->attrs[1], (int64_t)d->attrs[2], d->dtype, d->variant, s, err, cap);
-        case SF_OP_WINDOW_ATTENTION:
-            return sf_window_attention_launch(a[0], a[1], a[2], a[3], a[4], (void*)a[5], d->dims[0], d->dims[1], d->dims[2], d->dims[3],
-                                              d->dims[4], d->dims[5], nullptr, (float)d->attrs[0], d->dims[6], d->dims[7], d->dtype,
-                                              d->variant, s, err, cap);
+        case SF_OP_KV4_LOAD: {
+            const bool store = d->op == SF_OP_KV4_STORE;
+            const sf_rows r = {d->dims[1] * d->dims[2], d->dims[2]};
+            const sf_kv4_cache_args x = {(void*)a[store ? 0 : 2], (void*)a[store ? 1 : 3], a[store ? 2 : 1], (void*)a[store ? 3 : 0],
+                                         d->dims[0], d->dims[1], d->dims[2], d->dims[3], d->dims[4], r, r, d->dtype, d->variant};
+            return store ? sf_kv4_store(&x, s, err, cap) : sf_kv4_load(&x, s, err, cap);
+        }
+        case SF_OP_KV4_ATTENTION: {
+            const int64_t Hq = d->dims[1], D = d->dims[3];
+            const sf_rows r = {Hq * D, D};
+            const sf_kv4_attention_args x = {a[0], a[1], a[2], a[3], (void*)a[4], (void*)a[5], (uint64_t)d->dims[7], d->dims[0], Hq,
+                                             d->dims[2], D, d->dims[4], d->dims[5], d->dims[6], d->dims[6], r, r,
+                                             (int64_t)d->attrs[1], (int64_t)d->attrs[2], d->attrs[0], d->dtype, d->variant};
+            return sf_kv4_attention(&x, s, err, cap);
+        }
+        case SF_OP_WINDOW_ATTENTION: {
+            const int64_t Hq = d->dims[3], Hk = d->dims[4], D = d->dims[5];
+            const sf_rows q = {Hq * D, D}, k = {Hk * D, D};
+            const sf_window_attention_args x = {a[0], a[1], a[2], a[3], a[4], (void*)a[5], d->dims[0], d->dims[1], d->dims[2], Hq, Hk, D,
+                                                q, k, k, q, d->dims[6], d->dims[7], d->attrs[0], d->dtype, d->variant};
+            return sf_window_attention(&x, s, err, cap);
+        }
         default:
             return sf::fail(SF_EINVAL, err, cap, "unknown op %d", d->op);
     }

@@ -13,6 +13,9 @@
 
 #include <algorithm>
 #include <cmath>
+#include <initializer_list>
+#include <mutex>
+#include <type_traits>
 
 namespace {
 
@@ -102,6 +105,482 @@ __global__ void __launch_bounds__(128) window_general_kernel(const Args a, int D
     row_by_warp<T>(a, D, row, head, kb, p, (T*)a.o + row * a.ot + (int64_t)head * a.oh);
 }
 
+// ---- tensor-core kernel: D 64 / 128 ----------------------------------------------------------------
+//
+// The query heads of a kv head share its keys, so a tile's 128 rows are (token, head of the group) pairs:
+// TQ = 128 / g tokens with their g heads.  A window then costs a tile g times less padding, and short
+// prompts fill their rows.  A CTA takes two such tiles of consecutive tokens over one stream of key tiles
+// (each key and value tile is fetched once for 256 rows) and owns an SM:
+//   warp 0        TMA producer: both Q tiles, then K_j and V_j tiles of up to 128 keys, two slots each;
+//   warp 1        MMA issuer, in the order P0.V(j-1), S0(j), P1.V(j-1), S1(j): one tile's products run
+//                 under the other's softmax; S (then P over it) and O of both tiles fill TMEM;
+//   warp 2        zeroes the value rows behind a sequence's last key (0 times another sequence's NaN or
+//                 infinity would be NaN) and hands the tile on;
+//   warps 4..7    softmax of tile 0, a thread a row; warps 8..11 of tile 1.
+// Key tiles begin at the first key that the CTA's first token sees (a TMA coordinate along the tokens
+// needs no alignment), and the sinks in front of it are a tile of their own; a tile of n keys costs
+// n rounded up to 16 in both products and 32 in the softmax.  Tiles that every row sees in full skip the
+// mask.  Running max and sum in fp32; the max follows a score only past 2^8, so O is rarely rescaled.
+// P is rounded to the tensors' type (as the fp32 sum of the unrounded weights divides it, a weight is off
+// by half a step, which averages out over the keys).
+// A row that comes out NaN is computed again key by key: masked keys in its tiles may hold infinities or
+// NaN that their zero weights do not silence.
+
+constexpr int BOX = 128 * 128;       // 128 rows of 64 16-bit elements
+constexpr int TC_THREADS = 384;
+constexpr uint32_t O_COL = 256;      // S / P of tile t at column 128 t, O at 256 + 128 t
+
+__device__ sm100::KernelStatus g_window_status;
+
+struct __align__(8) Bars {
+    uint64_t q_full[2];
+    uint64_t k_full[2], k_empty[2];
+    uint64_t v_full[2], v_ready[2], v_empty[2];
+    uint64_t s_full[2], p_full[2][2], o_done[2];
+    uint32_t tmem_base;
+};
+
+template <int D>
+struct Layout {
+    static constexpr int DB = D / 64;
+    static constexpr int TILE = DB * BOX;
+    static constexpr int Q = 0;              // [2]
+    static constexpr int K = 2 * TILE;       // [2]
+    static constexpr int V = 4 * TILE;       // [2]
+    static constexpr int BARS = 6 * TILE;
+    static constexpr int BYTES = BARS + 256;
+};
+
+// The key tiles of a CTA: sinks [0, sink_end), then [low, high) in steps of 128.
+struct Walk {
+    int sink_end, sink_tiles, low, high, n;
+    int last[2];    // position of each tile's last token (-1: no tile)
+    int first[2];   // position of each tile's first token
+    int window, sinks;
+    __device__ __forceinline__ int start(int j) const { return j < sink_tiles ? 128 * j : low + 128 * (j - sink_tiles); }
+    // Keys of tile j that tile t's rows can see: [0, count).
+    __device__ __forceinline__ int count(int t, int j) const {
+        const int end = j < sink_tiles ? sink_end : min(high, last[t] + 1);
+        return max(0, min(128, end - start(j)));
+    }
+    __device__ __forceinline__ bool active(int t, int j) const {
+        if (last[t] < 0 || count(t, j) <= 0) return false;
+        if (j < sink_tiles || !window) return true;
+        const int s = start(j);
+        return s + 128 > first[t] - window + 1 || s < sinks;
+    }
+    // Every row of tile t sees all 128 keys of tile j.
+    __device__ __forceinline__ bool full(int t, int j) const {
+        const int s = start(j);
+        if (j < sink_tiles) return s + 128 <= sink_end;
+        return s + 127 <= first[t] && (!window || s > last[t] - window || s + 128 <= sinks);
+    }
+};
+
+// Bits [0, n) of a 32-bit word.
+__device__ __forceinline__ uint32_t below(int n) { return n <= 0 ? 0u : (n >= 32 ? 0xFFFFFFFFu : (1u << n) - 1u); }
+
+__device__ __forceinline__ float max3_nan(float a, float b, float c) {
+    float d;
+    asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+    return d;
+}
+
+// Running state of a row: `m` the max that weights are relative to (log2 units), `l` their sum.
+struct RowState {
+    float m, l;
+    // Take in a tile's row max; O (in TMEM) is rescaled when the max has grown by more than 2^8.
+    template <int D>
+    __device__ __forceinline__ float raise(float rmax, float scale_log2, uint32_t tmem_o, bool some) {
+        const float m_new = max3_nan(m, rmax * scale_log2, m);
+        const bool need = !(m_new <= m + 8.0f);
+        if (some) {
+            if (__any_sync(0xffffffffu, need)) {
+                const float alpha = need ? exp2f(m - m_new) : 1.0f;
+#pragma unroll 1
+                for (int c = 0; c < D / 32; ++c) {
+                    uint32_t r[32];
+                    sm100::tmem_ld_32x32b_x32(tmem_o + (uint32_t)(32 * c), r);
+                    sm100::tmem_ld_wait();
+#pragma unroll
+                    for (int i = 0; i < 32; ++i) r[i] = __float_as_uint(__uint_as_float(r[i]) * alpha);
+                    sm100::tmem_st_32x32b_x32(tmem_o + (uint32_t)(32 * c), r);
+                }
+                l *= alpha;
+            }
+        }
+        if (need) m = m_new;
+        return m == -INFINITY ? 0.f : m;
+    }
+};
+
+// 32 scores to weights (16 packed words), adding them up.
+template <typename T>
+__device__ __forceinline__ void weights32(const uint32_t* r, float scale_log2, float m, float2 (&acc)[2], uint32_t (&w)[16]) {
+    const float2 sc = sf::f2(scale_log2), nm = sf::f2(-m);
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+        const float2 x = sf::f2_fma(make_float2(__uint_as_float(r[2 * i]), __uint_as_float(r[2 * i + 1])), sc, nm);
+        const float2 p = make_float2(sf::ex2_ftz(x.x), sf::ex2_ftz(x.y));
+        acc[i & 1] = sf::f2_add(acc[i & 1], p);
+        w[i] = sf::Pair<T>::from_f2(p);
+    }
+}
+
+__device__ __forceinline__ float max32(const uint32_t* r, float m) {
+    float a[2] = {m, -INFINITY};
+#pragma unroll
+    for (int i = 0; i < 32; i += 4) {
+        a[0] = max3_nan(a[0], __uint_as_float(r[i]), __uint_as_float(r[i + 1]));
+        a[1] = max3_nan(a[1], __uint_as_float(r[i + 2]), __uint_as_float(r[i + 3]));
+    }
+    return max3_nan(a[0], a[1], a[1]);
+}
+
+template <typename T, int D>
+__global__ void __launch_bounds__(TC_THREADS, 1)
+    window_tc_kernel(const Args a, const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUtensorMap mk16,
+                     const __grid_constant__ CUtensorMap mv, const __grid_constant__ CUtensorMap mv16, int tq_tile) {
+    using L = Layout<D>;
+    constexpr int DB = L::DB;
+    constexpr bool BF16 = std::is_same<T, __nv_bfloat16>::value;
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+    Bars* bars = reinterpret_cast<Bars*>(smem + L::BARS);
+    sm100::KernelStatus* status = &g_window_status;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int kvh = blockIdx.y;
+
+    // ---- which tokens: sequence i owns the slots from cu[i] / TT + i on, later tiles (more keys) first ----
+    const int TT = 2 * tq_tile;
+    const int slot = gridDim.x - 1 - blockIdx.x;
+    int lo = 0, hi = a.seqs;
+    while (hi - lo > 1) {
+        const int step = (hi - lo + 31) >> 5;
+        const int i = lo + lane * step;
+        bool here = false;
+        if (i < hi) here = (int)(min((int64_t)max(0, __ldg(a.cu_q + i)), a.tq) / TT) + i <= slot;
+        const uint32_t yes = __ballot_sync(0xffffffffu, here);
+        const int k = yes ? 31 - __clz(yes) : 0;
+        lo = lo + k * step;
+        hi = min(hi, lo + step);
+    }
+    int64_t qb, qe, kb, ke;
+    bounds(a.cu_q, lo, a.tq, &qb, &qe);
+    bounds(a.cu_k, lo, a.tk, &kb, &ke);
+    const int64_t tok0 = qb + (int64_t)(slot - (int)(qb / TT) - lo) * TT;
+    if (tok0 < qb || tok0 >= qe) return;
+    const int rows_tok[2] = {(int)min((int64_t)tq_tile, qe - tok0), (int)max((int64_t)0, min((int64_t)tq_tile, qe - tok0 - tq_tile))};
+    const int pos0 = (int)((tok0 - qb) + (ke - kb) - (qe - qb));  // position of the CTA's first token
+    Walk w;
+    w.window = a.window;
+    w.sinks = a.sinks;
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+        w.first[t] = pos0 + t * tq_tile;
+        w.last[t] = rows_tok[t] ? w.first[t] + rows_tok[t] - 1 : -1;
+    }
+    w.high = max(0, max(w.last[0], w.last[1]) + 1);
+    w.low = a.window ? max(0, pos0 - a.window + 1) : 0;
+    w.sink_end = min(a.sinks, w.low);
+    w.sink_tiles = (w.sink_end + 127) >> 7;
+    w.n = w.high > 0 ? w.sink_tiles + ((w.high - w.low + 127) >> 7) : 0;
+
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < 2; ++i) {
+            sm100::mbar_init(&bars->q_full[i], 1);
+            sm100::mbar_init(&bars->k_full[i], 1);
+            sm100::mbar_init(&bars->k_empty[i], 1);
+            sm100::mbar_init(&bars->v_full[i], 1);
+            sm100::mbar_init(&bars->v_ready[i], 32);
+            sm100::mbar_init(&bars->v_empty[i], 1);
+            sm100::mbar_init(&bars->s_full[i], 1);
+            sm100::mbar_init(&bars->p_full[i][0], 128);
+            sm100::mbar_init(&bars->p_full[i][1], 128);
+            sm100::mbar_init(&bars->o_done[i], 1);
+        }
+        sm100::fence_mbar_init();
+    }
+    // Rows of the Q tiles that no copy writes.
+    const int qrows = tq_tile * a.group;
+    for (int i = threadIdx.x; i < 2 * DB * (128 - qrows) * 8; i += TC_THREADS) {
+        const int box = i / ((128 - qrows) * 8), rest = i % ((128 - qrows) * 8);
+        *reinterpret_cast<uint4*>(smem + L::Q + box * BOX + (qrows + rest / 8) * 128 + (rest % 8) * 16) = make_uint4(0, 0, 0, 0);
+    }
+    sm100::fence_proxy_async_smem();
+    if (warp == 1) {
+        sm100::tmem_alloc(&bars->tmem_base, 512);
+        sm100::tmem_relinquish();
+    }
+    sm100::tc_fence_before();
+    __syncthreads();
+    sm100::tc_fence_after();
+    const uint32_t tmem = bars->tmem_base;
+
+    if (warp < 4) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
+        if (warp == 0) {
+            if (lane == 0 && w.n > 0) {
+                for (int t = 0; t < 2; ++t) {
+                    if (w.last[t] < 0) continue;
+                    sm100::mbar_arrive_expect_tx(&bars->q_full[t], DB * qrows * 128);
+                    for (int b = 0; b < DB; ++b)
+                        sm100::tma_load_3d(smem + L::Q + (t * DB + b) * BOX, &mq, &bars->q_full[t], 64 * b, kvh * a.group, (int)tok0 + t * tq_tile);
+                }
+                int keys_in = 0, values_in = 0;  // tiles whose copies were issued
+                for (int j = 0; j < w.n; ++j) {
+                    const int st = j & 1;
+                    const uint32_t ph = (uint32_t)(j >> 1) & 1u;
+                    // Keys that some tile multiplies, in whole 16s.
+                    const int rows = (max(w.count(0, j), w.count(1, j)) + 15) & ~15;
+                    const int key = (int)kb + w.start(j);
+                    for (int kv = 0; kv < 2; ++kv) {
+                        uint64_t* empty = kv ? &bars->v_empty[st] : &bars->k_empty[st];
+                        uint64_t* full = kv ? &bars->v_full[st] : &bars->k_full[st];
+                        uint8_t* dst = smem + (kv ? L::V : L::K) + st * L::TILE;
+                        if (!sm100::mbar_wait(empty, ph ^ 1u, status, 120 + kv)) goto fetched;
+                        sm100::mbar_arrive_expect_tx(full, DB * rows * 128);
+                        ++(kv ? values_in : keys_in);
+                        for (int b = 0; b < DB; ++b) {
+                            if (rows == 128) {
+                                sm100::tma_load_3d(dst + b * BOX, kv ? &mv : &mk, full, 64 * b, kvh, key);
+                            } else {
+                                for (int r = 0; r < rows; r += 16)
+                                    sm100::tma_load_3d(dst + b * BOX + r * 128, kv ? &mv16 : &mk16, full, 64 * b, kvh, key + r);
+                            }
+                        }
+                    }
+                }
+            fetched:
+                // No copy is in flight when the CTA ends, also after a wait that gave up.
+                for (int t = 0; t < 2; ++t)
+                    if (w.last[t] >= 0) sm100::mbar_wait(&bars->q_full[t], 0, nullptr, 0);
+                for (int j = max(0, keys_in - 2); j < keys_in; ++j) sm100::mbar_wait(&bars->k_full[j & 1], (uint32_t)(j >> 1) & 1u, nullptr, 0);
+                for (int j = max(0, values_in - 2); j < values_in; ++j) sm100::mbar_wait(&bars->v_full[j & 1], (uint32_t)(j >> 1) & 1u, nullptr, 0);
+            }
+        } else if (warp == 1) {
+            if (lane == 0 && w.n > 0) {
+                constexpr uint32_t idesc_s = sm100::idesc_f16(128, 0, BF16);
+                constexpr uint32_t idesc_o = sm100::idesc_f16_bmn(128, D, BF16);
+                uint32_t turns[2] = {0, 0};  // tiles of P consumed
+                bool ok = true;
+                for (int j = 0; j <= w.n && ok; ++j) {
+                    for (int t = 0; t < 2 && ok; ++t) {
+                        if (j > 0 && w.active(t, j - 1)) {
+                            // O_t += P_t(j-1) . V(j-1), each half of the keys when its P is there.
+                            const int st = (j - 1) & 1;
+                            ok = sm100::mbar_wait(&bars->v_ready[st], (uint32_t)((j - 1) >> 1) & 1u, status, 122);
+                            const uint32_t sv = sm100::smem_u32(smem + L::V + st * L::TILE);
+                            const int steps = (w.count(t, j - 1) + 15) >> 4;
+                            for (int h = 0; h < 2 && ok; ++h) {
+                                ok = sm100::mbar_wait(&bars->p_full[t][h], turns[t] & 1u, status, 123);
+                                sm100::tc_fence_after();
+                                for (int kk = 4 * h; kk < min(steps, 4 * h + 4) && ok; ++kk)
+                                    sm100::mma_f16_ta(tmem + O_COL + 128u * t, tmem + 128u * t + (uint32_t)(32 * (kk >> 1) + 8 * (kk & 1)),
+                                                      sm100::smem_desc_mn_sw128(sv + (uint32_t)(kk * 16 * 128), BOX, 1024), idesc_o,
+                                                      turns[t] > 0 || kk > 0 ? 1u : 0u);
+                            }
+                            ++turns[t];
+                            if (ok && (t == 1 || !w.active(1, j - 1))) sm100::mma_commit(&bars->v_empty[st]);
+                        }
+                        if (ok && j < w.n && w.active(t, j)) {
+                            // S_t(j) = Q_t . K(j)^T over the columns that P_t(j-1) was read from (the pipe runs
+                            // this thread's products in order).
+                            const int st = j & 1;
+                            if (turns[t] == 0) ok = sm100::mbar_wait(&bars->q_full[t], 0, status, 124);
+                            ok = ok && sm100::mbar_wait(&bars->k_full[st], (uint32_t)(j >> 1) & 1u, status, 125);
+                            if (!ok) break;
+                            sm100::tc_fence_after();
+                            const uint32_t sq = sm100::smem_u32(smem + L::Q + t * L::TILE), sk = sm100::smem_u32(smem + L::K + st * L::TILE);
+                            const uint32_t n16 = (uint32_t)((w.count(t, j) + 15) & ~15);
+#pragma unroll
+                            for (int k = 0; k < D / 16; ++k) {
+                                const uint32_t off = (uint32_t)((k >> 2) * BOX + (k & 3) * 32);
+                                sm100::mma_f16(tmem + 128u * t, sm100::smem_desc_k_sw128(sq + off), sm100::smem_desc_k_sw128(sk + off),
+                                               idesc_s | ((n16 >> 3) << 17), k > 0 ? 1u : 0u);
+                            }
+                            sm100::mma_commit(&bars->s_full[t]);
+                            if (t == 1 || !w.active(1, j)) sm100::mma_commit(&bars->k_empty[st]);
+                        }
+                    }
+                }
+                // Also after a wait that gave up: the tensor pipe drains before TMEM is freed.
+                sm100::mma_commit(&bars->o_done[0]);
+                sm100::mma_commit(&bars->o_done[1]);
+            }
+        } else if (warp == 2) {
+            for (int j = 0; j < w.n; ++j) {
+                const int st = j & 1;
+                if (!__all_sync(0xffffffffu, sm100::mbar_wait(&bars->v_full[st], (uint32_t)(j >> 1) & 1u, status, 126))) break;
+                const int rows = (max(w.count(0, j), w.count(1, j)) + 15) & ~15;
+                const int real = (int)min((int64_t)rows, ke - kb - w.start(j));
+                for (int i = lane; i < DB * (rows - real) * 8; i += 32) {
+                    const int b = i / ((rows - real) * 8), rest = i % ((rows - real) * 8);
+                    *reinterpret_cast<uint4*>(smem + L::V + st * L::TILE + b * BOX + (real + rest / 8) * 128 + (rest % 8) * 16) = make_uint4(0, 0, 0, 0);
+                }
+                if (real < rows) sm100::fence_proxy_async_smem();
+                sm100::mbar_arrive(&bars->v_ready[st]);
+            }
+        }
+    } else {
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 224;");
+        const int t = (warp >> 2) - 1;
+        const int row = (warp & 3) * 32 + lane;
+        const int tok = row / a.group, head = kvh * a.group + row - tok * a.group;
+        const int n_tok = t ? rows_tok[1] : rows_tok[0];
+        const int first = t ? w.first[1] : w.first[0];
+        const bool live = row < qrows && tok < n_tok;
+        const int p = live ? first + tok : -1;
+        const uint32_t lane_off = (uint32_t)((warp & 3) * 32) << 16;
+        const uint32_t ts = tmem + 128u * t + lane_off, to = tmem + O_COL + 128u * t + lane_off;
+        RowState s{-INFINITY, 0.f};
+        uint32_t turn = 0;
+        bool ok = true;
+        for (int j = 0; j < w.n; ++j) {
+            if (!w.active(t, j)) continue;
+            if (!sm100::mbar_wait(&bars->s_full[t], turn & 1u, status, 127)) {
+                ok = false;
+                break;
+            }
+            sm100::tc_fence_after();
+            float2 acc[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+            if (w.full(t, j)) {
+                uint32_t r[128];
+#pragma unroll
+                for (int c = 0; c < 4; ++c) sm100::tmem_ld_32x32b_x32(ts + 32u * c, *reinterpret_cast<uint32_t(*)[32]>(&r[32 * c]));
+                sm100::tmem_ld_wait();
+                float mx = -INFINITY;
+#pragma unroll
+                for (int c = 0; c < 4; ++c) mx = max32(r + 32 * c, mx);
+                const float m = s.raise<D>(mx, a.scale_log2, to, turn > 0);
+#pragma unroll
+                for (int c = 0; c < 4; ++c) {
+                    uint32_t pw[16];
+                    weights32<T>(r + 32 * c, a.scale_log2, m, acc, pw);
+                    sm100::tmem_st_32x32b_x16(ts + 32u * c, pw);
+                    if (c & 1) {
+                        sm100::tmem_st_wait();
+                        sm100::tc_fence_before();
+                        sm100::mbar_arrive(&bars->p_full[t][c >> 1]);
+                    }
+                }
+            } else {
+                // Column c of the tile is seen when c < end and (c >= begin or c < sink).
+                const int start = w.start(j);
+                const bool in_sinks = j < w.sink_tiles;
+                const int end = in_sinks ? (p >= 0 ? w.sink_end - start : 0) : p + 1 - start;
+                const int begin = in_sinks || !a.window ? 0 : p - a.window + 1 - start;
+                const int sink = a.sinks - start;
+                const int chunks = (((w.count(t, j) + 15) & ~15) + 31) >> 5;
+                float mx = -INFINITY;
+#pragma unroll 1
+                for (int c = 0; c < chunks; ++c) {
+                    uint32_t r[32];
+                    sm100::tmem_ld_32x32b_x32(ts + 32u * c, r);
+                    sm100::tmem_ld_wait();
+                    const uint32_t seen = below(end - 32 * c) & (~below(begin - 32 * c) | below(sink - 32 * c));
+#pragma unroll
+                    for (int i = 0; i < 32; ++i)
+                        if (!(seen >> i & 1u)) r[i] = 0xff800000u;
+                    mx = max32(r, mx);
+                }
+                const float m = s.raise<D>(mx, a.scale_log2, to, turn > 0);
+#pragma unroll 1
+                for (int c = 0; c < chunks; ++c) {
+                    uint32_t r[32], pw[16];
+                    sm100::tmem_ld_32x32b_x32(ts + 32u * c, r);
+                    sm100::tmem_ld_wait();
+                    const uint32_t seen = below(end - 32 * c) & (~below(begin - 32 * c) | below(sink - 32 * c));
+#pragma unroll
+                    for (int i = 0; i < 32; ++i)
+                        if (!(seen >> i & 1u)) r[i] = 0xff800000u;
+                    weights32<T>(r, a.scale_log2, m, acc, pw);
+                    sm100::tmem_st_32x32b_x16(ts + 32u * c, pw);
+                }
+                sm100::tmem_st_wait();
+                sm100::tc_fence_before();
+                sm100::mbar_arrive(&bars->p_full[t][0]);
+                sm100::mbar_arrive(&bars->p_full[t][1]);
+            }
+            s.l += acc[0].x + acc[0].y + acc[1].x + acc[1].y;
+            ++turn;
+        }
+        // ---- O / l ----
+        T* out = (T*)a.o + (tok0 + t * tq_tile + tok) * a.ot + (int64_t)head * a.oh;
+        bool again = false;
+        if (w.n > 0) ok = sm100::mbar_wait(&bars->o_done[t], 0, status, 128) && ok;
+        sm100::tc_fence_after();
+        const bool none = turn == 0 || p < 0;
+        const float inv = 1.0f / s.l;
+#pragma unroll 1
+        for (int c = 0; c < D / 32; ++c) {
+            uint32_t r[32];
+            sm100::tmem_ld_32x32b_x32(to + 32u * c, r);
+            sm100::tmem_ld_wait();
+            if (live && ok) {
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    uint32_t o4[4];
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        float2 x = make_float2(__uint_as_float(r[8 * i + 2 * e]) * inv, __uint_as_float(r[8 * i + 2 * e + 1]) * inv);
+                        if (none) x = make_float2(0.f, 0.f);
+                        again |= x.x != x.x || x.y != x.y;
+                        o4[e] = sf::Pair<T>::from_f2(x);
+                    }
+                    *reinterpret_cast<uint4*>(out + 32 * c + 8 * i) = make_uint4(o4[0], o4[1], o4[2], o4[3]);
+                }
+            }
+        }
+        for (uint32_t todo = __ballot_sync(0xffffffffu, again); todo; todo &= todo - 1) {
+            const int src = __ffs(todo) - 1;
+            const int rw = (warp & 3) * 32 + src;
+            const int tk = rw / a.group, hd = kvh * a.group + rw - tk * a.group;
+            const int64_t qrow = tok0 + t * tq_tile + tk;
+            row_by_warp<T>(a, D, qrow, hd, kb, first + tk, (T*)a.o + qrow * a.ot + (int64_t)hd * a.oh);
+        }
+    }
+    sm100::tc_fence_before();
+    __syncthreads();
+    sm100::tc_fence_after();
+    if (warp == 1) sm100::tmem_dealloc(tmem, 512);
+}
+
+// Whether the tensor-core kernel takes these tensors; `rows` token and head strides of an [n, h, D] tensor.
+bool tc_rows(const void* p, int64_t token, int64_t head, int64_t n, int64_t h) {
+    return sf::aligned16(p) && (n <= 1 || (token > 0 && token % 8 == 0)) && (h <= 1 || (head > 0 && head % 8 == 0));
+}
+
+template <typename T, int D>
+int launch_tc(const Args& a, int64_t hk, bool* taken, cudaStream_t st, char* err, uint64_t cap) {
+    const bool bf16 = std::is_same<T, __nv_bfloat16>::value;
+    const int tq_tile = 128 / a.group;
+    auto map = [&](CUtensorMap* m, const void* p, int64_t token, int64_t head, int64_t n, int64_t h, int bh, int bn) {
+        return sf::tmap_3d_encode(m, p, D, h, n, h > 1 ? head * 2 : D * 2, n > 1 ? token * 2 : D * 2, 64, bh, bn, bf16);
+    };
+    CUtensorMap mq, mk, mk16, mv, mv16;
+    *taken = map(&mq, a.q, a.qt, a.qh, a.tq, a.heads, a.group, tq_tile) && map(&mk, a.k, a.kt, a.kh, a.tk, hk, 1, 128) &&
+             map(&mk16, a.k, a.kt, a.kh, a.tk, hk, 1, 16) && map(&mv, a.v, a.vt, a.vh, a.tk, hk, 1, 128) && map(&mv16, a.v, a.vt, a.vh, a.tk, hk, 1, 16);
+    if (!*taken) return SF_OK;
+    constexpr int smem = Layout<D>::BYTES + 1024 > 120 * 1024 ? Layout<D>::BYTES + 1024 : 120 * 1024;  // one CTA (all of TMEM) an SM
+    {
+        static std::mutex mu;
+        static uint64_t done = 0;
+        int dev = 0;
+        cudaGetDevice(&dev);
+        std::lock_guard<std::mutex> lock(mu);
+        if (dev >= 64 || !(done >> dev & 1)) {
+            const cudaError_t e = cudaFuncSetAttribute(window_tc_kernel<T, D>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+            if (e != cudaSuccess) return sf::fail(SF_EDEVICE, err, cap, "window_attention: %s", cudaGetErrorString(e));
+            if (dev < 64) done |= 1ull << dev;
+        }
+    }
+    const int64_t slots = a.tq / (2 * tq_tile) + a.seqs;
+    if (slots > 0x7fffffffLL) return sf::fail(SF_EINVAL, err, cap, "window_attention: grid too large");
+    window_tc_kernel<T, D><<<dim3((unsigned)slots, (unsigned)hk), TC_THREADS, smem, st>>>(a, mq, mk, mk16, mv, mv16, tq_tile);
+    return sf::check_launch("window_attention launch", err, cap);
+}
+
 template <typename T>
 int launch_general(const Args& a, int64_t D, cudaStream_t st, char* err, uint64_t cap) {
     if (D > 256) return sf::fail(SF_EINVAL, err, cap, "window_attention: D=%lld exceeds 256", (long long)D);
@@ -113,38 +592,58 @@ int launch_general(const Args& a, int64_t D, cudaStream_t st, char* err, uint64_
 
 }  // namespace
 
-int sf_window_attention_launch(const void* q, const void* k, const void* v, const void* cu_q, const void* cu_k, void* o, int64_t Tq, int64_t Tk,
-                               int64_t seqs, int64_t Hq, int64_t Hk, int64_t D, const int64_t* strides, float scale, int64_t window, int64_t sinks,
-                               int32_t dtype, int32_t variant, cudaStream_t st, char* err, uint64_t cap) {
+extern "C" int sf_window_attention(const sf_window_attention_args* x, void* stream, char* err, uint64_t cap) {
+    if (!x) return sf::fail(SF_EINVAL, err, cap, "window_attention: null arguments");
+    const int64_t Tq = x->Tq, Tk = x->Tk, seqs = x->seqs, Hq = x->Hq, Hk = x->Hk, D = x->D;
+    const float scale = (float)x->scale;
     if (Tq < 0 || Tk < 0 || seqs < 0 || Hq < 0 || Hk < 0 || D < 1) return sf::fail(SF_EINVAL, err, cap, "window_attention: bad sizes");
     if (Hq && (Hk == 0 || Hq % Hk)) return sf::fail(SF_EINVAL, err, cap, "window_attention: the query heads must be a multiple of the key heads");
-    if (Tq > 0x7fffffffLL || Tk > 0x7fffffffLL || seqs > 0x7fffffffLL || Hq > (1 << 20)) return sf::fail(SF_EINVAL, err, cap, "window_attention: size above 2^31 - 1");
+    if (Tq > 0x7fffffffLL || Tk > 0x7fffffffLL || seqs > 0x7fffffffLL || Hq > (1 << 20))
+        return sf::fail(SF_EINVAL, err, cap, "window_attention: size above 2^31 - 1");
     if (!(scale > 0.f) || !(scale < INFINITY)) return sf::fail(SF_EINVAL, err, cap, "window_attention: scale must be > 0");
-    if (window < 0 || sinks < 0) return sf::fail(SF_EINVAL, err, cap, "window_attention: window and sinks must be >= 0");
-    if (dtype != SF_DTYPE_F16 && dtype != SF_DTYPE_BF16) return sf::fail(SF_EINVAL, err, cap, "window_attention: dtype %d is not fp16/bf16", dtype);
+    if (x->window < 0 || x->sinks < 0) return sf::fail(SF_EINVAL, err, cap, "window_attention: window and sinks must be >= 0");
+    if (x->dtype != SF_DTYPE_F16 && x->dtype != SF_DTYPE_BF16) return sf::fail(SF_EINVAL, err, cap, "window_attention: dtype %d is not fp16/bf16", x->dtype);
+    for (const sf_rows* r : {&x->q_rows, &x->k_rows, &x->v_rows, &x->o_rows})
+        if (r->token < 0 || r->head < 0) return sf::fail(SF_EINVAL, err, cap, "window_attention: negative stride");
     if (Tq * Hq == 0 || seqs == 0) return SF_OK;
-    if (!q || !o || !cu_q || !cu_k || (Tk && (!k || !v))) return sf::fail(SF_EINVAL, err, cap, "window_attention: null tensor pointer");
-    const int64_t dense[8] = {Hq * D, D, Hk * D, D, Hk * D, D, Hq * D, D};
-    const int64_t* s = strides ? strides : dense;
-    for (int i = 0; i < 8; ++i)
-        if (s[i] < 0) return sf::fail(SF_EINVAL, err, cap, "window_attention: negative stride");
+    if (!x->q || !x->o || !x->cu_q || !x->cu_k || (Tk && (!x->k || !x->v))) return sf::fail(SF_EINVAL, err, cap, "window_attention: null tensor pointer");
     Args a = {};
-    a.q = q, a.k = k, a.v = v, a.o = o;
-    a.cu_q = (const int32_t*)cu_q, a.cu_k = (const int32_t*)cu_k;
-    a.qt = s[0], a.qh = s[1], a.kt = s[2], a.kh = s[3], a.vt = s[4], a.vh = s[5], a.ot = s[6], a.oh = s[7];
+    a.q = x->q, a.k = x->k, a.v = x->v, a.o = x->o;
+    a.cu_q = (const int32_t*)x->cu_q, a.cu_k = (const int32_t*)x->cu_k;
+    a.qt = x->q_rows.token, a.qh = x->q_rows.head, a.kt = x->k_rows.token, a.kh = x->k_rows.head;
+    a.vt = x->v_rows.token, a.vh = x->v_rows.head, a.ot = x->o_rows.token, a.oh = x->o_rows.head;
     a.tq = Tq, a.tk = Tk;
     a.seqs = (int)seqs, a.group = (int)(Hq / Hk), a.heads = (int)Hq;
-    a.window = (int)std::min<int64_t>(window, 0x7fffffff);
-    a.sinks = window ? (int)std::min<int64_t>(sinks, 0x7fffffff) : 0;
+    a.window = (int)std::min<int64_t>(x->window, 0x7fffffff);
+    a.sinks = x->window ? (int)std::min<int64_t>(x->sinks, 0x7fffffff) : 0;
     a.scale_log2 = scale * LOG2E;
-    if (variant == 1) return sf::fail(SF_EINVAL, err, cap, "window_attention: no tensor-core kernel yet");
-    if (dtype == SF_DTYPE_F16) return launch_general<__half>(a, D, st, err, cap);
+    cudaStream_t st = (cudaStream_t)stream;
+    const bool half = x->dtype == SF_DTYPE_F16;
+    const bool tc = (D == 64 || D == 128) && a.group <= 128 && Hk <= 65535 && Tk > 0 && tc_rows(a.q, a.qt, a.qh, Tq, Hq) && tc_rows(a.k, a.kt, a.kh, Tk, Hk) &&
+                    tc_rows(a.v, a.vt, a.vh, Tk, Hk) && tc_rows(a.o, a.ot, a.oh, Tq, Hq);
+    if (x->variant == 1 && !tc)
+        return sf::fail(SF_EINVAL, err, cap, "window_attention: the tensor-core variant needs D 64 or 128, at most 128 query heads a key head, 16-byte aligned tensors and strides");
+    if (tc && x->variant != 2) {
+        bool taken = false;
+        const int rc = D == 64 ? (half ? launch_tc<__half, 64>(a, Hk, &taken, st, err, cap) : launch_tc<__nv_bfloat16, 64>(a, Hk, &taken, st, err, cap))
+                               : (half ? launch_tc<__half, 128>(a, Hk, &taken, st, err, cap) : launch_tc<__nv_bfloat16, 128>(a, Hk, &taken, st, err, cap));
+        if (rc || taken) return rc;
+        if (x->variant == 1) return sf::fail(SF_EDEVICE, err, cap, "window_attention: the driver refused a tensor map");
+    }
+    if (half) return launch_general<__half>(a, D, st, err, cap);
     return launch_general<__nv_bfloat16>(a, D, st, err, cap);
 }
 
-extern "C" int sf_window_attention(const void* q, const void* k, const void* v, const void* cu_q, const void* cu_k, void* o, int64_t Tq, int64_t Tk,
-                                   int64_t seqs, int64_t Hq, int64_t Hk, int64_t D, const int64_t* strides, float scale, int64_t window,
-                                   int64_t sinks, int32_t dtype, int32_t variant, void* stream, char* err, uint64_t cap) {
-    return sf_window_attention_launch(q, k, v, cu_q, cu_k, o, Tq, Tk, seqs, Hq, Hk, D, strides, scale, window, sinks, dtype, variant, (cudaStream_t)stream,
-                                      err, cap);
+int sf_window_status_read(uint32_t* code, uint32_t* where, cudaStream_t stream) {
+    sm100::KernelStatus h{0, 0};
+    if (cudaMemcpyFromSymbolAsync(&h, g_window_status, sizeof(h), 0, cudaMemcpyDeviceToHost, stream) != cudaSuccess) return SF_EDEVICE;
+    if (cudaStreamSynchronize(stream) != cudaSuccess) return SF_EDEVICE;
+    if (h.code) {
+        const sm100::KernelStatus zero{0, 0};
+        cudaMemcpyToSymbolAsync(g_window_status, &zero, sizeof(zero), 0, cudaMemcpyHostToDevice, stream);
+        cudaStreamSynchronize(stream);
+    }
+    *code = h.code;
+    *where = h.where;
+    return SF_OK;
 }

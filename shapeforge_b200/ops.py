@@ -9,7 +9,6 @@ missing native library raises.
 from __future__ import annotations
 
 import functools
-import struct
 
 import torch
 
@@ -476,80 +475,102 @@ def mamba2_chunk_scan(x, dt, dA_cumsum, b_mat, c_mat, d_skip, states, out: torch
 
 
 # ---- serving operators: [tokens, heads, D] tensors with any token and head strides -----------------
+#
+# A decoding step makes these calls once a layer on a few tokens, so their host time counts: each tensor
+# is looked at once, and the arguments go down in one packed struct.
 
 
-def _check_rows(t: torch.Tensor, name: str, dtype: torch.dtype | None = None, written: bool = False) -> tuple[int, int]:
-    """Check a [tokens, heads, D] CUDA tensor with unit stride along D; return its token and head
-    strides in elements (0 along an axis of one entry, whose stride says nothing)."""
+def _gpu(t: torch.Tensor, name: str, dev: int | None = None) -> int:
+    """The index of the GPU ``t`` is on; refused on the CPU or when it is not GPU ``dev``."""
     if not isinstance(t, torch.Tensor):
         raise TypeError(f"{name} must be a torch.Tensor")
-    if not t.is_cuda:
+    index = t.get_device()
+    if index < 0:
         raise ValueError(f"{name} must be a CUDA tensor (there is no CPU path)")
+    if dev is not None and index != dev:
+        raise ValueError(f"tensors on more than one device (cuda:{dev}, {name} on cuda:{index})")
+    return index
+
+
+def _check_rows(t: torch.Tensor, name: str, dev: int | None = None, dtype: torch.dtype | None = None, shape=None,
+                written: bool = False) -> tuple[int, int]:
+    """Check a [tokens, heads, D] CUDA tensor with unit stride along D; return its token and head
+    strides in elements (0 along an axis of one entry, whose stride says nothing)."""
+    _gpu(t, name, dev)
     if dtype is not None and t.dtype != dtype:
         raise TypeError(f"{name} has dtype {t.dtype}, expected {dtype}")
-    if t.dim() != 3:
-        raise ValueError(f"{name} must have three axes (tokens, heads, D), got shape {tuple(t.shape)}")
-    n, h, d = t.shape
+    size = t.shape
+    if len(size) != 3:
+        raise ValueError(f"{name} must have three axes (tokens, heads, D), got shape {tuple(size)}")
+    if shape is not None and size != shape:
+        raise ValueError(f"{name} has shape {tuple(size)}, expected {tuple(shape)}")
+    n, h, d = size
     a, b, c = t.stride()
     if d > 1 and c != 1:
         raise ValueError(f"{name} must have unit stride along its last axis")
-    a, b = (a if n > 1 else 0), (b if h > 1 else 0)
-    if written and t.numel():
-        # Rows that share memory would be written by two threads: each axis must step over what the
-        # smaller one spans.
-        (near, many), (far, more) = sorted([(a, n), (b, h)])
-        if (many > 1 and near < d) or (more > 1 and far < (near * (many - 1) + d if many > 1 else d)):
+    if n <= 1:
+        a = 0
+    if h <= 1:
+        b = 0
+    if written and n * h:
+        # Rows that share memory would be written by two threads: the axis with the larger stride has
+        # to step over all that the other spans.
+        near, far = ((a, n), (b, h)) if (a <= b and n > 1) or h <= 1 else ((b, h), (a, n))
+        span = near[0] * (near[1] - 1) + d
+        if (near[1] > 1 and near[0] < d) or (far[1] > 1 and far[0] < span):
             raise ValueError(f"{name} has rows that overlap (strides {t.stride()})")
     return a, b
 
 
-def _check_index(t: torch.Tensor, name: str, length: int | None = None) -> None:
-    _check(t, name, torch.int32)
-    if t.dim() != 1 or (length is not None and t.shape[0] != length):
-        raise ValueError(f"{name} must be one axis of {'int32' if length is None else length} entries, got shape {tuple(t.shape)}")
+def _check_vector(t: torch.Tensor, name: str, dev: int, dtype: torch.dtype, length: int | None = None) -> None:
+    """Check a contiguous one-axis tensor of ``length`` entries."""
+    _gpu(t, name, dev)
+    if t.dtype != dtype:
+        raise TypeError(f"{name} has dtype {t.dtype}, expected {dtype}")
+    if t.dim() != 1 or (length is not None and t.shape[0] != length) or not t.is_contiguous():
+        raise ValueError(f"{name} must be contiguous with one axis{'' if length is None else f' of {length}'}, got shape {tuple(t.shape)}")
 
 
-def _on_tensors_device(name: str, tensors, *args) -> None:
-    """``_native.call`` with the tensors' GPU current (entered only when it is not), on the current
-    stream of that GPU; tensors on two GPUs are refused."""
-    dev = tensors[0].device
-    for t in tensors[1:]:
-        if t.device != dev:
-            raise ValueError(f"{name[3:]}: tensors on more than one device ({dev}, {t.device})")
-    if torch.cuda.current_device() == dev.index:
-        _native.call(name, *args, torch.cuda.current_stream().cuda_stream)
+def _launch(name: str, dev: int, *fields) -> None:
+    """Call a serving entry point on GPU ``dev``'s current stream, with that GPU current (the C ABI
+    launches on the thread's current device); entering it costs more than the launch, so only if need be."""
+    if torch.cuda.current_device() == dev:
+        _native.call_args(name, torch.cuda.current_stream().cuda_stream, *fields)
     else:
         with torch.cuda.device(dev):
-            _native.call(name, *args, torch.cuda.current_stream().cuda_stream)
+            _native.call_args(name, torch.cuda.current_stream().cuda_stream, *fields)
 
 
 def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, q_weight: torch.Tensor, k_weight: torch.Tensor, positions: torch.Tensor,
                  base: float = 10000.0, eps: float = 1e-6, rotary_dim: int | None = None, q_out: torch.Tensor | None = None,
-                 k_out: torch.Tensor | None = None) -> tuple[torch.Tensor, torch.Tensor]:
+                 k_out: torch.Tensor | None = None, variant: int = 0) -> tuple[torch.Tensor, torch.Tensor]:
     """Per-head RMS norm of queries ``q [T, Hq, D]`` and keys ``k [T, Hk, D]`` (weights ``[D]``) and the
     rotate-half rotary embedding of their first ``rotary_dim`` (default D) elements at ``positions [T]``
     (int32), in one pass; :func:`rmsnorm` then :func:`rope`, at any positions.  ``q`` and ``k`` may be
     views of a packed projection (unit stride along D); ``q_out`` / ``k_out`` may be ``q`` / ``k``
-    themselves (in place), otherwise they must not overlap the inputs.  Returns ``(q_out, k_out)``."""
-    qs, ks = _check_rows(q, "q"), _check_rows(k, "k", q.dtype)
+    themselves (in place), otherwise they must not overlap the inputs.  ``variant``: 0 = by shape, 1 =
+    vectorised (refused where it does not apply), 2 = general.  Returns ``(q_out, k_out)``."""
+    dev = _gpu(q, "q")
+    dtype = q.dtype
+    qs, ks = _check_rows(q, "q", dev), _check_rows(k, "k", dev, dtype)
     t, hq, d = q.shape
     hk = k.shape[1]
     if k.shape[0] != t or k.shape[2] != d:
         raise ValueError(f"k has shape {tuple(k.shape)}, expected [{t}, heads, {d}]")
-    for name, w in (("q_weight", q_weight), ("k_weight", k_weight)):
-        _check(w, name, q.dtype)
-        if w.numel() != d:
-            raise ValueError(f"{name} has {w.numel()} elements, expected D={d}")
-    _check_index(positions, "positions", t)
-    rotary = d if rotary_dim is None else int(rotary_dim)
-    q_out = torch.empty((t, hq, d), dtype=q.dtype, device=q.device) if q_out is None else q_out
-    k_out = torch.empty((t, hk, d), dtype=q.dtype, device=q.device) if k_out is None else k_out
-    qos, kos = _check_rows(q_out, "q_out", q.dtype, written=True), _check_rows(k_out, "k_out", q.dtype, written=True)
-    if q_out.shape != q.shape or k_out.shape != k.shape:
-        raise ValueError("q_out and k_out must have the shapes of q and k")
-    _on_tensors_device("sf_qk_norm_rope", (q, k, q_weight, k_weight, positions, q_out, k_out), q.data_ptr(), k.data_ptr(),
-                       q_weight.data_ptr(), k_weight.data_ptr(), positions.data_ptr(), q_out.data_ptr(), k_out.data_ptr(), t, hq, hk, d,
-                       struct.pack("8q", *qs, *ks, *qos, *kos), rotary, float(base), float(eps), _native.DTYPE_CODES[dtype_name(q)])
+    _check_vector(q_weight, "q_weight", dev, dtype, d)
+    _check_vector(k_weight, "k_weight", dev, dtype, d)
+    _check_vector(positions, "positions", dev, torch.int32, t)
+    if q_out is None:
+        q_out, qos = q.new_empty((t, hq, d)), (hq * d, d)
+    else:
+        qos = _check_rows(q_out, "q_out", dev, dtype, q.shape, written=True)
+    if k_out is None:
+        k_out, kos = k.new_empty((t, hk, d)), (hk * d, d)
+    else:
+        kos = _check_rows(k_out, "k_out", dev, dtype, k.shape, written=True)
+    _launch("sf_qk_norm_rope", dev, q.data_ptr(), k.data_ptr(), q_weight.data_ptr(), k_weight.data_ptr(), positions.data_ptr(),
+            q_out.data_ptr(), k_out.data_ptr(), t, hq, hk, d, d if rotary_dim is None else rotary_dim, *qs, *ks, *qos, *kos, base, eps,
+            _native.DTYPE_CODES[dtype_name(q)], variant)
     return q_out, k_out
 
 
@@ -563,11 +584,13 @@ def kv4_cache(num_pages: int, page_size: int, heads: int, dim: int, device: torc
     return torch.zeros((num_pages, heads, page_size // 16, 18 * dim), dtype=torch.uint8, device=device)
 
 
-def _check_cache(cache: torch.Tensor) -> tuple[int, int, int, int]:
+def _check_cache(cache: torch.Tensor, dev: int | None = None) -> tuple[int, int, int, int]:
     """(pages, heads, page size, D) of a 4-bit cache."""
-    _check(cache, "cache", torch.uint8)
-    if cache.dim() != 4 or cache.shape[3] not in (18 * 64, 18 * 128) or cache.shape[2] < 1:
-        raise ValueError(f"cache must be [pages, heads, page_size / 16, 18 * D], D 64 or 128, got {tuple(cache.shape)}")
+    _gpu(cache, "cache", dev)
+    if cache.dtype != torch.uint8:
+        raise TypeError(f"cache has dtype {cache.dtype}, expected torch.uint8")
+    if cache.dim() != 4 or cache.shape[3] not in (18 * 64, 18 * 128) or cache.shape[2] < 1 or not cache.is_contiguous():
+        raise ValueError(f"cache must be a contiguous [pages, heads, page_size / 16, 18 * D], D 64 or 128, got {tuple(cache.shape)}")
     pages, heads, tiles, record = cache.shape
     return pages, heads, 16 * tiles, record // 18
 
@@ -578,14 +601,13 @@ def kv4_store(k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor, cache: torc
     head get a bf16 minimum and scale = (max - min) / 15 and codes rint((x - minimum) / scale) in 0..15; a
     group that is not finite reads back as NaN.  A negative slot is padding and skipped, one past the
     cache is skipped and reported by :func:`kernel_status` (code 3).  The slots must differ."""
-    pages, heads, page, d = _check_cache(cache)
-    ks, vs = _check_rows(k, "k"), _check_rows(v, "v", k.dtype)
-    t = k.shape[0]
-    if k.shape != (t, heads, d) or v.shape != k.shape:
-        raise ValueError(f"k and v must be [T, {heads}, {d}] for this cache, got {tuple(k.shape)} and {tuple(v.shape)}")
-    _check_index(slots, "slots", t)
-    _on_tensors_device("sf_kv4_store", (k, v, slots, cache), k.data_ptr(), v.data_ptr(), slots.data_ptr(), cache.data_ptr(), t, heads, d,
-                       pages, page, struct.pack("4q", *ks, *vs), _native.DTYPE_CODES[dtype_name(k)])
+    dev = _gpu(k, "k")
+    pages, heads, page, d = _check_cache(cache, dev)
+    t = k.shape[0] if k.dim() else 0
+    ks, vs = _check_rows(k, "k", dev, None, (t, heads, d)), _check_rows(v, "v", dev, k.dtype, (t, heads, d))
+    _check_vector(slots, "slots", dev, torch.int32, t)
+    _launch("sf_kv4_store", dev, k.data_ptr(), v.data_ptr(), slots.data_ptr(), cache.data_ptr(), t, heads, d, pages, page, *ks, *vs,
+            _native.DTYPE_CODES[dtype_name(k)], 0)
     return cache
 
 
@@ -594,18 +616,24 @@ def kv4_load(cache: torch.Tensor, slots: torch.Tensor, dtype: torch.dtype = torc
     """Read the tokens at ``slots [T]`` (int32, in any order, repeated or not) of a 4-bit cache back as
     ``(k, v)``, each ``[T, H, D]`` in ``dtype`` (minimum + scale * code, rounded once), e.g. as the
     context of a prompt's next chunk for :func:`window_attention`.  Negative slots (and, reported by
-    :func:`kernel_status`, slots past the cache) read as zeros."""
+    :func:`kernel_status`, slots past the cache) read as zeros.  ``k_out`` / ``v_out`` set the type when
+    given."""
+    dev = _gpu(cache, "cache")
     pages, heads, page, d = _check_cache(cache)
-    _check_index(slots, "slots")
-    t = slots.shape[0]
-    dtype = dtype if k_out is None else k_out.dtype
-    k_out = torch.empty((t, heads, d), dtype=dtype, device=cache.device) if k_out is None else k_out
-    v_out = torch.empty((t, heads, d), dtype=dtype, device=cache.device) if v_out is None else v_out
-    ks, vs = _check_rows(k_out, "k_out", dtype, written=True), _check_rows(v_out, "v_out", dtype, written=True)
-    if k_out.shape != (t, heads, d) or v_out.shape != (t, heads, d):
-        raise ValueError(f"k_out and v_out must be [{t}, {heads}, {d}]")
-    _on_tensors_device("sf_kv4_load", (cache, slots, k_out, v_out), cache.data_ptr(), slots.data_ptr(), k_out.data_ptr(), v_out.data_ptr(),
-                       t, heads, d, pages, page, struct.pack("4q", *ks, *vs), _native.DTYPE_CODES[dtype_name(k_out)])
+    _check_vector(slots, "slots", dev, torch.int32)
+    shape = (slots.shape[0], heads, d)
+    given = k_out if k_out is not None else v_out
+    dtype = dtype if given is None else given.dtype
+    if k_out is None:
+        k_out, ks = cache.new_empty(shape, dtype=dtype), (heads * d, d)
+    else:
+        ks = _check_rows(k_out, "k_out", dev, dtype, shape, written=True)
+    if v_out is None:
+        v_out, vs = cache.new_empty(shape, dtype=dtype), (heads * d, d)
+    else:
+        vs = _check_rows(v_out, "v_out", dev, dtype, shape, written=True)
+    _launch("sf_kv4_load", dev, k_out.data_ptr(), v_out.data_ptr(), slots.data_ptr(), cache.data_ptr(), *shape, pages, page, *ks, *vs,
+            _native.DTYPE_CODES[dtype_name(k_out)], 0)
     return k_out, v_out
 
 
@@ -627,33 +655,36 @@ def kv4_attention(q: torch.Tensor, cache: torch.Tensor, block_table: torch.Tenso
     ``workspace`` (uint8, :func:`kv4_attention_workspace_bytes`) is allocated here when not given;
     calls that overlap on the GPU need one each.  ``variant``: 0 = by size, 1 = all requests' keys
     dealt evenly to all CTAs, 3 = a CTA a (request, head)."""
-    pages, heads, page, d = _check_cache(cache)
-    qs = _check_rows(q, "q")
-    b, hq = q.shape[:2]
-    if q.shape[2] != d or hq % heads:
+    dev = _gpu(q, "q")
+    dtype = q.dtype
+    pages, heads, page, d = _check_cache(cache, dev)
+    qs = _check_rows(q, "q", dev)
+    b, hq, qd = q.shape
+    if qd != d or heads == 0 or hq % heads:
         raise ValueError(f"q must be [B, a multiple of {heads}, {d}] for this cache, got {tuple(q.shape)}")
-    if not isinstance(block_table, torch.Tensor) or not block_table.is_cuda or block_table.dtype != torch.int32:
-        raise TypeError("block_table must be an int32 CUDA tensor")
+    _gpu(block_table, "block_table", dev)
+    if block_table.dtype != torch.int32:
+        raise TypeError(f"block_table has dtype {block_table.dtype}, expected torch.int32")
     if block_table.dim() != 2 or block_table.shape[0] != b or (block_table.shape[1] > 1 and block_table.stride(1) != 1):
         raise ValueError(f"block_table must be [{b}, width] with unit stride along a row")
     width = block_table.shape[1]
-    _check_index(seq_lens, "seq_lens", b)
-    out = torch.empty((b, hq, d), dtype=q.dtype, device=q.device) if out is None else out
-    os_ = _check_rows(out, "out", q.dtype, written=True)
-    if out.shape != q.shape:
-        raise ValueError(f"out must be {tuple(q.shape)}")
+    _check_vector(seq_lens, "seq_lens", dev, torch.int32, b)
+    if out is None:
+        out, os_ = q.new_empty((b, hq, d)), (hq * d, d)
+    else:
+        os_ = _check_rows(out, "out", dev, dtype, q.shape, written=True)
     if workspace is None:
         need = kv4_attention_workspace_bytes(b, hq, heads, d, page, width, window, sinks, variant)
         if need:
-            workspace = torch.empty(need, dtype=torch.uint8, device=q.device)
+            workspace = cache.new_empty(need)
     else:
-        _check(workspace, "workspace")
-    ws_ptr, ws_bytes = (0, 0) if workspace is None else (workspace.data_ptr(), workspace.numel() * workspace.element_size())
-    tensors = (q, cache, block_table, seq_lens, out) if workspace is None else (q, cache, block_table, seq_lens, out, workspace)
-    strides = struct.pack("5q", *qs, *os_, block_table.stride(0) if b > 1 else 0)
-    _on_tensors_device("sf_kv4_attention", tensors, q.data_ptr(), cache.data_ptr(), block_table.data_ptr(), seq_lens.data_ptr(),
-                       out.data_ptr(), ws_ptr, ws_bytes, b, hq, heads, d, pages, page, width, strides, float(scale), int(window), int(sinks),
-                       _native.DTYPE_CODES[dtype_name(q)], int(variant))
+        need = workspace.numel() * workspace.element_size()
+        _gpu(workspace, "workspace", dev)
+        if not workspace.is_contiguous():
+            raise ValueError("workspace must be contiguous")
+    _launch("sf_kv4_attention", dev, q.data_ptr(), cache.data_ptr(), block_table.data_ptr(), seq_lens.data_ptr(), out.data_ptr(),
+            0 if workspace is None else workspace.data_ptr(), need, b, hq, heads, d, pages, page, width,
+            block_table.stride(0) if b > 1 else 0, *qs, *os_, window, sinks, scale, _native.DTYPE_CODES[dtype_name(q)], variant)
     return out
 
 
@@ -669,23 +700,28 @@ def window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqle
     that belong to no sequence are left as they were.  D up to 256; D 64 and 128 with 16-byte aligned
     rows and at most 128 query heads a key head run on the tensor cores.  ``variant``: 0 = by shape, 1 =
     tensor cores (refused where they do not apply), 2 = general kernel."""
-    qs, ks, vs = _check_rows(q, "q"), _check_rows(k, "k", q.dtype), _check_rows(v, "v", q.dtype)
+    dev = _gpu(q, "q")
+    dtype = q.dtype
+    qs, ks = _check_rows(q, "q", dev), _check_rows(k, "k", dev, dtype)
+    vs = _check_rows(v, "v", dev, dtype, k.shape)
     tq, hq, d = q.shape
-    tk, hk, _ = k.shape
-    if k.shape[2] != d or v.shape != k.shape or hk == 0 or hq % hk:
-        raise ValueError(f"window_attention expects k and v of one shape [Tk, Hk, {d}] with Hk dividing {hq}, got {tuple(k.shape)} and {tuple(v.shape)}")
-    _check_index(cu_seqlens, "cu_seqlens")
-    cu_k = cu_seqlens if cu_seqlens_k is None else cu_seqlens_k
-    _check_index(cu_k, "cu_seqlens_k", cu_seqlens.shape[0])
+    tk, hk, kd = k.shape
+    if kd != d or hk == 0 or hq % hk:
+        raise ValueError(f"window_attention expects k and v [Tk, Hk, {d}] with Hk dividing {hq}, got {tuple(k.shape)}")
+    _check_vector(cu_seqlens, "cu_seqlens", dev, torch.int32)
     seqs = cu_seqlens.shape[0] - 1
     if seqs < 0:
         raise ValueError("cu_seqlens must have at least one entry")
-    out = torch.empty((tq, hq, d), dtype=q.dtype, device=q.device) if out is None else out
-    os_ = _check_rows(out, "out", q.dtype, written=True)
-    if out.shape != q.shape:
-        raise ValueError(f"out must be {tuple(q.shape)}")
-    _on_tensors_device("sf_window_attention", (q, k, v, cu_seqlens, cu_k, out), q.data_ptr(), k.data_ptr(), v.data_ptr(),
-                       cu_seqlens.data_ptr(), cu_k.data_ptr(), out.data_ptr(), tq, tk, seqs, hq, hk, d,
-                       struct.pack("8q", *qs, *ks, *vs, *os_), float(scale), int(window), int(sinks), _native.DTYPE_CODES[dtype_name(q)],
-                       int(variant))
+    if cu_seqlens_k is None:
+        cu_seqlens_k = cu_seqlens
+        if tk != tq:
+            raise ValueError(f"k has {tk} rows and q {tq}: cu_seqlens_k is needed")
+    else:
+        _check_vector(cu_seqlens_k, "cu_seqlens_k", dev, torch.int32, seqs + 1)
+    if out is None:
+        out, os_ = q.new_empty((tq, hq, d)), (hq * d, d)
+    else:
+        os_ = _check_rows(out, "out", dev, dtype, q.shape, written=True)
+    _launch("sf_window_attention", dev, q.data_ptr(), k.data_ptr(), v.data_ptr(), cu_seqlens.data_ptr(), cu_seqlens_k.data_ptr(),
+            out.data_ptr(), tq, tk, seqs, hq, hk, d, *qs, *ks, *vs, *os_, window, sinks, scale, _native.DTYPE_CODES[dtype_name(q)], variant)
     return out

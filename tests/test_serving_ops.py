@@ -4,7 +4,6 @@ definitions against themselves (the cache layout is one to one, the mask's corne
 from __future__ import annotations
 
 import math
-import struct
 
 import pytest
 import torch
@@ -15,85 +14,84 @@ from shapeforge_b200 import _native, ops
 BF16, F16, F32 = 1, 0, 2
 
 
-def refused(name, *args):
+def refused(name, fields):
     with pytest.raises(_native.SfError) as exc:
-        _native.call(name, *args)
+        _native.call_args(name, 0, *fields)
     assert exc.value.code == _native.SF_EINVAL
     return exc.value.message
 
 
-def norm_args(t=4, hq=2, hk=1, d=64, strides=None, rotary=64, base=1e4, eps=1e-6, dtype=BF16, ptr=16):
-    return (ptr,) * 7 + (t, hq, hk, d, strides, rotary, base, eps, dtype, None)
+def norm_args(t=4, hq=2, hk=1, d=64, strides=(128, 64, 64, 64) * 2, rotary=64, base=1e4, eps=1e-6, dtype=BF16, variant=0, ptr=16):
+    return (ptr,) * 7 + (t, hq, hk, d, rotary, *strides, base, eps, dtype, variant)
 
 
 @pytest.mark.parametrize("bad, word", [
     (dict(t=-1), "T"), (dict(d=0), "D"), (dict(rotary=63), "rotary"), (dict(rotary=66), "rotary"), (dict(rotary=-2), "rotary"),
     (dict(base=0.0), "base"), (dict(base=-2.0), "base"), (dict(base=math.nan), "base"), (dict(base=math.inf), "base"),
     (dict(eps=-1.0), "eps"), (dict(eps=math.nan), "eps"), (dict(dtype=F32), "dtype"), (dict(ptr=0), "null"),
-    (dict(strides=struct.pack("8q", 64, -1, 0, 0, 0, 0, 0, 0)), "stride"),
+    (dict(strides=(128, -1, 64, 64) * 2), "stride"), (dict(ptr=2, variant=1), "vectorised"), (dict(rotary=24, variant=1), "vectorised"),
+    (dict(strides=(129, 64, 64, 64) * 2, variant=1), "vectorised"),
 ])
 def test_qk_norm_rope_refusals(bad, word):
-    assert word in refused("sf_qk_norm_rope", *norm_args(**bad))
+    assert word in refused("sf_qk_norm_rope", norm_args(**bad))
 
 
-def cache_args(t=4, h=2, d=64, pages=3, page=32, strides=None, dtype=BF16, ptr=16, slots=16):
-    return (ptr, ptr, slots, ptr, t, h, d, pages, page, strides, dtype, None)
+def cache_args(t=4, h=2, d=64, pages=3, page=32, strides=(128, 64, 128, 64), dtype=BF16, ptr=16, slots=16):
+    return (ptr, ptr, slots, ptr, t, h, d, pages, page, *strides, dtype, 0)
 
 
 @pytest.mark.parametrize("bad, word", [
     (dict(t=-1), "negative"), (dict(d=96), "64 or 128"), (dict(page=24), "multiple of 16"), (dict(page=0), "multiple of 16"),
     (dict(pages=1 << 30), "2^31"), (dict(dtype=F32), "dtype"), (dict(ptr=0), "null"), (dict(slots=0), "null"), (dict(ptr=8), "aligned"),
-    (dict(h=70000), "heads"), (dict(strides=struct.pack("4q", 128, 64, 100, 64)), "multiples of 8"),
-    (dict(strides=struct.pack("4q", 128, -64, 128, 64)), "multiples of 8"),
+    (dict(h=70000), "heads"), (dict(strides=(128, 64, 100, 64)), "multiples of 8"), (dict(strides=(128, -64, 128, 64)), "multiples of 8"),
 ])
 @pytest.mark.parametrize("name", ["sf_kv4_store", "sf_kv4_load"])
 def test_kv4_cache_refusals(name, bad, word):
-    args = list(cache_args(**bad))
-    if name == "sf_kv4_load":
-        args[:4] = [args[3], args[2], args[0], args[1]]
-    assert word in refused(name, *args)
+    assert word in refused(name, cache_args(**bad))
 
 
-def decode_args(b=2, hq=4, hk=2, d=64, pages=3, page=32, width=2, strides=None, scale=0.1, window=0, sinks=0, dtype=BF16, variant=0, ptr=16,
-                ws=0, ws_bytes=0):
-    return (ptr,) * 5 + (ws, ws_bytes, b, hq, hk, d, pages, page, width, strides, scale, window, sinks, dtype, variant, None)
+def decode_args(b=2, hq=4, hk=2, d=64, pages=3, page=32, width=2, table_stride=2, strides=(256, 64, 256, 64), scale=0.1, window=0, sinks=0,
+                dtype=BF16, variant=0, ptr=16, ws=0, ws_bytes=0):
+    return (ptr,) * 5 + (ws, ws_bytes, b, hq, hk, d, pages, page, width, table_stride, *strides, window, sinks, scale, dtype, variant)
 
 
 @pytest.mark.parametrize("bad, word", [
     (dict(b=-1), "negative"), (dict(d=80), "64 or 128"), (dict(page=8), "multiple of 16"), (dict(hq=3), "multiple of the cache"),
     (dict(hk=0), "multiple of the cache"), (dict(scale=0.0), "scale"), (dict(scale=math.nan), "scale"), (dict(scale=math.inf), "scale"),
-    (dict(window=-1), "window"), (dict(sinks=-1), "sinks"), (dict(dtype=F32), "dtype"), (dict(ptr=0), "null"), (dict(ptr=4), "aligned"),
-    (dict(strides=struct.pack("5q", 256, 4, 256, 64, 2)), "multiples of 8"), (dict(strides=struct.pack("5q", 256, 64, 256, 64, -2)), "stride"),
+    (dict(scale=1e-60), "scale"), (dict(window=-1), "window"), (dict(sinks=-1), "sinks"), (dict(dtype=F32), "dtype"), (dict(ptr=0), "null"),
+    (dict(ptr=4), "aligned"), (dict(strides=(256, 4, 256, 64)), "multiples of 8"), (dict(table_stride=-2), "stride"),
     (dict(width=1000), "workspace"), (dict(width=1000, ws=16, ws_bytes=8), "workspace"), (dict(width=1000, ws=8, ws_bytes=1 << 40), "workspace"),
     (dict(pages=1 << 29), "2^31"), (dict(width=1 << 29), "2^31"), (dict(b=1 << 25, width=1 << 10), "too large"),
 ])
 def test_kv4_attention_refusals(bad, word):
-    assert word in refused("sf_kv4_attention", *decode_args(**bad))
+    assert word in refused("sf_kv4_attention", decode_args(**bad))
 
 
-def window_args(tq=4, tk=4, seqs=1, hq=4, hk=2, d=64, strides=None, scale=0.1, window=0, sinks=0, dtype=BF16, variant=0, ptr=16):
-    return (ptr,) * 6 + (tq, tk, seqs, hq, hk, d, strides, scale, window, sinks, dtype, variant, None)
+def window_args(tq=4, tk=4, seqs=1, hq=4, hk=2, d=64, strides=(256, 64, 128, 64, 128, 64, 256, 64), scale=0.1, window=0, sinks=0, dtype=BF16,
+                variant=0, ptr=16):
+    return (ptr,) * 6 + (tq, tk, seqs, hq, hk, d, *strides, window, sinks, scale, dtype, variant)
 
 
 @pytest.mark.parametrize("bad, word", [
     (dict(tq=-1), "sizes"), (dict(d=0), "sizes"), (dict(hq=3), "multiple"), (dict(hk=0), "multiple"), (dict(scale=0.0), "scale"),
     (dict(scale=-1.0), "scale"), (dict(scale=math.inf), "scale"), (dict(window=-1), "window"), (dict(sinks=-4), "sinks"),
     (dict(dtype=F32), "dtype"), (dict(ptr=0), "null"), (dict(tq=1 << 31), "2^31"), (dict(d=320), "256"),
-    (dict(strides=struct.pack("8q", 256, 64, 128, -64, 128, 64, 256, 64)), "stride"), (dict(d=96, variant=1), "tensor-core"),
-    (dict(ptr=8, variant=1), "tensor-core"), (dict(strides=struct.pack("8q", 257, 64, 128, 64, 128, 64, 256, 64), variant=1), "tensor-core"),
+    (dict(strides=(256, 64, 128, -64, 128, 64, 256, 64)), "stride"), (dict(d=96, variant=1), "tensor-core"),
+    (dict(ptr=8, variant=1), "tensor-core"), (dict(strides=(257, 64, 128, 64, 128, 64, 256, 64), variant=1), "tensor-core"),
+    (dict(hq=258, hk=2, variant=1), "tensor-core"),
 ])
 def test_window_attention_refusals(bad, word):
-    assert word in refused("sf_window_attention", *window_args(**bad))
+    assert word in refused("sf_window_attention", window_args(**bad))
 
 
 def test_calls_without_work_are_accepted_without_a_device():
     """Empty inputs return before any CUDA call, null pointers included."""
-    _native.call("sf_qk_norm_rope", *norm_args(t=0, ptr=0))
-    _native.call("sf_kv4_store", *cache_args(t=0, ptr=0))
-    _native.call("sf_kv4_load", *cache_args(t=0, ptr=0))
-    _native.call("sf_kv4_attention", *decode_args(b=0, ptr=0))
-    _native.call("sf_window_attention", *window_args(tq=0, ptr=0))
-    _native.call("sf_window_attention", *window_args(seqs=0, ptr=0))
+    _native.call_args("sf_qk_norm_rope", 0, *norm_args(t=0, ptr=0))
+    _native.call_args("sf_kv4_store", 0, *cache_args(t=0, ptr=0))
+    _native.call_args("sf_kv4_load", 0, *cache_args(t=0, ptr=0))
+    _native.call_args("sf_kv4_attention", 0, *decode_args(b=0, ptr=0))
+    _native.call_args("sf_window_attention", 0, *window_args(tq=0, ptr=0))
+    _native.call_args("sf_window_attention", 0, *window_args(seqs=0, ptr=0))
 
 
 def test_workspace_sizes():
@@ -111,13 +109,8 @@ def fake_cuda(t, index=0):
     """A CPU tensor that reports itself on GPU `index`, for the checks that run before a launch."""
 
     class Fake(torch.Tensor):
-        @property
-        def is_cuda(self):
-            return True
-
-        @property
-        def device(self):
-            return torch.device("cuda", index)
+        def get_device(self):
+            return index
 
     return torch.Tensor._make_subclass(Fake, t)
 
@@ -161,6 +154,7 @@ def test_python_refusals():
         (ValueError, lambda: ops.window_attention(q, k, k, cu, 0.1, cu_seqlens_k=fk(3, dtype=torch.int32))),
         (ValueError, lambda: ops.window_attention(q, k, k, fk(0, dtype=torch.int32), 0.1)),
         (TypeError, lambda: ops.window_attention(q, k, k, fk(2, dtype=torch.int64), 0.1)),
+        (ValueError, lambda: ops.window_attention(q, fk(5, 1, 64), fk(5, 1, 64), cu, 0.1)),
         (ValueError, lambda: ops.kv4_cache(4, 24, 2, 64, device="cpu")),
         (ValueError, lambda: ops.kv4_cache(4, 32, 2, 96, device="cpu")),
     ]
