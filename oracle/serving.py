@@ -89,19 +89,21 @@ class Attended:
     mass: torch.Tensor    # sum_j p_j |v_j - centre_j|: what a relative error of the weights p can move
     size: torch.Tensor    # sum_j p_j |v_j|
     peak: torch.Tensor    # max_j |v_j - centre_j| over seen keys
+    heaviest: torch.Tensor  # max_j p_j span_j, per row [.., 1]
     score: torch.Tensor   # max_j scale sum_d |q_d k_jd|, per row [.., 1]: what rounding in a score is relative to
 
 
-def attend(q, k, v, scale, seen, centre=None):
+def attend(q, k, v, scale, seen, centre=None, span=None):
     """q [R, D], k, v [S, D], seen [R, S] -> :class:`Attended` with [R, D] entries; rows that see
     nothing are zeros.  Unseen keys and values take no part, whatever they hold."""
     q, k, v = q.to(F64), k.to(F64), v.to(F64)
     dev = q.device
     centre = torch.zeros_like(v) if centre is None else centre.to(F64)
+    span = torch.zeros(v.shape[0], dtype=F64, device=dev) if span is None else span
     used = seen.any(0)
-    q, k, v, centre, seen = q, k[used], v[used], centre[used], seen[:, used]
+    k, v, centre, span, seen = k[used], v[used], centre[used], span[used], seen[:, used]
     out = [torch.zeros(q.shape[0], v.shape[1], dtype=F64, device=dev) for _ in range(4)]
-    score = torch.zeros(q.shape[0], 1, dtype=F64, device=dev)
+    score, heaviest = (torch.zeros(q.shape[0], 1, dtype=F64, device=dev) for _ in range(2))
     some = seen.any(1)
     if used.any() and some.any():
         w = torch.where(seen[some], q[some] @ k.T * scale, torch.full((), -math.inf, dtype=F64, device=dev))
@@ -121,8 +123,9 @@ def attend(q, k, v, scale, seen, centre=None):
         out[2][some] = p @ vz.abs()
         out[3][some] = off.amax(0, keepdim=True).expand(int(some.sum()), -1)
         bound = torch.where(seen[some], torch.nan_to_num(q[some].abs() @ k.abs().T * scale, nan=0.0, posinf=0.0), torch.zeros_like(w))
+        heaviest[some] = (p * span).amax(-1, keepdim=True)
         score[some] = bound.amax(-1, keepdim=True)
-    return Attended(*out, score)
+    return Attended(*out, heaviest, score)
 
 
 def window_mask(nq, nk, window, sinks, device="cpu"):
@@ -149,4 +152,4 @@ def window_attention(q, k, v, cu_q, cu_k, scale, window, sinks):
             for part, x in zip(parts, (r.value, r.mass, r.size, r.peak)):
                 part[a:b, h] = x
             score[a:b, h] = r.score
-    return inside, Attended(*parts, score)
+    return inside, Attended(*parts, torch.zeros_like(score), score)

@@ -13,9 +13,13 @@
 //  * K: an fp16 whose low bits are a code is the subnormal c 2^-24, exactly, so one AND makes two
 //    operands.  q is scaled by a power of two to [1, 2) a head (exact in fp16 down to 2^-24 of the
 //    head's largest) and by 16 where the code sits in the lower nibble of its byte.
-//  * V: 0x4300 | c is the bf16 128 + c; taking off 136 leaves c - 8 exactly.  Centred codes keep the
-//    fp32 accumulator from growing one-sided.  p s is rounded to bf16 (as flash attention rounds p);
-//    for fp16 tensors it is split into two bf16 parts, 16 bits in all.
+//  * V: with two keys' bytes side by side, 0x6400 | b is the fp16 1024 + b of a whole byte b = c + 16 c'
+//    (two neighbouring elements' codes) and clearing its low bits gives 1024 + 16 c'.  Both, less 1160
+//    and 1152, go through the MMA, and (c - 8) and (c' - 8) of the accumulators come from their
+//    difference and a factor 1/16 at the end: two integer operations a pair of codes.  Codes taken off
+//    their centre keep the fp32 accumulator from growing one-sided.  p s is an fp16 in a unit of each
+//    head's own that its largest p s so far sets, so what matters of it has 11 bits (flash attention's p
+//    has 8 or 11) whatever the values' range.
 //  * S^T = K q^T and O^T = V^T p^T (mma.sync m16n8k16, keys / elements in the 16 rows, 8 query heads
 //    in the columns): a group of up to 8 heads wastes no rows, the cache is the A operand straight
 //    from shared memory, and p becomes the next B operand by a transposing matrix move.  tcgen05
@@ -23,9 +27,11 @@
 //  * Each warp streams its own tiles (every 8th of the CTA's) through a ring of bulk copies, one
 //    record a copy; warps meet only at the end of a (request, head) to merge their softmax states.
 //  * Work is dealt in 16-key tiles: the tiles of all requests and heads in one line, an equal
-//    stretch for every CTA of one resident wave, whatever the lengths.  A (request, head) that
-//    spans CTAs leaves partial states in the workspace, joined by a second kernel in the order of
-//    the stretches (no atomics: the same call gives the same bits).
+//    stretch for every CTA of one resident wave, whatever the lengths; each (request, head) counts
+//    ITEM_COST tiles more for its start and end.  One that spans CTAs leaves partial states in the
+//    workspace, joined by a second kernel in the order of the stretches (no atomics: the same call
+//    gives the same bits).  The first copies of a CTA's next (request, head) are issued before the
+//    states of the one at hand are merged.
 #include "kv4.cuh"
 
 #include <algorithm>
@@ -41,6 +47,7 @@ namespace {
 constexpr int WARPS = 8;
 constexpr int THREADS = 32 * WARPS;
 constexpr int MAX_SMEM = 227 * 1024;
+constexpr int ITEM_COST = 12;  // what starting and merging a (request, head) costs, in tiles
 constexpr float LOG2E = 1.4426950408889634f;
 
 struct Args {
@@ -65,25 +72,30 @@ __device__ __forceinline__ void mma_f16(float (&d)[4], const uint32_t (&a)[4], u
                  : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
                  : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
-__device__ __forceinline__ void mma_bf16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-}
 // Transpose of an 8 x 8 matrix of 16-bit values held as an MMA fragment.
 __device__ __forceinline__ uint32_t transpose8(uint32_t x) {
     uint32_t y;
     asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
     return y;
 }
-__device__ __forceinline__ uint32_t bf16x2(float a, float b) { return sf::Pair<__nv_bfloat16>::from_f2(make_float2(a, b)); }
 __device__ __forceinline__ uint32_t f16x2(float a, float b) { return sf::Pair<__half>::from_f2(make_float2(a, b)); }
-// (128 + c) - 136 for two codes.
-__device__ __forceinline__ uint32_t centred(uint32_t x) {
-    const uint32_t u = (x & 0x000F000Fu) | 0x43004300u, off = 0x43084308u;
-    const __nv_bfloat162 d = __hsub2(*reinterpret_cast<const __nv_bfloat162*>(&u), *reinterpret_cast<const __nv_bfloat162*>(&off));
+// a - b on two fp16.
+__device__ __forceinline__ uint32_t sub2(uint32_t a, uint32_t b) {
+    const __half2 d = __hsub2(*reinterpret_cast<const __half2*>(&a), *reinterpret_cast<const __half2*>(&b));
     return *reinterpret_cast<const uint32_t*>(&d);
 }
+
+// The largest over the warp's keys (lanes of one t).
+__device__ __forceinline__ float2 over_keys(float2 v) {
+#pragma unroll
+    for (int off = 4; off < 32; off <<= 1) {
+        v.x = fmaxf(v.x, __shfl_xor_sync(0xffffffffu, v.x, off));
+        v.y = fmaxf(v.y, __shfl_xor_sync(0xffffffffu, v.y, off));
+    }
+    return v;
+}
+// 1 / u, and 0 for a unit that has vanished (what it counted has too).
+__device__ __forceinline__ float reciprocal(float u) { return u >= 0x1p-126f ? 1.0f / u : 0.f; }
 
 // The tiles a request's query sees: [0, sink_tiles) and [first, first + n - sink_tiles).
 struct Seen {
@@ -109,52 +121,51 @@ struct Smem {
     static constexpr int OUT = RING;                // [warp][head][PAD] fp32
     static constexpr int STAT = OUT + WARPS * HB * PAD * 4;  // [warp][head][2] fp32
     static constexpr int BARS = STAT + WARPS * HB * 8;
-    static constexpr int SCAN = BARS + WARPS * STAGES * 8;   // 8 warp sums, then the prefix of tiles
-    static constexpr int bytes(int B) { return SCAN + 64 + 4 * (B + 1); }
+    static constexpr int SCAN = BARS + WARPS * STAGES * 8;   // prefix of the requests' costs
+    static constexpr int bytes(int B) { return SCAN + 4 * (B + 1); }
 };
 
-// Exclusive prefix of the requests' tile counts into pre[0..B] (all threads of the CTA).
-__device__ __forceinline__ void scan_tiles(const Args& a, int* pre, int* sums) {
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+// What a request's (kv head, head block) counts in the line of tiles.
+__device__ __forceinline__ int cost_of(int tiles) { return tiles ? tiles + ITEM_COST : 0; }
+
+// Exclusive prefix of the requests' costs into pre[0..B].  Every warp computes and writes all of it (the
+// same values), so none waits for another.
+__device__ __forceinline__ void scan_costs(const Args& a, int* pre) {
+    const int lane = threadIdx.x & 31;
     int carry = 0;
-    for (int base = 0; base < a.B; base += THREADS) {
-        const int b = base + threadIdx.x;
-        const int n = b < a.B ? Seen(a, b).n : 0;
+#pragma unroll 2
+    for (int base = 0; base < a.B; base += 32) {
+        const int b = base + lane;
+        const int n = b < a.B ? cost_of(Seen(a, b).n) : 0;
         int inc = n;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
             const int up = __shfl_up_sync(0xffffffffu, inc, o);
             if (lane >= o) inc += up;
         }
-        if (lane == 31) sums[warp] = inc;
-        __syncthreads();
-        int before = carry, all = carry;
-#pragma unroll
-        for (int w = 0; w < WARPS; ++w) {
-            const int s = sums[w];
-            if (w < warp) before += s;
-            all += s;
-        }
-        if (b < a.B) pre[b] = before + inc - n;
-        carry = all;
-        __syncthreads();
+        if (b < a.B) pre[b] = carry + inc - n;
+        carry += __shfl_sync(0xffffffffu, inc, 31);
     }
-    if (threadIdx.x == 0) pre[a.B] = carry;
-    __syncthreads();
+    if (lane == 0) pre[a.B] = carry;
+    __syncwarp();
 }
+
+// A (request, kv head, head block) and the part [i0, i0 + n) of its `whole` tiles that is this CTA's;
+// n = -1: none is left.
+struct Part {
+    int b, kh, hb, i0, n, whole;
+};
 
 template <typename T, int NG, int NT>
 __global__ void __launch_bounds__(THREADS, NT == 1 ? 2 : 1) kv4_attention_kernel(const Args a) {
     using S = Smem<NG, NT>;
     using R = kv4::Record<NG>;
     constexpr int D = 64 * NG, HB = S::HB, ST = S::STAGES;
-    constexpr bool SPLIT_P = std::is_same<T, __half>::value;
     extern __shared__ __align__(128) uint8_t smem[];
     float* out_s = reinterpret_cast<float*>(smem + S::OUT);
     float* stat_s = reinterpret_cast<float*>(smem + S::STAT);
     uint64_t* bars = reinterpret_cast<uint64_t*>(smem + S::BARS);
-    int* sums = reinterpret_cast<int*>(smem + S::SCAN);
-    int* pre = reinterpret_cast<int*>(smem + S::SCAN + 64);
+    int* pre = reinterpret_cast<int*>(smem + S::SCAN);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int g = lane >> 2, t = lane & 3;
     const int row = (g & 1) ? 7 - (g >> 1) : g >> 1;  // the key of MMA row g; row g + 8 holds key row + 8
@@ -163,102 +174,123 @@ __global__ void __launch_bounds__(THREADS, NT == 1 ? 2 : 1) kv4_attention_kernel
         for (int i = 0; i < ST; ++i) sm100::mbar_init(&bars[warp * ST + i], 1);
         sm100::fence_mbar_init();
     }
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");  // the join may take its place; it waits for this grid
     const int per_b = a.Hk * a.blocks;
-    int64_t at = 0, end = 0;  // this CTA's stretch of the line of tiles
+    int64_t at = 0, end = 0;  // this CTA's stretch of the line
     int64_t share = 0;
-    int b = 0;
+    int b_at = 0;
     if (a.split) {
-        scan_tiles(a, pre, sums);
+        scan_costs(a, pre);
         const int64_t total = (int64_t)pre[a.B] * per_b;
         share = (total + gridDim.x - 1) / gridDim.x;
         if (share < WARPS) share = WARPS;  // at least a tile a warp
         at = min(total, (int64_t)blockIdx.x * share);
         end = min(total, at + share);
         if (threadIdx.x == 0) a.chain[2 * blockIdx.x + 1] = 0;
-        if (at < end) {  // the request the stretch starts in: pre[b] * per_b <= at < pre[b + 1] * per_b
-            int lo = 0, hi = a.B;
-            while (hi - lo > 1) {
-                const int mid = (lo + hi) >> 1;
-                if ((int64_t)pre[mid] * per_b <= at) lo = mid;
-                else hi = mid;
-            }
-            b = lo;
+        int hi = a.B;  // the request the stretch starts in: pre[b] * per_b <= at < pre[b + 1] * per_b
+        while (at < end && hi - b_at > 1) {
+            const int mid = (b_at + hi) >> 1;
+            if ((int64_t)pre[mid] * per_b <= at) b_at = mid;
+            else hi = mid;
         }
-        // Requests that see nothing belong to no stretch.
+    }
+    bool single = !a.split;  // the CTA's one item is still to come
+    auto next_part = [&]() {
+        Part x;
+        if (!a.split) {
+            x.b = blockIdx.x / per_b;
+            const int item = blockIdx.x - x.b * per_b;
+            x.kh = item / a.blocks;
+            x.hb = item - x.kh * a.blocks;
+            x.i0 = 0;
+            x.whole = Seen(a, x.b).n;
+            x.n = single ? x.whole : -1;
+            single = false;
+            return x;
+        }
+        do {
+            if (at >= end) {
+                x.n = -1;
+                return x;
+            }
+            while ((int64_t)pre[b_at + 1] * per_b <= at) ++b_at;
+            const int64_t off = at - (int64_t)pre[b_at] * per_b;
+            const int cost = pre[b_at + 1] - pre[b_at];
+            const int item = (int)(off / cost);
+            const int begin = (int)(off - (int64_t)item * cost);  // costs come first, then tiles
+            const int stop = (int)min((int64_t)cost, begin + (end - at));
+            x.b = b_at;
+            x.kh = item / a.blocks;
+            x.hb = item - x.kh * a.blocks;
+            x.whole = cost - ITEM_COST;
+            x.i0 = max(0, begin - ITEM_COST);
+            x.n = max(0, stop - ITEM_COST) - x.i0;
+            at += stop - begin;
+        } while (x.n == 0);
+        return x;
+    };
+
+    // ---- the ring: record numbers of the warp's tiles of a part, 32 at a time, and the first copies ----
+    uint32_t used = 0;  // tiles this warp has taken from its ring (stage = used % ST)
+    Part now = next_part();
+    int mine, issued, rec_now, rec_next;
+    auto tiles_of_warp = [&](const Part& x) { return x.n > warp ? (x.n - warp + WARPS - 1) / WARPS : 0; };
+    auto records = [&](const Part& x, const Seen& seen, int block) {  // of tiles 32 block + lane of this warp; -1: none, or no such page
+        const int k = 32 * block + lane;
+        if (k >= mine) return -1;
+        const int tile = seen.tile(x.i0 + warp + WARPS * k);
+        const int page = tile / a.tpp;
+        const int id = __ldg(a.table + (int64_t)x.b * a.tb + page);
+        if (id < 0 || id >= a.pages) {
+            kv4::report(g_kv4_attention_status, kv4::BAD_INDEX, kv4::AT_PAGE);
+            return -1;
+        }
+        return (id * a.Hk + x.kh) * a.tpp + (tile - page * a.tpp);
+    };
+    auto issue = [&](int k, int rec) {  // lane 0: tile k of the part, record `rec`, into its stage
+        const uint32_t stage = (used + (uint32_t)k) % ST;
+        uint64_t* bar = &bars[warp * ST + stage];
+        if (rec < 0) {
+            sm100::mbar_arrive(bar);
+        } else {
+            sm100::mbar_arrive_expect_tx(bar, R::BYTES);
+            sm100::bulk_load(sm100::smem_u32(smem) + (warp * ST + stage) * R::BYTES, a.cache + (int64_t)rec * R::BYTES, R::BYTES, bar);
+        }
+    };
+    auto start = [&](const Part& x) {
+        mine = tiles_of_warp(x);
+        issued = 0;
+        if (mine == 0) return;
+        const Seen seen(a, x.b);
+        rec_now = records(x, seen, 0);
+        rec_next = records(x, seen, 1);
+        for (; issued < min(mine, ST - 1); ++issued) {
+            const int rec = __shfl_sync(0xffffffffu, rec_now, issued);
+            if (lane == 0) issue(issued, rec);
+        }
+    };
+    start(now);
+
+    if (a.split) {  // requests that see nothing belong to no stretch
         for (int e = blockIdx.x; e < a.B; e += gridDim.x)
             if (pre[e + 1] == pre[e])
                 for (int i = threadIdx.x; i < a.Hk * a.group * D; i += THREADS)
                     ((T*)a.o)[(int64_t)e * a.ob + (int64_t)(i / D) * a.oh + i % D] = sf::Dt<T>::from_f(0.f);
-    } else {
-        b = blockIdx.x / per_b;
     }
-    if (blockIdx.x == 0 && threadIdx.x < 32)
+    if (blockIdx.x == 0 && warp == 0)
         for (int e = lane; e < a.B; e += 32)
             if (__ldg(a.lens + e) > a.width * a.tpp * 16) kv4::report(g_kv4_attention_status, kv4::BAD_INDEX, kv4::AT_LENGTH);
-    __syncwarp();
 
-    uint32_t used = 0;  // tiles this warp has taken from its ring (stage = used % ST)
-    bool ok = true;     // a copy that never lands ends the warp's work
-    bool first_stretch = true;
-    while (true) {
-        // ---- the next (request, kv head, head block) and the part of its tiles that is this CTA's ----
-        int kh, hb, i0, n, whole;
-        if (a.split) {
-            if (at >= end) break;
-            while ((int64_t)pre[b + 1] * per_b <= at) ++b;
-            const int64_t off = at - (int64_t)pre[b] * per_b;
-            whole = pre[b + 1] - pre[b];
-            const int item = (int)(off / whole);
-            kh = item / a.blocks;
-            hb = item - kh * a.blocks;
-            i0 = (int)(off - (int64_t)item * whole);
-            n = (int)min((int64_t)(whole - i0), end - at);
-        } else {
-            if (!first_stretch) break;
-            const int item = blockIdx.x - b * per_b;
-            kh = item / a.blocks;
-            hb = item - kh * a.blocks;
-            i0 = 0;
-        }
+    while (now.n >= 0) {
+        const int b = now.b;
         const Seen seen(a, b);
-        if (!a.split) whole = n = seen.n;
-        const int head0 = kh * a.group + hb * HB;          // first query head of the block
-        const int heads = min(HB, a.group - hb * HB);
-
-        // ---- the ring: record numbers of this warp's tiles, 32 at a time, and the first copies ----
-        const int mine = n > warp ? (n - warp + WARPS - 1) / WARPS : 0;
-        auto records = [&](int block) {  // of tiles 32 block + lane of this warp; -1: none, or no such page
-            const int k = 32 * block + lane;
-            if (k >= mine) return -1;
-            const int tile = seen.tile(i0 + warp + WARPS * k);
-            const int page = tile / a.tpp;
-            const int id = __ldg(a.table + (int64_t)b * a.tb + page);
-            if (id < 0 || id >= a.pages) {
-                kv4::report(g_kv4_attention_status, kv4::BAD_INDEX, kv4::AT_PAGE);
-                return -1;
-            }
-            return (id * a.Hk + kh) * a.tpp + (tile - page * a.tpp);
-        };
-        int rec_now = records(0), rec_next = records(1);
-        auto issue = [&](int k, int rec) {  // lane 0: tile k of this warp, record `rec`, into its stage
-            const uint32_t stage = (used + (uint32_t)k) % ST;
-            uint64_t* bar = &bars[warp * ST + stage];
-            if (rec < 0) {
-                sm100::mbar_arrive(bar);
-            } else {
-                sm100::mbar_arrive_expect_tx(bar, R::BYTES);
-                sm100::bulk_load(sm100::smem_u32(smem) + (warp * ST + stage) * R::BYTES, a.cache + (int64_t)rec * R::BYTES, R::BYTES, bar);
-            }
-        };
-        int issued = ok ? min(mine, ST - 1) : 0;
-        for (int k = 0; k < issued; ++k) {
-            const int rec = __shfl_sync(0xffffffffu, rec_now, k);
-            if (lane == 0) issue(k, rec);
-        }
+        const int head0 = now.kh * a.group + now.hb * HB;  // first query head of the block
+        const int heads = min(HB, a.group - now.hb * HB);
+        uint32_t bad = __ballot_sync(0xffffffffu, mine && rec_now < 0);  // of a block of 32 tiles: nothing was copied
 
         // ---- q as the B operand: the lane's elements 64 G + 16 t + 0..15 of heads g (+ 8) ----
         uint32_t qf[NT][8 * NG];
-        float fac[NT][2], qs[NT][2][NG];  // of heads 2t, 2t + 1
+        float2 fac[NT], qs[NT][NG];  // of heads 2t, 2t + 1
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
             const int h = nt * 8 + g;
@@ -304,90 +336,84 @@ __global__ void __launch_bounds__(THREADS, NT == 1 ? 2 : 1) kv4_attention_kernel
                     f[3] = f16x2(e[3] * up, e[7] * up);
                 }
             const float down = __uint_as_float((ex + 10u) << 23) * a.scale_log2;  // 2^(ex - 137) 2^20
+            fac[nt] = make_float2(__shfl_sync(0xffffffffu, down, 8 * t), __shfl_sync(0xffffffffu, down, 8 * t + 4));
 #pragma unroll
-            for (int c = 0; c < 2; ++c) {
-                fac[nt][c] = __shfl_sync(0xffffffffu, down, 4 * (2 * t + c));
-#pragma unroll
-                for (int G = 0; G < NG; ++G) qs[nt][c][G] = __shfl_sync(0xffffffffu, sum[G] * a.scale_log2, 4 * (2 * t + c));
-            }
+            for (int G = 0; G < NG; ++G)
+                qs[nt][G] = make_float2(__shfl_sync(0xffffffffu, sum[G] * a.scale_log2, 8 * t), __shfl_sync(0xffffffffu, sum[G] * a.scale_log2, 8 * t + 4));
         }
 
-        float o[NT][4 * NG][4];     // O^T: row g element 64 G + 8 g + m, row g + 8 the element 4 further; heads 2t, 2t + 1
-        float m[NT][2], l[NT][2], pm[NT][2][NG];
+        // O^T, heads 2t, 2t + 1, elements 64 G + 8 g + 4 i + 0..3 for i < 2: [4 G + i] whole bytes (rows g
+        // and g + 8 are the lower and upper pair of elements), [4 G + 2 + i] their upper codes times 16.
+        float o[NT][4 * NG][4];
+        float2 m[NT], l[NT], pm[NT][NG];
+        float2 unit[NT], per_unit[NT];  // O is in this unit, a head each; the largest p s is at most 2^8 of it
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
             for (int i = 0; i < 4 * NG; ++i)
 #pragma unroll
                 for (int c = 0; c < 4; ++c) o[nt][i][c] = 0.f;
+            m[nt] = sf::f2(-INFINITY);
+            l[nt] = unit[nt] = per_unit[nt] = sf::f2(0.f);
 #pragma unroll
-            for (int c = 0; c < 2; ++c) {
-                m[nt][c] = -INFINITY;
-                l[nt][c] = 0.f;
-#pragma unroll
-                for (int G = 0; G < NG; ++G) pm[nt][c][G] = 0.f;
-            }
+            for (int G = 0; G < NG; ++G) pm[nt][G] = sf::f2(0.f);
         }
 
         // ---- the warp's tiles ----
+        const uint8_t* ring = smem + warp * ST * R::BYTES;
+        // Tiles that may hold keys past either end of what is seen: the last, the last of the sinks and
+        // the first behind them.
+        const int edge0 = seen.sink_tiles - 1 - now.i0, edge1 = seen.sink_tiles - now.i0, edge2 = seen.n - 1 - now.i0;
         for (int k = 0; k < mine; ++k) {
             if (k && (k & 31) == 0) {
                 rec_now = rec_next;
-                rec_next = records((k >> 5) + 1);
+                bad = __ballot_sync(0xffffffffu, rec_now < 0);
+                rec_next = records(now, seen, (k >> 5) + 1);
             }
             __syncwarp();  // every lane is done with the stage that the next copy overwrites
-            if (issued < mine && ok) {
+            if (issued < mine) {
                 const int rec = __shfl_sync(0xffffffffu, (issued >> 5) == (k >> 5) ? rec_now : rec_next, issued & 31);
                 if (lane == 0) issue(issued, rec);
                 ++issued;
             }
             const uint32_t turn = used + (uint32_t)k;
-            if (!ok && k >= issued) break;  // a copy gave up: only those in flight are still waited for
-            ok &= sm100::mbar_wait(&bars[warp * ST + turn % ST], (turn / ST) & 1u, g_kv4_attention_status + 1, kv4::AT_WAIT);
-            ok = __all_sync(0xffffffffu, ok);
-            const bool there = __shfl_sync(0xffffffffu, rec_now, k & 31) >= 0;
-            if (!ok || !there) continue;
-            const uint8_t* rec = smem + (warp * ST + turn % ST) * R::BYTES;
+            // A copy that never lands leaves its status; the numbers are void then, and the waits that
+            // follow end early.
+            sm100::mbar_wait(&bars[warp * ST + turn % ST], (turn / ST) & 1u, g_kv4_attention_status + 1, kv4::AT_WAIT);
+            __syncwarp();
+            if (bad >> (k & 31) & 1u) continue;
+            const uint8_t* rec = ring + (turn % ST) * R::BYTES;
 
-            const int key0 = seen.tile(i0 + warp + WARPS * k) * 16;
-            bool v0 = true, v1 = true;  // keys `row` and `row + 8` are seen
-            const bool partly = key0 + 16 > seen.len || (key0 < seen.low && key0 + 16 > a.sinks);
-            if (partly) {
-                const int j = key0 + row;
-                v0 = j < seen.len && (j >= seen.low || j < a.sinks);
-                v1 = j + 8 < seen.len && (j + 8 >= seen.low || j + 8 < a.sinks);
-            }
-            // (scale, minimum) of the lane's two keys.
-            float ks[2][NG], km[2][NG], vs[2][NG], vm[2][NG];
+            // (scale, minimum) of the lane's keys `row` and `row + 8`; of the values the minimum is the
+            // centre's, minimum + 8 scale.
+            float2 kp[2][NG], vp[2][NG];
 #pragma unroll
-            for (int r = 0; r < 2; ++r)
+            for (int r = 0; r < 2; ++r) {
+                uint32_t kw[NG], vw[NG];
+                if constexpr (NG == 2) {
+                    *reinterpret_cast<uint2*>(kw) = *reinterpret_cast<const uint2*>(rec + R::KP + (row + 8 * r) * 8);
+                    *reinterpret_cast<uint2*>(vw) = *reinterpret_cast<const uint2*>(rec + R::VP + (row + 8 * r) * 8);
+                } else {
+                    kw[0] = *reinterpret_cast<const uint32_t*>(rec + R::KP + (row + 8 * r) * 4);
+                    vw[0] = *reinterpret_cast<const uint32_t*>(rec + R::VP + (row + 8 * r) * 4);
+                }
 #pragma unroll
                 for (int G = 0; G < NG; ++G) {
-                    const float2 kp = sf::Pair<__nv_bfloat16>::to_f2(*reinterpret_cast<const uint32_t*>(rec + R::KP + ((row + 8 * r) * NG + G) * 4));
-                    const float2 vp = sf::Pair<__nv_bfloat16>::to_f2(*reinterpret_cast<const uint32_t*>(rec + R::VP + ((row + 8 * r) * NG + G) * 4));
-                    ks[r][G] = kp.x;
-                    km[r][G] = kp.y;
-                    const bool v = r ? v1 : v0;
-                    vs[r][G] = v ? vp.x : 0.f;
-                    vm[r][G] = v ? fmaf(8.f, vp.x, vp.y) : 0.f;
+                    kp[r][G] = sf::Pair<__nv_bfloat16>::to_f2(kw[G]);
+                    vp[r][G] = sf::Pair<__nv_bfloat16>::to_f2(vw[G]);
+                    vp[r][G].y = fmaf(8.f, vp[r][G].x, vp[r][G].y);
                 }
+            }
             // S^T = K q^T, a group at a time.
-            float s[NT][4];
+            float2 s[NT][2];  // [row, row + 8], heads 2t, 2t + 1
             uint32_t kw[2][2 * NG];
 #pragma unroll
             for (int r = 0; r < 2; ++r) {
                 const uint8_t* p = rec + R::K + (row + 8 * r) * R::ROW + t * 8 * NG;
-#pragma unroll
-                for (int i = 0; i < NG; ++i) {
-                    if constexpr (NG == 2) {
-                        if (i == 0) {
-                            const uint4 w = *reinterpret_cast<const uint4*>(p);
-                            kw[r][0] = w.x, kw[r][1] = w.y, kw[r][2] = w.z, kw[r][3] = w.w;
-                        }
-                    } else {
-                        const uint2 w = *reinterpret_cast<const uint2*>(p);
-                        kw[r][0] = w.x, kw[r][1] = w.y;
-                    }
+                if constexpr (NG == 2) {
+                    *reinterpret_cast<uint4*>(kw[r]) = *reinterpret_cast<const uint4*>(p);
+                } else {
+                    *reinterpret_cast<uint2*>(kw[r]) = *reinterpret_cast<const uint2*>(p);
                 }
             }
 #pragma unroll
@@ -397,9 +423,9 @@ __global__ void __launch_bounds__(THREADS, NT == 1 ? 2 : 1) kv4_attention_kernel
                 for (int nt = 0; nt < NT; ++nt) acc[nt][0] = acc[nt][1] = acc[nt][2] = acc[nt][3] = 0.f;
 #pragma unroll
                 for (int h2 = 0; h2 < 2; ++h2) {
-                    const uint32_t x = kw[0][2 * G + h2], y = kw[1][2 * G + h2];
+                    const uint32_t x = kw[0][2 * G + h2], y = kw[1][2 * G + h2], x8 = x >> 8, y8 = y >> 8;
                     const uint32_t a0[4] = {x & 0x000F000Fu, y & 0x000F000Fu, x & 0x00F000F0u, y & 0x00F000F0u};
-                    const uint32_t a1[4] = {(x >> 8) & 0x000F000Fu, (y >> 8) & 0x000F000Fu, (x >> 8) & 0x00F000F0u, (y >> 8) & 0x00F000F0u};
+                    const uint32_t a1[4] = {x8 & 0x000F000Fu, y8 & 0x000F000Fu, x8 & 0x00F000F0u, y8 & 0x00F000F0u};
 #pragma unroll
                     for (int nt = 0; nt < NT; ++nt) {
                         const uint32_t* f = &qf[nt][(2 * G + h2) * 4];
@@ -410,77 +436,101 @@ __global__ void __launch_bounds__(THREADS, NT == 1 ? 2 : 1) kv4_attention_kernel
 #pragma unroll
                 for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-                    for (int c = 0; c < 4; ++c) {
-                        const int r = c >> 1, h = c & 1;
-                        const float dot = acc[nt][c] * ks[r][G];
-                        const float low = km[r][G] * qs[nt][h][G];
-                        const float v = fmaf(dot, fac[nt][h], low);
-                        s[nt][c] = G == 0 ? v : s[nt][c] + v;
+                    for (int r = 0; r < 2; ++r) {
+                        const float2 low = G == 0 ? sf::f2_mul(sf::f2(kp[r][G].y), qs[nt][G]) : sf::f2_fma(sf::f2(kp[r][G].y), qs[nt][G], s[nt][r]);
+                        s[nt][r] = sf::f2_fma(make_float2(acc[nt][2 * r], acc[nt][2 * r + 1]), sf::f2_mul(sf::f2(kp[r][G].x), fac[nt]), low);
                     }
             }
-            if (partly) {
+            const int at_tile = warp + WARPS * k;
+            if (at_tile == edge0 || at_tile == edge1 || at_tile == edge2) {
+                const int j = seen.tile(now.i0 + at_tile) * 16 + row;
 #pragma unroll
-                for (int nt = 0; nt < NT; ++nt) {
-                    if (!v0) s[nt][0] = s[nt][1] = -INFINITY;
-                    if (!v1) s[nt][2] = s[nt][3] = -INFINITY;
+                for (int r = 0; r < 2; ++r) {
+                    if (j + 8 * r < seen.len && (j + 8 * r >= seen.low || j + 8 * r < a.sinks)) continue;
+#pragma unroll
+                    for (int nt = 0; nt < NT; ++nt) s[nt][r] = sf::f2(-INFINITY);
+#pragma unroll
+                    for (int G = 0; G < NG; ++G) vp[r][G] = sf::f2(0.f);
                 }
             }
-            // The running max follows only when a score passes it by 2^8: p stays within fp32 and
-            // bf16 range and the final division takes the stale max out again.
+            // The running max follows only when a score passes it by 2^8: p stays within fp32 and fp16
+            // range and the final division takes the stale max out again.  O follows through its unit.
             bool grow = false;
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) {
+                grow |= fmaxf(s[nt][0].x, s[nt][1].x) > m[nt].x + 8.f;
+                grow |= fmaxf(s[nt][0].y, s[nt][1].y) > m[nt].y + 8.f;
+            }
+            if (__any_sync(0xffffffffu, grow)) {
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt) {
+                    float2 mx = over_keys(make_float2(fmaxf(s[nt][0].x, s[nt][1].x), fmaxf(s[nt][0].y, s[nt][1].y)));
+                    mx = make_float2(fmaxf(mx.x, m[nt].x), fmaxf(mx.y, m[nt].y));
+                    const float2 f = make_float2(m[nt].x == mx.x ? 1.f : exp2f(m[nt].x - mx.x), m[nt].y == mx.y ? 1.f : exp2f(m[nt].y - mx.y));
+                    m[nt] = mx;
+                    l[nt] = sf::f2_mul(l[nt], f);
+                    unit[nt] = sf::f2_mul(unit[nt], f);
+                    per_unit[nt] = make_float2(reciprocal(unit[nt].x), reciprocal(unit[nt].y));
+#pragma unroll
+                    for (int G = 0; G < NG; ++G) pm[nt][G] = sf::f2_mul(pm[nt][G], f);
+                }
+            }
+            // p, its sum, and p s.
+            float2 w[NT][NG][2];
+            grow = false;
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) {
+                const float2 nm = make_float2(m[nt].x == -INFINITY ? 0.f : -m[nt].x, m[nt].y == -INFINITY ? 0.f : -m[nt].y);
+                float2 top = sf::f2(0.f);
+#pragma unroll
+                for (int r = 0; r < 2; ++r) {
+                    float2 p = sf::f2_add(s[nt][r], nm);
+                    p = make_float2(sf::ex2_ftz(p.x), sf::ex2_ftz(p.y));
+                    l[nt] = sf::f2_add(l[nt], p);
+#pragma unroll
+                    for (int G = 0; G < NG; ++G) {
+                        pm[nt][G] = sf::f2_fma(p, sf::f2(vp[r][G].y), pm[nt][G]);
+                        w[nt][G][r] = sf::f2_mul(p, sf::f2(vp[r][G].x));
+                        top = make_float2(fmaxf(top.x, w[nt][G][r].x), fmaxf(top.y, w[nt][G][r].y));
+                    }
+                }
+                grow |= top.x > 256.f * unit[nt].x || top.y > 256.f * unit[nt].y;
+            }
+            if (__any_sync(0xffffffffu, grow)) {
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt) {
+                    float2 top = sf::f2(0.f);
+#pragma unroll
+                    for (int G = 0; G < NG; ++G)
+#pragma unroll
+                        for (int r = 0; r < 2; ++r) top = make_float2(fmaxf(top.x, w[nt][G][r].x), fmaxf(top.y, w[nt][G][r].y));
+                    top = over_keys(top);
+                    // Where this head's own weights fit its unit stays.
+                    const float2 u = make_float2(top.x > 256.f * unit[nt].x ? fmaxf(top.x, 0x1p-126f) : unit[nt].x,
+                                                 top.y > 256.f * unit[nt].y ? fmaxf(top.y, 0x1p-126f) : unit[nt].y);
+                    per_unit[nt] = make_float2(reciprocal(u.x), reciprocal(u.y));
+                    const float2 f = sf::f2_mul(unit[nt], per_unit[nt]);
+                    unit[nt] = u;
+#pragma unroll
+                    for (int i = 0; i < 4 * NG; ++i) {
+                        o[nt][i][0] *= f.x;
+                        o[nt][i][1] *= f.y;
+                        o[nt][i][2] *= f.x;
+                        o[nt][i][3] *= f.y;
+                    }
+                }
+            }
+            // p s in the unit, as the B operand of O^T = V^T p^T.
+            uint32_t pf[NT][NG][2];
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-                for (int h = 0; h < 2; ++h) grow |= fmaxf(s[nt][h], s[nt][h + 2]) > m[nt][h] + 8.f;
-            if (__any_sync(0xffffffffu, grow)) {
-#pragma unroll
-                for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-                    for (int h = 0; h < 2; ++h) {
-                        float mx = fmaxf(s[nt][h], s[nt][h + 2]);
-#pragma unroll
-                        for (int off = 4; off < 32; off <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, off));
-                        mx = fmaxf(mx, m[nt][h]);
-                        const float f = m[nt][h] == mx ? 1.f : exp2f(m[nt][h] - mx);
-                        m[nt][h] = mx;
-                        l[nt][h] *= f;
-#pragma unroll
-                        for (int G = 0; G < NG; ++G) pm[nt][h][G] *= f;
-#pragma unroll
-                        for (int i = 0; i < 4 * NG; ++i) {
-                            o[nt][i][h] *= f;
-                            o[nt][i][h + 2] *= f;
-                        }
-                    }
-            }
-            // p, its sum, and p s as the B operand of O^T = V^T p^T.
-            uint32_t pf[NT][NG][2], pl[NT][NG][2];
-#pragma unroll
-            for (int nt = 0; nt < NT; ++nt) {
-                float p[4];
-#pragma unroll
-                for (int c = 0; c < 4; ++c) {
-                    const float mm = m[nt][c & 1];
-                    p[c] = sf::ex2_ftz(s[nt][c] - (mm == -INFINITY ? 0.f : mm));
-                }
-                l[nt][0] += p[0] + p[2];
-                l[nt][1] += p[1] + p[3];
-#pragma unroll
-                for (int G = 0; G < NG; ++G) {
-                    pm[nt][0][G] = fmaf(p[0], vm[0][G], fmaf(p[2], vm[1][G], pm[nt][0][G]));
-                    pm[nt][1][G] = fmaf(p[1], vm[0][G], fmaf(p[3], vm[1][G], pm[nt][1][G]));
+                for (int G = 0; G < NG; ++G)
 #pragma unroll
                     for (int r = 0; r < 2; ++r) {
-                        const float w0 = p[2 * r] * vs[r][G], w1 = p[2 * r + 1] * vs[r][G];
-                        const uint32_t hi = bf16x2(w0, w1);
-                        pf[nt][G][r] = transpose8(hi);
-                        if (SPLIT_P) {
-                            const float2 back = sf::Pair<__nv_bfloat16>::to_f2(hi);
-                            pl[nt][G][r] = transpose8(bf16x2(w0 - back.x, w1 - back.y));
-                        }
+                        const float2 x = sf::f2_mul(w[nt][G][r], per_unit[nt]);
+                        pf[nt][G][r] = transpose8(f16x2(x.x, x.y));
                     }
-                }
-            }
             // O^T += V^T p^T: the lane reads its 8 elements a group of keys t, 7 - t, 8 + t, 15 - t.
             uint32_t vw[4][NG];
 #pragma unroll
@@ -488,62 +538,77 @@ __global__ void __launch_bounds__(THREADS, NT == 1 ? 2 : 1) kv4_attention_kernel
                 const int key = (i & 1 ? 7 - t : t) + 8 * (i >> 1);
                 const uint8_t* p = rec + R::V + key * R::ROW + (g ^ (4 * ((key >> 1) & 1))) * 4 * NG;
                 if constexpr (NG == 2) {
-                    const uint2 w = *reinterpret_cast<const uint2*>(p);
-                    vw[i][0] = w.x, vw[i][1] = w.y;
+                    *reinterpret_cast<uint2*>(vw[i]) = *reinterpret_cast<const uint2*>(p);
                 } else {
                     vw[i][0] = *reinterpret_cast<const uint32_t*>(p);
                 }
             }
 #pragma unroll
-            for (int G = 0; G < NG; ++G) {
-                // Codes 0..3 and 4..7 of two keys side by side in the halves of a word.
-                const uint32_t x0 = __byte_perm(vw[0][G], vw[1][G], 0x5410), x1 = __byte_perm(vw[0][G], vw[1][G], 0x7632);
-                const uint32_t y0 = __byte_perm(vw[2][G], vw[3][G], 0x5410), y1 = __byte_perm(vw[2][G], vw[3][G], 0x7632);
+            for (int G = 0; G < NG; ++G)
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const uint32_t af[4] = {centred(x0 >> (4 * i)), centred(x1 >> (4 * i)), centred(y0 >> (4 * i)), centred(y1 >> (4 * i))};
+                for (int i = 0; i < 2; ++i) {
+                    // Elements 4 i .. 4 i + 3 (two bytes) of two keys side by side in the halves of a word.
+                    const uint32_t x = __byte_perm(vw[0][G], vw[1][G], i ? 0x7632 : 0x5410), y = __byte_perm(vw[2][G], vw[3][G], i ? 0x7632 : 0x5410);
+                    const uint32_t b[4] = {(x & 0x00FF00FFu) | 0x64006400u, __byte_perm(x, 0x64646464u, 0x4341), (y & 0x00FF00FFu) | 0x64006400u,
+                                           __byte_perm(y, 0x64646464u, 0x4341)};
+                    uint32_t all[4], up[4];
+#pragma unroll
+                    for (int c = 0; c < 4; ++c) {
+                        all[c] = sub2(b[c], 0x64886488u);                 // 1024 + byte - 1160
+                        up[c] = sub2(b[c] & 0xFFF0FFF0u, 0x64806480u);    // 1024 + 16 code - 1152
+                    }
 #pragma unroll
                     for (int nt = 0; nt < NT; ++nt) {
-                        mma_bf16(o[nt][4 * G + i], af, pf[nt][G][0], pf[nt][G][1]);
-                        if (SPLIT_P) mma_bf16(o[nt][4 * G + i], af, pl[nt][G][0], pl[nt][G][1]);
+                        mma_f16(o[nt][4 * G + i], all, pf[nt][G][0], pf[nt][G][1]);
+                        mma_f16(o[nt][4 * G + 2 + i], up, pf[nt][G][0], pf[nt][G][1]);
                     }
                 }
-            }
         }
-        used += (uint32_t)issued;  // = mine, unless a copy gave up
+        used += (uint32_t)mine;
+        const Part done = now;
+        const int64_t done_at = at;
+        __syncwarp();
+        now = next_part();
+        start(now);
 
         // ---- the warps' states side by side, then one sum over them ----
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
+        for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+            for (int off = 4; off < 32; off <<= 1) {
+                l[nt].x += __shfl_xor_sync(0xffffffffu, l[nt].x, off);
+                l[nt].y += __shfl_xor_sync(0xffffffffu, l[nt].y, off);
+#pragma unroll
+                for (int G = 0; G < NG; ++G) {
+                    pm[nt][G].x += __shfl_xor_sync(0xffffffffu, pm[nt][G].x, off);
+                    pm[nt][G].y += __shfl_xor_sync(0xffffffffu, pm[nt][G].y, off);
+                }
+            }
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
-                float sum = l[nt][h], add[NG];
-#pragma unroll
-                for (int G = 0; G < NG; ++G) add[G] = pm[nt][h][G];
-#pragma unroll
-                for (int off = 4; off < 32; off <<= 1) {
-                    sum += __shfl_xor_sync(0xffffffffu, sum, off);
-#pragma unroll
-                    for (int G = 0; G < NG; ++G) add[G] += __shfl_xor_sync(0xffffffffu, add[G], off);
-                }
                 const int head = nt * 8 + 2 * t + h;
                 if (g == 0) {
-                    stat_s[(warp * HB + head) * 2] = m[nt][h];
-                    stat_s[(warp * HB + head) * 2 + 1] = sum;
+                    stat_s[(warp * HB + head) * 2] = h ? m[nt].y : m[nt].x;
+                    stat_s[(warp * HB + head) * 2 + 1] = h ? l[nt].y : l[nt].x;
                 }
                 float* dst = out_s + (warp * HB + head) * S::PAD + 8 * g;
 #pragma unroll
                 for (int G = 0; G < NG; ++G) {
-                    *reinterpret_cast<float4*>(dst + 64 * G) =
-                        make_float4(o[nt][4 * G][h] + add[G], o[nt][4 * G + 1][h] + add[G], o[nt][4 * G + 2][h] + add[G], o[nt][4 * G + 3][h] + add[G]);
-                    *reinterpret_cast<float4*>(dst + 64 * G + 4) = make_float4(o[nt][4 * G][h + 2] + add[G], o[nt][4 * G + 1][h + 2] + add[G],
-                                                                               o[nt][4 * G + 2][h + 2] + add[G], o[nt][4 * G + 3][h + 2] + add[G]);
+                    const float add = h ? pm[nt][G].y : pm[nt][G].x, u = h ? unit[nt].y : unit[nt].x;
+#pragma unroll
+                    for (int i = 0; i < 2; ++i) {
+                        const float *all = o[nt][4 * G + i], *up = o[nt][4 * G + 2 + i];
+                        *reinterpret_cast<float4*>(dst + 64 * G + 4 * i) =
+                            make_float4(fmaf(all[h] - up[h], u, add), fmaf(up[h], u * 0.0625f, add), fmaf(all[h + 2] - up[h + 2], u, add),
+                                        fmaf(up[h + 2], u * 0.0625f, add));
+                    }
                 }
             }
+        }
         __syncthreads();
-        const bool all_mine = n == whole;
-        const int slot = 2 * blockIdx.x + (first_stretch && i0 > 0 ? 0 : 1);
-        const int active = min(n, WARPS);  // warps that had tiles
+        const bool all_mine = done.n == done.whole;
+        const int slot = 2 * blockIdx.x + (done.i0 > 0 ? 0 : 1);
+        const int active = min(done.n, WARPS);  // warps that had tiles
         for (int e = threadIdx.x; e < HB * (D / 4); e += THREADS) {
             const int head = e / (D / 4), d = 4 * (e % (D / 4));
             float mx = -INFINITY;
@@ -562,7 +627,7 @@ __global__ void __launch_bounds__(THREADS, NT == 1 ? 2 : 1) kv4_attention_kernel
             }
             if (all_mine) {
                 if (head < heads) {
-                    const float inv = n == 0 ? 0.f : 1.0f / sum;
+                    const float inv = done.n == 0 ? 0.f : 1.0f / sum;
                     T* dst = (T*)a.o + (int64_t)b * a.ob + (int64_t)(head0 + head) * a.oh + d;
                     *reinterpret_cast<uint2*>(dst) = make_uint2(sf::Pair<T>::from_f2(make_float2(acc.x * inv, acc.y * inv)),
                                                                 sf::Pair<T>::from_f2(make_float2(acc.z * inv, acc.w * inv)));
@@ -572,71 +637,59 @@ __global__ void __launch_bounds__(THREADS, NT == 1 ? 2 : 1) kv4_attention_kernel
                 if (d == 0) *reinterpret_cast<float2*>(a.stat + ((int64_t)slot * HB + head) * 2) = make_float2(mx, sum);
             }
         }
-        if (a.split) {
-            // An item that starts here and goes on in the CTAs behind is joined from here.
-            if (threadIdx.x == 0 && i0 == 0 && n < whole) {
-                a.chain[2 * blockIdx.x] = b * per_b + kh * a.blocks + hb;
-                a.chain[2 * blockIdx.x + 1] = (int)((at + whole - 1) / share) - blockIdx.x + 1;
-            }
-            at += n;
+        // An item that starts here and goes on in the CTAs behind is joined from here.
+        if (threadIdx.x == 0 && done.i0 == 0 && !all_mine) {
+            a.chain[2 * blockIdx.x] = b * per_b + done.kh * a.blocks + done.hb;
+            a.chain[2 * blockIdx.x + 1] = (int)((done_at - done.n + done.whole - 1) / share) - blockIdx.x + 1;
         }
-        first_stretch = false;
         __syncthreads();
     }
 }
 
-// Join the pieces of the items that span CTAs: one block a (first CTA, head), 4 warps over the pieces.
+// Join the pieces of the items that span CTAs: one block a (first CTA, head), its warps over the pieces.
+constexpr int JOIN_WARPS = 8;
 template <typename T, int D, int HB>
-__global__ void __launch_bounds__(128) kv4_join_kernel(const Args a) {
+__global__ void __launch_bounds__(32 * JOIN_WARPS) kv4_join_kernel(const Args a) {
     asm volatile("griddepcontrol.wait;" ::: "memory");
     const int first = blockIdx.x, head = blockIdx.y;
-    const int pieces = a.chain[2 * first + 1];
+    const int2 chain = *reinterpret_cast<const int2*>(a.chain + 2 * first);
+    const int pieces = chain.y, item = chain.x;
     if (pieces == 0) return;
-    const int item = a.chain[2 * first];
     const int per_b = a.Hk * a.blocks;
     const int b = item / per_b, kh = (item - b * per_b) / a.blocks, hb = item - b * per_b - kh * a.blocks;
     if (hb * HB + head >= a.group) return;
-    __shared__ float acc_s[4][D];
-    __shared__ float stat_s[4][2];
+    __shared__ float acc_s[JOIN_WARPS][D];
     constexpr int E = D / 32;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    float m = -INFINITY, l = 0.f, acc[E];
+    // The first piece is its CTA's last part, the others their CTAs' first.
+    auto slot = [&](int p) { return ((int64_t)2 * (first + p) + (p == 0 ? 1 : 0)) * HB + head; };
+    float m = -INFINITY, l = 0.f;
+    for (int p = lane; p < pieces; p += 32) m = fmaxf(m, a.stat[slot(p) * 2]);
+    m = sf::warp_max(m);
+    const float shift = m == -INFINITY ? 0.f : m;
+    for (int p = lane; p < pieces; p += 32) {
+        const float2 st = *reinterpret_cast<const float2*>(a.stat + slot(p) * 2);
+        l = fmaf(exp2f(st.x - shift), st.y, l);
+    }
+    l = sf::warp_sum(l);
+    float acc[E];
 #pragma unroll
     for (int e = 0; e < E; ++e) acc[e] = 0.f;
-    for (int p = warp; p < pieces; p += 4) {
-        // The first piece is its CTA's last stretch, the others their CTAs' first.
-        const int64_t slot = (int64_t)2 * (first + p) + (p == 0 ? 1 : 0);
-        const float2 st = *reinterpret_cast<const float2*>(a.stat + (slot * HB + head) * 2);
-        const float* src = a.part + (slot * HB + head) * D + E * lane;
-        float x[E];
+#pragma unroll 4
+    for (int p = warp; p < pieces; p += JOIN_WARPS) {
+        const float f = exp2f(a.stat[slot(p) * 2] - shift);
+        const float* src = a.part + slot(p) * D + E * lane;
 #pragma unroll
-        for (int e = 0; e < E; ++e) x[e] = src[e];
-        const float mx = fmaxf(m, st.x);
-        const float f0 = m == mx ? 1.f : exp2f(m - mx), f1 = st.x == mx ? 1.f : exp2f(st.x - mx);
-        l = l * f0 + st.y * f1;
-#pragma unroll
-        for (int e = 0; e < E; ++e) acc[e] = acc[e] * f0 + x[e] * f1;
-        m = mx;
+        for (int e = 0; e < E; ++e) acc[e] = fmaf(f, src[e], acc[e]);
     }
 #pragma unroll
     for (int e = 0; e < E; ++e) acc_s[warp][E * lane + e] = acc[e];
-    if (lane == 0) {
-        stat_s[warp][0] = m;
-        stat_s[warp][1] = l;
-    }
     __syncthreads();
     if (threadIdx.x >= D) return;
-    float mx = -INFINITY, sum = 0.f, out = 0.f;
+    float out = 0.f;
 #pragma unroll
-    for (int w = 0; w < 4; ++w) mx = fmaxf(mx, stat_s[w][0]);
-#pragma unroll
-    for (int w = 0; w < 4; ++w) {
-        if (w >= pieces) break;
-        const float f = stat_s[w][0] == mx ? 1.f : exp2f(stat_s[w][0] - mx);
-        sum += f * stat_s[w][1];
-        out += f * acc_s[w][threadIdx.x];
-    }
-    ((T*)a.o)[(int64_t)b * a.ob + (int64_t)(kh * a.group + hb * HB + head) * a.oh + threadIdx.x] = sf::Dt<T>::from_f(out / sum);
+    for (int w = 0; w < JOIN_WARPS; ++w) out += acc_s[w][threadIdx.x];
+    ((T*)a.o)[(int64_t)b * a.ob + (int64_t)(kh * a.group + hb * HB + head) * a.oh + threadIdx.x] = sf::Dt<T>::from_f(out / l);
 }
 
 // Most tiles a request can see, from the table's width, window and sinks alone.
@@ -699,7 +752,7 @@ int launch_t(Args a, const Plan& p, cudaStream_t st, char* err, uint64_t cap) {
     // The join starts while the last CTAs of the first kernel run, and waits for all of it.
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)p.grid, (unsigned)std::min(HB, a.group));
-    cfg.blockDim = dim3(128);
+    cfg.blockDim = dim3(32 * JOIN_WARPS);
     cfg.stream = st;
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -746,8 +799,8 @@ extern "C" int sf_kv4_attention(const sf_kv4_attention_args* x, void* stream, ch
         return sf::fail(SF_EINVAL, err, cap, "kv4_attention: q, out and the cache must be 16-byte aligned");
     const int64_t tpp = page_size / 16;
     if (pages * Hk > 0x7fffffffLL / tpp) return sf::fail(SF_EINVAL, err, cap, "kv4_attention: more than 2^31 - 1 records");
-    // The tiles of all requests are counted in 32 bits.
-    if (B > 0x7fffffffLL / std::max<int64_t>(1, width * tpp)) return sf::fail(SF_EINVAL, err, cap, "kv4_attention: requests x table width too large");
+    // The costs of all requests are summed in 32 bits.
+    if (B > 0x7fffffffLL / (width * tpp + ITEM_COST)) return sf::fail(SF_EINVAL, err, cap, "kv4_attention: requests x table width too large");
     const Plan p = plan_of(B, Hq, Hk, D, width, tpp, window, sinks, x->variant);
     if (B * Hk > 0x7fffffffLL / p.blocks) return sf::fail(SF_EINVAL, err, cap, "kv4_attention: grid too large");
     if (p.split && (!x->workspace || x->workspace_bytes < workspace_of(p, D) || !sf::aligned16(x->workspace)))
