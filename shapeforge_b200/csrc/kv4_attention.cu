@@ -11,8 +11,9 @@
 //   o       = sum_j (p_j s_jG) (c_j - 8) + p_j (m_jG + 8 s_jG)  scales go into p, which is small.
 //
 //  * K: an fp16 whose low bits are a code is the subnormal c 2^-24, exactly, so one AND makes two
-//    operands.  q is scaled by a power of two to [1, 2) a head (exact in fp16 down to 2^-24 of the
-//    head's largest) and by 16 where the code sits in the lower nibble of its byte.
+//    operands.  The block's q are scaled by one power of two to at most 2^11 (an fp16 holds them exactly
+//    down to 2^-25 of the largest) and by 16 where the code sits in the lower nibble of its byte.  The
+//    minima's part is one bf16 MMA of its own: minima are bf16, sum(q_G) goes in as three bf16 parts.
 //  * V: with two keys' bytes side by side, 0x6400 | b is the fp16 1024 + b of a whole byte b = c + 16 c'
 //    (two neighbouring elements' codes) and clearing its low bits gives 1024 + 16 c'.  Both, less 1160
 //    and 1152, go through the MMA, and (c - 8) and (c' - 8) of the accumulators come from their
@@ -47,7 +48,10 @@ namespace {
 constexpr int WARPS = 8;
 constexpr int THREADS = 32 * WARPS;
 constexpr int MAX_SMEM = 227 * 1024;
-constexpr int ITEM_COST = 12;  // what starting and merging a (request, head) costs, in tiles
+constexpr int ITEM_COST = 16;  // what starting and merging a (request, head) costs, in tiles
+constexpr float NO_MAX = -3e38f;  // the running max before any score
+// Smallest unit of a head's p s: p / unit stays finite for p up to 2^8.
+constexpr float UNIT_FLOOR = 0x1p-118f;
 constexpr float LOG2E = 1.4426950408889634f;
 
 struct Args {
@@ -72,6 +76,17 @@ __device__ __forceinline__ void mma_f16(float (&d)[4], const uint32_t (&a)[4], u
                  : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
                  : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
+// The same onto zero.
+__device__ __forceinline__ void mma_f16_first(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+                 : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.f));
+}
+__device__ __forceinline__ void mma_bf16_k8_first(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t b) {
+    asm volatile("mma.sync.aligned.m16n8k8.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5}, {%6}, {%7,%7,%7,%7};"
+                 : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+                 : "r"(a0), "r"(a1), "r"(b), "f"(0.f));
+}
 // Transpose of an 8 x 8 matrix of 16-bit values held as an MMA fragment.
 __device__ __forceinline__ uint32_t transpose8(uint32_t x) {
     uint32_t y;
@@ -94,9 +109,6 @@ __device__ __forceinline__ float2 over_keys(float2 v) {
     }
     return v;
 }
-// 1 / u, and 0 for a unit that has vanished (what it counted has too).
-__device__ __forceinline__ float reciprocal(float u) { return u >= 0x1p-126f ? 1.0f / u : 0.f; }
-
 // The tiles a request's query sees: [0, sink_tiles) and [first, first + n - sink_tiles).
 struct Seen {
     int len, low;  // keys j < len with j >= low or j < sinks
@@ -111,6 +123,21 @@ struct Seen {
     __device__ __forceinline__ int tile(int i) const { return i < sink_tiles ? i : first + (i - sink_tiles); }
 };
 
+// A (request, kv head, head block) and the part [i0, i0 + n) of its `whole` tiles that is this CTA's;
+// n = -1: none is left.
+struct Part {
+    int b, item, i0, n, whole;  // item = kv head x head blocks + head block
+};
+// A warp's place in its CTA's stretch [at, end) of the line: the next part begins at `into` of item `item`
+// of request b.  It changes once a part and would take ten registers from the loop over the tiles, so it
+// is kept in shared memory, each warp its own copy.
+struct Line {
+    int64_t at, end;
+    int b, item, into;
+    Part next;
+};
+static_assert(sizeof(Line) <= 64, "");
+
 template <int NG, int NT>
 struct Smem {
     static constexpr int D = 64 * NG;
@@ -121,7 +148,9 @@ struct Smem {
     static constexpr int OUT = RING;                // [warp][head][PAD] fp32
     static constexpr int STAT = OUT + WARPS * HB * PAD * 4;  // [warp][head][2] fp32
     static constexpr int BARS = STAT + WARPS * HB * 8;
-    static constexpr int SCAN = BARS + WARPS * STAGES * 8;   // prefix of the requests' costs
+    static constexpr int AHEAD = BARS + (WARPS * STAGES + 2) * 8;  // [warp][64] record numbers of the next part
+    static constexpr int LINE = AHEAD + WARPS * 64 * 4;            // [warp] Line
+    static constexpr int SCAN = LINE + WARPS * 64;                 // prefix of the requests' costs
     static constexpr int bytes(int B) { return SCAN + 4 * (B + 1); }
 };
 
@@ -150,12 +179,6 @@ __device__ __forceinline__ void scan_costs(const Args& a, int* pre) {
     __syncwarp();
 }
 
-// A (request, kv head, head block) and the part [i0, i0 + n) of its `whole` tiles that is this CTA's;
-// n = -1: none is left.
-struct Part {
-    int b, kh, hb, i0, n, whole;
-};
-
 template <typename T, int NG, int NT>
 __global__ void __launch_bounds__(THREADS, NT == 1 ? 2 : 1) kv4_attention_kernel(const Args a) {
     using S = Smem<NG, NT>;
@@ -170,74 +193,89 @@ __global__ void __launch_bounds__(THREADS, NT == 1 ? 2 : 1) kv4_attention_kernel
     const int g = lane >> 2, t = lane & 3;
     const int row = (g & 1) ? 7 - (g >> 1) : g >> 1;  // the key of MMA row g; row g + 8 holds key row + 8
 
+    uint64_t* merged = bars + WARPS * ST;  // the staged states have been read (one arrival a warp)
     if (lane == 0) {
         for (int i = 0; i < ST; ++i) sm100::mbar_init(&bars[warp * ST + i], 1);
+        if (warp == 0) sm100::mbar_init(merged, WARPS);
         sm100::fence_mbar_init();
     }
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");  // the join may take its place; it waits for this grid
     const int per_b = a.Hk * a.blocks;
-    int64_t at = 0, end = 0;  // this CTA's stretch of the line
-    int64_t share = 0;
-    int b_at = 0;
+    Line* line = reinterpret_cast<Line*>(smem + S::LINE + 64 * warp);
+    auto share_of = [&]() {  // tiles and costs a CTA, at least a tile a warp
+        const int64_t total = (int64_t)pre[a.B] * per_b;
+        return max((int64_t)WARPS, (total + gridDim.x - 1) / gridDim.x);
+    };
     if (a.split) {
         scan_costs(a, pre);
-        const int64_t total = (int64_t)pre[a.B] * per_b;
-        share = (total + gridDim.x - 1) / gridDim.x;
-        if (share < WARPS) share = WARPS;  // at least a tile a warp
-        at = min(total, (int64_t)blockIdx.x * share);
-        end = min(total, at + share);
+        const int64_t total = (int64_t)pre[a.B] * per_b, share = share_of();
+        Line x = {};
+        x.at = min(total, (int64_t)blockIdx.x * share);
+        x.end = min(total, x.at + share);
         if (threadIdx.x == 0) a.chain[2 * blockIdx.x + 1] = 0;
-        int hi = a.B;  // the request the stretch starts in: pre[b] * per_b <= at < pre[b + 1] * per_b
-        while (at < end && hi - b_at > 1) {
-            const int mid = (b_at + hi) >> 1;
-            if ((int64_t)pre[mid] * per_b <= at) b_at = mid;
-            else hi = mid;
-        }
-    }
-    bool single = !a.split;  // the CTA's one item is still to come
-    auto next_part = [&]() {
-        Part x;
-        if (!a.split) {
-            x.b = blockIdx.x / per_b;
-            const int item = blockIdx.x - x.b * per_b;
-            x.kh = item / a.blocks;
-            x.hb = item - x.kh * a.blocks;
-            x.i0 = 0;
-            x.whole = Seen(a, x.b).n;
-            x.n = single ? x.whole : -1;
-            single = false;
-            return x;
-        }
-        do {
-            if (at >= end) {
-                x.n = -1;
-                return x;
+        if (x.at < x.end) {
+            int hi = a.B;  // pre[b] * per_b <= at < pre[b + 1] * per_b
+            while (hi - x.b > 1) {
+                const int mid = (x.b + hi) >> 1;
+                if ((int64_t)pre[mid] * per_b <= x.at) x.b = mid;
+                else hi = mid;
             }
-            while ((int64_t)pre[b_at + 1] * per_b <= at) ++b_at;
-            const int64_t off = at - (int64_t)pre[b_at] * per_b;
-            const int cost = pre[b_at + 1] - pre[b_at];
-            const int item = (int)(off / cost);
-            const int begin = (int)(off - (int64_t)item * cost);  // costs come first, then tiles
-            const int stop = (int)min((int64_t)cost, begin + (end - at));
-            x.b = b_at;
-            x.kh = item / a.blocks;
-            x.hb = item - x.kh * a.blocks;
-            x.whole = cost - ITEM_COST;
-            x.i0 = max(0, begin - ITEM_COST);
-            x.n = max(0, stop - ITEM_COST) - x.i0;
-            at += stop - begin;
-        } while (x.n == 0);
-        return x;
+            const int64_t off = x.at - (int64_t)pre[x.b] * per_b;
+            const int cost = pre[x.b + 1] - pre[x.b];
+            x.item = (int)(off / cost);
+            x.into = (int)(off - (int64_t)x.item * cost);
+        }
+        if (lane == 0) *line = x;
+    } else if (lane == 0) {
+        Line x = {};
+        x.end = 1;  // the CTA's one item is still to come
+        x.b = blockIdx.x / per_b;
+        x.item = blockIdx.x - x.b * per_b;
+        *line = x;
+    }
+    __syncwarp();
+    // The next part, by lane 0 into line->next.
+    auto step = [&]() {
+        if (lane == 0) {
+            Line y = *line;
+            Part& x = y.next;
+            x.n = -1;
+            if (!a.split) {
+                if (y.at < y.end) {
+                    const int n = Seen(a, y.b).n;
+                    x = {y.b, y.item, 0, n, n};
+                    y.at = y.end;
+                }
+            } else {
+                while (y.at < y.end) {
+                    const int cost = pre[y.b + 1] - pre[y.b];
+                    const int stop = (int)min((int64_t)cost, y.into + (y.end - y.at));  // costs come first, then tiles
+                    x = {y.b, y.item, max(0, y.into - ITEM_COST), 0, cost - ITEM_COST};
+                    const int n = max(0, stop - ITEM_COST) - x.i0;
+                    x.n = n > 0 ? n : -1;
+                    y.at += stop - y.into;
+                    y.into = 0;
+                    if (stop == cost && ++y.item == per_b) {
+                        y.item = 0;
+                        do ++y.b;
+                        while (y.at < y.end && pre[y.b + 1] == pre[y.b]);
+                    }
+                    if (n > 0) break;
+                }
+            }
+            *line = y;
+        }
+        __syncwarp();
     };
 
-    // ---- the ring: record numbers of the warp's tiles of a part, 32 at a time, and the first copies ----
+    // ---- the ring ----
     uint32_t used = 0;  // tiles this warp has taken from its ring (stage = used % ST)
-    Part now = next_part();
-    int mine, issued, rec_now, rec_next;
+    int* ahead = reinterpret_cast<int*>(smem + S::AHEAD) + 64 * warp;
     auto tiles_of_warp = [&](const Part& x) { return x.n > warp ? (x.n - warp + WARPS - 1) / WARPS : 0; };
-    auto records = [&](const Part& x, const Seen& seen, int block) {  // of tiles 32 block + lane of this warp; -1: none, or no such page
+    // Record numbers of tiles 32 block + lane of this warp; -1: none, or no such page.
+    auto records = [&](const Part& x, const Seen& seen, int block) {
         const int k = 32 * block + lane;
-        if (k >= mine) return -1;
+        if (k >= tiles_of_warp(x)) return -1;
         const int tile = seen.tile(x.i0 + warp + WARPS * k);
         const int page = tile / a.tpp;
         const int id = __ldg(a.table + (int64_t)x.b * a.tb + page);
@@ -245,7 +283,7 @@ __global__ void __launch_bounds__(THREADS, NT == 1 ? 2 : 1) kv4_attention_kernel
             kv4::report(g_kv4_attention_status, kv4::BAD_INDEX, kv4::AT_PAGE);
             return -1;
         }
-        return (id * a.Hk + x.kh) * a.tpp + (tile - page * a.tpp);
+        return (id * a.Hk + x.item / a.blocks) * a.tpp + (tile - page * a.tpp);
     };
     auto issue = [&](int k, int rec) {  // lane 0: tile k of the part, record `rec`, into its stage
         const uint32_t stage = (used + (uint32_t)k) % ST;
@@ -257,19 +295,44 @@ __global__ void __launch_bounds__(THREADS, NT == 1 ? 2 : 1) kv4_attention_kernel
             sm100::bulk_load(sm100::smem_u32(smem) + (warp * ST + stage) * R::BYTES, a.cache + (int64_t)rec * R::BYTES, R::BYTES, bar);
         }
     };
-    auto start = [&](const Part& x) {
-        mine = tiles_of_warp(x);
-        issued = 0;
-        if (mine == 0) return;
+    // A part's first 64 record numbers, looked up long before they are needed.
+    auto look_up = [&](const Part& x) {
+        if (x.n <= 0) return;
         const Seen seen(a, x.b);
-        rec_now = records(x, seen, 0);
-        rec_next = records(x, seen, 1);
-        for (; issued < min(mine, ST - 1); ++issued) {
+        ahead[lane] = records(x, seen, 0);
+        ahead[32 + lane] = records(x, seen, 1);
+        __syncwarp();
+    };
+    int mine, issued, rec_now, rec_next;
+    uint4 raw[NT][NG][2];  // the lane's elements 64 G + 16 t + 0..15 of heads g (+ 8)
+    // Begin a part that has been looked up: its first copies and its queries.
+    auto begin = [&](const Part& x) {
+        if (x.n < 0) return;
+        mine = tiles_of_warp(x);
+        rec_now = x.n ? ahead[lane] : -1;
+        rec_next = x.n ? ahead[32 + lane] : -1;
+        for (issued = 0; issued < min(mine, ST - 1); ++issued) {
             const int rec = __shfl_sync(0xffffffffu, rec_now, issued);
             if (lane == 0) issue(issued, rec);
         }
+        const int kh = x.item / a.blocks, hb = x.item - kh * a.blocks;
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int G = 0; G < NG; ++G) {
+                const int h = hb * HB + nt * 8 + g;
+                raw[nt][G][0] = raw[nt][G][1] = make_uint4(0, 0, 0, 0);
+                if (h < a.group && mine) {
+                    const T* src = (const T*)a.q + (int64_t)x.b * a.qb + (int64_t)(kh * a.group + h) * a.qh + 64 * G + 16 * t;
+                    raw[nt][G][0] = *reinterpret_cast<const uint4*>(src);
+                    raw[nt][G][1] = *reinterpret_cast<const uint4*>(src + 8);
+                }
+            }
     };
-    start(now);
+    step();
+    Part now = line->next;
+    look_up(now);
+    begin(now);
 
     if (a.split) {  // requests that see nothing belong to no stretch
         for (int e = blockIdx.x; e < a.B; e += gridDim.x)
@@ -280,81 +343,89 @@ __global__ void __launch_bounds__(THREADS, NT == 1 ? 2 : 1) kv4_attention_kernel
     if (blockIdx.x == 0 && warp == 0)
         for (int e = lane; e < a.B; e += 32)
             if (__ldg(a.lens + e) > a.width * a.tpp * 16) kv4::report(g_kv4_attention_status, kv4::BAD_INDEX, kv4::AT_LENGTH);
+    __syncthreads();  // `merged` is initialised
 
-    while (now.n >= 0) {
-        const int b = now.b;
-        const Seen seen(a, b);
-        const int head0 = now.kh * a.group + now.hb * HB;  // first query head of the block
-        const int heads = min(HB, a.group - now.hb * HB);
+    for (uint32_t round = 0; now.n >= 0; ++round) {
+        const Seen seen(a, now.b);
+        const int64_t now_end = line->at;  // behind this part
+        __syncwarp();
+        step();
+        look_up(line->next);
         uint32_t bad = __ballot_sync(0xffffffffu, mine && rec_now < 0);  // of a block of 32 tiles: nothing was copied
 
-        // ---- q as the B operand: the lane's elements 64 G + 16 t + 0..15 of heads g (+ 8) ----
-        uint32_t qf[NT][8 * NG];
-        float2 fac[NT], qs[NT][NG];  // of heads 2t, 2t + 1
+        // ---- q as the B operand ----
+        uint32_t qf[NT][8 * NG], qlow[NT];
+        float fac;
+        {
+            float amax = 0.f;
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt) {
-            const int h = nt * 8 + g;
-            float x[NG][16];
-            float amax = 0.f, sum[NG];
+            for (int nt = 0; nt < NT; ++nt) {
+                float sum[NG];
 #pragma unroll
-            for (int G = 0; G < NG; ++G) {
-                sum[G] = 0.f;
-                const T* src = (const T*)a.q + (int64_t)b * a.qb + (int64_t)(head0 + h) * a.qh + 64 * G + 16 * t;
-                uint4 raw[2] = {};
-                if (h < heads) {
-                    raw[0] = *reinterpret_cast<const uint4*>(src);
-                    raw[1] = *reinterpret_cast<const uint4*>(src + 8);
+                for (int G = 0; G < NG; ++G) {
+                    const uint32_t w[8] = {raw[nt][G][0].x, raw[nt][G][0].y, raw[nt][G][0].z, raw[nt][G][0].w,
+                                           raw[nt][G][1].x, raw[nt][G][1].y, raw[nt][G][1].z, raw[nt][G][1].w};
+                    float2 two = sf::f2(0.f);
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) {
+                        const float2 f = sf::Pair<T>::to_f2(w[i]);
+                        amax = fmaxf(amax, fmaxf(fabsf(f.x), fabsf(f.y)));
+                        two = sf::f2_add(two, f);
+                    }
+                    sum[G] = two.x + two.y;
+#pragma unroll
+                    for (int o = 1; o <= 2; o <<= 1) sum[G] += __shfl_xor_sync(0xffffffffu, sum[G], o);
                 }
-                const uint32_t w[8] = {raw[0].x, raw[0].y, raw[0].z, raw[0].w, raw[1].x, raw[1].y, raw[1].z, raw[1].w};
+                // Of sum(q_G), G = 0, 1, the lane's t-th bf16 part: t = 0, 1, 2 make up 24 bits.
+                float part[2] = {sum[0] * a.scale_log2, NG == 2 ? sum[NG - 1] * a.scale_log2 : 0.f};
+                qlow[nt] = 0;
 #pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    const float2 f = sf::Pair<T>::to_f2(w[i]);
-                    x[G][2 * i] = f.x;
-                    x[G][2 * i + 1] = f.y;
-                    amax = fmaxf(amax, fmaxf(fabsf(f.x), fabsf(f.y)));
-                    sum[G] += f.x + f.y;
+                for (int i = 0; i < 3; ++i) {
+                    const uint32_t w = sf::Pair<__nv_bfloat16>::from_f2(make_float2(part[0], part[1]));
+                    const float2 back = sf::Pair<__nv_bfloat16>::to_f2(w);
+                    if (t == i) qlow[nt] = w;
+                    part[0] -= back.x;
+                    part[1] -= back.y;
                 }
             }
-#pragma unroll
-            for (int o = 1; o <= 2; o <<= 1) {
-                amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
-#pragma unroll
-                for (int G = 0; G < NG; ++G) sum[G] += __shfl_xor_sync(0xffffffffu, sum[G], o);
-            }
+            amax = sf::warp_max(amax);
             // amax 2^(137 - ex) in [2^10, 2^11): times 16 it is still an fp16.
             const uint32_t ex = min(max(__float_as_uint(amax) >> 23, 10u), 244u);
             const float up = __uint_as_float((264u - ex) << 23);
+            fac = __uint_as_float((ex + 10u) << 23) * a.scale_log2;  // 2^(ex - 137) 2^20
 #pragma unroll
-            for (int G = 0; G < NG; ++G)
+            for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-                for (int h2 = 0; h2 < 2; ++h2) {
-                    const float* e = &x[G][8 * h2];
-                    uint32_t* f = &qf[nt][(2 * G + h2) * 4];
-                    f[0] = f16x2(e[0] * up * 16.f, e[4] * up * 16.f);
-                    f[1] = f16x2(e[1] * up, e[5] * up);
-                    f[2] = f16x2(e[2] * up * 16.f, e[6] * up * 16.f);
-                    f[3] = f16x2(e[3] * up, e[7] * up);
-                }
-            const float down = __uint_as_float((ex + 10u) << 23) * a.scale_log2;  // 2^(ex - 137) 2^20
-            fac[nt] = make_float2(__shfl_sync(0xffffffffu, down, 8 * t), __shfl_sync(0xffffffffu, down, 8 * t + 4));
+                for (int G = 0; G < NG; ++G)
 #pragma unroll
-            for (int G = 0; G < NG; ++G)
-                qs[nt][G] = make_float2(__shfl_sync(0xffffffffu, sum[G] * a.scale_log2, 8 * t), __shfl_sync(0xffffffffu, sum[G] * a.scale_log2, 8 * t + 4));
+                    for (int h2 = 0; h2 < 2; ++h2) {
+                        const uint4 r4 = raw[nt][G][h2];
+                        const float2 e01 = sf::Pair<T>::to_f2(r4.x), e23 = sf::Pair<T>::to_f2(r4.y), e45 = sf::Pair<T>::to_f2(r4.z),
+                                     e67 = sf::Pair<T>::to_f2(r4.w);
+                        uint32_t* f = &qf[nt][(2 * G + h2) * 4];
+                        const float up16 = up * 16.f;
+                        f[0] = f16x2(e01.x * up16, e45.x * up16);
+                        f[1] = f16x2(e01.y * up, e45.y * up);
+                        f[2] = f16x2(e23.x * up16, e67.x * up16);
+                        f[3] = f16x2(e23.y * up, e67.y * up);
+                    }
         }
 
         // O^T, heads 2t, 2t + 1, elements 64 G + 8 g + 4 i + 0..3 for i < 2: [4 G + i] whole bytes (rows g
         // and g + 8 are the lower and upper pair of elements), [4 G + 2 + i] their upper codes times 16.
         float o[NT][4 * NG][4];
-        float2 m[NT], l[NT], pm[NT][NG];
-        float2 unit[NT], per_unit[NT];  // O is in this unit, a head each; the largest p s is at most 2^8 of it
+        float2 nm[NT], l[NT], pm[NT][NG];  // minus the max that weights are relative to, their sum, sum p (minimum + 8 scale)
+        float2 unit[NT], per_unit[NT];     // O is in this unit, a head each; the largest p s is at most 2^8 of it
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
             for (int i = 0; i < 4 * NG; ++i)
 #pragma unroll
                 for (int c = 0; c < 4; ++c) o[nt][i][c] = 0.f;
-            m[nt] = sf::f2(-INFINITY);
-            l[nt] = unit[nt] = per_unit[nt] = sf::f2(0.f);
+            nm[nt] = sf::f2(-NO_MAX);
+            l[nt] = sf::f2(0.f);
+            unit[nt] = sf::f2(UNIT_FLOOR);
+            per_unit[nt] = sf::f2(1.0f / UNIT_FLOOR);
 #pragma unroll
             for (int G = 0; G < NG; ++G) pm[nt][G] = sf::f2(0.f);
         }
@@ -384,43 +455,30 @@ __global__ void __launch_bounds__(THREADS, NT == 1 ? 2 : 1) kv4_attention_kernel
             if (bad >> (k & 31) & 1u) continue;
             const uint8_t* rec = ring + (turn % ST) * R::BYTES;
 
-            // (scale, minimum) of the lane's keys `row` and `row + 8`; of the values the minimum is the
-            // centre's, minimum + 8 scale.
-            float2 kp[2][NG], vp[2][NG];
-#pragma unroll
-            for (int r = 0; r < 2; ++r) {
-                uint32_t kw[NG], vw[NG];
-                if constexpr (NG == 2) {
-                    *reinterpret_cast<uint2*>(kw) = *reinterpret_cast<const uint2*>(rec + R::KP + (row + 8 * r) * 8);
-                    *reinterpret_cast<uint2*>(vw) = *reinterpret_cast<const uint2*>(rec + R::VP + (row + 8 * r) * 8);
-                } else {
-                    kw[0] = *reinterpret_cast<const uint32_t*>(rec + R::KP + (row + 8 * r) * 4);
-                    vw[0] = *reinterpret_cast<const uint32_t*>(rec + R::VP + (row + 8 * r) * 4);
-                }
-#pragma unroll
-                for (int G = 0; G < NG; ++G) {
-                    kp[r][G] = sf::Pair<__nv_bfloat16>::to_f2(kw[G]);
-                    vp[r][G] = sf::Pair<__nv_bfloat16>::to_f2(vw[G]);
-                    vp[r][G].y = fmaf(8.f, vp[r][G].x, vp[r][G].y);
-                }
-            }
-            // S^T = K q^T, a group at a time.
-            float2 s[NT][2];  // [row, row + 8], heads 2t, 2t + 1
-            uint32_t kw[2][2 * NG];
+            // Scales and minima of the lane's keys `row` and `row + 8`.
+            uint32_t kp[2][NG], vp[2][NG], kw[2][2 * NG];
 #pragma unroll
             for (int r = 0; r < 2; ++r) {
                 const uint8_t* p = rec + R::K + (row + 8 * r) * R::ROW + t * 8 * NG;
                 if constexpr (NG == 2) {
+                    *reinterpret_cast<uint2*>(kp[r]) = *reinterpret_cast<const uint2*>(rec + R::KP + (row + 8 * r) * 8);
+                    *reinterpret_cast<uint2*>(vp[r]) = *reinterpret_cast<const uint2*>(rec + R::VP + (row + 8 * r) * 8);
                     *reinterpret_cast<uint4*>(kw[r]) = *reinterpret_cast<const uint4*>(p);
                 } else {
+                    kp[r][0] = *reinterpret_cast<const uint32_t*>(rec + R::KP + (row + 8 * r) * 4);
+                    vp[r][0] = *reinterpret_cast<const uint32_t*>(rec + R::VP + (row + 8 * r) * 4);
                     *reinterpret_cast<uint2*>(kw[r]) = *reinterpret_cast<const uint2*>(p);
                 }
             }
+            // S^T = K q^T: the minima's part, then a group at a time.
+            float s[NT][4];  // [row, row + 8] x heads 2t, 2t + 1
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt)
+                mma_bf16_k8_first(s[nt], NG == 2 ? __byte_perm(kp[0][0], kp[0][NG - 1], 0x7632) : kp[0][0] >> 16,
+                                  NG == 2 ? __byte_perm(kp[1][0], kp[1][NG - 1], 0x7632) : kp[1][0] >> 16, qlow[nt]);
 #pragma unroll
             for (int G = 0; G < NG; ++G) {
                 float acc[NT][4];
-#pragma unroll
-                for (int nt = 0; nt < NT; ++nt) acc[nt][0] = acc[nt][1] = acc[nt][2] = acc[nt][3] = 0.f;
 #pragma unroll
                 for (int h2 = 0; h2 < 2; ++h2) {
                     const uint32_t x = kw[0][2 * G + h2], y = kw[1][2 * G + h2], x8 = x >> 8, y8 = y >> 8;
@@ -429,17 +487,20 @@ __global__ void __launch_bounds__(THREADS, NT == 1 ? 2 : 1) kv4_attention_kernel
 #pragma unroll
                     for (int nt = 0; nt < NT; ++nt) {
                         const uint32_t* f = &qf[nt][(2 * G + h2) * 4];
-                        mma_f16(acc[nt], a0, f[0], f[1]);
+                        if (h2 == 0) mma_f16_first(acc[nt], a0, f[0], f[1]);
+                        else mma_f16(acc[nt], a0, f[0], f[1]);
                         mma_f16(acc[nt], a1, f[2], f[3]);
                     }
                 }
 #pragma unroll
-                for (int nt = 0; nt < NT; ++nt)
+                for (int r = 0; r < 2; ++r) {
+                    const float kf = __uint_as_float(kp[r][G] << 16) * fac;
 #pragma unroll
-                    for (int r = 0; r < 2; ++r) {
-                        const float2 low = G == 0 ? sf::f2_mul(sf::f2(kp[r][G].y), qs[nt][G]) : sf::f2_fma(sf::f2(kp[r][G].y), qs[nt][G], s[nt][r]);
-                        s[nt][r] = sf::f2_fma(make_float2(acc[nt][2 * r], acc[nt][2 * r + 1]), sf::f2_mul(sf::f2(kp[r][G].x), fac[nt]), low);
+                    for (int nt = 0; nt < NT; ++nt) {
+                        s[nt][2 * r] = fmaf(acc[nt][2 * r], kf, s[nt][2 * r]);
+                        s[nt][2 * r + 1] = fmaf(acc[nt][2 * r + 1], kf, s[nt][2 * r + 1]);
                     }
+                }
             }
             const int at_tile = warp + WARPS * k;
             if (at_tile == edge0 || at_tile == edge1 || at_tile == edge2) {
@@ -448,67 +509,82 @@ __global__ void __launch_bounds__(THREADS, NT == 1 ? 2 : 1) kv4_attention_kernel
                 for (int r = 0; r < 2; ++r) {
                     if (j + 8 * r < seen.len && (j + 8 * r >= seen.low || j + 8 * r < a.sinks)) continue;
 #pragma unroll
-                    for (int nt = 0; nt < NT; ++nt) s[nt][r] = sf::f2(-INFINITY);
+                    for (int nt = 0; nt < NT; ++nt) s[nt][2 * r] = s[nt][2 * r + 1] = -INFINITY;
 #pragma unroll
-                    for (int G = 0; G < NG; ++G) vp[r][G] = sf::f2(0.f);
+                    for (int G = 0; G < NG; ++G) vp[r][G] = 0;
                 }
             }
             // The running max follows only when a score passes it by 2^8: p stays within fp32 and fp16
             // range and the final division takes the stale max out again.  O follows through its unit.
-            bool grow = false;
+            float2 d[NT][2];
+            float over = -INFINITY;
 #pragma unroll
-            for (int nt = 0; nt < NT; ++nt) {
-                grow |= fmaxf(s[nt][0].x, s[nt][1].x) > m[nt].x + 8.f;
-                grow |= fmaxf(s[nt][0].y, s[nt][1].y) > m[nt].y + 8.f;
-            }
-            if (__any_sync(0xffffffffu, grow)) {
-#pragma unroll
-                for (int nt = 0; nt < NT; ++nt) {
-                    float2 mx = over_keys(make_float2(fmaxf(s[nt][0].x, s[nt][1].x), fmaxf(s[nt][0].y, s[nt][1].y)));
-                    mx = make_float2(fmaxf(mx.x, m[nt].x), fmaxf(mx.y, m[nt].y));
-                    const float2 f = make_float2(m[nt].x == mx.x ? 1.f : exp2f(m[nt].x - mx.x), m[nt].y == mx.y ? 1.f : exp2f(m[nt].y - mx.y));
-                    m[nt] = mx;
-                    l[nt] = sf::f2_mul(l[nt], f);
-                    unit[nt] = sf::f2_mul(unit[nt], f);
-                    per_unit[nt] = make_float2(reciprocal(unit[nt].x), reciprocal(unit[nt].y));
-#pragma unroll
-                    for (int G = 0; G < NG; ++G) pm[nt][G] = sf::f2_mul(pm[nt][G], f);
-                }
-            }
-            // p, its sum, and p s.
-            float2 w[NT][NG][2];
-            grow = false;
-#pragma unroll
-            for (int nt = 0; nt < NT; ++nt) {
-                const float2 nm = make_float2(m[nt].x == -INFINITY ? 0.f : -m[nt].x, m[nt].y == -INFINITY ? 0.f : -m[nt].y);
-                float2 top = sf::f2(0.f);
+            for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
                 for (int r = 0; r < 2; ++r) {
-                    float2 p = sf::f2_add(s[nt][r], nm);
-                    p = make_float2(sf::ex2_ftz(p.x), sf::ex2_ftz(p.y));
-                    l[nt] = sf::f2_add(l[nt], p);
-#pragma unroll
-                    for (int G = 0; G < NG; ++G) {
-                        pm[nt][G] = sf::f2_fma(p, sf::f2(vp[r][G].y), pm[nt][G]);
-                        w[nt][G][r] = sf::f2_mul(p, sf::f2(vp[r][G].x));
-                        top = make_float2(fmaxf(top.x, w[nt][G][r].x), fmaxf(top.y, w[nt][G][r].y));
-                    }
+                    d[nt][r] = sf::f2_add(make_float2(s[nt][2 * r], s[nt][2 * r + 1]), nm[nt]);
+                    over = fmaxf(over, fmaxf(d[nt][r].x, d[nt][r].y));
                 }
-                grow |= top.x > 256.f * unit[nt].x || top.y > 256.f * unit[nt].y;
-            }
-            if (__any_sync(0xffffffffu, grow)) {
+            if (__any_sync(0xffffffffu, over > 8.f)) {
 #pragma unroll
                 for (int nt = 0; nt < NT; ++nt) {
-                    float2 top = sf::f2(0.f);
+                    float2 mx = over_keys(make_float2(fmaxf(s[nt][0], s[nt][2]), fmaxf(s[nt][1], s[nt][3])));
+                    mx = make_float2(fmaxf(mx.x, -nm[nt].x), fmaxf(mx.y, -nm[nt].y));
+                    const float2 f = make_float2(exp2f(-nm[nt].x - mx.x), exp2f(-nm[nt].y - mx.y));
+                    nm[nt] = make_float2(-mx.x, -mx.y);
+                    l[nt] = sf::f2_mul(l[nt], f);
+                    unit[nt] = sf::f2_mul(unit[nt], f);
+                    // A unit that vanishes takes along what it counted.
+                    unit[nt] = make_float2(fmaxf(unit[nt].x, UNIT_FLOOR), fmaxf(unit[nt].y, UNIT_FLOOR));
+                    per_unit[nt] = make_float2(1.0f / unit[nt].x, 1.0f / unit[nt].y);
 #pragma unroll
-                    for (int G = 0; G < NG; ++G)
+                    for (int G = 0; G < NG; ++G) pm[nt][G] = sf::f2_mul(pm[nt][G], f);
 #pragma unroll
-                        for (int r = 0; r < 2; ++r) top = make_float2(fmaxf(top.x, w[nt][G][r].x), fmaxf(top.y, w[nt][G][r].y));
+                    for (int r = 0; r < 2; ++r) d[nt][r] = sf::f2_add(make_float2(s[nt][2 * r], s[nt][2 * r + 1]), nm[nt]);
+                }
+            }
+            // p, its sum, and p s in O's unit.
+            float2 x[NT][NG][2];
+            over = 0.f;
+#pragma unroll
+            for (int r = 0; r < 2; ++r) {
+                float vs[NG], vm[NG];
+#pragma unroll
+                for (int G = 0; G < NG; ++G) {
+                    vs[G] = __uint_as_float(vp[r][G] << 16);
+                    vm[G] = fmaf(8.f, vs[G], __uint_as_float(vp[r][G] & 0xFFFF0000u));
+                }
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt) {
+                    const float2 p = make_float2(sf::ex2_ftz(d[nt][r].x), sf::ex2_ftz(d[nt][r].y));
+                    l[nt] = sf::f2_add(l[nt], p);
+                    const float2 pu = sf::f2_mul(p, per_unit[nt]);
+#pragma unroll
+                    for (int G = 0; G < NG; ++G) {
+                        pm[nt][G] = make_float2(fmaf(p.x, vm[G], pm[nt][G].x), fmaf(p.y, vm[G], pm[nt][G].y));
+                        x[nt][G][r] = make_float2(pu.x * vs[G], pu.y * vs[G]);
+                        over = fmaxf(over, fmaxf(x[nt][G][r].x, x[nt][G][r].y));
+                    }
+                }
+            }
+            if (__any_sync(0xffffffffu, over > 256.f)) {
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt) {
+                    // The head's largest p s, formed without the unit (2^126 at first).
+                    float2 w[NG][2], top = sf::f2(0.f);
+#pragma unroll
+                    for (int r = 0; r < 2; ++r)
+#pragma unroll
+                        for (int G = 0; G < NG; ++G) {
+                            const float vs = __uint_as_float(vp[r][G] << 16);
+                            w[G][r] = make_float2(sf::ex2_ftz(d[nt][r].x) * vs, sf::ex2_ftz(d[nt][r].y) * vs);
+                            top = make_float2(fmaxf(top.x, w[G][r].x), fmaxf(top.y, w[G][r].y));
+                        }
                     top = over_keys(top);
-                    // Where this head's own weights fit its unit stays.
-                    const float2 u = make_float2(top.x > 256.f * unit[nt].x ? fmaxf(top.x, 0x1p-126f) : unit[nt].x,
-                                                 top.y > 256.f * unit[nt].y ? fmaxf(top.y, 0x1p-126f) : unit[nt].y);
-                    per_unit[nt] = make_float2(reciprocal(u.x), reciprocal(u.y));
+                    // Where this head's own weights fit, its unit stays.
+                    const float2 u = make_float2(top.x > 256.f * unit[nt].x ? fmaxf(top.x, UNIT_FLOOR) : unit[nt].x,
+                                                 top.y > 256.f * unit[nt].y ? fmaxf(top.y, UNIT_FLOOR) : unit[nt].y);
+                    per_unit[nt] = make_float2(1.0f / u.x, 1.0f / u.y);
                     const float2 f = sf::f2_mul(unit[nt], per_unit[nt]);
                     unit[nt] = u;
 #pragma unroll
@@ -518,19 +594,19 @@ __global__ void __launch_bounds__(THREADS, NT == 1 ? 2 : 1) kv4_attention_kernel
                         o[nt][i][2] *= f.x;
                         o[nt][i][3] *= f.y;
                     }
+#pragma unroll
+                    for (int G = 0; G < NG; ++G)
+#pragma unroll
+                        for (int r = 0; r < 2; ++r) x[nt][G][r] = sf::f2_mul(w[G][r], per_unit[nt]);
                 }
             }
-            // p s in the unit, as the B operand of O^T = V^T p^T.
-            uint32_t pf[NT][NG][2];
+            uint32_t pf[NT][NG][2];  // the B operand of O^T = V^T p^T
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
                 for (int G = 0; G < NG; ++G)
 #pragma unroll
-                    for (int r = 0; r < 2; ++r) {
-                        const float2 x = sf::f2_mul(w[nt][G][r], per_unit[nt]);
-                        pf[nt][G][r] = transpose8(f16x2(x.x, x.y));
-                    }
+                    for (int r = 0; r < 2; ++r) pf[nt][G][r] = transpose8(f16x2(x[nt][G][r].x, x[nt][G][r].y));
             // O^T += V^T p^T: the lane reads its 8 elements a group of keys t, 7 - t, 8 + t, 15 - t.
             uint32_t vw[4][NG];
 #pragma unroll
@@ -548,9 +624,9 @@ __global__ void __launch_bounds__(THREADS, NT == 1 ? 2 : 1) kv4_attention_kernel
 #pragma unroll
                 for (int i = 0; i < 2; ++i) {
                     // Elements 4 i .. 4 i + 3 (two bytes) of two keys side by side in the halves of a word.
-                    const uint32_t x = __byte_perm(vw[0][G], vw[1][G], i ? 0x7632 : 0x5410), y = __byte_perm(vw[2][G], vw[3][G], i ? 0x7632 : 0x5410);
-                    const uint32_t b[4] = {(x & 0x00FF00FFu) | 0x64006400u, __byte_perm(x, 0x64646464u, 0x4341), (y & 0x00FF00FFu) | 0x64006400u,
-                                           __byte_perm(y, 0x64646464u, 0x4341)};
+                    const uint32_t u = __byte_perm(vw[0][G], vw[1][G], i ? 0x7632 : 0x5410), w = __byte_perm(vw[2][G], vw[3][G], i ? 0x7632 : 0x5410);
+                    const uint32_t b[4] = {(u & 0x00FF00FFu) | 0x64006400u, __byte_perm(u, 0x64646464u, 0x4341), (w & 0x00FF00FFu) | 0x64006400u,
+                                           __byte_perm(w, 0x64646464u, 0x4341)};
                     uint32_t all[4], up[4];
 #pragma unroll
                     for (int c = 0; c < 4; ++c) {
@@ -565,13 +641,10 @@ __global__ void __launch_bounds__(THREADS, NT == 1 ? 2 : 1) kv4_attention_kernel
                 }
         }
         used += (uint32_t)mine;
-        const Part done = now;
-        const int64_t done_at = at;
-        __syncwarp();
-        now = next_part();
-        start(now);
 
         // ---- the warps' states side by side, then one sum over them ----
+        if (round) sm100::mbar_wait(merged, (round - 1) & 1u, g_kv4_attention_status + 1, kv4::AT_WAIT);
+        __syncwarp();
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
@@ -587,10 +660,8 @@ __global__ void __launch_bounds__(THREADS, NT == 1 ? 2 : 1) kv4_attention_kernel
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
                 const int head = nt * 8 + 2 * t + h;
-                if (g == 0) {
-                    stat_s[(warp * HB + head) * 2] = h ? m[nt].y : m[nt].x;
-                    stat_s[(warp * HB + head) * 2 + 1] = h ? l[nt].y : l[nt].x;
-                }
+                if (g == 0)
+                    *reinterpret_cast<float2*>(stat_s + (warp * HB + head) * 2) = make_float2(h ? -nm[nt].y : -nm[nt].x, h ? l[nt].y : l[nt].x);
                 float* dst = out_s + (warp * HB + head) * S::PAD + 8 * g;
 #pragma unroll
                 for (int G = 0; G < NG; ++G) {
@@ -605,30 +676,38 @@ __global__ void __launch_bounds__(THREADS, NT == 1 ? 2 : 1) kv4_attention_kernel
                 }
             }
         }
+        const Part done = now;
+        now = line->next;
+        begin(now);
         __syncthreads();
         const bool all_mine = done.n == done.whole;
+        const int kh = done.item / a.blocks, hb = done.item - kh * a.blocks;
         const int slot = 2 * blockIdx.x + (done.i0 > 0 ? 0 : 1);
         const int active = min(done.n, WARPS);  // warps that had tiles
         for (int e = threadIdx.x; e < HB * (D / 4); e += THREADS) {
             const int head = e / (D / 4), d = 4 * (e % (D / 4));
-            float mx = -INFINITY;
-            for (int w = 0; w < active; ++w) mx = fmaxf(mx, stat_s[(w * HB + head) * 2]);
-            float sum = 0.f;
+            float mx = NO_MAX, sum = 0.f, mw[WARPS];
+#pragma unroll
+            for (int w = 0; w < WARPS; ++w) {
+                mw[w] = w < active ? stat_s[(w * HB + head) * 2] : NO_MAX;
+                mx = fmaxf(mx, mw[w]);
+            }
             float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-            for (int w = 0; w < active; ++w) {
-                const float mw = stat_s[(w * HB + head) * 2];
-                const float f = mw == -INFINITY && mx != -INFINITY ? 0.f : (mw == mx ? 1.f : exp2f(mw - mx));
-                const float4 x = *reinterpret_cast<const float4*>(out_s + (w * HB + head) * S::PAD + d);
+#pragma unroll
+            for (int w = 0; w < WARPS; ++w) {
+                if (w >= active) break;
+                const float f = exp2f(mw[w] - mx);
+                const float4 y = *reinterpret_cast<const float4*>(out_s + (w * HB + head) * S::PAD + d);
                 sum = fmaf(f, stat_s[(w * HB + head) * 2 + 1], sum);
-                acc.x = fmaf(f, x.x, acc.x);
-                acc.y = fmaf(f, x.y, acc.y);
-                acc.z = fmaf(f, x.z, acc.z);
-                acc.w = fmaf(f, x.w, acc.w);
+                acc.x = fmaf(f, y.x, acc.x);
+                acc.y = fmaf(f, y.y, acc.y);
+                acc.z = fmaf(f, y.z, acc.z);
+                acc.w = fmaf(f, y.w, acc.w);
             }
             if (all_mine) {
-                if (head < heads) {
+                if (hb * HB + head < a.group) {
                     const float inv = done.n == 0 ? 0.f : 1.0f / sum;
-                    T* dst = (T*)a.o + (int64_t)b * a.ob + (int64_t)(head0 + head) * a.oh + d;
+                    T* dst = (T*)a.o + (int64_t)done.b * a.ob + (int64_t)(kh * a.group + hb * HB + head) * a.oh + d;
                     *reinterpret_cast<uint2*>(dst) = make_uint2(sf::Pair<T>::from_f2(make_float2(acc.x * inv, acc.y * inv)),
                                                                 sf::Pair<T>::from_f2(make_float2(acc.z * inv, acc.w * inv)));
                 }
@@ -639,10 +718,12 @@ __global__ void __launch_bounds__(THREADS, NT == 1 ? 2 : 1) kv4_attention_kernel
         }
         // An item that starts here and goes on in the CTAs behind is joined from here.
         if (threadIdx.x == 0 && done.i0 == 0 && !all_mine) {
-            a.chain[2 * blockIdx.x] = b * per_b + done.kh * a.blocks + done.hb;
-            a.chain[2 * blockIdx.x + 1] = (int)((done_at - done.n + done.whole - 1) / share) - blockIdx.x + 1;
+            const int64_t share = share_of();
+            a.chain[2 * blockIdx.x] = done.b * per_b + done.item;
+            a.chain[2 * blockIdx.x + 1] = (int)((now_end - done.n + done.whole - 1) / share) - blockIdx.x + 1;
         }
-        __syncthreads();
+        __syncwarp();
+        if (lane == 0) sm100::mbar_arrive(merged);
     }
 }
 
@@ -663,13 +744,12 @@ __global__ void __launch_bounds__(32 * JOIN_WARPS) kv4_join_kernel(const Args a)
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     // The first piece is its CTA's last part, the others their CTAs' first.
     auto slot = [&](int p) { return ((int64_t)2 * (first + p) + (p == 0 ? 1 : 0)) * HB + head; };
-    float m = -INFINITY, l = 0.f;
+    float m = NO_MAX, l = 0.f;
     for (int p = lane; p < pieces; p += 32) m = fmaxf(m, a.stat[slot(p) * 2]);
     m = sf::warp_max(m);
-    const float shift = m == -INFINITY ? 0.f : m;
     for (int p = lane; p < pieces; p += 32) {
         const float2 st = *reinterpret_cast<const float2*>(a.stat + slot(p) * 2);
-        l = fmaf(exp2f(st.x - shift), st.y, l);
+        l = fmaf(exp2f(st.x - m), st.y, l);
     }
     l = sf::warp_sum(l);
     float acc[E];
@@ -677,7 +757,7 @@ __global__ void __launch_bounds__(32 * JOIN_WARPS) kv4_join_kernel(const Args a)
     for (int e = 0; e < E; ++e) acc[e] = 0.f;
 #pragma unroll 4
     for (int p = warp; p < pieces; p += JOIN_WARPS) {
-        const float f = exp2f(a.stat[slot(p) * 2] - shift);
+        const float f = exp2f(a.stat[slot(p) * 2] - m);
         const float* src = a.part + slot(p) * D + E * lane;
 #pragma unroll
         for (int e = 0; e < E; ++e) acc[e] = fmaf(f, src[e], acc[e]);
