@@ -154,26 +154,31 @@ struct Layout {
 // The key tiles of a CTA: sinks [0, sink_end), then [low, high) in steps of 128.
 struct Walk {
     int sink_end, sink_tiles, low, high, n;
-    int last[2];    // position of each tile's last token (-1: no tile)
-    int first[2];   // position of each tile's first token
-    int window, sinks;
     __device__ __forceinline__ int start(int j) const { return j < sink_tiles ? 128 * j : low + 128 * (j - sink_tiles); }
-    // Keys of tile j that tile t's rows can see: [0, count).
-    __device__ __forceinline__ int count(int t, int j) const {
-        const int end = j < sink_tiles ? sink_end : min(high, last[t] + 1);
-        return max(0, min(128, end - start(j)));
+};
+
+// What one of the CTA's two row tiles makes of them.
+struct Span {
+    int first, last;  // positions of its first and last token (last < 0: no token that sees a key)
+    int skip;         // the window's first tile is left out (it ends before the tile's own window)
+    int end;          // keys below this are seen by some row
+    int front;        // keys from here on are inside every row's window
+    __device__ __forceinline__ Span(const Args& a, const Walk& w, int first_, int tokens) {
+        first = first_;
+        last = tokens > 0 ? first_ + tokens - 1 : -1;
+        end = min(w.high, last + 1);
+        front = a.window ? last - a.window + 1 : 0;
+        skip = a.window && w.low + 128 <= first - a.window + 1 && w.low >= a.sinks;
     }
-    __device__ __forceinline__ bool active(int t, int j) const {
-        if (last[t] < 0 || count(t, j) <= 0) return false;
-        if (j < sink_tiles || !window) return true;
-        const int s = start(j);
-        return s + 128 > first[t] - window + 1 || s < sinks;
+    // Keys [0, count) of tile j can be seen.
+    __device__ __forceinline__ int count(const Walk& w, int j) const { return max(0, min(128, (j < w.sink_tiles ? w.sink_end : end) - w.start(j))); }
+    __device__ __forceinline__ bool active(const Walk& w, int j) const {
+        return last >= 0 && (j < w.sink_tiles || (w.start(j) < end && !(skip && j == w.sink_tiles)));
     }
-    // Every row of tile t sees all 128 keys of tile j.
-    __device__ __forceinline__ bool full(int t, int j) const {
-        const int s = start(j);
-        if (j < sink_tiles) return s + 128 <= sink_end;
-        return s + 127 <= first[t] && (!window || s > last[t] - window || s + 128 <= sinks);
+    // Every row sees all 128 keys of tile j.
+    __device__ __forceinline__ bool full(const Walk& w, int j, int sinks) const {
+        const int s = w.start(j);
+        return j < w.sink_tiles ? s + 128 <= w.sink_end : s + 127 <= first && (s >= front || s + 128 <= sinks);
     }
 };
 
@@ -273,18 +278,12 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
     const int rows_tok[2] = {(int)min((int64_t)tq_tile, qe - tok0), (int)max((int64_t)0, min((int64_t)tq_tile, qe - tok0 - tq_tile))};
     const int pos0 = (int)((tok0 - qb) + (ke - kb) - (qe - qb));  // position of the CTA's first token
     Walk w;
-    w.window = a.window;
-    w.sinks = a.sinks;
-#pragma unroll
-    for (int t = 0; t < 2; ++t) {
-        w.first[t] = pos0 + t * tq_tile;
-        w.last[t] = rows_tok[t] ? w.first[t] + rows_tok[t] - 1 : -1;
-    }
-    w.high = max(0, max(w.last[0], w.last[1]) + 1);
+    w.high = max(0, pos0 + rows_tok[0] + rows_tok[1]);
     w.low = a.window ? max(0, pos0 - a.window + 1) : 0;
     w.sink_end = min(a.sinks, w.low);
     w.sink_tiles = (w.sink_end + 127) >> 7;
     w.n = w.high > 0 ? w.sink_tiles + ((w.high - w.low + 127) >> 7) : 0;
+    const Span span0(a, w, pos0, rows_tok[0]), span1(a, w, pos0 + tq_tile, rows_tok[1]);
 
     if (threadIdx.x == 0) {
         for (int i = 0; i < 2; ++i) {
@@ -318,11 +317,11 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
     const uint32_t tmem = bars->tmem_base;
 
     if (warp < 4) {
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 80;");
         if (warp == 0) {
             if (lane == 0 && w.n > 0) {
                 for (int t = 0; t < 2; ++t) {
-                    if (w.last[t] < 0) continue;
+                    if ((t ? span1.last : span0.last) < 0) continue;
                     sm100::mbar_arrive_expect_tx(&bars->q_full[t], DB * qrows * 128);
                     for (int b = 0; b < DB; ++b)
                         sm100::tma_load_3d(smem + L::Q + (t * DB + b) * BOX, &mq, &bars->q_full[t], 64 * b, kvh * a.group, (int)tok0 + t * tq_tile);
@@ -332,7 +331,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
                     const int st = j & 1;
                     const uint32_t ph = (uint32_t)(j >> 1) & 1u;
                     // Keys that some tile multiplies, in whole 16s.
-                    const int rows = (max(w.count(0, j), w.count(1, j)) + 15) & ~15;
+                    const int rows = (max(span0.count(w, j), span1.count(w, j)) + 15) & ~15;
                     const int key = (int)kb + w.start(j);
                     for (int kv = 0; kv < 2; ++kv) {
                         uint64_t* empty = kv ? &bars->v_empty[st] : &bars->k_empty[st];
@@ -354,7 +353,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
             fetched:
                 // No copy is in flight when the CTA ends, also after a wait that gave up.
                 for (int t = 0; t < 2; ++t)
-                    if (w.last[t] >= 0) sm100::mbar_wait(&bars->q_full[t], 0, nullptr, 0);
+                    if ((t ? span1.last : span0.last) >= 0) sm100::mbar_wait(&bars->q_full[t], 0, nullptr, 0);
                 for (int j = max(0, keys_in - 2); j < keys_in; ++j) sm100::mbar_wait(&bars->k_full[j & 1], (uint32_t)(j >> 1) & 1u, nullptr, 0);
                 for (int j = max(0, values_in - 2); j < values_in; ++j) sm100::mbar_wait(&bars->v_full[j & 1], (uint32_t)(j >> 1) & 1u, nullptr, 0);
             }
@@ -362,47 +361,59 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
             if (lane == 0 && w.n > 0) {
                 constexpr uint32_t idesc_s = sm100::idesc_f16(128, 0, BF16);
                 constexpr uint32_t idesc_o = sm100::idesc_f16_bmn(128, D, BF16);
-                uint32_t turns[2] = {0, 0};  // tiles of P consumed
+                const uint64_t dq = sm100::smem_desc_k_sw128(sm100::smem_u32(smem + L::Q)), dk = sm100::smem_desc_k_sw128(sm100::smem_u32(smem + L::K)),
+                               dv = sm100::smem_desc_mn_sw128(sm100::smem_u32(smem + L::V), BOX, 1024);
+                constexpr uint32_t NEXT = L::TILE >> 4;  // from one tile to the next in a descriptor's address field
+                uint32_t turns0 = 0, turns1 = 0;         // tiles of P consumed
                 bool ok = true;
-                for (int j = 0; j <= w.n && ok; ++j) {
-                    for (int t = 0; t < 2 && ok; ++t) {
-                        if (j > 0 && w.active(t, j - 1)) {
-                            // O_t += P_t(j-1) . V(j-1), each half of the keys when its P is there.
-                            const int st = (j - 1) & 1;
-                            ok = sm100::mbar_wait(&bars->v_ready[st], (uint32_t)((j - 1) >> 1) & 1u, status, 122);
-                            const uint32_t sv = sm100::smem_u32(smem + L::V + st * L::TILE);
-                            const int steps = (w.count(t, j - 1) + 15) >> 4;
-                            for (int h = 0; h < 2 && ok; ++h) {
-                                ok = sm100::mbar_wait(&bars->p_full[t][h], turns[t] & 1u, status, 123);
-                                sm100::tc_fence_after();
-                                for (int kk = 4 * h; kk < min(steps, 4 * h + 4) && ok; ++kk)
-                                    sm100::mma_f16_ta(tmem + O_COL + 128u * t, tmem + 128u * t + (uint32_t)(32 * (kk >> 1) + 8 * (kk & 1)),
-                                                      sm100::smem_desc_mn_sw128(sv + (uint32_t)(kk * 16 * 128), BOX, 1024), idesc_o,
-                                                      turns[t] > 0 || kk > 0 ? 1u : 0u);
-                            }
-                            ++turns[t];
-                            if (ok && (t == 1 || !w.active(1, j - 1))) sm100::mma_commit(&bars->v_empty[st]);
-                        }
-                        if (ok && j < w.n && w.active(t, j)) {
-                            // S_t(j) = Q_t . K(j)^T over the columns that P_t(j-1) was read from (the pipe runs
-                            // this thread's products in order).
-                            const int st = j & 1;
-                            if (turns[t] == 0) ok = sm100::mbar_wait(&bars->q_full[t], 0, status, 124);
-                            ok = ok && sm100::mbar_wait(&bars->k_full[st], (uint32_t)(j >> 1) & 1u, status, 125);
-                            if (!ok) break;
-                            sm100::tc_fence_after();
-                            const uint32_t sq = sm100::smem_u32(smem + L::Q + t * L::TILE), sk = sm100::smem_u32(smem + L::K + st * L::TILE);
-                            const uint32_t n16 = (uint32_t)((w.count(t, j) + 15) & ~15);
+                // O_t += P_t(j) . V(j), each half of the keys when its P is there.
+                auto pv = [&](int t, const Span& sp, int j, uint32_t& turn, bool last_user) {
+                    const int st = j & 1;
+                    ok = ok && sm100::mbar_wait(&bars->v_ready[st], (uint32_t)(j >> 1) & 1u, status, 122);
+                    const int steps = (sp.count(w, j) + 15) >> 4;
+                    const uint64_t d = dv + st * NEXT;
+                    const uint32_t to = tmem + O_COL + 128u * t, tp = tmem + 128u * t;
 #pragma unroll
-                            for (int k = 0; k < D / 16; ++k) {
-                                const uint32_t off = (uint32_t)((k >> 2) * BOX + (k & 3) * 32);
-                                sm100::mma_f16(tmem + 128u * t, sm100::smem_desc_k_sw128(sq + off), sm100::smem_desc_k_sw128(sk + off),
-                                               idesc_s | ((n16 >> 3) << 17), k > 0 ? 1u : 0u);
-                            }
-                            sm100::mma_commit(&bars->s_full[t]);
-                            if (t == 1 || !w.active(1, j)) sm100::mma_commit(&bars->k_empty[st]);
-                        }
+                    for (int h = 0; h < 2; ++h) {
+                        ok = ok && sm100::mbar_wait(&bars->p_full[t][h], turn & 1u, status, 123);
+                        if (!ok) return;
+                        sm100::tc_fence_after();
+#pragma unroll
+                        for (int kk = 4 * h; kk < 4 * h + 4; ++kk)
+                            if (kk < steps)
+                                sm100::mma_f16_ta(to, tp + (uint32_t)(32 * (kk >> 1) + 8 * (kk & 1)), d + kk * (16 * 128 >> 4), idesc_o,
+                                                  kk > 0 ? 1u : (turn > 0 ? 1u : 0u));
                     }
+                    ++turn;
+                    if (last_user) sm100::mma_commit(&bars->v_empty[st]);
+                };
+                // S_t(j) = Q_t . K(j)^T over the columns that P_t was read from (the pipe runs this thread's
+                // products in order).
+                auto qk = [&](int t, const Span& sp, int j, uint32_t turn, bool last_user) {
+                    const int st = j & 1;
+                    if (turn == 0) ok = ok && sm100::mbar_wait(&bars->q_full[t], 0, status, 124);
+                    ok = ok && sm100::mbar_wait(&bars->k_full[st], (uint32_t)(j >> 1) & 1u, status, 125);
+                    if (!ok) return;
+                    sm100::tc_fence_after();
+                    const uint32_t n16 = (uint32_t)((sp.count(w, j) + 15) & ~15);
+                    const uint64_t da = dq + t * NEXT, db = dk + st * NEXT;
+#pragma unroll
+                    for (int k = 0; k < D / 16; ++k) {
+                        const uint32_t off = (uint32_t)((k >> 2) * BOX + (k & 3) * 32) >> 4;
+                        sm100::mma_f16(tmem + 128u * t, da + off, db + off, idesc_s | ((n16 >> 3) << 17), k > 0 ? 1u : 0u);
+                    }
+                    sm100::mma_commit(&bars->s_full[t]);
+                    if (last_user) sm100::mma_commit(&bars->k_empty[st]);
+                };
+                bool was0 = false, was1 = false;
+                for (int j = 0; j <= w.n && ok; ++j) {
+                    const bool now0 = j < w.n && span0.active(w, j), now1 = j < w.n && span1.active(w, j);
+                    if (was0) pv(0, span0, j - 1, turns0, !was1);
+                    if (ok && now0) qk(0, span0, j, turns0, !now1);
+                    if (ok && was1) pv(1, span1, j - 1, turns1, true);
+                    if (ok && now1) qk(1, span1, j, turns1, true);
+                    was0 = now0;
+                    was1 = now1;
                 }
                 // Also after a wait that gave up: the tensor pipe drains before TMEM is freed.
                 sm100::mma_commit(&bars->o_done[0]);
@@ -412,7 +423,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
             for (int j = 0; j < w.n; ++j) {
                 const int st = j & 1;
                 if (!__all_sync(0xffffffffu, sm100::mbar_wait(&bars->v_full[st], (uint32_t)(j >> 1) & 1u, status, 126))) break;
-                const int rows = (max(w.count(0, j), w.count(1, j)) + 15) & ~15;
+                const int rows = (max(span0.count(w, j), span1.count(w, j)) + 15) & ~15;
                 const int real = (int)min((int64_t)rows, ke - kb - w.start(j));
                 for (int i = lane; i < DB * (rows - real) * 8; i += 32) {
                     const int b = i / ((rows - real) * 8), rest = i % ((rows - real) * 8);
@@ -423,12 +434,13 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
             }
         }
     } else {
-        asm volatile("setmaxnreg.inc.sync.aligned.u32 224;");
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
         const int t = (warp >> 2) - 1;
         const int row = (warp & 3) * 32 + lane;
         const int tok = row / a.group, head = kvh * a.group + row - tok * a.group;
         const int n_tok = t ? rows_tok[1] : rows_tok[0];
-        const int first = t ? w.first[1] : w.first[0];
+        const Span span = t ? span1 : span0;
+        const int first = span.first;
         const bool live = row < qrows && tok < n_tok;
         const int p = live ? first + tok : -1;
         const uint32_t lane_off = (uint32_t)((warp & 3) * 32) << 16;
@@ -437,14 +449,14 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
         uint32_t turn = 0;
         bool ok = true;
         for (int j = 0; j < w.n; ++j) {
-            if (!w.active(t, j)) continue;
+            if (!span.active(w, j)) continue;
             if (!sm100::mbar_wait(&bars->s_full[t], turn & 1u, status, 127)) {
                 ok = false;
                 break;
             }
             sm100::tc_fence_after();
             float2 acc[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
-            if (w.full(t, j)) {
+            if (span.full(w, j, a.sinks)) {
                 uint32_t r[128];
 #pragma unroll
                 for (int c = 0; c < 4; ++c) sm100::tmem_ld_32x32b_x32(ts + 32u * c, *reinterpret_cast<uint32_t(*)[32]>(&r[32 * c]));
@@ -471,7 +483,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
                 const int end = in_sinks ? (p >= 0 ? w.sink_end - start : 0) : p + 1 - start;
                 const int begin = in_sinks || !a.window ? 0 : p - a.window + 1 - start;
                 const int sink = a.sinks - start;
-                const int chunks = (((w.count(t, j) + 15) & ~15) + 31) >> 5;
+                const int chunks = (((span.count(w, j) + 15) & ~15) + 31) >> 5;
                 float mx = -INFINITY;
 #pragma unroll 1
                 for (int c = 0; c < chunks; ++c) {
