@@ -113,7 +113,10 @@ __global__ void __launch_bounds__(128) window_general_kernel(const Args a, int D
 // (each key and value tile is fetched once for 256 rows) and owns an SM:
 //   warp 0        TMA producer: both Q tiles, then K_j and V_j tiles of up to 128 keys, two slots each;
 //   warp 1        MMA issuer, in the order P0.V(j-1), S0(j), P1.V(j-1), S1(j): one tile's products run
-//                 under the other's softmax; S (then P over it) and O of both tiles fill TMEM;
+//                 under the other's softmax; S (then P over it) and O of both tiles fill TMEM.  (An
+//                 issuer a tile let both tiles wait, then compute, at the same time: 498 against 402 us
+//                 at 16384 tokens, window 4096, 16 heads on 2.)  Its operands are kept uniform over the
+//                 warp: issued from one divergent lane a product cost ~130 cycles against the pipe's 64;
 //   warp 2        zeroes the value rows behind a sequence's last key (0 times another sequence's NaN or
 //                 infinity would be NaN) and hands the tile on;
 //   warps 4..7    softmax of tile 0, a thread a row; warps 8..11 of tile 1.
@@ -128,6 +131,7 @@ __global__ void __launch_bounds__(128) window_general_kernel(const Args a, int D
 
 constexpr int BOX = 128 * 128;       // 128 rows of 64 16-bit elements
 constexpr int TC_THREADS = 384;
+constexpr int FIRST_KEYS = 96;       // keys of a tile whose P is handed over first, then the rest
 constexpr uint32_t O_COL = 256;      // S / P of tile t at column 128 t, O at 256 + 128 t
 
 __device__ sm100::KernelStatus g_window_status;
@@ -151,6 +155,10 @@ struct Layout {
     static constexpr int BYTES = BARS + 256;
 };
 
+// A value that all lanes share, told to the compiler: what is computed from it, loops and branches
+// included, can run on the uniform datapath, where the tensor instructions take their operands from.
+__device__ __forceinline__ int uniform(int x) { return __shfl_sync(0xffffffffu, x, 0); }
+
 // The key tiles of a CTA: sinks [0, sink_end), then [low, high) in steps of 128.
 struct Walk {
     int sink_end, sink_tiles, low, high, n;
@@ -168,7 +176,7 @@ struct Span {
         last = tokens > 0 ? first_ + tokens - 1 : -1;
         end = min(w.high, last + 1);
         front = a.window ? last - a.window + 1 : 0;
-        skip = a.window && w.low + 128 <= first - a.window + 1 && w.low >= a.sinks;
+        skip = a.window && last >= 0 && w.low + 128 <= first - a.window + 1 && w.low >= a.sinks ? 1 : 0;
     }
     // Keys [0, count) of tile j can be seen.
     __device__ __forceinline__ int count(const Walk& w, int j) const { return max(0, min(128, (j < w.sink_tiles ? w.sink_end : end) - w.start(j))); }
@@ -189,6 +197,60 @@ __device__ __forceinline__ float max3_nan(float a, float b, float c) {
     float d;
     asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
     return d;
+}
+
+// The products' tcgen05.mma, issued by the one lane with `lead`, as predicated instructions of a warp that
+// runs together: descriptors and addresses then stay in uniform registers, and several go into one block
+// that forms the predicate once.  A descriptor is given as its two words; offsets go onto the address
+// field of the lower one.
+#define SF_DESC(reg, lo, hi, off) "add.u32 x, " lo ", " off ";\nmov.b64 " reg ", {x, " hi "};\n"
+#define SF_QK_STEP(off, acc) SF_DESC("da", "%1", "%2", off) SF_DESC("db", "%3", "%4", off) "@q tcgen05.mma.cta_group::1.kind::f16 [%0], da, db, %5, " acc ";\n"
+#define SF_QK_BEGIN "{\n.reg .pred p, f, q;\n.reg .b32 x;\n.reg .b64 da, db;\nsetp.ne.b32 q, %6, 0;\nsetp.eq.b32 p, %6, %6;\nsetp.ne.b32 f, %6, %6;\n"
+#define SF_QK_ARGS(d, a, b, idesc, lead) \
+    "r"(d), "r"((uint32_t)(a)), "r"((uint32_t)((a) >> 32)), "r"((uint32_t)(b)), "r"((uint32_t)((b) >> 32)), "r"(idesc), "r"(lead)
+// S = Q . K^T, D / 16 products; in a tile of 128 rows 16 elements of D are 2 on in the address field, 64 are a box.
+template <int D>
+__device__ __forceinline__ void issue_qk(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t lead) {
+    if constexpr (D == 128) {
+        asm volatile(SF_QK_BEGIN SF_QK_STEP("0", "f") SF_QK_STEP("2", "p") SF_QK_STEP("4", "p") SF_QK_STEP("6", "p") SF_QK_STEP("1024", "p")
+                         SF_QK_STEP("1026", "p") SF_QK_STEP("1028", "p") SF_QK_STEP("1030", "p") "}\n" ::SF_QK_ARGS(d, a, b, idesc, lead)
+                     : "memory");
+    } else {
+        asm volatile(SF_QK_BEGIN SF_QK_STEP("0", "f") SF_QK_STEP("2", "p") SF_QK_STEP("4", "p") SF_QK_STEP("6", "p") "}\n" ::SF_QK_ARGS(d, a, b, idesc, lead)
+                     : "memory");
+    }
+}
+// O += P . V over 32 keys (P of 32 keys lies in 16 columns of every 32, 16 keys of V are 128 on) or over 16.
+#define SF_PV_STEP(col, off, acc) "add.u32 y, %1, " col ";\n" SF_DESC("db", "%2", "%3", off) "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [y], db, %4, " acc ";\n"
+__device__ __forceinline__ void issue_pv32(uint32_t d, uint32_t p, uint64_t v, uint32_t idesc, uint32_t accumulate, uint32_t lead) {
+    asm volatile("{\n.reg .pred p, f, q;\n.reg .b32 x, y;\n.reg .b64 db;\nsetp.ne.b32 q, %6, 0;\nsetp.eq.b32 p, %6, %6;\nsetp.ne.b32 f, %5, 0;\n" SF_PV_STEP(
+                     "0", "0", "f") SF_PV_STEP("8", "128", "p") "}\n" ::"r"(d),
+                 "r"(p), "r"((uint32_t)v), "r"((uint32_t)(v >> 32)), "r"(idesc), "r"(accumulate), "r"(lead)
+                 : "memory");
+}
+__device__ __forceinline__ void issue_pv16(uint32_t d, uint32_t p, uint64_t v, uint32_t idesc, uint32_t accumulate, uint32_t lead) {
+    asm volatile("{\n.reg .pred f, q;\n.reg .b32 x, y;\n.reg .b64 db;\nsetp.ne.b32 q, %6, 0;\nsetp.ne.b32 f, %5, 0;\n" SF_PV_STEP("0", "0", "f") "}\n" ::"r"(d),
+                 "r"(p), "r"((uint32_t)v), "r"((uint32_t)(v >> 32)), "r"(idesc), "r"(accumulate), "r"(lead)
+                 : "memory");
+}
+__device__ __forceinline__ void commit(uint64_t* bar, uint32_t lead) {
+    asm volatile(
+        "{\n"
+        ".reg .pred q;\n"
+        "setp.ne.b32 q, %1, 0;\n"
+        "@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n"
+        "}\n" ::"r"(sm100::smem_u32(bar)),
+        "r"(lead)
+        : "memory");
+}
+
+// mbar_wait for the hand-overs between products and softmax: reading the clock for the time limit costs some
+// hundred cycles, so it begins only after waits that together outlast any product.
+__device__ __forceinline__ bool wait_soon(uint64_t* bar, uint32_t parity, sm100::KernelStatus* st, uint32_t where) {
+#pragma unroll 1
+    for (int i = 0; i < 256; ++i)
+        if (sm100::mbar_try_wait(bar, parity)) return true;
+    return sm100::mbar_wait(bar, parity, st, where);
 }
 
 // Running state of a row: `m` the max that weights are relative to (log2 units), `l` their sum.
@@ -253,7 +315,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
     Bars* bars = reinterpret_cast<Bars*>(smem + L::BARS);
     sm100::KernelStatus* status = &g_window_status;
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int warp = uniform(threadIdx.x >> 5), lane = threadIdx.x & 31;
     const int kvh = blockIdx.y;
 
     // ---- which tokens: sequence i owns the slots from cu[i] / TT + i on, later tiles (more keys) first ----
@@ -275,11 +337,11 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
     bounds(a.cu_k, lo, a.tk, &kb, &ke);
     const int64_t tok0 = qb + (int64_t)(slot - (int)(qb / TT) - lo) * TT;
     if (tok0 < qb || tok0 >= qe) return;
-    const int rows_tok[2] = {(int)min((int64_t)tq_tile, qe - tok0), (int)max((int64_t)0, min((int64_t)tq_tile, qe - tok0 - tq_tile))};
-    const int pos0 = (int)((tok0 - qb) + (ke - kb) - (qe - qb));  // position of the CTA's first token
+    const int rows_tok[2] = {uniform((int)min((int64_t)tq_tile, qe - tok0)), uniform((int)max((int64_t)0, min((int64_t)tq_tile, qe - tok0 - tq_tile)))};
+    const int pos0 = uniform((int)((tok0 - qb) + (ke - kb) - (qe - qb)));  // position of the CTA's first token
     Walk w;
-    w.high = max(0, pos0 + rows_tok[0] + rows_tok[1]);
-    w.low = a.window ? max(0, pos0 - a.window + 1) : 0;
+    w.high = uniform(max(0, pos0 + rows_tok[0] + rows_tok[1]));
+    w.low = uniform(a.window ? max(0, pos0 - a.window + 1) : 0);
     w.sink_end = min(a.sinks, w.low);
     w.sink_tiles = (w.sink_end + 127) >> 7;
     w.n = w.high > 0 ? w.sink_tiles + ((w.high - w.low + 127) >> 7) : 0;
@@ -314,7 +376,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
     sm100::tc_fence_before();
     __syncthreads();
     sm100::tc_fence_after();
-    const uint32_t tmem = bars->tmem_base;
+    const uint32_t tmem = uniform(bars->tmem_base);
 
     if (warp < 4) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 80;");
@@ -358,66 +420,98 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
                 for (int j = max(0, values_in - 2); j < values_in; ++j) sm100::mbar_wait(&bars->v_full[j & 1], (uint32_t)(j >> 1) & 1u, nullptr, 0);
             }
         } else if (warp == 1) {
-            if (lane == 0 && w.n > 0) {
+            if (w.n > 0) {
+                const uint32_t lead = sm100::elect_one();
                 constexpr uint32_t idesc_s = sm100::idesc_f16(128, 0, BF16);
                 constexpr uint32_t idesc_o = sm100::idesc_f16_bmn(128, D, BF16);
+                constexpr uint32_t NEXT = L::TILE >> 4;  // from one tile to the next in a descriptor's address field
                 const uint64_t dq = sm100::smem_desc_k_sw128(sm100::smem_u32(smem + L::Q)), dk = sm100::smem_desc_k_sw128(sm100::smem_u32(smem + L::K)),
                                dv = sm100::smem_desc_mn_sw128(sm100::smem_u32(smem + L::V), BOX, 1024);
-                constexpr uint32_t NEXT = L::TILE >> 4;  // from one tile to the next in a descriptor's address field
-                uint32_t turns0 = 0, turns1 = 0;         // tiles of P consumed
+                // The lanes wait each for itself and agree once a step on whether a wait gave up.
                 bool ok = true;
-                // O_t += P_t(j) . V(j), each half of the keys when its P is there.
-                auto pv = [&](int t, const Span& sp, int j, uint32_t& turn, bool last_user) {
-                    const int st = j & 1;
-                    ok = ok && sm100::mbar_wait(&bars->v_ready[st], (uint32_t)(j >> 1) & 1u, status, 122);
-                    const int steps = (sp.count(w, j) + 15) >> 4;
-                    const uint64_t d = dv + st * NEXT;
+                auto wait = [&](uint64_t* bar, uint32_t parity, uint32_t where) { ok &= wait_soon(bar, parity, status, where); };
+                // O_t += P_t(j) . V(j) over `keys` keys, the first of them as soon as their P is there.
+                auto pv = [&](int t, int j, int keys, uint32_t turn) {
+                    const uint64_t d = dv + (j & 1) * NEXT;
                     const uint32_t to = tmem + O_COL + 128u * t, tp = tmem + 128u * t;
-#pragma unroll
+#pragma unroll 1
                     for (int h = 0; h < 2; ++h) {
-                        ok = ok && sm100::mbar_wait(&bars->p_full[t][h], turn & 1u, status, 123);
-                        if (!ok) return;
+                        wait(&bars->p_full[t][h], turn & 1u, 123);
+                        __syncwarp();
                         sm100::tc_fence_after();
-#pragma unroll
-                        for (int kk = 4 * h; kk < 4 * h + 4; ++kk)
-                            if (kk < steps)
-                                sm100::mma_f16_ta(to, tp + (uint32_t)(32 * (kk >> 1) + 8 * (kk & 1)), d + kk * (16 * 128 >> 4), idesc_o,
-                                                  kk > 0 ? 1u : (turn > 0 ? 1u : 0u));
+                        const int steps = min((keys + 15) >> 4, h ? 8 : FIRST_KEYS / 16);
+#pragma unroll 1
+                        for (int kk = h ? FIRST_KEYS / 16 : 0; kk < steps; ++kk)
+                            issue_pv16(to, tp + (uint32_t)(32 * (kk >> 1) + 8 * (kk & 1)), d + kk * 128, idesc_o, kk > 0 || turn > 0 ? 1u : 0u, lead);
                     }
-                    ++turn;
-                    if (last_user) sm100::mma_commit(&bars->v_empty[st]);
                 };
                 // S_t(j) = Q_t . K(j)^T over the columns that P_t was read from (the pipe runs this thread's
                 // products in order).
-                auto qk = [&](int t, const Span& sp, int j, uint32_t turn, bool last_user) {
-                    const int st = j & 1;
-                    if (turn == 0) ok = ok && sm100::mbar_wait(&bars->q_full[t], 0, status, 124);
-                    ok = ok && sm100::mbar_wait(&bars->k_full[st], (uint32_t)(j >> 1) & 1u, status, 125);
-                    if (!ok) return;
-                    sm100::tc_fence_after();
-                    const uint32_t n16 = (uint32_t)((sp.count(w, j) + 15) & ~15);
-                    const uint64_t da = dq + t * NEXT, db = dk + st * NEXT;
-#pragma unroll
-                    for (int k = 0; k < D / 16; ++k) {
-                        const uint32_t off = (uint32_t)((k >> 2) * BOX + (k & 3) * 32) >> 4;
-                        sm100::mma_f16(tmem + 128u * t, da + off, db + off, idesc_s | ((n16 >> 3) << 17), k > 0 ? 1u : 0u);
-                    }
-                    sm100::mma_commit(&bars->s_full[t]);
-                    if (last_user) sm100::mma_commit(&bars->k_empty[st]);
+                auto qk = [&](int t, int j, int keys) {
+                    issue_qk<D>(tmem + 128u * t, dq + t * NEXT, dk + (j & 1) * NEXT, idesc_s | ((uint32_t)((keys + 15) >> 4) << 18), lead);
+                    commit(&bars->s_full[t], lead);
                 };
-                bool was0 = false, was1 = false;
-                for (int j = 0; j <= w.n && ok; ++j) {
-                    const bool now0 = j < w.n && span0.active(w, j), now1 = j < w.n && span1.active(w, j);
-                    if (was0) pv(0, span0, j - 1, turns0, !was1);
-                    if (ok && now0) qk(0, span0, j, turns0, !now1);
-                    if (ok && was1) pv(1, span1, j - 1, turns1, true);
-                    if (ok && now1) qk(1, span1, j, turns1, true);
-                    was0 = now0;
-                    was1 = now1;
+                // A step between two tiles of 128 keys for both row tiles, key tile j in slot ST: nothing to
+                // decide, since every instruction here is on the way from one softmax to the next.
+                uint32_t turns0 = 0, turns1 = 0;  // tiles of P consumed
+                auto whole_step = [&](auto slot, uint32_t k_parity, uint32_t v_parity) {
+                    constexpr int ST = decltype(slot)::value;
+                    const uint64_t v = dv + (1 - ST) * NEXT, k = dk + ST * NEXT;
+                    constexpr uint32_t idesc = sm100::idesc_f16(128, 128, BF16);
+                    wait(&bars->v_ready[1 - ST], v_parity, 122);
+                    wait(&bars->k_full[ST], k_parity, 125);
+#pragma unroll
+                    for (int t = 0; t < 2; ++t) {
+                        const uint32_t turn = t ? turns1 : turns0, to = tmem + O_COL + 128u * t, tp = tmem + 128u * t;
+#pragma unroll
+                        for (int h = 0; h < 2; ++h) {
+                            wait(&bars->p_full[t][h], turn & 1u, 123);
+                            __syncwarp();
+                            sm100::tc_fence_after();
+#pragma unroll
+                            for (int c = h ? FIRST_KEYS / 32 : 0; c < (h ? 4 : FIRST_KEYS / 32); ++c)
+                                issue_pv32(to, tp + 32u * c, v + 256 * c, idesc_o, c > 0 || turn > 0 ? 1u : 0u, lead);
+                        }
+                        if (t == 1) commit(&bars->v_empty[1 - ST], lead);
+                        issue_qk<D>(tp, dq + t * NEXT, k, idesc, lead);
+                        commit(&bars->s_full[t], lead);
+                    }
+                    commit(&bars->k_empty[ST], lead);
+                    ++turns0;
+                    ++turns1;
+                };
+                // Tiles [whole0, whole1) have 128 keys for both.
+                const int whole0 = w.sink_tiles + (span0.skip | span1.skip), whole1 = span0.last >= 0 && span1.last >= 0 ? w.sink_tiles + (min(span0.end, span1.end) - w.low) / 128 : 0;
+                if (span0.last >= 0) wait(&bars->q_full[0], 0, 124);
+                if (span1.last >= 0) wait(&bars->q_full[1], 0, 124);
+                int keys0 = 0, keys1 = 0;         // of tile j - 1, 0: it is not for that row tile
+                for (int j = 0; j <= w.n; ++j) {
+                    const int next0 = j < w.n && span0.active(w, j) ? span0.count(w, j) : 0, next1 = j < w.n && span1.active(w, j) ? span1.count(w, j) : 0;
+                    if (j > 0) wait(&bars->v_ready[(j - 1) & 1], (uint32_t)((j - 1) >> 1) & 1u, 122);
+                    if (keys0) pv(0, j - 1, keys0, turns0++);
+                    if (j < w.n) wait(&bars->k_full[j & 1], (uint32_t)(j >> 1) & 1u, 125);
+                    __syncwarp();
+                    sm100::tc_fence_after();
+                    if (next0) qk(0, j, next0);
+                    if (keys1) pv(1, j - 1, keys1, turns1++);
+                    if (j > 0) commit(&bars->v_empty[(j - 1) & 1], lead);
+                    if (next1) qk(1, j, next1);
+                    if (j < w.n) commit(&bars->k_empty[j & 1], lead);
+                    keys0 = next0;
+                    keys1 = next1;
+                    if (__any_sync(0xffffffffu, !ok)) break;
+                    if (j >= whole0 && j + 1 < whole1) {
+#pragma unroll 1
+                        while (j + 1 < whole1 && !__any_sync(0xffffffffu, !ok)) {
+                            ++j;
+                            if (j & 1) whole_step(std::integral_constant<int, 1>{}, (uint32_t)(j >> 1) & 1u, (uint32_t)((j - 1) >> 1) & 1u);
+                            else whole_step(std::integral_constant<int, 0>{}, (uint32_t)(j >> 1) & 1u, (uint32_t)((j - 1) >> 1) & 1u);
+                        }
+                    }
                 }
                 // Also after a wait that gave up: the tensor pipe drains before TMEM is freed.
-                sm100::mma_commit(&bars->o_done[0]);
-                sm100::mma_commit(&bars->o_done[1]);
+                commit(&bars->o_done[0], lead);
+                commit(&bars->o_done[1], lead);
             }
         } else if (warp == 2) {
             for (int j = 0; j < w.n; ++j) {
@@ -450,14 +544,14 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
         bool ok = true;
         for (int j = 0; j < w.n; ++j) {
             if (!span.active(w, j)) continue;
-            if (!sm100::mbar_wait(&bars->s_full[t], turn & 1u, status, 127)) {
+            if (!wait_soon(&bars->s_full[t], turn & 1u, status, 127)) {
                 ok = false;
                 break;
             }
             sm100::tc_fence_after();
             float2 acc[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+            uint32_t r[128];
             if (span.full(w, j, a.sinks)) {
-                uint32_t r[128];
 #pragma unroll
                 for (int c = 0; c < 4; ++c) sm100::tmem_ld_32x32b_x32(ts + 32u * c, *reinterpret_cast<uint32_t(*)[32]>(&r[32 * c]));
                 sm100::tmem_ld_wait();
@@ -470,43 +564,41 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
                     uint32_t pw[16];
                     weights32<T>(r + 32 * c, a.scale_log2, m, acc, pw);
                     sm100::tmem_st_32x32b_x16(ts + 32u * c, pw);
-                    if (c & 1) {
+                    if (c == FIRST_KEYS / 32 - 1 || c == 3) {
                         sm100::tmem_st_wait();
                         sm100::tc_fence_before();
-                        sm100::mbar_arrive(&bars->p_full[t][c >> 1]);
+                        sm100::mbar_arrive(&bars->p_full[t][c == 3]);
                     }
                 }
             } else {
-                // Column c of the tile is seen when c < end and (c >= begin or c < sink).
+                // 32 columns at a time, as many as the tile has.  Column c of the tile is seen when c < end
+                // and (c >= begin or c < sink).
+                const int chunks = (span.count(w, j) + 31) >> 5;
                 const int start = w.start(j);
                 const bool in_sinks = j < w.sink_tiles;
                 const int end = in_sinks ? (p >= 0 ? w.sink_end - start : 0) : p + 1 - start;
                 const int begin = in_sinks || !a.window ? 0 : p - a.window + 1 - start;
                 const int sink = a.sinks - start;
-                const int chunks = (((span.count(w, j) + 15) & ~15) + 31) >> 5;
+#pragma unroll
+                for (int c = 0; c < 4; ++c)
+                    if (c < chunks) sm100::tmem_ld_32x32b_x32(ts + 32u * c, *reinterpret_cast<uint32_t(*)[32]>(&r[32 * c]));
+                sm100::tmem_ld_wait();
                 float mx = -INFINITY;
-#pragma unroll 1
-                for (int c = 0; c < chunks; ++c) {
-                    uint32_t r[32];
-                    sm100::tmem_ld_32x32b_x32(ts + 32u * c, r);
-                    sm100::tmem_ld_wait();
+#pragma unroll
+                for (int c = 0; c < 4; ++c) {
+                    if (c >= chunks) continue;
                     const uint32_t seen = below(end - 32 * c) & (~below(begin - 32 * c) | below(sink - 32 * c));
 #pragma unroll
                     for (int i = 0; i < 32; ++i)
-                        if (!(seen >> i & 1u)) r[i] = 0xff800000u;
-                    mx = max32(r, mx);
+                        if (!(seen >> i & 1u)) r[32 * c + i] = 0xff800000u;
+                    mx = max32(r + 32 * c, mx);
                 }
                 const float m = s.raise<D>(mx, a.scale_log2, to, turn > 0);
-#pragma unroll 1
-                for (int c = 0; c < chunks; ++c) {
-                    uint32_t r[32], pw[16];
-                    sm100::tmem_ld_32x32b_x32(ts + 32u * c, r);
-                    sm100::tmem_ld_wait();
-                    const uint32_t seen = below(end - 32 * c) & (~below(begin - 32 * c) | below(sink - 32 * c));
 #pragma unroll
-                    for (int i = 0; i < 32; ++i)
-                        if (!(seen >> i & 1u)) r[i] = 0xff800000u;
-                    weights32<T>(r, a.scale_log2, m, acc, pw);
+                for (int c = 0; c < 4; ++c) {
+                    if (c >= chunks) continue;
+                    uint32_t pw[16];
+                    weights32<T>(r + 32 * c, a.scale_log2, m, acc, pw);
                     sm100::tmem_st_32x32b_x16(ts + 32u * c, pw);
                 }
                 sm100::tmem_st_wait();
