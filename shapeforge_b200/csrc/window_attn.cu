@@ -126,8 +126,8 @@ __global__ void __launch_bounds__(128) window_general_kernel(const Args a, int D
 // mask.  Running max and sum in fp32; the max follows a score only past 2^8, so O is rarely rescaled.
 // P is rounded to the tensors' type (as the fp32 sum of the unrounded weights divides it, a weight is off
 // by half a step, which averages out over the keys).
-// A row that comes out NaN is computed again key by key: masked keys in its tiles may hold infinities or
-// NaN that their zero weights do not silence.
+// A row that comes out NaN (or infinite) is computed again key by key: masked keys in its tiles may hold
+// infinities or NaN that their zero weights do not silence.
 
 constexpr int BOX = 128 * 128;       // 128 rows of 64 16-bit elements
 constexpr int TC_THREADS = 384;
@@ -318,36 +318,9 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
     const int warp = uniform(threadIdx.x >> 5), lane = threadIdx.x & 31;
     const int kvh = blockIdx.y;
 
-    // ---- which tokens: sequence i owns the slots from cu[i] / TT + i on, later tiles (more keys) first ----
-    const int TT = 2 * tq_tile;
-    const int slot = gridDim.x - 1 - blockIdx.x;
-    int lo = 0, hi = a.seqs;
-    while (hi - lo > 1) {
-        const int step = (hi - lo + 31) >> 5;
-        const int i = lo + lane * step;
-        bool here = false;
-        if (i < hi) here = (int)(min((int64_t)max(0, __ldg(a.cu_q + i)), a.tq) / TT) + i <= slot;
-        const uint32_t yes = __ballot_sync(0xffffffffu, here);
-        const int k = yes ? 31 - __clz(yes) : 0;
-        lo = lo + k * step;
-        hi = min(hi, lo + step);
-    }
-    int64_t qb, qe, kb, ke;
-    bounds(a.cu_q, lo, a.tq, &qb, &qe);
-    bounds(a.cu_k, lo, a.tk, &kb, &ke);
-    const int64_t tok0 = qb + (int64_t)(slot - (int)(qb / TT) - lo) * TT;
-    if (tok0 < qb || tok0 >= qe) return;
-    const int rows_tok[2] = {uniform((int)min((int64_t)tq_tile, qe - tok0)), uniform((int)max((int64_t)0, min((int64_t)tq_tile, qe - tok0 - tq_tile)))};
-    const int pos0 = uniform((int)((tok0 - qb) + (ke - kb) - (qe - qb)));  // position of the CTA's first token
-    Walk w;
-    w.high = uniform(max(0, pos0 + rows_tok[0] + rows_tok[1]));
-    w.low = uniform(a.window ? max(0, pos0 - a.window + 1) : 0);
-    w.sink_end = min(a.sinks, w.low);
-    w.sink_tiles = (w.sink_end + 127) >> 7;
-    w.n = w.high > 0 ? w.sink_tiles + ((w.high - w.low + 127) >> 7) : 0;
-    const Span span0(a, w, pos0, rows_tok[0]), span1(a, w, pos0 + tq_tile, rows_tok[1]);
-
+    // Set-up that needs no lengths runs while the search below waits for them.
     if (threadIdx.x == 0) {
+        for (const CUtensorMap* m : {&mq, &mk, &mk16, &mv, &mv16}) sm100::tma_prefetch_desc(m);
         for (int i = 0; i < 2; ++i) {
             sm100::mbar_init(&bars->q_full[i], 1);
             sm100::mbar_init(&bars->k_full[i], 1);
@@ -369,6 +342,51 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
         *reinterpret_cast<uint4*>(smem + L::Q + box * BOX + (qrows + rest / 8) * 128 + (rest % 8) * 16) = make_uint4(0, 0, 0, 0);
     }
     sm100::fence_proxy_async_smem();
+
+    // ---- which tokens: sequence i owns the slots from cu[i] / TT + i on, later tiles (more keys) first ----
+    const int TT = 2 * tq_tile;
+    const int slot = gridDim.x - 1 - blockIdx.x;
+    int lo = 0, hi = a.seqs;
+    int qb, qe, kb, ke;
+    int q_here = 0, k_here = 0;  // both tables at lo + lane, after a round in steps of one
+    bool at_hand = false;
+    while (hi - lo > 1 || !at_hand) {
+        const int step = max(1, (hi - lo + 31) >> 5);
+        const int i = min(lo + lane * step, a.seqs);
+        q_here = __ldg(a.cu_q + i);
+        if (step == 1) k_here = __ldg(a.cu_k + i);
+        const bool here = lo + lane * step < hi && min(max(0, q_here), (int)a.tq) / TT + i <= slot;
+        const uint32_t yes = __ballot_sync(0xffffffffu, here);
+        const int k = yes ? 31 - __clz(yes) : 0;
+        if (step == 1) {
+            at_hand = true;
+            // The bounds come from the lanes k and k + 1.
+            const int top_q = k < 31 ? __shfl_sync(0xffffffffu, q_here, min(k + 1, 31)) : __ldg(a.cu_q + lo + 32);
+            const int top_k = k < 31 ? __shfl_sync(0xffffffffu, k_here, min(k + 1, 31)) : __ldg(a.cu_k + lo + 32);
+            qb = min(max(0, __shfl_sync(0xffffffffu, q_here, k)), (int)a.tq);
+            qe = max(qb, min(top_q, (int)a.tq));
+            kb = min(max(0, __shfl_sync(0xffffffffu, k_here, k)), (int)a.tk);
+            ke = max(kb, min(top_k, (int)a.tk));
+            lo += k;
+            hi = lo;
+        } else {
+            lo = lo + k * step;
+            hi = min(hi, lo + step);
+        }
+    }
+    const int64_t tok_at = qb + (int64_t)(slot - qb / TT - lo) * TT;
+    if (tok_at < qb || tok_at >= qe) return;  // a slot that rounding left over
+    const int tok0 = uniform((int)tok_at);
+    const int rows_tok[2] = {min(tq_tile, qe - tok0), max(0, min(tq_tile, qe - tok0 - tq_tile))};
+    const int pos0 = uniform((tok0 - qb) + (ke - kb) - (qe - qb));  // position of the CTA's first token
+    Walk w;
+    w.high = max(0, pos0 + uniform(rows_tok[0] + rows_tok[1]));
+    w.low = uniform(a.window ? max(0, pos0 - a.window + 1) : 0);
+    w.sink_end = min(a.sinks, w.low);
+    w.sink_tiles = (w.sink_end + 127) >> 7;
+    w.n = w.high > 0 ? w.sink_tiles + ((w.high - w.low + 127) >> 7) : 0;
+    const Span span0(a, w, pos0, uniform(rows_tok[0])), span1(a, w, pos0 + tq_tile, uniform(rows_tok[1]));
+
     if (warp == 1) {
         sm100::tmem_alloc(&bars->tmem_base, 512);
         sm100::tmem_relinquish();
@@ -386,7 +404,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
                     if ((t ? span1.last : span0.last) < 0) continue;
                     sm100::mbar_arrive_expect_tx(&bars->q_full[t], DB * qrows * 128);
                     for (int b = 0; b < DB; ++b)
-                        sm100::tma_load_3d(smem + L::Q + (t * DB + b) * BOX, &mq, &bars->q_full[t], 64 * b, kvh * a.group, (int)tok0 + t * tq_tile);
+                        sm100::tma_load_3d(smem + L::Q + (t * DB + b) * BOX, &mq, &bars->q_full[t], 64 * b, kvh * a.group, tok0 + t * tq_tile);
                 }
                 int keys_in = 0, values_in = 0;  // tiles whose copies were issued
                 for (int j = 0; j < w.n; ++j) {
@@ -394,7 +412,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
                     const uint32_t ph = (uint32_t)(j >> 1) & 1u;
                     // Keys that some tile multiplies, in whole 16s.
                     const int rows = (max(span0.count(w, j), span1.count(w, j)) + 15) & ~15;
-                    const int key = (int)kb + w.start(j);
+                    const int key = kb + w.start(j);
                     for (int kv = 0; kv < 2; ++kv) {
                         uint64_t* empty = kv ? &bars->v_empty[st] : &bars->k_empty[st];
                         uint64_t* full = kv ? &bars->v_full[st] : &bars->k_full[st];
@@ -434,15 +452,16 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
                 auto pv = [&](int t, int j, int keys, uint32_t turn) {
                     const uint64_t d = dv + (j & 1) * NEXT;
                     const uint32_t to = tmem + O_COL + 128u * t, tp = tmem + 128u * t;
-#pragma unroll 1
+#pragma unroll
                     for (int h = 0; h < 2; ++h) {
                         wait(&bars->p_full[t][h], turn & 1u, 123);
                         __syncwarp();
                         sm100::tc_fence_after();
-                        const int steps = min((keys + 15) >> 4, h ? 8 : FIRST_KEYS / 16);
-#pragma unroll 1
-                        for (int kk = h ? FIRST_KEYS / 16 : 0; kk < steps; ++kk)
-                            issue_pv16(to, tp + (uint32_t)(32 * (kk >> 1) + 8 * (kk & 1)), d + kk * 128, idesc_o, kk > 0 || turn > 0 ? 1u : 0u, lead);
+#pragma unroll
+                        for (int c = h ? FIRST_KEYS / 32 : 0; c < (h ? 4 : FIRST_KEYS / 32); ++c) {
+                            if (keys > 32 * c + 16) issue_pv32(to, tp + 32u * c, d + 256 * c, idesc_o, c > 0 || turn > 0 ? 1u : 0u, lead);
+                            else if (keys > 32 * c) issue_pv16(to, tp + 32u * c, d + 256 * c, idesc_o, c > 0 || turn > 0 ? 1u : 0u, lead);
+                        }
                     }
                 };
                 // S_t(j) = Q_t . K(j)^T over the columns that P_t was read from (the pipe runs this thread's
@@ -485,15 +504,18 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
                 if (span0.last >= 0) wait(&bars->q_full[0], 0, 124);
                 if (span1.last >= 0) wait(&bars->q_full[1], 0, 124);
                 int keys0 = 0, keys1 = 0;         // of tile j - 1, 0: it is not for that row tile
-                for (int j = 0; j <= w.n; ++j) {
+                int j = 0;
+                for (; j <= w.n; ++j) {
                     const int next0 = j < w.n && span0.active(w, j) ? span0.count(w, j) : 0, next1 = j < w.n && span1.active(w, j) ? span1.count(w, j) : 0;
                     if (j > 0) wait(&bars->v_ready[(j - 1) & 1], (uint32_t)((j - 1) >> 1) & 1u, 122);
                     if (keys0) pv(0, j - 1, keys0, turns0++);
+                    if (j == w.n) commit(&bars->o_done[0], lead);
                     if (j < w.n) wait(&bars->k_full[j & 1], (uint32_t)(j >> 1) & 1u, 125);
                     __syncwarp();
                     sm100::tc_fence_after();
                     if (next0) qk(0, j, next0);
                     if (keys1) pv(1, j - 1, keys1, turns1++);
+                    if (j == w.n) commit(&bars->o_done[1], lead);
                     if (j > 0) commit(&bars->v_empty[(j - 1) & 1], lead);
                     if (next1) qk(1, j, next1);
                     if (j < w.n) commit(&bars->k_empty[j & 1], lead);
@@ -509,16 +531,18 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
                         }
                     }
                 }
-                // Also after a wait that gave up: the tensor pipe drains before TMEM is freed.
-                commit(&bars->o_done[0], lead);
-                commit(&bars->o_done[1], lead);
+                // After a wait that gave up the tensor pipe still drains before TMEM is freed.
+                if (j < w.n) {
+                    commit(&bars->o_done[0], lead);
+                    commit(&bars->o_done[1], lead);
+                }
             }
         } else if (warp == 2) {
             for (int j = 0; j < w.n; ++j) {
                 const int st = j & 1;
                 if (!__all_sync(0xffffffffu, sm100::mbar_wait(&bars->v_full[st], (uint32_t)(j >> 1) & 1u, status, 126))) break;
                 const int rows = (max(span0.count(w, j), span1.count(w, j)) + 15) & ~15;
-                const int real = (int)min((int64_t)rows, ke - kb - w.start(j));
+                const int real = min(rows, ke - kb - w.start(j));
                 for (int i = lane; i < DB * (rows - real) * 8; i += 32) {
                     const int b = i / ((rows - real) * 8), rest = i % ((rows - real) * 8);
                     *reinterpret_cast<uint4*>(smem + L::V + st * L::TILE + b * BOX + (real + rest / 8) * 128 + (rest % 8) * 16) = make_uint4(0, 0, 0, 0);
@@ -531,7 +555,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
         asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
         const int t = (warp >> 2) - 1;
         const int row = (warp & 3) * 32 + lane;
-        const int tok = row / a.group, head = kvh * a.group + row - tok * a.group;
+        const int tok = row / a.group;
         const int n_tok = t ? rows_tok[1] : rows_tok[0];
         const Span span = t ? span1 : span0;
         const int first = span.first;
@@ -610,37 +634,50 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
             ++turn;
         }
         // ---- O / l ----
-        T* out = (T*)a.o + (tok0 + t * tq_tile + tok) * a.ot + (int64_t)head * a.oh;
-        bool again = false;
-        if (w.n > 0) ok = sm100::mbar_wait(&bars->o_done[t], 0, status, 128) && ok;
+        // Through the tile's Q buffer (its products are done), so that 16 (8) lanes store a whole row; a
+        // row's 16-byte pieces are turned by its number to spread over the banks.
+        float2 nan = sf::f2(0.f);
+        if (w.n > 0) ok = wait_soon(&bars->o_done[t], 0, status, 128) && ok;
         sm100::tc_fence_after();
         const bool none = turn == 0 || p < 0;
         const float inv = 1.0f / s.l;
+        constexpr int PIECES = D / 8;
+        uint4* stage = reinterpret_cast<uint4*>(smem + L::Q + t * L::TILE) + (warp & 3) * 32 * PIECES;
 #pragma unroll 1
         for (int c = 0; c < D / 32; ++c) {
             uint32_t r[32];
             sm100::tmem_ld_32x32b_x32(to + 32u * c, r);
             sm100::tmem_ld_wait();
-            if (live && ok) {
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    uint32_t o4[4];
+            for (int i = 0; i < 4; ++i) {
+                uint32_t o4[4];
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        float2 x = make_float2(__uint_as_float(r[8 * i + 2 * e]) * inv, __uint_as_float(r[8 * i + 2 * e + 1]) * inv);
-                        if (none) x = make_float2(0.f, 0.f);
-                        again |= x.x != x.x || x.y != x.y;
-                        o4[e] = sf::Pair<T>::from_f2(x);
-                    }
-                    *reinterpret_cast<uint4*>(out + 32 * c + 8 * i) = make_uint4(o4[0], o4[1], o4[2], o4[3]);
+                for (int e = 0; e < 4; ++e) {
+                    float2 x = make_float2(__uint_as_float(r[8 * i + 2 * e]) * inv, __uint_as_float(r[8 * i + 2 * e + 1]) * inv);
+                    if (none) x = make_float2(0.f, 0.f);
+                    nan = sf::f2_fma(x, sf::f2(0.f), nan);  // 0, or NaN once a NaN or an infinity has passed
+                    o4[e] = sf::Pair<T>::from_f2(x);
                 }
+                stage[lane * PIECES + ((4 * c + i) ^ (lane & 7))] = make_uint4(o4[0], o4[1], o4[2], o4[3]);
             }
         }
+        const bool again = live && ok && !(nan.x + nan.y == 0.f);
+        const int64_t mine = (int64_t)(tok0 + t * tq_tile + tok) * a.ot + (int64_t)(kvh * a.group + row - tok * a.group) * a.oh;
+        __syncwarp();
+        const uint32_t written = __ballot_sync(0xffffffffu, live && ok);
+#pragma unroll 4
+        for (int i = lane; i < 32 * PIECES; i += 32) {
+            const int rl = i / PIECES, piece = i % PIECES;
+            const int64_t at = __shfl_sync(0xffffffffu, mine, rl);
+            const uint4 x = stage[rl * PIECES + (piece ^ (rl & 7))];
+            if (written >> rl & 1u) *reinterpret_cast<uint4*>((T*)a.o + at + 8 * piece) = x;
+        }
+        __syncwarp();
         for (uint32_t todo = __ballot_sync(0xffffffffu, again); todo; todo &= todo - 1) {
             const int src = __ffs(todo) - 1;
             const int rw = (warp & 3) * 32 + src;
             const int tk = rw / a.group, hd = kvh * a.group + rw - tk * a.group;
-            const int64_t qrow = tok0 + t * tq_tile + tk;
+            const int64_t qrow = (int64_t)tok0 + t * tq_tile + tk;
             row_by_warp<T>(a, D, qrow, hd, kb, first + tk, (T*)a.o + qrow * a.ot + (int64_t)hd * a.oh);
         }
     }
