@@ -41,34 +41,25 @@ __device__ __forceinline__ void sincos_turns(double turns, float* s, float* c) {
 }
 
 template <typename T>
-struct Row {
-    uint4 a, b;  // the lane's two chunks
-};
-
-template <typename T>
-__device__ __forceinline__ void unpack8(const uint4& u, float (&v)[8]) {
-    const uint32_t w[4] = {u.x, u.y, u.z, u.w};
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const float2 f = sf::Pair<T>::to_f2(w[i]);
-        v[2 * i] = f.x;
-        v[2 * i + 1] = f.y;
-    }
+__device__ __forceinline__ void unpack8(const uint4& u, float2 (&v)[4]) {
+    v[0] = sf::Pair<T>::to_f2(u.x);
+    v[1] = sf::Pair<T>::to_f2(u.y);
+    v[2] = sf::Pair<T>::to_f2(u.z);
+    v[3] = sf::Pair<T>::to_f2(u.w);
 }
 
 template <typename T>
-__device__ __forceinline__ uint4 pack8(const float (&v)[8]) {
-    uint32_t w[4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) w[i] = sf::Pair<T>::from_f2(make_float2(v[2 * i], v[2 * i + 1]));
-    return make_uint4(w[0], w[1], w[2], w[3]);
+__device__ __forceinline__ uint4 pack8(const float2 (&v)[4]) {
+    return make_uint4(sf::Pair<T>::from_f2(v[0]), sf::Pair<T>::from_f2(v[1]), sf::Pair<T>::from_f2(v[2]), sf::Pair<T>::from_f2(v[3]));
 }
 
 // LPR lanes a row (a power of two >= D / 16); `items` = tokens x head parts, one warp an item.
 template <typename T, int LPR>
-__global__ void __launch_bounds__(256) qk_norm_rope_kernel(const Side q, const Side k, const int32_t* __restrict__ position, int64_t tokens,
-                                                           int hq, int hk, int D, int r, double ratio, float eps, int parts) {
+__global__ void __launch_bounds__(256, 2) qk_norm_rope_kernel(const Side q, const Side k, const int32_t* __restrict__ position, int64_t tokens,
+                                                              int hq, int hk, int D, int r, double ratio, float eps, int parts) {
     constexpr int RPW = 32 / LPR;  // rows a warp holds at once
+    // Both weights, in the lanes' order: 16 bytes a chunk (in registers they would cost a third of the warps).
+    __shared__ uint4 w_s[2][2][32];
     const int lane = threadIdx.x & 31;
     const int p = lane % LPR, sub = lane / LPR;
     const bool live = p < D / 16;
@@ -76,6 +67,16 @@ __global__ void __launch_bounds__(256) qk_norm_rope_kernel(const Side q, const S
     // Element offsets of the lane's chunks.
     const int e0 = turned ? 8 * p : 2 * r + 16 * (p - r / 8);
     const int e1 = turned ? e0 + r : e0 + 8;
+    if (threadIdx.x < LPR && live) {
+        if (hq) {
+            w_s[0][0][p] = *reinterpret_cast<const uint4*>((const T*)q.w + e0);
+            w_s[0][1][p] = *reinterpret_cast<const uint4*>((const T*)q.w + e1);
+        }
+        if (hk) {
+            w_s[1][0][p] = *reinterpret_cast<const uint4*>((const T*)k.w + e0);
+            w_s[1][1][p] = *reinterpret_cast<const uint4*>((const T*)k.w + e1);
+        }
+    }
     // base^(-i/r) / 2 pi of the lane's 8 angles: the first by repeated squaring, then by `ratio`.
     double turn0 = 0.15915494309189533577;
     if (turned) {
@@ -85,17 +86,7 @@ __global__ void __launch_bounds__(256) qk_norm_rope_kernel(const Side q, const S
             sq *= sq;
         }
     }
-    uint4 wq0 = {}, wq1 = {}, wk0 = {}, wk1 = {};
-    if (live) {
-        if (hq) {
-            wq0 = *reinterpret_cast<const uint4*>((const T*)q.w + e0);
-            wq1 = *reinterpret_cast<const uint4*>((const T*)q.w + e1);
-        }
-        if (hk) {
-            wk0 = *reinterpret_cast<const uint4*>((const T*)k.w + e0);
-            wk1 = *reinterpret_cast<const uint4*>((const T*)k.w + e1);
-        }
-    }
+    __syncthreads();
     const float inv_d = 1.0f / (float)D;
     const int rows = hq + hk;
     const int groups = (rows + RPW - 1) / RPW;
@@ -103,66 +94,82 @@ __global__ void __launch_bounds__(256) qk_norm_rope_kernel(const Side q, const S
     const int64_t items = tokens * parts;
     const int64_t step = (int64_t)gridDim.x * (blockDim.x >> 5);
     for (int64_t item = (int64_t)blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5); item < items; item += step) {
-        const int64_t t = item / parts;
+        const int64_t t = parts == 1 ? item : item / parts;
         const int g0 = (int)(item - t * parts) * per, g1 = min(groups, g0 + per);
-        const int32_t pos = __ldg(position + t);
-        float sn[8], cs[8];
-        bool have = false;
-        for (int g = g0; g < g1; g += 2) {
-            uint4 a[2], b[2];
-            int row[2];
-#pragma unroll
-            for (int u = 0; u < 2; ++u) {
-                row[u] = (g + u) * RPW + sub;
-                const bool ok = live && g + u < g1 && row[u] < rows;
-                if (!ok) row[u] = -1;
-                a[u] = b[u] = make_uint4(0, 0, 0, 0);
-                if (ok) {
-                    const bool isq = row[u] < hq;
-                    const T* x = isq ? (const T*)q.x + t * q.xt + (int64_t)row[u] * q.xh : (const T*)k.x + t * k.xt + (int64_t)(row[u] - hq) * k.xh;
-                    a[u] = *reinterpret_cast<const uint4*>(x + e0);
-                    b[u] = *reinterpret_cast<const uint4*>(x + e1);
-                }
+        const T* xq = (const T*)q.x + t * q.xt;
+        const T* xk = (const T*)k.x + t * k.xt;
+        // Row of group g for this lane, -1: none.
+        auto row_of = [&](int g) {
+            const int row = g * RPW + sub;
+            return live && g < g1 && row < rows ? row : -1;
+        };
+        auto load = [&](int row, uint4& a, uint4& b) {
+            a = b = make_uint4(0, 0, 0, 0);
+            if (row >= 0) {
+                const T* x = row < hq ? xq + row * q.xh : xk + (row - hq) * k.xh;
+                a = *reinterpret_cast<const uint4*>(x + e0);
+                b = *reinterpret_cast<const uint4*>(x + e1);
             }
-            if (!have) {  // while the first rows are on their way
-                have = true;
-                double f = turn0;
+        };
+        uint4 na[2], nb[2];
 #pragma unroll
-                for (int j = 0; j < 8; ++j) {
-                    sn[j] = 0.f;
-                    cs[j] = 1.f;
-                    if (turned) sincos_turns((double)pos * f, &sn[j], &cs[j]);
+        for (int u = 0; u < 2; ++u) load(row_of(g0 + u), na[u], nb[u]);
+        // Sines and cosines while the first rows are on their way.
+        const double pos = (double)__ldg(position + t);
+        float2 sn[4], cs[4];
+        {
+            double f = turn0;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                sn[j] = sf::f2(0.f);
+                cs[j] = sf::f2(1.f);
+                if (turned) {
+                    sincos_turns(pos * f, &sn[j].x, &cs[j].x);
+                    f *= ratio;
+                    sincos_turns(pos * f, &sn[j].y, &cs[j].y);
                     f *= ratio;
                 }
             }
+        }
+        for (int g = g0; g < g1; g += 2) {
+            uint4 a[2], b[2];
 #pragma unroll
             for (int u = 0; u < 2; ++u) {
-                float va[8], vb[8];
+                a[u] = na[u];
+                b[u] = nb[u];
+                load(row_of(g + 2 + u), na[u], nb[u]);
+            }
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+                const int row = row_of(g + u);
+                float2 va[4], vb[4];
                 unpack8<T>(a[u], va);
                 unpack8<T>(b[u], vb);
-                float2 ss = make_float2(0.f, 0.f);
+                float2 ss = sf::f2_mul(va[0], va[0]);
 #pragma unroll
-                for (int j = 0; j < 8; ++j) {
-                    const float2 x2 = make_float2(va[j], vb[j]);
-                    ss = sf::f2_fma(x2, x2, ss);
-                }
+                for (int j = 1; j < 4; ++j) ss = sf::f2_fma(va[j], va[j], ss);
+#pragma unroll
+                for (int j = 0; j < 4; ++j) ss = sf::f2_fma(vb[j], vb[j], ss);
                 float sum = ss.x + ss.y;
 #pragma unroll
                 for (int o = LPR / 2; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-                if (row[u] < 0) continue;
-                const float rs = rsqrtf(fmaf(sum, inv_d, eps));
-                const bool isq = row[u] < hq;
-                float w0[8], w1[8], o0[8], o1[8];
-                unpack8<T>(isq ? wq0 : wk0, w0);
-                unpack8<T>(isq ? wq1 : wk1, w1);
+                if (row < 0) continue;
+                const float2 rs = sf::f2(rsqrtf(fmaf(sum, inv_d, eps)));
+                const bool isq = row < hq;
+                float2 w0[4], w1[4], o0[4], o1[4];
+                unpack8<T>(w_s[isq ? 0 : 1][0][p], w0);
+                unpack8<T>(w_s[isq ? 0 : 1][1][p], w1);
 #pragma unroll
-                for (int j = 0; j < 8; ++j) {
-                    const float y0 = va[j] * rs * w0[j], y1 = vb[j] * rs * w1[j];
-                    // Plain products and sums where nothing turns keep an infinite partner out.
-                    o0[j] = turned ? y0 * cs[j] - y1 * sn[j] : y0;
-                    o1[j] = turned ? y0 * sn[j] + y1 * cs[j] : y1;
+                for (int j = 0; j < 4; ++j) {
+                    const float2 y0 = sf::f2_mul(sf::f2_mul(va[j], rs), w0[j]), y1 = sf::f2_mul(sf::f2_mul(vb[j], rs), w1[j]);
+                    o0[j] = y0;
+                    o1[j] = y1;
+                    if (turned) {  // where nothing turns an infinite partner would leave NaN
+                        o0[j] = make_float2(fmaf(-y1.x, sn[j].x, y0.x * cs[j].x), fmaf(-y1.y, sn[j].y, y0.y * cs[j].y));
+                        o1[j] = sf::f2_fma(y1, cs[j], sf::f2_mul(y0, sn[j]));
+                    }
                 }
-                T* y = isq ? (T*)q.y + t * q.yt + (int64_t)row[u] * q.yh : (T*)k.y + t * k.yt + (int64_t)(row[u] - hq) * k.yh;
+                T* y = isq ? (T*)q.y + t * q.yt + row * q.yh : (T*)k.y + t * k.yt + (row - hq) * k.yh;
                 *reinterpret_cast<uint4*>(y + e0) = pack8<T>(o0);
                 *reinterpret_cast<uint4*>(y + e1) = pack8<T>(o1);
             }

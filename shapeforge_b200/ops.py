@@ -533,12 +533,13 @@ def _check_vector(t: torch.Tensor, name: str, dev: int, dtype: torch.dtype, leng
 
 def _launch(name: str, dev: int, *fields) -> None:
     """Call a serving entry point on GPU ``dev``'s current stream, with that GPU current (the C ABI
-    launches on the thread's current device); entering it costs more than the launch, so only if need be."""
+    launches on the thread's current device); entering it costs more than the launch, so only if need be.
+    The stream comes as the raw handle: a ``torch.cuda.Stream`` object would cost 3 us of a 12 us call."""
     if torch.cuda.current_device() == dev:
-        _native.call_args(name, torch.cuda.current_stream().cuda_stream, *fields)
+        _native.call_args(name, torch._C._cuda_getCurrentRawStream(dev), *fields)
     else:
         with torch.cuda.device(dev):
-            _native.call_args(name, torch.cuda.current_stream().cuda_stream, *fields)
+            _native.call_args(name, torch._C._cuda_getCurrentRawStream(dev), *fields)
 
 
 def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, q_weight: torch.Tensor, k_weight: torch.Tensor, positions: torch.Tensor,
