@@ -25,8 +25,8 @@
 //    in the columns): a group of up to 8 heads wastes no rows, the cache is the A operand straight
 //    from shared memory, and p becomes the next B operand by a transposing matrix move.  tcgen05
 //    would need the expanded operands written back to shared memory, several times the cache's bytes.
-//  * Each warp streams its own tiles (every 8th of the CTA's) through a ring of bulk copies, one
-//    record a copy; warps meet only at the end of a (request, head) to merge their softmax states.
+//  * Each warp streams its own tiles (every 4th of the CTA's) through a ring of bulk copies, one record a
+//    copy; warps meet only at the end of a (request, head) to merge their softmax states.
 //  * Work is dealt in 16-key tiles: the tiles of all requests and heads in one line, an equal
 //    stretch for every CTA of one resident wave, whatever the lengths; each (request, head) counts
 //    ITEM_COST tiles more for its start and end.  One that spans CTAs leaves partial states in the
@@ -45,10 +45,16 @@ __device__ sm100::KernelStatus g_kv4_attention_status[2];
 
 namespace {
 
-constexpr int WARPS = 8;
+// Four warps a CTA and several CTAs an SM, so that one's tiles run while another starts or merges an item
+// (12 warps in one CTA: 87.7 against 83.3 us for 32 requests of 8192 keys on average, 64 heads on 8); with
+// one head tile (8 query heads) the registers allow a warp two key tiles side by side at a step.
+constexpr int WARPS = 4;
 constexpr int THREADS = 32 * WARPS;
+constexpr int ctas_of(int nt) { return nt == 1 ? 3 : 2; }
+constexpr int tiles_of_step(int nt) { return nt == 1 ? 2 : 1; }
 constexpr int MAX_SMEM = 227 * 1024;
-constexpr int ITEM_COST = 16;  // what starting and merging a (request, head) costs, in tiles
+constexpr int LEAST = 4 * WARPS;  // tiles and costs a CTA has at least (one a warp: 13.3 against 11.6 us for one request of 4097 keys)
+constexpr int ITEM_COST = 24;  // what starting and merging a (request, head) costs, in tiles
 constexpr float NO_MAX = -3e38f;  // the running max before any score
 // Smallest unit of a head's p s: p / unit stays finite for p up to 2^8.
 constexpr float UNIT_FLOOR = 0x1p-118f;
@@ -142,9 +148,11 @@ template <int NG, int NT>
 struct Smem {
     static constexpr int D = 64 * NG;
     static constexpr int HB = 8 * NT;               // query heads of a block
-    static constexpr int STAGES = 4;
+    static constexpr int TS = tiles_of_step(NT);
+    static constexpr int STAGES = TS == 2 ? 3 : 4;  // steps
+    static constexpr int STAGE = TS * kv4::Record<NG>::BYTES;
     static constexpr int PAD = D + 4;               // row stride of the staged outputs
-    static constexpr int RING = WARPS * STAGES * kv4::Record<NG>::BYTES;
+    static constexpr int RING = WARPS * STAGES * STAGE;
     static constexpr int OUT = RING;                // [warp][head][PAD] fp32
     static constexpr int STAT = OUT + WARPS * HB * PAD * 4;  // [warp][head][2] fp32
     static constexpr int BARS = STAT + WARPS * HB * 8;
@@ -180,10 +188,10 @@ __device__ __forceinline__ void scan_costs(const Args& a, int* pre) {
 }
 
 template <typename T, int NG, int NT>
-__global__ void __launch_bounds__(THREADS, NT == 1 ? 2 : 1) kv4_attention_kernel(const Args a) {
+__global__ void __launch_bounds__(THREADS, ctas_of(NT)) kv4_attention_kernel(const Args a) {
     using S = Smem<NG, NT>;
     using R = kv4::Record<NG>;
-    constexpr int D = 64 * NG, HB = S::HB, ST = S::STAGES;
+    constexpr int D = 64 * NG, HB = S::HB, ST = S::STAGES, TS = S::TS;
     extern __shared__ __align__(128) uint8_t smem[];
     float* out_s = reinterpret_cast<float*>(smem + S::OUT);
     float* stat_s = reinterpret_cast<float*>(smem + S::STAT);
@@ -202,9 +210,9 @@ __global__ void __launch_bounds__(THREADS, NT == 1 ? 2 : 1) kv4_attention_kernel
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");  // the join may take its place; it waits for this grid
     const int per_b = a.Hk * a.blocks;
     Line* line = reinterpret_cast<Line*>(smem + S::LINE + 64 * warp);
-    auto share_of = [&]() {  // tiles and costs a CTA, at least a tile a warp
+    auto share_of = [&]() {  // tiles and costs a CTA
         const int64_t total = (int64_t)pre[a.B] * per_b;
-        return max((int64_t)WARPS, (total + gridDim.x - 1) / gridDim.x);
+        return max((int64_t)LEAST, (total + gridDim.x - 1) / gridDim.x);
     };
     if (a.split) {
         scan_costs(a, pre);
@@ -269,7 +277,7 @@ __global__ void __launch_bounds__(THREADS, NT == 1 ? 2 : 1) kv4_attention_kernel
     };
 
     // ---- the ring ----
-    uint32_t used = 0;  // tiles this warp has taken from its ring (stage = used % ST)
+    uint32_t used = 0;  // steps this warp has taken from its ring (stage = used % ST)
     int* ahead = reinterpret_cast<int*>(smem + S::AHEAD) + 64 * warp;
     auto tiles_of_warp = [&](const Part& x) { return x.n > warp ? (x.n - warp + WARPS - 1) / WARPS : 0; };
     // Record numbers of tiles 32 block + lane of this warp; -1: none, or no such page.
@@ -285,15 +293,22 @@ __global__ void __launch_bounds__(THREADS, NT == 1 ? 2 : 1) kv4_attention_kernel
         }
         return (id * a.Hk + x.item / a.blocks) * a.tpp + (tile - page * a.tpp);
     };
-    auto issue = [&](int k, int rec) {  // lane 0: tile k of the part, record `rec`, into its stage
+    // Lane 0: the records of step k (-1: none) into its stage.
+    auto issue = [&](int k, const int (&rec)[TS]) {
         const uint32_t stage = (used + (uint32_t)k) % ST;
         uint64_t* bar = &bars[warp * ST + stage];
-        if (rec < 0) {
+        uint32_t bytes = 0;
+#pragma unroll
+        for (int u = 0; u < TS; ++u) bytes += rec[u] < 0 ? 0 : R::BYTES;
+        if (bytes == 0) {
             sm100::mbar_arrive(bar);
-        } else {
-            sm100::mbar_arrive_expect_tx(bar, R::BYTES);
-            sm100::bulk_load(sm100::smem_u32(smem) + (warp * ST + stage) * R::BYTES, a.cache + (int64_t)rec * R::BYTES, R::BYTES, bar);
+            return;
         }
+        sm100::mbar_arrive_expect_tx(bar, bytes);
+#pragma unroll
+        for (int u = 0; u < TS; ++u)
+            if (rec[u] >= 0)
+                sm100::bulk_load(sm100::smem_u32(smem) + (warp * ST + stage) * S::STAGE + u * R::BYTES, a.cache + (int64_t)rec[u] * R::BYTES, R::BYTES, bar);
     };
     // A part's first 64 record numbers, looked up long before they are needed.
     auto look_up = [&](const Part& x) {
@@ -303,16 +318,18 @@ __global__ void __launch_bounds__(THREADS, NT == 1 ? 2 : 1) kv4_attention_kernel
         ahead[32 + lane] = records(x, seen, 1);
         __syncwarp();
     };
-    int mine, issued, rec_now, rec_next;
+    int steps, issued, rec_now, rec_next;  // of the warp: steps in the part, steps whose copies are issued
     uint4 raw[NT][NG][2];  // the lane's elements 64 G + 16 t + 0..15 of heads g (+ 8)
     // Begin a part that has been looked up: its first copies and its queries.
     auto begin = [&](const Part& x) {
         if (x.n < 0) return;
-        mine = tiles_of_warp(x);
+        steps = (tiles_of_warp(x) + TS - 1) / TS;
         rec_now = x.n ? ahead[lane] : -1;
         rec_next = x.n ? ahead[32 + lane] : -1;
-        for (issued = 0; issued < min(mine, ST - 1); ++issued) {
-            const int rec = __shfl_sync(0xffffffffu, rec_now, issued);
+        for (issued = 0; issued < min(steps, ST - 1); ++issued) {
+            int rec[TS];
+#pragma unroll
+            for (int u = 0; u < TS; ++u) rec[u] = __shfl_sync(0xffffffffu, rec_now, TS * issued + u);
             if (lane == 0) issue(issued, rec);
         }
         const int kh = x.item / a.blocks, hb = x.item - kh * a.blocks;
@@ -322,7 +339,7 @@ __global__ void __launch_bounds__(THREADS, NT == 1 ? 2 : 1) kv4_attention_kernel
             for (int G = 0; G < NG; ++G) {
                 const int h = hb * HB + nt * 8 + g;
                 raw[nt][G][0] = raw[nt][G][1] = make_uint4(0, 0, 0, 0);
-                if (h < a.group && mine) {
+                if (h < a.group && steps) {
                     const T* src = (const T*)a.q + (int64_t)x.b * a.qb + (int64_t)(kh * a.group + h) * a.qh + 64 * G + 16 * t;
                     raw[nt][G][0] = *reinterpret_cast<const uint4*>(src);
                     raw[nt][G][1] = *reinterpret_cast<const uint4*>(src + 8);
@@ -351,7 +368,7 @@ __global__ void __launch_bounds__(THREADS, NT == 1 ? 2 : 1) kv4_attention_kernel
         __syncwarp();
         step();
         look_up(line->next);
-        uint32_t bad = __ballot_sync(0xffffffffu, mine && rec_now < 0);  // of a block of 32 tiles: nothing was copied
+        uint32_t bad = __ballot_sync(0xffffffffu, steps && rec_now < 0);  // of a block of 32 tiles: nothing was copied
 
         // ---- q as the B operand ----
         uint32_t qf[NT][8 * NG], qlow[NT];
@@ -431,19 +448,22 @@ __global__ void __launch_bounds__(THREADS, NT == 1 ? 2 : 1) kv4_attention_kernel
         }
 
         // ---- the warp's tiles ----
-        const uint8_t* ring = smem + warp * ST * R::BYTES;
+        const uint8_t* ring = smem + warp * ST * S::STAGE;
         // Tiles that may hold keys past either end of what is seen: the last, the last of the sinks and
         // the first behind them.
         const int edge0 = seen.sink_tiles - 1 - now.i0, edge1 = seen.sink_tiles - now.i0, edge2 = seen.n - 1 - now.i0;
-        for (int k = 0; k < mine; ++k) {
-            if (k && (k & 31) == 0) {
+        for (int k = 0; k < steps; ++k) {
+            if (k && (TS * k & 31) == 0) {
                 rec_now = rec_next;
                 bad = __ballot_sync(0xffffffffu, rec_now < 0);
-                rec_next = records(now, seen, (k >> 5) + 1);
+                rec_next = records(now, seen, (TS * k >> 5) + 1);
             }
             __syncwarp();  // every lane is done with the stage that the next copy overwrites
-            if (issued < mine) {
-                const int rec = __shfl_sync(0xffffffffu, (issued >> 5) == (k >> 5) ? rec_now : rec_next, issued & 31);
+            if (issued < steps) {
+                const int from = TS * issued >> 5 == TS * k >> 5 ? rec_now : rec_next;
+                int rec[TS];
+#pragma unroll
+                for (int u = 0; u < TS; ++u) rec[u] = __shfl_sync(0xffffffffu, from, (TS * issued + u) & 31);
                 if (lane == 0) issue(issued, rec);
                 ++issued;
             }
@@ -452,83 +472,91 @@ __global__ void __launch_bounds__(THREADS, NT == 1 ? 2 : 1) kv4_attention_kernel
             // follow end early.
             sm100::mbar_wait(&bars[warp * ST + turn % ST], (turn / ST) & 1u, g_kv4_attention_status + 1, kv4::AT_WAIT);
             __syncwarp();
-            if (bad >> (k & 31) & 1u) continue;
-            const uint8_t* rec = ring + (turn % ST) * R::BYTES;
+            const uint32_t none = bad >> (TS * k & 31);
+            if ((none & ((1u << TS) - 1u)) == (1u << TS) - 1u) continue;
+            const uint8_t* rec = ring + (turn % ST) * S::STAGE;
 
-            // Scales and minima of the lane's keys `row` and `row + 8`.
-            uint32_t kp[2][NG], vp[2][NG], kw[2][2 * NG];
+            // Scales and minima of the lane's keys `row` and `row + 8` of each tile.
+            uint32_t vp[TS][2][NG];
+            float s[TS][NT][4];  // S^T: [row, row + 8] x heads 2t, 2t + 1
 #pragma unroll
-            for (int r = 0; r < 2; ++r) {
-                const uint8_t* p = rec + R::K + (row + 8 * r) * R::ROW + t * 8 * NG;
-                if constexpr (NG == 2) {
-                    *reinterpret_cast<uint2*>(kp[r]) = *reinterpret_cast<const uint2*>(rec + R::KP + (row + 8 * r) * 8);
-                    *reinterpret_cast<uint2*>(vp[r]) = *reinterpret_cast<const uint2*>(rec + R::VP + (row + 8 * r) * 8);
-                    *reinterpret_cast<uint4*>(kw[r]) = *reinterpret_cast<const uint4*>(p);
-                } else {
-                    kp[r][0] = *reinterpret_cast<const uint32_t*>(rec + R::KP + (row + 8 * r) * 4);
-                    vp[r][0] = *reinterpret_cast<const uint32_t*>(rec + R::VP + (row + 8 * r) * 4);
-                    *reinterpret_cast<uint2*>(kw[r]) = *reinterpret_cast<const uint2*>(p);
-                }
-            }
-            // S^T = K q^T: the minima's part, then a group at a time.
-            float s[NT][4];  // [row, row + 8] x heads 2t, 2t + 1
-#pragma unroll
-            for (int nt = 0; nt < NT; ++nt)
-                mma_bf16_k8_first(s[nt], NG == 2 ? __byte_perm(kp[0][0], kp[0][NG - 1], 0x7632) : kp[0][0] >> 16,
-                                  NG == 2 ? __byte_perm(kp[1][0], kp[1][NG - 1], 0x7632) : kp[1][0] >> 16, qlow[nt]);
-#pragma unroll
-            for (int G = 0; G < NG; ++G) {
-                float acc[NT][4];
-#pragma unroll
-                for (int h2 = 0; h2 < 2; ++h2) {
-                    const uint32_t x = kw[0][2 * G + h2], y = kw[1][2 * G + h2], x8 = x >> 8, y8 = y >> 8;
-                    const uint32_t a0[4] = {x & 0x000F000Fu, y & 0x000F000Fu, x & 0x00F000F0u, y & 0x00F000F0u};
-                    const uint32_t a1[4] = {x8 & 0x000F000Fu, y8 & 0x000F000Fu, x8 & 0x00F000F0u, y8 & 0x00F000F0u};
-#pragma unroll
-                    for (int nt = 0; nt < NT; ++nt) {
-                        const uint32_t* f = &qf[nt][(2 * G + h2) * 4];
-                        if (h2 == 0) mma_f16_first(acc[nt], a0, f[0], f[1]);
-                        else mma_f16(acc[nt], a0, f[0], f[1]);
-                        mma_f16(acc[nt], a1, f[2], f[3]);
-                    }
-                }
+            for (int u = 0; u < TS; ++u) {
+                const uint8_t* tile = rec + u * R::BYTES;
+                uint32_t kp[2][NG], kw[2][2 * NG];
 #pragma unroll
                 for (int r = 0; r < 2; ++r) {
-                    const float kf = __uint_as_float(kp[r][G] << 16) * fac;
-#pragma unroll
-                    for (int nt = 0; nt < NT; ++nt) {
-                        s[nt][2 * r] = fmaf(acc[nt][2 * r], kf, s[nt][2 * r]);
-                        s[nt][2 * r + 1] = fmaf(acc[nt][2 * r + 1], kf, s[nt][2 * r + 1]);
+                    const uint8_t* p = tile + R::K + (row + 8 * r) * R::ROW + t * 8 * NG;
+                    if constexpr (NG == 2) {
+                        *reinterpret_cast<uint2*>(kp[r]) = *reinterpret_cast<const uint2*>(tile + R::KP + (row + 8 * r) * 8);
+                        *reinterpret_cast<uint2*>(vp[u][r]) = *reinterpret_cast<const uint2*>(tile + R::VP + (row + 8 * r) * 8);
+                        *reinterpret_cast<uint4*>(kw[r]) = *reinterpret_cast<const uint4*>(p);
+                    } else {
+                        kp[r][0] = *reinterpret_cast<const uint32_t*>(tile + R::KP + (row + 8 * r) * 4);
+                        vp[u][r][0] = *reinterpret_cast<const uint32_t*>(tile + R::VP + (row + 8 * r) * 4);
+                        *reinterpret_cast<uint2*>(kw[r]) = *reinterpret_cast<const uint2*>(p);
                     }
                 }
-            }
-            const int at_tile = warp + WARPS * k;
-            if (at_tile == edge0 || at_tile == edge1 || at_tile == edge2) {
-                const int j = seen.tile(now.i0 + at_tile) * 16 + row;
+                // S^T = K q^T: the minima's part, then a group at a time.
 #pragma unroll
-                for (int r = 0; r < 2; ++r) {
-                    if (j + 8 * r < seen.len && (j + 8 * r >= seen.low || j + 8 * r < a.sinks)) continue;
+                for (int nt = 0; nt < NT; ++nt)
+                    mma_bf16_k8_first(s[u][nt], NG == 2 ? __byte_perm(kp[0][0], kp[0][NG - 1], 0x7632) : kp[0][0] >> 16,
+                                      NG == 2 ? __byte_perm(kp[1][0], kp[1][NG - 1], 0x7632) : kp[1][0] >> 16, qlow[nt]);
 #pragma unroll
-                    for (int nt = 0; nt < NT; ++nt) s[nt][2 * r] = s[nt][2 * r + 1] = -INFINITY;
+                for (int G = 0; G < NG; ++G) {
+                    float acc[NT][4];
 #pragma unroll
-                    for (int G = 0; G < NG; ++G) vp[r][G] = 0;
+                    for (int h2 = 0; h2 < 2; ++h2) {
+                        const uint32_t x = kw[0][2 * G + h2], y = kw[1][2 * G + h2], x8 = x >> 8, y8 = y >> 8;
+                        const uint32_t a0[4] = {x & 0x000F000Fu, y & 0x000F000Fu, x & 0x00F000F0u, y & 0x00F000F0u};
+                        const uint32_t a1[4] = {x8 & 0x000F000Fu, y8 & 0x000F000Fu, x8 & 0x00F000F0u, y8 & 0x00F000F0u};
+#pragma unroll
+                        for (int nt = 0; nt < NT; ++nt) {
+                            const uint32_t* f = &qf[nt][(2 * G + h2) * 4];
+                            if (h2 == 0) mma_f16_first(acc[nt], a0, f[0], f[1]);
+                            else mma_f16(acc[nt], a0, f[0], f[1]);
+                            mma_f16(acc[nt], a1, f[2], f[3]);
+                        }
+                    }
+#pragma unroll
+                    for (int r = 0; r < 2; ++r) {
+                        const float kf = __uint_as_float(kp[r][G] << 16) * fac;
+#pragma unroll
+                        for (int nt = 0; nt < NT; ++nt) {
+                            s[u][nt][2 * r] = fmaf(acc[nt][2 * r], kf, s[u][nt][2 * r]);
+                            s[u][nt][2 * r + 1] = fmaf(acc[nt][2 * r + 1], kf, s[u][nt][2 * r + 1]);
+                        }
+                    }
+                }
+                const int at_tile = warp + WARPS * (TS * k + u);
+                if (at_tile == edge0 || at_tile == edge1 || at_tile == edge2 || (none >> u & 1u)) {
+                    const int j = seen.tile(now.i0 + at_tile) * 16 + row;
+#pragma unroll
+                    for (int r = 0; r < 2; ++r) {
+                        if (!(none >> u & 1u) && j + 8 * r < seen.len && (j + 8 * r >= seen.low || j + 8 * r < a.sinks)) continue;
+#pragma unroll
+                        for (int nt = 0; nt < NT; ++nt) s[u][nt][2 * r] = s[u][nt][2 * r + 1] = -INFINITY;
+#pragma unroll
+                        for (int G = 0; G < NG; ++G) vp[u][r][G] = 0;
+                    }
                 }
             }
             // The running max follows only when a score passes it by 2^8: p stays within fp32 and fp16
             // range and the final division takes the stale max out again.  O follows through its unit.
-            float2 d[NT][2];
             float over = -INFINITY;
 #pragma unroll
-            for (int nt = 0; nt < NT; ++nt)
+            for (int u = 0; u < TS; ++u)
 #pragma unroll
-                for (int r = 0; r < 2; ++r) {
-                    d[nt][r] = sf::f2_add(make_float2(s[nt][2 * r], s[nt][2 * r + 1]), nm[nt]);
-                    over = fmaxf(over, fmaxf(d[nt][r].x, d[nt][r].y));
-                }
+                for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                    for (int r = 0; r < 2; ++r)
+                        over = fmaxf(over, fmaxf(s[u][nt][2 * r] + nm[nt].x, s[u][nt][2 * r + 1] + nm[nt].y));
             if (__any_sync(0xffffffffu, over > 8.f)) {
 #pragma unroll
                 for (int nt = 0; nt < NT; ++nt) {
-                    float2 mx = over_keys(make_float2(fmaxf(s[nt][0], s[nt][2]), fmaxf(s[nt][1], s[nt][3])));
+                    float2 mx = make_float2(fmaxf(s[0][nt][0], s[0][nt][2]), fmaxf(s[0][nt][1], s[0][nt][3]));
+                    if constexpr (TS == 2)
+                        mx = make_float2(fmaxf(mx.x, fmaxf(s[TS - 1][nt][0], s[TS - 1][nt][2])), fmaxf(mx.y, fmaxf(s[TS - 1][nt][1], s[TS - 1][nt][3])));
+                    mx = over_keys(mx);
                     mx = make_float2(fmaxf(mx.x, -nm[nt].x), fmaxf(mx.y, -nm[nt].y));
                     const float2 f = make_float2(exp2f(-nm[nt].x - mx.x), exp2f(-nm[nt].y - mx.y));
                     nm[nt] = make_float2(-mx.x, -mx.y);
@@ -539,54 +567,54 @@ __global__ void __launch_bounds__(THREADS, NT == 1 ? 2 : 1) kv4_attention_kernel
                     per_unit[nt] = make_float2(1.0f / unit[nt].x, 1.0f / unit[nt].y);
 #pragma unroll
                     for (int G = 0; G < NG; ++G) pm[nt][G] = sf::f2_mul(pm[nt][G], f);
-#pragma unroll
-                    for (int r = 0; r < 2; ++r) d[nt][r] = sf::f2_add(make_float2(s[nt][2 * r], s[nt][2 * r + 1]), nm[nt]);
                 }
             }
-            // p, its sum, and p s in O's unit.
-            float2 x[NT][NG][2];
+            // p over the scores, its sum, and the largest p s in O's unit.
             over = 0.f;
 #pragma unroll
-            for (int r = 0; r < 2; ++r) {
-                float vs[NG], vm[NG];
+            for (int u = 0; u < TS; ++u)
 #pragma unroll
-                for (int G = 0; G < NG; ++G) {
-                    vs[G] = __uint_as_float(vp[r][G] << 16);
-                    vm[G] = fmaf(8.f, vs[G], __uint_as_float(vp[r][G] & 0xFFFF0000u));
-                }
-#pragma unroll
-                for (int nt = 0; nt < NT; ++nt) {
-                    const float2 p = make_float2(sf::ex2_ftz(d[nt][r].x), sf::ex2_ftz(d[nt][r].y));
-                    l[nt] = sf::f2_add(l[nt], p);
-                    const float2 pu = sf::f2_mul(p, per_unit[nt]);
+                for (int r = 0; r < 2; ++r) {
+                    float vs[NG], vm[NG];
 #pragma unroll
                     for (int G = 0; G < NG; ++G) {
-                        pm[nt][G] = make_float2(fmaf(p.x, vm[G], pm[nt][G].x), fmaf(p.y, vm[G], pm[nt][G].y));
-                        x[nt][G][r] = make_float2(pu.x * vs[G], pu.y * vs[G]);
-                        over = fmaxf(over, fmaxf(x[nt][G][r].x, x[nt][G][r].y));
+                        vs[G] = __uint_as_float(vp[u][r][G] << 16);
+                        vm[G] = fmaf(8.f, vs[G], __uint_as_float(vp[u][r][G] & 0xFFFF0000u));
+                    }
+                    const float top = NG == 2 ? fmaxf(vs[0], vs[NG - 1]) : vs[0];
+#pragma unroll
+                    for (int nt = 0; nt < NT; ++nt) {
+                        float2 p = sf::f2_add(make_float2(s[u][nt][2 * r], s[u][nt][2 * r + 1]), nm[nt]);
+                        p = make_float2(sf::ex2_ftz(p.x), sf::ex2_ftz(p.y));
+                        l[nt] = sf::f2_add(l[nt], p);
+#pragma unroll
+                        for (int G = 0; G < NG; ++G) pm[nt][G] = make_float2(fmaf(p.x, vm[G], pm[nt][G].x), fmaf(p.y, vm[G], pm[nt][G].y));
+                        const float2 pu = sf::f2_mul(p, per_unit[nt]);
+                        over = fmaxf(over, fmaxf(pu.x * top, pu.y * top));
+                        s[u][nt][2 * r] = p.x;
+                        s[u][nt][2 * r + 1] = p.y;
                     }
                 }
-            }
             if (__any_sync(0xffffffffu, over > 256.f)) {
 #pragma unroll
                 for (int nt = 0; nt < NT; ++nt) {
-                    // The head's largest p s, formed without the unit (2^126 at first).
-                    float2 w[NG][2], top = sf::f2(0.f);
+                    float2 top = sf::f2(0.f);  // the head's largest p s
 #pragma unroll
-                    for (int r = 0; r < 2; ++r)
+                    for (int u = 0; u < TS; ++u)
 #pragma unroll
-                        for (int G = 0; G < NG; ++G) {
-                            const float vs = __uint_as_float(vp[r][G] << 16);
-                            w[G][r] = make_float2(sf::ex2_ftz(d[nt][r].x) * vs, sf::ex2_ftz(d[nt][r].y) * vs);
-                            top = make_float2(fmaxf(top.x, w[G][r].x), fmaxf(top.y, w[G][r].y));
-                        }
+                        for (int r = 0; r < 2; ++r)
+#pragma unroll
+                            for (int G = 0; G < NG; ++G) {
+                                const float vs = __uint_as_float(vp[u][r][G] << 16);
+                                top = make_float2(fmaxf(top.x, s[u][nt][2 * r] * vs), fmaxf(top.y, s[u][nt][2 * r + 1] * vs));
+                            }
                     top = over_keys(top);
                     // Where this head's own weights fit, its unit stays.
-                    const float2 u = make_float2(top.x > 256.f * unit[nt].x ? fmaxf(top.x, UNIT_FLOOR) : unit[nt].x,
-                                                 top.y > 256.f * unit[nt].y ? fmaxf(top.y, UNIT_FLOOR) : unit[nt].y);
-                    per_unit[nt] = make_float2(1.0f / u.x, 1.0f / u.y);
+                    const float2 un = make_float2(top.x > 256.f * unit[nt].x ? fmaxf(top.x, UNIT_FLOOR) : unit[nt].x,
+                                                  top.y > 256.f * unit[nt].y ? fmaxf(top.y, UNIT_FLOOR) : unit[nt].y);
+                    per_unit[nt] = make_float2(1.0f / un.x, 1.0f / un.y);
                     const float2 f = sf::f2_mul(unit[nt], per_unit[nt]);
-                    unit[nt] = u;
+                    unit[nt] = un;
 #pragma unroll
                     for (int i = 0; i < 4 * NG; ++i) {
                         o[nt][i][0] *= f.x;
@@ -594,53 +622,58 @@ __global__ void __launch_bounds__(THREADS, NT == 1 ? 2 : 1) kv4_attention_kernel
                         o[nt][i][2] *= f.x;
                         o[nt][i][3] *= f.y;
                     }
-#pragma unroll
-                    for (int G = 0; G < NG; ++G)
-#pragma unroll
-                        for (int r = 0; r < 2; ++r) x[nt][G][r] = sf::f2_mul(w[G][r], per_unit[nt]);
                 }
             }
-            uint32_t pf[NT][NG][2];  // the B operand of O^T = V^T p^T
 #pragma unroll
-            for (int nt = 0; nt < NT; ++nt)
+            for (int u = 0; u < TS; ++u) {
+                const uint8_t* tile = rec + u * R::BYTES;
+                uint32_t pf[NT][NG][2];  // p s in O's unit, the B operand of O^T = V^T p^T
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                    for (int r = 0; r < 2; ++r) {
+                        const float2 pu = sf::f2_mul(make_float2(s[u][nt][2 * r], s[u][nt][2 * r + 1]), per_unit[nt]);
+#pragma unroll
+                        for (int G = 0; G < NG; ++G) {
+                            const float vs = __uint_as_float(vp[u][r][G] << 16);
+                            pf[nt][G][r] = transpose8(f16x2(pu.x * vs, pu.y * vs));
+                        }
+                    }
+                // O^T += V^T p^T: the lane reads its 8 elements a group of keys t, 7 - t, 8 + t, 15 - t.
+                uint32_t vw[4][NG];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const int key = (i & 1 ? 7 - t : t) + 8 * (i >> 1);
+                    const uint8_t* p = tile + R::V + key * R::ROW + (g ^ (4 * ((key >> 1) & 1))) * 4 * NG;
+                    if constexpr (NG == 2) {
+                        *reinterpret_cast<uint2*>(vw[i]) = *reinterpret_cast<const uint2*>(p);
+                    } else {
+                        vw[i][0] = *reinterpret_cast<const uint32_t*>(p);
+                    }
+                }
 #pragma unroll
                 for (int G = 0; G < NG; ++G)
 #pragma unroll
-                    for (int r = 0; r < 2; ++r) pf[nt][G][r] = transpose8(f16x2(x[nt][G][r].x, x[nt][G][r].y));
-            // O^T += V^T p^T: the lane reads its 8 elements a group of keys t, 7 - t, 8 + t, 15 - t.
-            uint32_t vw[4][NG];
+                    for (int i = 0; i < 2; ++i) {
+                        // Elements 4 i .. 4 i + 3 (two bytes) of two keys side by side in the halves of a word.
+                        const uint32_t y = __byte_perm(vw[0][G], vw[1][G], i ? 0x7632 : 0x5410), w = __byte_perm(vw[2][G], vw[3][G], i ? 0x7632 : 0x5410);
+                        const uint32_t b[4] = {(y & 0x00FF00FFu) | 0x64006400u, __byte_perm(y, 0x64646464u, 0x4341), (w & 0x00FF00FFu) | 0x64006400u,
+                                               __byte_perm(w, 0x64646464u, 0x4341)};
+                        uint32_t all[4], up[4];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const int key = (i & 1 ? 7 - t : t) + 8 * (i >> 1);
-                const uint8_t* p = rec + R::V + key * R::ROW + (g ^ (4 * ((key >> 1) & 1))) * 4 * NG;
-                if constexpr (NG == 2) {
-                    *reinterpret_cast<uint2*>(vw[i]) = *reinterpret_cast<const uint2*>(p);
-                } else {
-                    vw[i][0] = *reinterpret_cast<const uint32_t*>(p);
-                }
+                        for (int c = 0; c < 4; ++c) {
+                            all[c] = sub2(b[c], 0x64886488u);                 // 1024 + byte - 1160
+                            up[c] = sub2(b[c] & 0xFFF0FFF0u, 0x64806480u);    // 1024 + 16 code - 1152
+                        }
+#pragma unroll
+                        for (int nt = 0; nt < NT; ++nt) {
+                            mma_f16(o[nt][4 * G + i], all, pf[nt][G][0], pf[nt][G][1]);
+                            mma_f16(o[nt][4 * G + 2 + i], up, pf[nt][G][0], pf[nt][G][1]);
+                        }
+                    }
             }
-#pragma unroll
-            for (int G = 0; G < NG; ++G)
-#pragma unroll
-                for (int i = 0; i < 2; ++i) {
-                    // Elements 4 i .. 4 i + 3 (two bytes) of two keys side by side in the halves of a word.
-                    const uint32_t u = __byte_perm(vw[0][G], vw[1][G], i ? 0x7632 : 0x5410), w = __byte_perm(vw[2][G], vw[3][G], i ? 0x7632 : 0x5410);
-                    const uint32_t b[4] = {(u & 0x00FF00FFu) | 0x64006400u, __byte_perm(u, 0x64646464u, 0x4341), (w & 0x00FF00FFu) | 0x64006400u,
-                                           __byte_perm(w, 0x64646464u, 0x4341)};
-                    uint32_t all[4], up[4];
-#pragma unroll
-                    for (int c = 0; c < 4; ++c) {
-                        all[c] = sub2(b[c], 0x64886488u);                 // 1024 + byte - 1160
-                        up[c] = sub2(b[c] & 0xFFF0FFF0u, 0x64806480u);    // 1024 + 16 code - 1152
-                    }
-#pragma unroll
-                    for (int nt = 0; nt < NT; ++nt) {
-                        mma_f16(o[nt][4 * G + i], all, pf[nt][G][0], pf[nt][G][1]);
-                        mma_f16(o[nt][4 * G + 2 + i], up, pf[nt][G][0], pf[nt][G][1]);
-                    }
-                }
         }
-        used += (uint32_t)mine;
+        used += (uint32_t)steps;
 
         // ---- the warps' states side by side, then one sum over them ----
         if (round) sm100::mbar_wait(merged, (round - 1) & 1u, g_kv4_attention_status + 1, kv4::AT_WAIT);
@@ -727,49 +760,57 @@ __global__ void __launch_bounds__(THREADS, NT == 1 ? 2 : 1) kv4_attention_kernel
     }
 }
 
-// Join the pieces of the items that span CTAs: one block a (first CTA, head), its warps over the pieces.
-constexpr int JOIN_WARPS = 8;
+// Join the pieces of the items that span CTAs: blocks of JOIN_HEADS heads of a first CTA's item (spread over
+// SMs, since one SM alone takes a microsecond to fetch the pieces), JOIN warps a head, each over every
+// JOIN-th piece.
+constexpr int JOIN = 4, JOIN_HEADS = 1;
 template <typename T, int D, int HB>
-__global__ void __launch_bounds__(32 * JOIN_WARPS) kv4_join_kernel(const Args a) {
+__global__ void __launch_bounds__(32 * JOIN_HEADS * JOIN) kv4_join_kernel(const Args a) {
+    constexpr int E = D / 32;
+    __shared__ float acc_s[JOIN_HEADS][JOIN][D], l_s[JOIN_HEADS][JOIN];
     asm volatile("griddepcontrol.wait;" ::: "memory");
-    const int first = blockIdx.x, head = blockIdx.y;
+    const int first = blockIdx.x, hs = threadIdx.x / (32 * JOIN), head = blockIdx.y * JOIN_HEADS + hs, part = (threadIdx.x >> 5) % JOIN, lane = threadIdx.x & 31;
     const int2 chain = *reinterpret_cast<const int2*>(a.chain + 2 * first);
     const int pieces = chain.y, item = chain.x;
     if (pieces == 0) return;
     const int per_b = a.Hk * a.blocks;
     const int b = item / per_b, kh = (item - b * per_b) / a.blocks, hb = item - b * per_b - kh * a.blocks;
-    if (hb * HB + head >= a.group) return;
-    __shared__ float acc_s[JOIN_WARPS][D];
-    constexpr int E = D / 32;
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const bool there = hb * HB + head < a.group;
     // The first piece is its CTA's last part, the others their CTAs' first.
     auto slot = [&](int p) { return ((int64_t)2 * (first + p) + (p == 0 ? 1 : 0)) * HB + head; };
-    float m = NO_MAX, l = 0.f;
-    for (int p = lane; p < pieces; p += 32) m = fmaxf(m, a.stat[slot(p) * 2]);
-    m = sf::warp_max(m);
-    for (int p = lane; p < pieces; p += 32) {
-        const float2 st = *reinterpret_cast<const float2*>(a.stat + slot(p) * 2);
-        l = fmaf(exp2f(st.x - m), st.y, l);
-    }
-    l = sf::warp_sum(l);
-    float acc[E];
+    float m = NO_MAX, l = 0.f, acc[E];
 #pragma unroll
     for (int e = 0; e < E; ++e) acc[e] = 0.f;
+    if (there) {
+        for (int p = lane; p < pieces; p += 32) m = fmaxf(m, a.stat[slot(p) * 2]);
+        m = sf::warp_max(m);
 #pragma unroll 4
-    for (int p = warp; p < pieces; p += JOIN_WARPS) {
-        const float f = exp2f(a.stat[slot(p) * 2] - m);
-        const float* src = a.part + slot(p) * D + E * lane;
+        for (int p = part; p < pieces; p += JOIN) {
+            const float2 st = *reinterpret_cast<const float2*>(a.stat + slot(p) * 2);
+            float x[E];
+            if constexpr (E == 4) *reinterpret_cast<float4*>(x) = *reinterpret_cast<const float4*>(a.part + slot(p) * D + E * lane);
+            else *reinterpret_cast<float2*>(x) = *reinterpret_cast<const float2*>(a.part + slot(p) * D + E * lane);
+            const float f = exp2f(st.x - m);
+            l = fmaf(f, st.y, l);
 #pragma unroll
-        for (int e = 0; e < E; ++e) acc[e] = fmaf(f, src[e], acc[e]);
+            for (int e = 0; e < E; ++e) acc[e] = fmaf(f, x[e], acc[e]);
+        }
+#pragma unroll
+        for (int e = 0; e < E; ++e) acc_s[hs][part][E * lane + e] = acc[e];
+        if (lane == 0) l_s[hs][part] = l;
     }
-#pragma unroll
-    for (int e = 0; e < E; ++e) acc_s[warp][E * lane + e] = acc[e];
     __syncthreads();
-    if (threadIdx.x >= D) return;
-    float out = 0.f;
+    if (!there || part) return;
 #pragma unroll
-    for (int w = 0; w < JOIN_WARPS; ++w) out += acc_s[w][threadIdx.x];
-    ((T*)a.o)[(int64_t)b * a.ob + (int64_t)(kh * a.group + hb * HB + head) * a.oh + threadIdx.x] = sf::Dt<T>::from_f(out / l);
+    for (int w = 1; w < JOIN; ++w) {
+        l += l_s[hs][w];
+#pragma unroll
+        for (int e = 0; e < E; ++e) acc[e] += acc_s[hs][w][E * lane + e];
+    }
+    const float inv = 1.0f / l;
+    T* out = (T*)a.o + (int64_t)b * a.ob + (int64_t)(kh * a.group + hb * HB + head) * a.oh + E * lane;
+#pragma unroll
+    for (int e = 0; e < E; e += 2) *reinterpret_cast<uint32_t*>(out + e) = sf::Pair<T>::from_f2(make_float2(acc[e] * inv, acc[e + 1] * inv));
 }
 
 // Most tiles a request can see, from the table's width, window and sinks alone.
@@ -791,14 +832,16 @@ Plan plan_of(int64_t B, int64_t Hq, int64_t Hk, int64_t D, int64_t width, int64_
     p.nt = group > 8 ? 2 : 1;
     p.blocks = (int)((group + 8 * p.nt - 1) / (8 * p.nt));
     const int64_t items = B * Hk * p.blocks;
-    const int64_t wave = (int64_t)sf::sm_count() * (p.nt == 1 ? 2 : 1);
+    const int64_t wave = (int64_t)sf::sm_count() * ctas_of(p.nt);
     const int64_t tiles = most_tiles(width, tpp, window, sinks);
-    // Whole items a CTA while an item is at most two tiles a warp: nothing to join, no second
-    // launch.  Longer items are cut so that every CTA gets the same number of tiles.
-    p.split = tiles > 2 * WARPS;
+    // Whole items a CTA while an item is at most four tiles a warp: nothing to join, no second
+    // launch.  Longer items are cut so that every CTA gets the same number of tiles.  (Above 1024
+    // requests the items balance the CTAs by themselves, and the prefix of the costs would take the
+    // shared memory.)
+    p.split = tiles > LEAST && B <= 1024;
     if (variant == 3) p.split = false;
     if (variant == 1) p.split = true;
-    p.grid = (int)(p.split ? std::min(wave, std::max<int64_t>(1, (items * tiles + WARPS - 1) / WARPS)) : items);
+    p.grid = (int)(p.split ? std::min(wave, std::max<int64_t>(1, (items * (tiles + ITEM_COST) + LEAST - 1) / LEAST)) : items);
     return p;
 }
 
@@ -831,8 +874,8 @@ int launch_t(Args a, const Plan& p, cudaStream_t st, char* err, uint64_t cap) {
     if (rc || !p.split) return rc;
     // The join starts while the last CTAs of the first kernel run, and waits for all of it.
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned)p.grid, (unsigned)std::min(HB, a.group));
-    cfg.blockDim = dim3(32 * JOIN_WARPS);
+    cfg.gridDim = dim3((unsigned)p.grid, (unsigned)((std::min(HB, a.group) + JOIN_HEADS - 1) / JOIN_HEADS));
+    cfg.blockDim = dim3(32 * JOIN_HEADS * JOIN);
     cfg.stream = st;
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
