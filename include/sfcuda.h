@@ -332,17 +332,22 @@ SF_API int sf_kv4_attention(const sf_kv4_attention_args* args, void* stream, cha
  * (window 0: all j <= p).  A query that sees nothing gives zeros; rows of no sequence are left as they
  * were.  D <= 256; tcgen05 kernel for D in {64, 128}, 16-byte aligned tensors, strides that are
  * multiples of 8 elements and at most 128 query heads a key head (variant 1 forces it), general kernel
- * otherwise (variant 2).
+ * otherwise (variant 2).  With a workspace (16-byte aligned, sf_window_attention_workspace_bytes bytes, no
+ * initial content; two calls that overlap on the GPU need one each) few queries with many keys are split
+ * over the keys and joined; with none, or with variant 4, they are not.
  */
 typedef struct sf_window_attention_args {
     const void *q, *k, *v, *cu_q, *cu_k;
-    void* o;
+    void *o, *workspace;
+    uint64_t workspace_bytes;
     int64_t Tq, Tk, seqs, Hq, Hk, D;
     sf_rows q_rows, k_rows, v_rows, o_rows;
     int64_t window, sinks;
     double scale;
     int32_t dtype, variant;
 } sf_window_attention_args;
+SF_API uint64_t sf_window_attention_workspace_bytes(int64_t Tq, int64_t Tk, int64_t seqs, int64_t Hq, int64_t Hk, int64_t D,
+               int64_t window, int64_t sinks);
 SF_API int sf_window_attention(const sf_window_attention_args* args, void* stream, char* err, uint64_t cap);
 
 /*

@@ -102,7 +102,7 @@ ARGS = {
     "sf_kv4_store": struct.Struct("4P 5q 4q 2i"),
     "sf_kv4_load": struct.Struct("4P 5q 4q 2i"),
     "sf_kv4_attention": struct.Struct("6P Q 8q 4q 2q d 2i"),
-    "sf_window_attention": struct.Struct("6P 6q 8q 2q d 2i"),
+    "sf_window_attention": struct.Struct("7P Q 6q 8q 2q d 2i"),
 }
 
 _P = ctypes.c_void_p
@@ -146,6 +146,7 @@ SIGNATURES: dict[str, tuple[object, tuple]] = {
     "sf_kv4_load": (ctypes.c_int, (_P, _P, *_ERR)),
     "sf_kv4_attention_workspace_bytes": (_U64, (_I64,) * 8 + (_I32,)),
     "sf_kv4_attention": (ctypes.c_int, (_P, _P, *_ERR)),
+    "sf_window_attention_workspace_bytes": (_U64, (_I64,) * 8),
     "sf_window_attention": (ctypes.c_int, (_P, _P, *_ERR)),
     "sf_gemm_nt": (ctypes.c_int, (_P, _P, _P, _I64, _I64, _I64, _I32, _P, *_ERR)),
     "sf_gemm_nn_workspace_bytes": (_U64, (_I64, _I64, _I64, _I32)),

@@ -221,7 +221,7 @@ static int dispatch(const sf_op_desc* d, const void* const* a, cudaStream_t s, c
         case SF_OP_WINDOW_ATTENTION: {
             const int64_t Hq = d->dims[3], Hk = d->dims[4], D = d->dims[5];
             const sf_rows q = {Hq * D, D}, k = {Hk * D, D};
-            const sf_window_attention_args x = {a[0], a[1], a[2], a[3], a[4], (void*)a[5], d->dims[0], d->dims[1], d->dims[2], Hq, Hk, D,
+            const sf_window_attention_args x = {a[0], a[1], a[2], a[3], a[4], (void*)a[5], nullptr, 0, d->dims[0], d->dims[1], d->dims[2], Hq, Hk, D,
                                                 q, k, k, q, d->dims[6], d->dims[7], d->attrs[0], d->dtype, d->variant};
             return sf_window_attention(&x, s, err, cap);
         }

@@ -30,6 +30,8 @@ struct Args {
     int seqs, group, heads;                  // sequences, query heads a kv head, query heads
     int window, sinks;
     float scale_log2;
+    int splits;          // CTAs that share a row tile's keys; above 1 each leaves its state for the join:
+    float *part, *stat;  // [splits][tq][heads][D] unnormalised outputs, [splits][tq][heads][2] running max, sum
 };
 
 // Keys [0, sinks) and [low, high) of a query at position p.
@@ -159,10 +161,12 @@ struct Layout {
 // included, can run on the uniform datapath, where the tensor instructions take their operands from.
 __device__ __forceinline__ int uniform(int x) { return __shfl_sync(0xffffffffu, x, 0); }
 
-// The key tiles of a CTA: sinks [0, sink_end), then [low, high) in steps of 128.
+// The key tiles of a CTA: sinks [0, sink_end), then [low, high) in steps of 128; of these the n from `base` on
+// are this split's (tile j below is j - base of the CTA's own).
 struct Walk {
-    int sink_end, sink_tiles, low, high, n;
-    __device__ __forceinline__ int start(int j) const { return j < sink_tiles ? 128 * j : low + 128 * (j - sink_tiles); }
+    int sink_end, sink_tiles, low, high, base, n;
+    __device__ __forceinline__ bool in_sinks(int j) const { return j + base < sink_tiles; }
+    __device__ __forceinline__ int start(int j) const { return in_sinks(j) ? 128 * (j + base) : low + 128 * (j + base - sink_tiles); }
 };
 
 // What one of the CTA's two row tiles makes of them.
@@ -179,16 +183,54 @@ struct Span {
         skip = a.window && last >= 0 && w.low + 128 <= first - a.window + 1 && w.low >= a.sinks ? 1 : 0;
     }
     // Keys [0, count) of tile j can be seen.
-    __device__ __forceinline__ int count(const Walk& w, int j) const { return max(0, min(128, (j < w.sink_tiles ? w.sink_end : end) - w.start(j))); }
+    __device__ __forceinline__ int count(const Walk& w, int j) const { return max(0, min(128, (w.in_sinks(j) ? w.sink_end : end) - w.start(j))); }
     __device__ __forceinline__ bool active(const Walk& w, int j) const {
-        return last >= 0 && (j < w.sink_tiles || (w.start(j) < end && !(skip && j == w.sink_tiles)));
+        return last >= 0 && (w.in_sinks(j) || (w.start(j) < end && !(skip && j + w.base == w.sink_tiles)));
     }
     // Every row sees all 128 keys of tile j.
     __device__ __forceinline__ bool full(const Walk& w, int j, int sinks) const {
         const int s = w.start(j);
-        return j < w.sink_tiles ? s + 128 <= w.sink_end : s + 127 <= first && (s >= front || s + 128 <= sinks);
+        return w.in_sinks(j) ? s + 128 <= w.sink_end : s + 127 <= first && (s >= front || s + 128 <= sinks);
     }
 };
+
+// Where a CTA's tokens lie: its sequence's rows and keys, its first token and that one's position.
+struct Where {
+    int qe, kb, ke, tok0, pos0;
+};
+// Sequence i owns the slots from cu_q[i] / TT + i on, TT tokens each, which leaves out no token whatever the
+// lengths and needs no prefix of tile counts; false: a slot without tokens.  Every lane of the warp.
+__device__ __forceinline__ bool locate(const Args& a, int TT, int slot, Where* w) {
+    const int lane = threadIdx.x & 31;
+    int lo = 0, hi = a.seqs, qb = 0;
+    while (true) {
+        const int step = max(1, (hi - lo + 31) >> 5);
+        const int i = min(lo + lane * step, a.seqs);
+        const int q_here = __ldg(a.cu_q + i), k_here = step == 1 ? __ldg(a.cu_k + i) : 0;
+        const bool here = lo + lane * step < hi && min(max(0, q_here), (int)a.tq) / TT + i <= slot;
+        const uint32_t yes = __ballot_sync(0xffffffffu, here);
+        const int k = yes ? 31 - __clz(yes) : 0;
+        if (step > 1) {
+            lo = lo + k * step;
+            hi = min(hi, lo + step);
+            continue;
+        }
+        // The bounds come from the lanes k and k + 1.
+        const int top_q = k < 31 ? __shfl_sync(0xffffffffu, q_here, min(k + 1, 31)) : __ldg(a.cu_q + lo + 32);
+        const int top_k = k < 31 ? __shfl_sync(0xffffffffu, k_here, min(k + 1, 31)) : __ldg(a.cu_k + lo + 32);
+        qb = min(max(0, __shfl_sync(0xffffffffu, q_here, k)), (int)a.tq);
+        w->qe = max(qb, min(top_q, (int)a.tq));
+        w->kb = min(max(0, __shfl_sync(0xffffffffu, k_here, k)), (int)a.tk);
+        w->ke = max(w->kb, min(top_k, (int)a.tk));
+        lo += k;
+        break;
+    }
+    const int64_t at = qb + (int64_t)(slot - qb / TT - lo) * TT;
+    if (at < qb || at >= w->qe) return false;
+    w->tok0 = uniform((int)at);
+    w->pos0 = (w->tok0 - qb) + (w->ke - w->kb) - (w->qe - qb);
+    return true;
+}
 
 // Bits [0, n) of a 32-bit word.
 __device__ __forceinline__ uint32_t below(int n) { return n <= 0 ? 0u : (n >= 32 ? 0xFFFFFFFFu : (1u << n) - 1u); }
@@ -343,48 +385,24 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
     }
     sm100::fence_proxy_async_smem();
 
-    // ---- which tokens: sequence i owns the slots from cu[i] / TT + i on, later tiles (more keys) first ----
-    const int TT = 2 * tq_tile;
-    const int slot = gridDim.x - 1 - blockIdx.x;
-    int lo = 0, hi = a.seqs;
-    int qb, qe, kb, ke;
-    int q_here = 0, k_here = 0;  // both tables at lo + lane, after a round in steps of one
-    bool at_hand = false;
-    while (hi - lo > 1 || !at_hand) {
-        const int step = max(1, (hi - lo + 31) >> 5);
-        const int i = min(lo + lane * step, a.seqs);
-        q_here = __ldg(a.cu_q + i);
-        if (step == 1) k_here = __ldg(a.cu_k + i);
-        const bool here = lo + lane * step < hi && min(max(0, q_here), (int)a.tq) / TT + i <= slot;
-        const uint32_t yes = __ballot_sync(0xffffffffu, here);
-        const int k = yes ? 31 - __clz(yes) : 0;
-        if (step == 1) {
-            at_hand = true;
-            // The bounds come from the lanes k and k + 1.
-            const int top_q = k < 31 ? __shfl_sync(0xffffffffu, q_here, min(k + 1, 31)) : __ldg(a.cu_q + lo + 32);
-            const int top_k = k < 31 ? __shfl_sync(0xffffffffu, k_here, min(k + 1, 31)) : __ldg(a.cu_k + lo + 32);
-            qb = min(max(0, __shfl_sync(0xffffffffu, q_here, k)), (int)a.tq);
-            qe = max(qb, min(top_q, (int)a.tq));
-            kb = min(max(0, __shfl_sync(0xffffffffu, k_here, k)), (int)a.tk);
-            ke = max(kb, min(top_k, (int)a.tk));
-            lo += k;
-            hi = lo;
-        } else {
-            lo = lo + k * step;
-            hi = min(hi, lo + step);
-        }
-    }
-    const int64_t tok_at = qb + (int64_t)(slot - qb / TT - lo) * TT;
-    if (tok_at < qb || tok_at >= qe) return;  // a slot that rounding left over
-    const int tok0 = uniform((int)tok_at);
-    const int rows_tok[2] = {min(tq_tile, qe - tok0), max(0, min(tq_tile, qe - tok0 - tq_tile))};
-    const int pos0 = uniform((tok0 - qb) + (ke - kb) - (qe - qb));  // position of the CTA's first token
+    Where at;
+    const bool found = locate(a, 2 * tq_tile, gridDim.x - 1 - blockIdx.x, &at);
+    if (!found) return;  // a slot that rounding left over
+    const int tok0 = at.tok0, kb = at.kb, ke = at.ke;
+    const int rows_tok[2] = {min(tq_tile, at.qe - tok0), max(0, min(tq_tile, at.qe - tok0 - tq_tile))};
+    const int pos0 = uniform(at.pos0);
     Walk w;
     w.high = max(0, pos0 + uniform(rows_tok[0] + rows_tok[1]));
     w.low = uniform(a.window ? max(0, pos0 - a.window + 1) : 0);
     w.sink_end = min(a.sinks, w.low);
     w.sink_tiles = (w.sink_end + 127) >> 7;
     w.n = w.high > 0 ? w.sink_tiles + ((w.high - w.low + 127) >> 7) : 0;
+    w.base = 0;
+    if (a.splits > 1) {
+        const int n = w.n;
+        w.base = (int)((int64_t)n * blockIdx.z / a.splits);
+        w.n = (int)((int64_t)n * (blockIdx.z + 1) / a.splits) - w.base;
+    }
     const Span span0(a, w, pos0, uniform(rows_tok[0])), span1(a, w, pos0 + tq_tile, uniform(rows_tok[1]));
 
     if (warp == 1) {
@@ -500,7 +518,8 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
                     ++turns1;
                 };
                 // Tiles [whole0, whole1) have 128 keys for both.
-                const int whole0 = w.sink_tiles + (span0.skip | span1.skip), whole1 = span0.last >= 0 && span1.last >= 0 ? w.sink_tiles + (min(span0.end, span1.end) - w.low) / 128 : 0;
+                const int whole0 = w.sink_tiles + (span0.skip | span1.skip) - w.base;
+                const int whole1 = span0.last >= 0 && span1.last >= 0 ? min(w.n, w.sink_tiles + (min(span0.end, span1.end) - w.low) / 128 - w.base) : 0;
                 if (span0.last >= 0) wait(&bars->q_full[0], 0, 124);
                 if (span1.last >= 0) wait(&bars->q_full[1], 0, 124);
                 int keys0 = 0, keys1 = 0;         // of tile j - 1, 0: it is not for that row tile
@@ -599,7 +618,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
                 // and (c >= begin or c < sink).
                 const int chunks = (span.count(w, j) + 31) >> 5;
                 const int start = w.start(j);
-                const bool in_sinks = j < w.sink_tiles;
+                const bool in_sinks = w.in_sinks(j);
                 const int end = in_sinks ? (p >= 0 ? w.sink_end - start : 0) : p + 1 - start;
                 const int begin = in_sinks || !a.window ? 0 : p - a.window + 1 - start;
                 const int sink = a.sinks - start;
@@ -639,46 +658,76 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
         float2 nan = sf::f2(0.f);
         if (w.n > 0) ok = wait_soon(&bars->o_done[t], 0, status, 128) && ok;
         sm100::tc_fence_after();
-        const bool none = turn == 0 || p < 0;
-        const float inv = 1.0f / s.l;
-        constexpr int PIECES = D / 8;
-        uint4* stage = reinterpret_cast<uint4*>(smem + L::Q + t * L::TILE) + (warp & 3) * 32 * PIECES;
+        if (a.splits > 1) {
+            // The row's state for the join, O as it is: half its columns at a time through the Q buffer.
+            const bool own = live && ok;
+            const int64_t row_at = ((int64_t)blockIdx.z * a.tq + tok0 + t * tq_tile + tok) * a.heads + kvh * a.group + row - tok * a.group;
+            if (own) *reinterpret_cast<float2*>(a.stat + 2 * row_at) = make_float2(turn ? s.m : -INFINITY, s.l);
+            const uint32_t written = __ballot_sync(0xffffffffu, own);
+            constexpr int PIECES = D / 8;  // 16-byte pieces of half a row
+            uint4* stage = reinterpret_cast<uint4*>(smem + L::Q + t * L::TILE) + (warp & 3) * 32 * PIECES;
 #pragma unroll 1
-        for (int c = 0; c < D / 32; ++c) {
-            uint32_t r[32];
-            sm100::tmem_ld_32x32b_x32(to + 32u * c, r);
-            sm100::tmem_ld_wait();
+            for (int half = 0; half < 2 && turn; ++half) {
+#pragma unroll 1
+                for (int c = 0; c < D / 64; ++c) {
+                    uint32_t r[32];
+                    sm100::tmem_ld_32x32b_x32(to + (uint32_t)(half * D / 2 + 32 * c), r);
+                    sm100::tmem_ld_wait();
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                uint32_t o4[4];
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    float2 x = make_float2(__uint_as_float(r[8 * i + 2 * e]) * inv, __uint_as_float(r[8 * i + 2 * e + 1]) * inv);
-                    if (none) x = make_float2(0.f, 0.f);
-                    nan = sf::f2_fma(x, sf::f2(0.f), nan);  // 0, or NaN once a NaN or an infinity has passed
-                    o4[e] = sf::Pair<T>::from_f2(x);
+                    for (int i = 0; i < 8; ++i) stage[lane * PIECES + ((8 * c + i) ^ (lane & 7))] = make_uint4(r[4 * i], r[4 * i + 1], r[4 * i + 2], r[4 * i + 3]);
                 }
-                stage[lane * PIECES + ((4 * c + i) ^ (lane & 7))] = make_uint4(o4[0], o4[1], o4[2], o4[3]);
-            }
-        }
-        const bool again = live && ok && !(nan.x + nan.y == 0.f);
-        const int64_t mine = (int64_t)(tok0 + t * tq_tile + tok) * a.ot + (int64_t)(kvh * a.group + row - tok * a.group) * a.oh;
-        __syncwarp();
-        const uint32_t written = __ballot_sync(0xffffffffu, live && ok);
+                __syncwarp();
 #pragma unroll 4
-        for (int i = lane; i < 32 * PIECES; i += 32) {
-            const int rl = i / PIECES, piece = i % PIECES;
-            const int64_t at = __shfl_sync(0xffffffffu, mine, rl);
-            const uint4 x = stage[rl * PIECES + (piece ^ (rl & 7))];
-            if (written >> rl & 1u) *reinterpret_cast<uint4*>((T*)a.o + at + 8 * piece) = x;
-        }
-        __syncwarp();
-        for (uint32_t todo = __ballot_sync(0xffffffffu, again); todo; todo &= todo - 1) {
-            const int src = __ffs(todo) - 1;
-            const int rw = (warp & 3) * 32 + src;
-            const int tk = rw / a.group, hd = kvh * a.group + rw - tk * a.group;
-            const int64_t qrow = (int64_t)tok0 + t * tq_tile + tk;
-            row_by_warp<T>(a, D, qrow, hd, kb, first + tk, (T*)a.o + qrow * a.ot + (int64_t)hd * a.oh);
+                for (int i = lane; i < 32 * PIECES; i += 32) {
+                    const int rl = i / PIECES, piece = i % PIECES;
+                    const int64_t at = __shfl_sync(0xffffffffu, row_at, rl);
+                    const uint4 x = stage[rl * PIECES + (piece ^ (rl & 7))];
+                    if (written >> rl & 1u) *reinterpret_cast<uint4*>(a.part + at * D + half * D / 2 + 4 * piece) = x;
+                }
+                __syncwarp();
+            }
+        } else {
+            const bool none = turn == 0 || p < 0;
+            const float inv = 1.0f / s.l;
+            constexpr int PIECES = D / 8;
+            uint4* stage = reinterpret_cast<uint4*>(smem + L::Q + t * L::TILE) + (warp & 3) * 32 * PIECES;
+#pragma unroll 1
+            for (int c = 0; c < D / 32; ++c) {
+                uint32_t r[32];
+                sm100::tmem_ld_32x32b_x32(to + 32u * c, r);
+                sm100::tmem_ld_wait();
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    uint32_t o4[4];
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        float2 x = make_float2(__uint_as_float(r[8 * i + 2 * e]) * inv, __uint_as_float(r[8 * i + 2 * e + 1]) * inv);
+                        if (none) x = make_float2(0.f, 0.f);
+                        nan = sf::f2_fma(x, sf::f2(0.f), nan);  // 0, or NaN once a NaN or an infinity has passed
+                        o4[e] = sf::Pair<T>::from_f2(x);
+                    }
+                    stage[lane * PIECES + ((4 * c + i) ^ (lane & 7))] = make_uint4(o4[0], o4[1], o4[2], o4[3]);
+                }
+            }
+            const bool again = live && ok && !(nan.x + nan.y == 0.f);
+            const int64_t mine = (int64_t)(tok0 + t * tq_tile + tok) * a.ot + (int64_t)(kvh * a.group + row - tok * a.group) * a.oh;
+            __syncwarp();
+            const uint32_t written = __ballot_sync(0xffffffffu, live && ok);
+#pragma unroll 4
+            for (int i = lane; i < 32 * PIECES; i += 32) {
+                const int rl = i / PIECES, piece = i % PIECES;
+                const int64_t at = __shfl_sync(0xffffffffu, mine, rl);
+                const uint4 x = stage[rl * PIECES + (piece ^ (rl & 7))];
+                if (written >> rl & 1u) *reinterpret_cast<uint4*>((T*)a.o + at + 8 * piece) = x;
+            }
+            __syncwarp();
+            for (uint32_t todo = __ballot_sync(0xffffffffu, again); todo; todo &= todo - 1) {
+                const int src = __ffs(todo) - 1;
+                const int rw = (warp & 3) * 32 + src;
+                const int tk = rw / a.group, hd = kvh * a.group + rw - tk * a.group;
+                const int64_t qrow = (int64_t)tok0 + t * tq_tile + tk;
+                row_by_warp<T>(a, D, qrow, hd, kb, first + tk, (T*)a.o + qrow * a.ot + (int64_t)hd * a.oh);
+            }
         }
     }
     sm100::tc_fence_before();
@@ -687,13 +736,94 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
     if (warp == 1) sm100::tmem_dealloc(tmem, 512);
 }
 
+// Join the splits of every row, a warp a row; the CTAs and their rows are those of the kernel above.
+template <typename T, int D>
+__global__ void __launch_bounds__(256) window_join_kernel(const Args a, int tq_tile) {
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    Where at;
+    if (!locate(a, 2 * tq_tile, blockIdx.x, &at)) return;
+    const int lane = threadIdx.x & 31, kvh = blockIdx.y;
+    const int tokens = min(2 * tq_tile, at.qe - at.tok0);
+    constexpr int E = D / 32;
+    for (int r = threadIdx.x >> 5; r < tokens * a.group; r += 8) {
+        const int tok = r / a.group, head = kvh * a.group + r - tok * a.group;
+        const int64_t row = at.tok0 + tok, row_at = row * a.heads + head, all = a.tq * a.heads;
+        float m = -INFINITY;
+        for (int z = lane; z < a.splits; z += 32) {
+            const float mz = a.stat[2 * (z * all + row_at)];
+            m = mz > m || mz != mz ? mz : m;
+        }
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) {
+            const float other = __shfl_xor_sync(0xffffffffu, m, o);
+            m = other > m || other != other ? other : m;
+        }
+        float l = 0.f, acc[E];
+#pragma unroll
+        for (int e = 0; e < E; ++e) acc[e] = 0.f;
+#pragma unroll 4
+        for (int z = 0; z < a.splits; ++z) {
+            const float2 st = *reinterpret_cast<const float2*>(a.stat + 2 * (z * all + row_at));
+            if (st.x == -INFINITY) continue;  // that split saw nothing and left no output
+            float x[E];
+            if constexpr (E == 4) *reinterpret_cast<float4*>(x) = *reinterpret_cast<const float4*>(a.part + (z * all + row_at) * D + E * lane);
+            else *reinterpret_cast<float2*>(x) = *reinterpret_cast<const float2*>(a.part + (z * all + row_at) * D + E * lane);
+            const float f = exp2f(st.x - m);
+            l = fmaf(f, st.y, l);
+#pragma unroll
+            for (int e = 0; e < E; ++e) acc[e] = fmaf(f, x[e], acc[e]);
+        }
+        const int p = at.pos0 + tok;
+        const float inv = 1.0f / l;
+        bool again = false;
+        T* out = (T*)a.o + row * a.ot + (int64_t)head * a.oh;
+#pragma unroll
+        for (int e = 0; e < E; e += 2) {
+            float2 x = make_float2(acc[e] * inv, acc[e + 1] * inv);
+            if (p < 0) x = make_float2(0.f, 0.f);
+            again |= !(x.x * 0.f + x.y * 0.f == 0.f);
+            *reinterpret_cast<uint32_t*>(out + E * lane + e) = sf::Pair<T>::from_f2(x);
+        }
+        if (__any_sync(0xffffffffu, again)) {
+            __syncwarp();
+            row_by_warp<T>(a, D, row, head, at.kb, p, out);
+        }
+    }
+}
+
+// CTAs that share a row tile's keys.  A tile of 128 keys takes a CTA about 1.5 us, a CTA's start and end
+// about three of them, and a row's state leaves and comes back through L2: the number of splits with the
+// least sum of waves x (tiles + 3) and the join.  The lengths are on the GPU, so the tiles are those of
+// sequences of equal length; the number of CTAs is known but for the rounding of each sequence.
+int64_t splits_of(int64_t Tq, int64_t Tk, int64_t seqs, int64_t Hq, int64_t Hk, int64_t D, int64_t window, int64_t sinks) {
+    const int64_t group = Hq / Hk;
+    if ((D != 64 && D != 128) || group > 128 || Tk == 0 || seqs == 0) return 1;
+    const int64_t tt = 2 * (128 / group), ctas = (Tq / tt + seqs) * Hk;
+    int64_t keys = Tk / seqs;
+    if (window) keys = std::min(keys, window + tt + (sinks ? std::min<int64_t>(sinks, keys) : 0));
+    const int64_t tiles = (keys + 127) / 128;
+    double best = 1e30;
+    int64_t pick = 1;
+    for (int64_t z : {1, 2, 3, 4, 6, 8, 12, 16, 24, 32}) {
+        if (z > 1 && tiles / z < 2) break;
+        const int64_t waves = (ctas * z + sf::sm_count() - 1) / sf::sm_count();
+        double cost = (double)waves * ((tiles + z - 1) / z + 3);
+        if (z > 1) cost += 3 + (double)Tq * Hq * D * 8 * z / 9e6;  // 9 MB of states in a tile's time
+        if (cost < best) {
+            best = cost;
+            pick = z;
+        }
+    }
+    return pick;
+}
+
 // Whether the tensor-core kernel takes these tensors; `rows` token and head strides of an [n, h, D] tensor.
 bool tc_rows(const void* p, int64_t token, int64_t head, int64_t n, int64_t h) {
     return sf::aligned16(p) && (n <= 1 || (token > 0 && token % 8 == 0)) && (h <= 1 || (head > 0 && head % 8 == 0));
 }
 
 template <typename T, int D>
-int launch_tc(const Args& a, int64_t hk, bool* taken, cudaStream_t st, char* err, uint64_t cap) {
+int launch_tc(Args a, int64_t hk, bool* taken, cudaStream_t st, char* err, uint64_t cap) {
     const bool bf16 = std::is_same<T, __nv_bfloat16>::value;
     const int tq_tile = 128 / a.group;
     auto map = [&](CUtensorMap* m, const void* p, int64_t token, int64_t head, int64_t n, int64_t h, int bh, int bn) {
@@ -718,8 +848,21 @@ int launch_tc(const Args& a, int64_t hk, bool* taken, cudaStream_t st, char* err
     }
     const int64_t slots = a.tq / (2 * tq_tile) + a.seqs;
     if (slots > 0x7fffffffLL) return sf::fail(SF_EINVAL, err, cap, "window_attention: grid too large");
-    window_tc_kernel<T, D><<<dim3((unsigned)slots, (unsigned)hk), TC_THREADS, smem, st>>>(a, mq, mk, mk16, mv, mv16, tq_tile);
-    return sf::check_launch("window_attention launch", err, cap);
+    window_tc_kernel<T, D><<<dim3((unsigned)slots, (unsigned)hk, (unsigned)a.splits), TC_THREADS, smem, st>>>(a, mq, mk, mk16, mv, mv16, tq_tile);
+    int rc = sf::check_launch("window_attention launch", err, cap);
+    if (rc || a.splits == 1) return rc;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)slots, (unsigned)hk);
+    cfg.blockDim = dim3(256);
+    cfg.stream = st;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    const cudaError_t e = cudaLaunchKernelEx(&cfg, window_join_kernel<T, D>, (const Args)a, (int)tq_tile);
+    if (e != cudaSuccess) return sf::fail(SF_EDEVICE, err, cap, "window_attention join launch: %s", cudaGetErrorString(e));
+    return SF_OK;
 }
 
 template <typename T>
@@ -732,6 +875,13 @@ int launch_general(const Args& a, int64_t D, cudaStream_t st, char* err, uint64_
 }
 
 }  // namespace
+
+extern "C" uint64_t sf_window_attention_workspace_bytes(int64_t Tq, int64_t Tk, int64_t seqs, int64_t Hq, int64_t Hk, int64_t D, int64_t window,
+                                                        int64_t sinks) {
+    if (Tq <= 0 || Tk <= 0 || seqs <= 0 || Hq <= 0 || Hk <= 0 || Hq % Hk || window < 0 || sinks < 0) return 0;
+    const int64_t z = splits_of(Tq, Tk, seqs, Hq, Hk, D, window, sinks);
+    return z > 1 ? (uint64_t)(z * Tq * Hq * (D + 2) * 4) : 0;
+}
 
 extern "C" int sf_window_attention(const sf_window_attention_args* x, void* stream, char* err, uint64_t cap) {
     if (!x) return sf::fail(SF_EINVAL, err, cap, "window_attention: null arguments");
@@ -758,6 +908,15 @@ extern "C" int sf_window_attention(const sf_window_attention_args* x, void* stre
     a.window = (int)std::min<int64_t>(x->window, 0x7fffffff);
     a.sinks = x->window ? (int)std::min<int64_t>(x->sinks, 0x7fffffff) : 0;
     a.scale_log2 = scale * LOG2E;
+    a.splits = 1;
+    if (x->variant != 4) {
+        const int64_t z = splits_of(Tq, Tk, seqs, Hq, Hk, D, x->window, x->sinks);
+        if (z > 1 && x->workspace && sf::aligned16(x->workspace) && x->workspace_bytes >= (uint64_t)(z * Tq * Hq * (D + 2) * 4)) {
+            a.splits = (int)z;
+            a.part = (float*)x->workspace;
+            a.stat = a.part + z * Tq * Hq * D;
+        }
+    }
     cudaStream_t st = (cudaStream_t)stream;
     const bool half = x->dtype == SF_DTYPE_F16;
     const bool tc = (D == 64 || D == 128) && a.group <= 128 && Hk <= 65535 && Tk > 0 && tc_rows(a.q, a.qt, a.qh, Tq, Hq) && tc_rows(a.k, a.kt, a.kh, Tk, Hk) &&

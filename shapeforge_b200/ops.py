@@ -531,6 +531,13 @@ def _check_vector(t: torch.Tensor, name: str, dev: int, dtype: torch.dtype, leng
         raise ValueError(f"{name} must be contiguous with one axis{'' if length is None else f' of {length}'}, got shape {tuple(t.shape)}")
 
 
+def _workspace_bytes(t: torch.Tensor, dev: int) -> int:
+    _gpu(t, "workspace", dev)
+    if not t.is_contiguous():
+        raise ValueError("workspace must be contiguous")
+    return t.numel() * t.element_size()
+
+
 def _launch(name: str, dev: int, *fields) -> None:
     """Call a serving entry point on GPU ``dev``'s current stream, with that GPU current (the C ABI
     launches on the thread's current device); entering it costs more than the launch, so only if need be.
@@ -679,18 +686,22 @@ def kv4_attention(q: torch.Tensor, cache: torch.Tensor, block_table: torch.Tenso
         if need:
             workspace = cache.new_empty(need)
     else:
-        need = workspace.numel() * workspace.element_size()
-        _gpu(workspace, "workspace", dev)
-        if not workspace.is_contiguous():
-            raise ValueError("workspace must be contiguous")
+        need = _workspace_bytes(workspace, dev)
     _launch("sf_kv4_attention", dev, q.data_ptr(), cache.data_ptr(), block_table.data_ptr(), seq_lens.data_ptr(), out.data_ptr(),
             0 if workspace is None else workspace.data_ptr(), need, b, hq, heads, d, pages, page, width,
             block_table.stride(0) if b > 1 else 0, *qs, *os_, window, sinks, scale, _native.DTYPE_CODES[dtype_name(q)], variant)
     return out
 
 
+def window_attention_workspace_bytes(q_tokens: int, k_tokens: int, sequences: int, q_heads: int, kv_heads: int, dim: int, window: int = 0,
+                                     sinks: int = 0) -> int:
+    """Workspace bytes of :func:`window_attention` (0 when the keys of a row tile stay with one CTA)."""
+    return int(_native.load().sf_window_attention_workspace_bytes(q_tokens, k_tokens, sequences, q_heads, kv_heads, dim, window, sinks))
+
+
 def window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqlens: torch.Tensor, scale: float, window: int = 0, sinks: int = 0,
-                     cu_seqlens_k: torch.Tensor | None = None, out: torch.Tensor | None = None, variant: int = 0) -> torch.Tensor:
+                     cu_seqlens_k: torch.Tensor | None = None, out: torch.Tensor | None = None, workspace: torch.Tensor | None = None,
+                     variant: int = 0) -> torch.Tensor:
     """Causal attention of packed prompts with grouped heads, a sliding window and sinks.
 
     ``q [Tq, Hq, D]``, ``k, v [Tk, Hk, D]`` (unit stride along D, Hq a multiple of Hk); sequence ``s`` has
@@ -699,8 +710,10 @@ def window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqle
     keys ``j <= p`` with ``j > p - window`` or ``j < sinks`` (``window`` 0: all ``j <= p``), so a prompt's next
     chunk comes with its whole context as keys.  A query that sees nothing gives zeros; rows of ``out``
     that belong to no sequence are left as they were.  D up to 256; D 64 and 128 with 16-byte aligned
-    rows and at most 128 query heads a key head run on the tensor cores.  ``variant``: 0 = by shape, 1 =
-    tensor cores (refused where they do not apply), 2 = general kernel."""
+    rows and at most 128 query heads a key head run on the tensor cores, where few queries with many keys
+    are split over the keys by way of ``workspace`` (uint8, :func:`window_attention_workspace_bytes`,
+    allocated here when not given; calls that overlap on the GPU need one each).  ``variant``: 0 = by
+    shape, 1 = tensor cores (refused where they do not apply), 2 = general kernel, 4 = unsplit."""
     dev = _gpu(q, "q")
     dtype = q.dtype
     qs, ks = _check_rows(q, "q", dev), _check_rows(k, "k", dev, dtype)
@@ -723,6 +736,12 @@ def window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqle
         out, os_ = q.new_empty((tq, hq, d)), (hq * d, d)
     else:
         os_ = _check_rows(out, "out", dev, dtype, q.shape, written=True)
+    if workspace is None:
+        need = 0 if variant in (2, 4) else window_attention_workspace_bytes(tq, tk, seqs, hq, hk, d, window, sinks)
+        if need:
+            workspace = q.new_empty(need, dtype=torch.uint8)
+    else:
+        need = _workspace_bytes(workspace, dev)
     _launch("sf_window_attention", dev, q.data_ptr(), k.data_ptr(), v.data_ptr(), cu_seqlens.data_ptr(), cu_seqlens_k.data_ptr(),
-            out.data_ptr(), tq, tk, seqs, hq, hk, d, *qs, *ks, *vs, *os_, window, sinks, scale, _native.DTYPE_CODES[dtype_name(q)], variant)
+            out.data_ptr(), 0 if workspace is None else workspace.data_ptr(), need, tq, tk, seqs, hq, hk, d, *qs, *ks, *vs, *os_, window, sinks, scale, _native.DTYPE_CODES[dtype_name(q)], variant)
     return out

@@ -69,7 +69,7 @@ def test_kv4_attention_refusals(bad, word):
 
 def window_args(tq=4, tk=4, seqs=1, hq=4, hk=2, d=64, strides=(256, 64, 128, 64, 128, 64, 256, 64), scale=0.1, window=0, sinks=0, dtype=BF16,
                 variant=0, ptr=16):
-    return (ptr,) * 6 + (tq, tk, seqs, hq, hk, d, *strides, window, sinks, scale, dtype, variant)
+    return (ptr,) * 6 + (0, 0, tq, tk, seqs, hq, hk, d, *strides, window, sinks, scale, dtype, variant)
 
 
 @pytest.mark.parametrize("bad, word", [
@@ -103,6 +103,16 @@ def test_workspace_sizes():
     assert size(1, 32, 8, 128, 64, 1000) <= big       # never more than one resident wave's pieces
     assert size(0, 32, 8, 128, 64, 1000) == 0
     assert size(4, 32, 8, 128, 64, 4, variant=1) > 0 and size(4, 32, 8, 128, 64, 1000, variant=3) == 0
+
+
+def test_window_workspace_sizes():
+    """Split only where CTAs are few and keys are many."""
+    size = ops.window_attention_workspace_bytes
+    assert size(16384, 16384, 1, 16, 2, 128, window=4096, sinks=4) == 0 and size(1203, 1203, 9, 32, 8, 128, window=128, sinks=4) == 0
+    one = size(1, 32768, 1, 32, 8, 128)
+    assert one > 0 and one % (32 * 130 * 4) == 0 and 8 <= one // (32 * 130 * 4) <= 32
+    assert size(1, 32768, 1, 32, 8, 96) == 0 and size(1, 32768, 1, 129, 1, 64) == 0 and size(0, 9, 1, 8, 8, 64) == 0
+    assert size(1, 32768, 1, 32, 8, 128, window=100) == 0
 
 
 def fake_cuda(t, index=0):

@@ -497,6 +497,58 @@ def test_window_attention(case, dtype, variant):
     check_window(out, q, k, v, cu_q, cu_k, d**-0.5, window, sinks, variant, before)
 
 
+SPLIT = [
+    # query lengths, contexts in front, Hq, Hk, D, window, sinks: few queries, many keys
+    ([1], [4000], 8, 2, 128, 0, 0),
+    ([1, 3, 40], [3000, 100, 2000], 4, 4, 64, 0, 0),
+    ([2, 0, 30], [1500, 700, -10], 14, 2, 128, 0, 0),
+    ([5, 1], [2600, 2100], 16, 1, 64, 1500, 4),
+    ([9], [3333], 3, 1, 128, 2000, 300),
+    ([130], [1900], 12, 4, 128, 0, 0),
+]
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+@pytest.mark.parametrize("case", SPLIT, ids=[f"{'_'.join(map(str, c[0]))}+{'_'.join(map(str, c[1]))}-{'x'.join(map(str, c[2:]))}" for c in SPLIT])
+def test_window_attention_split_over_keys(case, dtype):
+    lq, ctx, hq, hk, d, window, sinks = case
+    g, dt = gen(31), TD[dtype]
+    lk = [max(0, a + b) for a, b in zip(lq, ctx)]
+    cu_q, cu_k = cu(lq), cu(lk)
+    q = randn(g, sum(lq) + 2, hq, d, dtype=dt)
+    k, v = randn(g, sum(lk), hk, d, dtype=dt), randn(g, sum(lk), hk, d, dtype=dt)
+    need = ops.window_attention_workspace_bytes(q.shape[0], k.shape[0], len(lq), hq, hk, d, window, sinks)
+    assert need > 0
+    ws = torch.full((need + 64,), 0xFF, dtype=torch.uint8, device="cuda")   # NaN everywhere it is not written
+    out = torch.full_like(q, 7.5)
+    before = out.clone()
+    ops.window_attention(q, k, v, cu_q.cuda(), d**-0.5, window=window, sinks=sinks, cu_seqlens_k=cu_k.cuda(), out=out, workspace=ws[:need])
+    check_window(out, q, k, v, cu_q, cu_k, d**-0.5, window, sinks, 0, before)
+    assert (ws[need:] == 0xFF).all()
+    for _ in range(2):
+        assert torch.equal(ops.window_attention(q, k, v, cu_q.cuda(), d**-0.5, window=window, sinks=sinks, cu_seqlens_k=cu_k.cuda(),
+                                                out=before.clone()), out)
+    # Without a workspace of that size, or asked to, the keys stay together.
+    for kw in (dict(workspace=ws[: need - 16]), dict(variant=4)):
+        whole = ops.window_attention(q, k, v, cu_q.cuda(), d**-0.5, window=window, sinks=sinks, cu_seqlens_k=cu_k.cuda(), out=before.clone(), **kw)
+        check_window(whole, q, k, v, cu_q, cu_k, d**-0.5, window, sinks, 0, before)
+
+
+def test_window_attention_split_masked_specials():
+    """What a query does not see stays out of its result when its keys are split, and what it sees comes in."""
+    g = gen(32)
+    q, k, v = randn(g, 3, 4, 128, dtype=torch.bfloat16), randn(g, 2000, 2, 128, dtype=torch.bfloat16), randn(g, 2000, 2, 128, dtype=torch.bfloat16)
+    c, ck = cu([3]), cu([2000])
+    clean = ops.window_attention(q, k, v, c.cuda(), 0.09, cu_seqlens_k=ck.cuda())
+    assert ops.window_attention_workspace_bytes(3, 2000, 1, 4, 2, 128) > 0
+    v[1998], k[1999, 1] = math.nan, math.inf   # seen by the last two queries and the last one
+    out = ops.window_attention(q, k, v, c.cuda(), 0.09, cu_seqlens_k=ck.cuda())
+    assert torch.isfinite(out[0]).all() and torch.isnan(out[1:]).all()
+    _, r = serving.window_attention(q, k.nan_to_num(0, 0, 0), v.nan_to_num(0, 0, 0), c.tolist(), ck.tolist(), 0.09, 0, 0)
+    close(out[0], r.value[0], attention_slack(r, 128, 2000, 2.0**-8)[0])
+    assert (clean[0] - out[0]).abs().max() < 1e-2
+
+
 @pytest.mark.parametrize("d", [8, 20, 80, 96, 256])
 def test_window_attention_other_head_sizes(d):
     g = gen(15)
@@ -653,9 +705,12 @@ def test_captured_replayed_and_on_other_streams():
         a = ops.kv4_attention(q, cache, table, pos + 1, d**-0.5)
         b = ops.kv4_attention(q, cache, table, pos + 1, d**-0.5, window=64, sinks=4)
         c = ops.window_attention(q, k, one[:, hq + hk :], cu_one, d**-0.5)
-        return a, b, c
+        kl, vl = ops.kv4_load(cache, every)
+        e = ops.window_attention(q, kl, vl, cu_one, d**-0.5, cu_seqlens_k=cu_all)  # split over the keys
+        return a, b, c, e
 
-    cu_one = i32([0, 1, 2])
+    cu_one, cu_all, every = i32([0, 1, 2]), i32([0, 900, 2048]), torch.arange(2048, device="cuda", dtype=torch.int32)
+    assert ops.window_attention_workspace_bytes(2, 2048, 2, hq, hk, d) > 0
     side = torch.cuda.Stream()
     side.wait_stream(torch.cuda.current_stream())
     with torch.cuda.stream(side):
