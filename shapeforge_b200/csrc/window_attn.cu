@@ -736,7 +736,9 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
     if (warp == 1) sm100::tmem_dealloc(tmem, 512);
 }
 
-// Join the splits of every row, a warp a row; the CTAs and their rows are those of the kernel above.
+// Join the splits of every row, a warp a row.  Tokens are found as in the kernel above; its 256 rows are dealt
+// to blocks of JOIN_ROWS, since a row is two dependent trips to L2 and little else.
+constexpr int JOIN_ROWS = 16;
 template <typename T, int D>
 __global__ void __launch_bounds__(256) window_join_kernel(const Args a, int tq_tile) {
     asm volatile("griddepcontrol.wait;" ::: "memory");
@@ -745,7 +747,8 @@ __global__ void __launch_bounds__(256) window_join_kernel(const Args a, int tq_t
     const int lane = threadIdx.x & 31, kvh = blockIdx.y;
     const int tokens = min(2 * tq_tile, at.qe - at.tok0);
     constexpr int E = D / 32;
-    for (int r = threadIdx.x >> 5; r < tokens * a.group; r += 8) {
+    const int end = min(tokens * a.group, (int)(blockIdx.z + 1) * JOIN_ROWS);
+    for (int r = blockIdx.z * JOIN_ROWS + (threadIdx.x >> 5); r < end; r += 8) {
         const int tok = r / a.group, head = kvh * a.group + r - tok * a.group;
         const int64_t row = at.tok0 + tok, row_at = row * a.heads + head, all = a.tq * a.heads;
         float m = -INFINITY;
@@ -852,7 +855,7 @@ int launch_tc(Args a, int64_t hk, bool* taken, cudaStream_t st, char* err, uint6
     int rc = sf::check_launch("window_attention launch", err, cap);
     if (rc || a.splits == 1) return rc;
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned)slots, (unsigned)hk);
+    cfg.gridDim = dim3((unsigned)slots, (unsigned)hk, (unsigned)((2 * tq_tile * a.group + JOIN_ROWS - 1) / JOIN_ROWS));
     cfg.blockDim = dim3(256);
     cfg.stream = st;
     cudaLaunchAttribute attr[1];
