@@ -736,61 +736,75 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
     if (warp == 1) sm100::tmem_dealloc(tmem, 512);
 }
 
-// Join the splits of every row, a warp a row.  Tokens are found as in the kernel above; its 256 rows are dealt
-// to blocks of JOIN_ROWS, since a row is two dependent trips to L2 and little else.
+// Join the splits of every row.  Tokens are found as in the kernel above; its 256 rows are dealt to blocks of
+// JOIN_ROWS.  A warp takes its ROWS rows side by side, each split's state in turn onto a running max, so the
+// trips to L2 overlap: 1536 tokens, 28 heads of 128 and 8200 keys in 3 parts take 206 us in all with a row at a
+// time behind its max, 197 so, 198 and 200 in blocks of 32 and 64 rows.
 constexpr int JOIN_ROWS = 16;
 template <typename T, int D>
 __global__ void __launch_bounds__(256) window_join_kernel(const Args a, int tq_tile) {
     asm volatile("griddepcontrol.wait;" ::: "memory");
     Where at;
     if (!locate(a, 2 * tq_tile, blockIdx.x, &at)) return;
+    constexpr int ROWS = JOIN_ROWS / 8, E = D / 32;
     const int lane = threadIdx.x & 31, kvh = blockIdx.y;
-    const int tokens = min(2 * tq_tile, at.qe - at.tok0);
-    constexpr int E = D / 32;
-    const int end = min(tokens * a.group, (int)(blockIdx.z + 1) * JOIN_ROWS);
-    for (int r = blockIdx.z * JOIN_ROWS + (threadIdx.x >> 5); r < end; r += 8) {
-        const int tok = r / a.group, head = kvh * a.group + r - tok * a.group;
-        const int64_t row = at.tok0 + tok, row_at = row * a.heads + head, all = a.tq * a.heads;
-        float m = -INFINITY;
-        for (int z = lane; z < a.splits; z += 32) {
-            const float mz = a.stat[2 * (z * all + row_at)];
-            m = mz > m || mz != mz ? mz : m;
+    const int r0 = blockIdx.z * JOIN_ROWS + (threadIdx.x >> 5) * ROWS;
+    const int rows = min(ROWS, min(2 * tq_tile, at.qe - at.tok0) * a.group - r0);
+    if (rows <= 0) return;
+    const int64_t all = a.tq * a.heads;
+    int64_t row_at[ROWS];
+    float m[ROWS], l[ROWS], acc[ROWS][E];
+#pragma unroll
+    for (int i = 0; i < ROWS; ++i) {
+        const int r = r0 + min(i, rows - 1), tok = r / a.group;
+        row_at[i] = (int64_t)(at.tok0 + tok) * a.heads + kvh * a.group + r - tok * a.group;
+        m[i] = -INFINITY;
+        l[i] = 0.f;
+#pragma unroll
+        for (int e = 0; e < E; ++e) acc[i][e] = 0.f;
+    }
+    for (int z = 0; z < a.splits; ++z) {
+        float2 st[ROWS];
+        float x[ROWS][E];
+#pragma unroll
+        for (int i = 0; i < ROWS; ++i) {
+            const int64_t from = z * all + row_at[i];
+            st[i] = *reinterpret_cast<const float2*>(a.stat + 2 * from);
+            if constexpr (E == 4) *reinterpret_cast<float4*>(x[i]) = *reinterpret_cast<const float4*>(a.part + from * D + E * lane);
+            else *reinterpret_cast<float2*>(x[i]) = *reinterpret_cast<const float2*>(a.part + from * D + E * lane);
         }
 #pragma unroll
-        for (int o = 16; o > 0; o >>= 1) {
-            const float other = __shfl_xor_sync(0xffffffffu, m, o);
-            m = other > m || other != other ? other : m;
-        }
-        float l = 0.f, acc[E];
+        for (int i = 0; i < ROWS; ++i) {
+            if (st[i].x == -INFINITY) continue;  // that split saw nothing and left no output
+            const float mn = st[i].x > m[i] || st[i].x != st[i].x ? st[i].x : m[i];
+            const float f = exp2f(m[i] - mn), g = exp2f(st[i].x - mn);
+            m[i] = mn;
+            l[i] = l[i] * f + st[i].y * g;
 #pragma unroll
-        for (int e = 0; e < E; ++e) acc[e] = 0.f;
-#pragma unroll 4
-        for (int z = 0; z < a.splits; ++z) {
-            const float2 st = *reinterpret_cast<const float2*>(a.stat + 2 * (z * all + row_at));
-            if (st.x == -INFINITY) continue;  // that split saw nothing and left no output
-            float x[E];
-            if constexpr (E == 4) *reinterpret_cast<float4*>(x) = *reinterpret_cast<const float4*>(a.part + (z * all + row_at) * D + E * lane);
-            else *reinterpret_cast<float2*>(x) = *reinterpret_cast<const float2*>(a.part + (z * all + row_at) * D + E * lane);
-            const float f = exp2f(st.x - m);
-            l = fmaf(f, st.y, l);
-#pragma unroll
-            for (int e = 0; e < E; ++e) acc[e] = fmaf(f, x[e], acc[e]);
+            for (int e = 0; e < E; ++e) acc[i][e] = acc[i][e] * f + x[i][e] * g;
         }
-        const int p = at.pos0 + tok;
-        const float inv = 1.0f / l;
+    }
+    uint32_t todo = 0;  // rows to compute key by key
+#pragma unroll
+    for (int i = 0; i < ROWS; ++i) {
+        if (i >= rows) break;
+        const int tok = (r0 + i) / a.group, head = kvh * a.group + r0 + i - tok * a.group, p = at.pos0 + tok;
+        const float inv = 1.0f / l[i];
         bool again = false;
-        T* out = (T*)a.o + row * a.ot + (int64_t)head * a.oh;
+        T* out = (T*)a.o + (int64_t)(at.tok0 + tok) * a.ot + (int64_t)head * a.oh;
 #pragma unroll
         for (int e = 0; e < E; e += 2) {
-            float2 x = make_float2(acc[e] * inv, acc[e + 1] * inv);
-            if (p < 0) x = make_float2(0.f, 0.f);
-            again |= !(x.x * 0.f + x.y * 0.f == 0.f);
-            *reinterpret_cast<uint32_t*>(out + E * lane + e) = sf::Pair<T>::from_f2(x);
+            float2 v = make_float2(acc[i][e] * inv, acc[i][e + 1] * inv);
+            if (p < 0) v = make_float2(0.f, 0.f);
+            again |= !(v.x * 0.f + v.y * 0.f == 0.f);
+            *reinterpret_cast<uint32_t*>(out + E * lane + e) = sf::Pair<T>::from_f2(v);
         }
-        if (__any_sync(0xffffffffu, again)) {
-            __syncwarp();
-            row_by_warp<T>(a, D, row, head, at.kb, p, out);
-        }
+        if (__any_sync(0xffffffffu, again)) todo |= 1u << i;
+    }
+    for (; todo; todo &= todo - 1) {
+        const int r = r0 + __ffs(todo) - 1, tok = r / a.group, head = kvh * a.group + r - tok * a.group;
+        __syncwarp();
+        row_by_warp<T>(a, D, at.tok0 + tok, head, at.kb, at.pos0 + tok, (T*)a.o + (int64_t)(at.tok0 + tok) * a.ot + (int64_t)head * a.oh);
     }
 }
 
@@ -807,11 +821,12 @@ int64_t splits_of(int64_t Tq, int64_t Tk, int64_t seqs, int64_t Hq, int64_t Hk, 
     int64_t keys = Tk / seqs;
     if (window) keys = std::min(keys, window + tt + (sinks ? std::min<int64_t>(sinks, keys) : 0));
     const int64_t tiles = (keys + 127) / 128;
+    const int64_t sms = sf::sm_count();
     double best = 1e30;
     int64_t pick = 1;
     for (int64_t z : {1, 2, 3, 4, 6, 8, 12, 16, 24, 32}) {
         if (z > 1 && tiles / z < 2) break;
-        const int64_t waves = (ctas * z + sf::sm_count() - 1) / sf::sm_count();
+        const int64_t waves = (ctas * z + sms - 1) / sms;
         double cost = (double)waves * ((tiles + z - 1) / z + 3);
         if (z > 1) cost += 3 + (double)Tq * Hq * D * 8 * z / 9e6;  // 9 MB of states in a tile's time
         if (cost < best) {

@@ -569,11 +569,11 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, q_weight: torch.Tensor, k_wei
     _check_vector(k_weight, "k_weight", dev, dtype, d)
     _check_vector(positions, "positions", dev, torch.int32, t)
     if q_out is None:
-        q_out, qos = q.new_empty((t, hq, d)), (hq * d, d)
+        q_out, qos = q.new_empty(t, hq, d), (hq * d, d)
     else:
         qos = _check_rows(q_out, "q_out", dev, dtype, q.shape, written=True)
     if k_out is None:
-        k_out, kos = k.new_empty((t, hk, d)), (hk * d, d)
+        k_out, kos = k.new_empty(t, hk, d), (hk * d, d)
     else:
         kos = _check_rows(k_out, "k_out", dev, dtype, k.shape, written=True)
     _launch("sf_qk_norm_rope", dev, q.data_ptr(), k.data_ptr(), q_weight.data_ptr(), k_weight.data_ptr(), positions.data_ptr(),
@@ -633,11 +633,11 @@ def kv4_load(cache: torch.Tensor, slots: torch.Tensor, dtype: torch.dtype = torc
     given = k_out if k_out is not None else v_out
     dtype = dtype if given is None else given.dtype
     if k_out is None:
-        k_out, ks = cache.new_empty(shape, dtype=dtype), (heads * d, d)
+        k_out, ks = cache.new_empty(*shape, dtype=dtype), (heads * d, d)
     else:
         ks = _check_rows(k_out, "k_out", dev, dtype, shape, written=True)
     if v_out is None:
-        v_out, vs = cache.new_empty(shape, dtype=dtype), (heads * d, d)
+        v_out, vs = cache.new_empty(*shape, dtype=dtype), (heads * d, d)
     else:
         vs = _check_rows(v_out, "v_out", dev, dtype, shape, written=True)
     _launch("sf_kv4_load", dev, k_out.data_ptr(), v_out.data_ptr(), slots.data_ptr(), cache.data_ptr(), *shape, pages, page, *ks, *vs,
@@ -649,6 +649,12 @@ def kv4_attention_workspace_bytes(batch: int, q_heads: int, kv_heads: int, dim: 
                                   sinks: int = 0, variant: int = 0) -> int:
     """Workspace bytes of :func:`kv4_attention` (0 when a request's keys stay with one CTA)."""
     return int(_native.load().sf_kv4_attention_workspace_bytes(batch, q_heads, kv_heads, dim, page_size, table_width, window, sinks, variant))
+
+
+@functools.lru_cache(maxsize=512)
+def _kv4_attention_need(dev: int, *sizes: int) -> int:
+    """The sizes' workspace bytes on GPU ``dev``: a decode loop asks for the same ones again and again."""
+    return kv4_attention_workspace_bytes(*sizes)
 
 
 def kv4_attention(q: torch.Tensor, cache: torch.Tensor, block_table: torch.Tensor, seq_lens: torch.Tensor, scale: float, window: int = 0,
@@ -678,11 +684,11 @@ def kv4_attention(q: torch.Tensor, cache: torch.Tensor, block_table: torch.Tenso
     width = block_table.shape[1]
     _check_vector(seq_lens, "seq_lens", dev, torch.int32, b)
     if out is None:
-        out, os_ = q.new_empty((b, hq, d)), (hq * d, d)
+        out, os_ = q.new_empty(b, hq, d), (hq * d, d)
     else:
         os_ = _check_rows(out, "out", dev, dtype, q.shape, written=True)
     if workspace is None:
-        need = kv4_attention_workspace_bytes(b, hq, heads, d, page, width, window, sinks, variant)
+        need = _kv4_attention_need(dev, b, hq, heads, d, page, width, window, sinks, variant)
         if need:
             workspace = cache.new_empty(need)
     else:
@@ -697,6 +703,11 @@ def window_attention_workspace_bytes(q_tokens: int, k_tokens: int, sequences: in
                                      sinks: int = 0) -> int:
     """Workspace bytes of :func:`window_attention` (0 when the keys of a row tile stay with one CTA)."""
     return int(_native.load().sf_window_attention_workspace_bytes(q_tokens, k_tokens, sequences, q_heads, kv_heads, dim, window, sinks))
+
+
+@functools.lru_cache(maxsize=512)
+def _window_attention_need(dev: int, *sizes: int) -> int:
+    return window_attention_workspace_bytes(*sizes)
 
 
 def window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqlens: torch.Tensor, scale: float, window: int = 0, sinks: int = 0,
@@ -733,11 +744,11 @@ def window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqle
     else:
         _check_vector(cu_seqlens_k, "cu_seqlens_k", dev, torch.int32, seqs + 1)
     if out is None:
-        out, os_ = q.new_empty((tq, hq, d)), (hq * d, d)
+        out, os_ = q.new_empty(tq, hq, d), (hq * d, d)
     else:
         os_ = _check_rows(out, "out", dev, dtype, q.shape, written=True)
     if workspace is None:
-        need = 0 if variant in (2, 4) else window_attention_workspace_bytes(tq, tk, seqs, hq, hk, d, window, sinks)
+        need = 0 if variant in (2, 4) else _window_attention_need(dev, tq, tk, seqs, hq, hk, d, window, sinks)
         if need:
             workspace = q.new_empty(need, dtype=torch.uint8)
     else:
