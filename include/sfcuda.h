@@ -305,8 +305,8 @@ SF_API int sf_kv4_load(const sf_kv4_cache_args* args, void* stream, char* err, u
  * lens[b] tokens (the query's own last); token j sits at row j % page_size of page table[b, j / page_size],
  * table [B, width] with table_stride elements from row to row.  Seen are j >= lens[b] - window or
  * j < sinks (window 0: all).  lens[b] <= 0 gives zeros; a length past the table is cut to it, a page id
- * outside the cache hides its tokens, both reported through sf_kernel_status (code 3).  q and o 16-byte
- * aligned, strides multiples of 8 elements.  workspace: 16-byte aligned,
+ * outside the cache hides its tokens, both reported through sf_kernel_status (code 3); zeros where every
+ * token is hidden.  q and o 16-byte aligned, strides multiples of 8 elements.  workspace: 16-byte aligned,
  * sf_kv4_attention_workspace_bytes bytes (0: may be NULL), no initial content; two calls that overlap
  * on the GPU need one each.  variant 1 deals every request's keys to all CTAs, 3 keeps a (request,
  * head) to a CTA, 0 decides by size.

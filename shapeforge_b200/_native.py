@@ -219,7 +219,11 @@ def call_args(name: str, stream: int, *fields) -> None:
         buf = _err.buf
     except AttributeError:
         buf = _err.buf = ctypes.create_string_buffer(ERR_CAP)
-    rc = getattr(_lib or load(), name)(ARGS[name].pack(*fields), stream, buf, ERR_CAP)
+    try:
+        packed = ARGS[name].pack(*fields)
+    except struct.error as exc:
+        raise ValueError(f"{name}: {exc}") from exc
+    rc = getattr(_lib or load(), name)(packed, stream, buf, ERR_CAP)
     if rc != SF_OK:
         raise SfError(int(rc), buf.value.decode(errors="replace") or name)
 

@@ -739,7 +739,7 @@ __global__ void __launch_bounds__(THREADS, ctas_of(NT)) kv4_attention_kernel(con
             }
             if (all_mine) {
                 if (hb * HB + head < a.group) {
-                    const float inv = done.n == 0 ? 0.f : 1.0f / sum;
+                    const float inv = sum == 0.f ? 0.f : 1.0f / sum;  // 0: every key was hidden
                     T* dst = (T*)a.o + (int64_t)done.b * a.ob + (int64_t)(kh * a.group + hb * HB + head) * a.oh + d;
                     *reinterpret_cast<uint2*>(dst) = make_uint2(sf::Pair<T>::from_f2(make_float2(acc.x * inv, acc.y * inv)),
                                                                 sf::Pair<T>::from_f2(make_float2(acc.z * inv, acc.w * inv)));
@@ -807,7 +807,7 @@ __global__ void __launch_bounds__(32 * JOIN_HEADS * JOIN) kv4_join_kernel(const 
 #pragma unroll
         for (int e = 0; e < E; ++e) acc[e] += acc_s[hs][w][E * lane + e];
     }
-    const float inv = 1.0f / l;
+    const float inv = l == 0.f ? 0.f : 1.0f / l;  // 0: every key was hidden
     T* out = (T*)a.o + (int64_t)b * a.ob + (int64_t)(kh * a.group + hb * HB + head) * a.oh + E * lane;
 #pragma unroll
     for (int e = 0; e < E; e += 2) *reinterpret_cast<uint32_t*>(out + e) = sf::Pair<T>::from_f2(make_float2(acc[e] * inv, acc[e + 1] * inv));
@@ -911,6 +911,7 @@ extern "C" int sf_kv4_attention(const sf_kv4_attention_args* x, void* stream, ch
         return sf::fail(SF_EINVAL, err, cap, "kv4_attention: more than 2^31 - 1 slots");
     if (Hq && (Hk == 0 || Hq % Hk)) return sf::fail(SF_EINVAL, err, cap, "kv4_attention: the query heads must be a multiple of the cache's heads");
     if (!(scale > 0.f) || !(scale < INFINITY)) return sf::fail(SF_EINVAL, err, cap, "kv4_attention: scale must be > 0");
+    if (x->variant != 0 && x->variant != 1 && x->variant != 3) return sf::fail(SF_EINVAL, err, cap, "kv4_attention: no variant %d", x->variant);
     if (window < 0 || sinks < 0) return sf::fail(SF_EINVAL, err, cap, "kv4_attention: window and sinks must be >= 0");
     if (x->dtype != SF_DTYPE_F16 && x->dtype != SF_DTYPE_BF16) return sf::fail(SF_EINVAL, err, cap, "kv4_attention: dtype %d is not fp16/bf16", x->dtype);
     for (int64_t s : {x->q_rows.token, x->q_rows.head, x->o_rows.token, x->o_rows.head})

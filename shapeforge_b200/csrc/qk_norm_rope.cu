@@ -267,6 +267,7 @@ extern "C" int sf_qk_norm_rope(const sf_qk_norm_rope_args* x, void* stream, char
     const int64_t T = x->T, Hq = x->Hq, Hk = x->Hk, D = x->D;
     if (T < 0 || Hq < 0 || Hk < 0 || Hq + Hk > (1 << 20) || D < 1 || D > (1 << 20))
         return sf::fail(SF_EINVAL, err, cap, "qk_norm_rope: need T, Hq, Hk >= 0 and D >= 1");
+    if (x->variant < 0 || x->variant > 2) return sf::fail(SF_EINVAL, err, cap, "qk_norm_rope: no variant %d", x->variant);
     if (x->rotary < 0 || x->rotary % 2 || x->rotary > D) return sf::fail(SF_EINVAL, err, cap, "qk_norm_rope: rotary must be even and at most D");
     if (!(x->base > 0) || !std::isfinite(x->base)) return sf::fail(SF_EINVAL, err, cap, "qk_norm_rope: base must be > 0");
     if (!(x->eps >= 0)) return sf::fail(SF_EINVAL, err, cap, "qk_norm_rope: eps must be >= 0");

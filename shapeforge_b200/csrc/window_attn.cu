@@ -912,6 +912,8 @@ extern "C" int sf_window_attention(const sf_window_attention_args* x, void* stre
     if (Tq > 0x7fffffffLL || Tk > 0x7fffffffLL || seqs > 0x7fffffffLL || Hq > (1 << 20))
         return sf::fail(SF_EINVAL, err, cap, "window_attention: size above 2^31 - 1");
     if (!(scale > 0.f) || !(scale < INFINITY)) return sf::fail(SF_EINVAL, err, cap, "window_attention: scale must be > 0");
+    if (x->variant != 0 && x->variant != 1 && x->variant != 2 && x->variant != 4)
+        return sf::fail(SF_EINVAL, err, cap, "window_attention: no variant %d", x->variant);
     if (x->window < 0 || x->sinks < 0) return sf::fail(SF_EINVAL, err, cap, "window_attention: window and sinks must be >= 0");
     if (x->dtype != SF_DTYPE_F16 && x->dtype != SF_DTYPE_BF16) return sf::fail(SF_EINVAL, err, cap, "window_attention: dtype %d is not fp16/bf16", x->dtype);
     for (const sf_rows* r : {&x->q_rows, &x->k_rows, &x->v_rows, &x->o_rows})

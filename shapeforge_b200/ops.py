@@ -9,6 +9,7 @@ missing native library raises.
 from __future__ import annotations
 
 import functools
+import operator
 
 import torch
 
@@ -531,6 +532,13 @@ def _check_vector(t: torch.Tensor, name: str, dev: int, dtype: torch.dtype, leng
         raise ValueError(f"{name} must be contiguous with one axis{'' if length is None else f' of {length}'}, got shape {tuple(t.shape)}")
 
 
+def _count(x: int, name: str) -> int:
+    x = operator.index(x)
+    if not 0 <= x < 1 << 63:
+        raise ValueError(f"{name} must be >= 0 and below 2^63, got {x}")
+    return x
+
+
 def _workspace_bytes(t: torch.Tensor, dev: int) -> int:
     _gpu(t, "workspace", dev)
     if not t.is_contiguous():
@@ -665,11 +673,13 @@ def kv4_attention(q: torch.Tensor, cache: torch.Tensor, block_table: torch.Tenso
     (int32, rows may be strided) holds each request's pages in order, ``seq_lens [B]`` (int32) its tokens
     in the cache, the query's own last.  Token ``j`` is seen when ``j >= seq_len - window`` or ``j <
     sinks`` (``window`` 0: all).  A length of 0 gives zeros; a length past the table is cut to it and a
-    page id outside the cache hides its tokens, both reported by :func:`kernel_status` (code 3).
+    page id outside the cache hides its tokens, both reported by :func:`kernel_status` (code 3); a request
+    with every token hidden gives zeros.  q and ``out`` need 16-byte aligned rows and must not overlap.
     ``workspace`` (uint8, :func:`kv4_attention_workspace_bytes`) is allocated here when not given;
     calls that overlap on the GPU need one each.  ``variant``: 0 = by size, 1 = all requests' keys
     dealt evenly to all CTAs, 3 = a CTA a (request, head)."""
     dev = _gpu(q, "q")
+    window, sinks = _count(window, "window"), _count(sinks, "sinks")
     dtype = q.dtype
     pages, heads, page, d = _check_cache(cache, dev)
     qs = _check_rows(q, "q", dev)
@@ -720,12 +730,13 @@ def window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqle
     rows).  Query ``i`` of a sequence with nq queries and nk keys sits at ``p = i + nk - nq`` and sees the
     keys ``j <= p`` with ``j > p - window`` or ``j < sinks`` (``window`` 0: all ``j <= p``), so a prompt's next
     chunk comes with its whole context as keys.  A query that sees nothing gives zeros; rows of ``out``
-    that belong to no sequence are left as they were.  D up to 256; D 64 and 128 with 16-byte aligned
+    that belong to no sequence are left as they were.  ``out`` must not overlap the inputs.  D up to 256; D 64 and 128 with 16-byte aligned
     rows and at most 128 query heads a key head run on the tensor cores, where few queries with many keys
     are split over the keys by way of ``workspace`` (uint8, :func:`window_attention_workspace_bytes`,
     allocated here when not given; calls that overlap on the GPU need one each).  ``variant``: 0 = by
     shape, 1 = tensor cores (refused where they do not apply), 2 = general kernel, 4 = unsplit."""
     dev = _gpu(q, "q")
+    window, sinks = _count(window, "window"), _count(sinks, "sinks")
     dtype = q.dtype
     qs, ks = _check_rows(q, "q", dev), _check_rows(k, "k", dev, dtype)
     vs = _check_rows(v, "v", dev, dtype, k.shape)

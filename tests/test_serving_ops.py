@@ -219,3 +219,26 @@ def test_mask_definition():
     assert m.tolist() == [[True, True, True, False, False], [True, False, True, True, False], [True, False, False, True, True]]
     assert not serving.window_mask(3, 1, 0, 0)[0].any()      # a query in front of the first key
     assert serving.window_mask(1, 4, 0, 9).all()
+
+
+def test_unknown_variants_are_refused():
+    for name, args, bad in (("sf_qk_norm_rope", norm_args, (-1, 3)), ("sf_kv4_attention", decode_args, (-1, 2, 4)),
+                            ("sf_window_attention", window_args, (-1, 3, 5))):
+        for variant in bad:
+            assert f"no variant {variant}" in refused(name, args(variant=variant))
+
+
+def test_numbers_that_are_no_sizes_are_refused():
+    q, k, cu = fk(4, 2, 64), fk(4, 1, 64), fk(2, dtype=torch.int32)
+    cache, table, lens = fk(3, 1, 2, 18 * 64, dtype=torch.uint8), fk(4, 2, dtype=torch.int32), fk(4, dtype=torch.int32)
+    for kind, extra in ((TypeError, dict(window=1.5)), (TypeError, dict(sinks=None)), (ValueError, dict(sinks=1 << 70)), (ValueError, dict(window=-1))):
+        with pytest.raises(kind):
+            ops.kv4_attention(q, cache, table, lens, 0.1, out=fk(4, 2, 64), workspace=fk(16, dtype=torch.uint8), **extra)
+        with pytest.raises(kind):
+            ops.window_attention(q, k, k, cu, 0.1, out=fk(4, 2, 64), workspace=fk(16, dtype=torch.uint8), **extra)
+    with pytest.raises(ValueError, match="sf_qk_norm_rope"):
+        _native.call_args("sf_qk_norm_rope", 0, *norm_args(rotary=6.4))
+
+
+def test_above_1024_requests_a_cta_takes_a_whole_one():
+    assert ops.kv4_attention_workspace_bytes(1024, 4, 2, 64, 16, 400) > 0 and ops.kv4_attention_workspace_bytes(1025, 4, 2, 64, 16, 400) == 0

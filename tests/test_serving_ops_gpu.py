@@ -788,3 +788,105 @@ def test_generic_dispatch_and_timed_batches():
     ws, one = torch.empty(need, dtype=torch.uint8, device="cuda"), torch.empty(2, 4, 64, device="cuda", dtype=torch.bfloat16)
     run("kv4_attention", (2, 4, 2, 64, 3, 16, 3, need), (0.125, 20, 1), (qo, cache, table, lens, one, ws), variant=1)
     assert torch.equal(one, ops.kv4_attention(qo[:2].contiguous(), cache, table, lens, 0.125, window=20, sinks=1, variant=1))
+
+
+# ---- the ends of the range ----------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("variant", [0, 1, 3])
+def test_kv4_attention_with_every_page_hidden(variant):
+    """A request whose pages all lie outside the cache sees nothing, like one of length 0; its neighbour is as ever."""
+    g = gen(40)
+    cache, kq, vq = filled_cache(g, 4, 16, 2, 128, torch.bfloat16)
+    q = randn(g, 3, 8, 128, dtype=torch.bfloat16)
+    for n in (16, 400):
+        table = torch.full((3, 25), -1, dtype=torch.int32, device="cuda")
+        table[1] = torch.arange(25, device="cuda") % 4
+        table[2] = 4
+        out = ops.kv4_attention(q, cache, table, i32([n, n, n]), 0.1, variant=variant)
+        assert ops.kernel_status() == (3, 112)
+        assert not out[0].any() and not out[2].any()
+        check_decode(out[1:2], q[1:2], kq, vq, 16, table[1:2], [n], 0.1, 0, 0)
+    none = ops.kv4_cache(0, 16, 2, 128)
+    out = ops.kv4_attention(q, none, table, i32([5, 400, 0]), 0.1, variant=variant)
+    assert ops.kernel_status() == (3, 112) and not out.any()
+    assert not ops.kv4_load(none, i32([-1, 0, 7]))[0].any()
+    assert ops.kernel_status()[0] == 3
+
+
+@pytest.mark.parametrize("variant", [0, 1, 3])
+@pytest.mark.parametrize("batch", [70, 1023, 1030])
+def test_kv4_attention_many_requests(batch, variant):
+    """More requests than a warp scans at a time, and more than the keys are dealt evenly for; lengths 0 among them."""
+    g = gen(41)
+    h, d, page, width = 1, 64, 16, 40
+    cache, kq, vq = filled_cache(g, 300, page, h, d, torch.float16)
+    table = torch.randint(300, (batch, width), device="cuda", generator=g).to(torch.int32)
+    lens = torch.randint(width * page + 1, (batch,), device="cuda", generator=g) * (torch.rand(batch, device="cuda", generator=g) > 0.3)
+    q = randn(g, batch, 3, d, dtype=torch.float16)
+    out = ops.kv4_attention(q, cache, table, lens.to(torch.int32), 0.1, variant=variant)
+    some = [0, 1, 31, 32, 33, 64, batch // 2, batch - 2, batch - 1]
+    check_decode(out[some], q[some], kq, vq, page, table[some], lens[some].tolist(), 0.1, 0, 0)
+    assert not out[lens == 0].any()
+    # The same request gives close to the same wherever it stands (the split's order of sums differs).
+    alone = torch.cat([ops.kv4_attention(q[i : i + 1], cache, table[i : i + 1], lens[i : i + 1].to(torch.int32), 0.1) for i in range(0, batch, 9)])
+    # Each is off by at most half a step, 2^-11 of the weights' mass and 14 2^-23 17 n 8 max p (n <= 640, max p < 0.02):
+    # under 2^-8 of the largest value.
+    assert (alone.float() - out[::9].float()).abs().max() <= 2.0**-7 * out.float().abs().max()
+
+
+@pytest.mark.parametrize("variant", [0, 2])
+@pytest.mark.parametrize("seqs", [33, 100, 1500, 40000])
+def test_window_attention_many_sequences(seqs, variant):
+    """More sequences than a warp looks at in one step of its search, most of them short or empty."""
+    g = gen(42)
+    lens = torch.randint(0, 4, (seqs,), device="cuda", generator=g) * (torch.rand(seqs, device="cuda", generator=g) > 0.5)
+    lens[seqs // 2], lens[-1] = 70, 0
+    more = torch.randint(0, 3, (seqs,), device="cuda", generator=g)
+    cu_q = torch.cat([lens.new_zeros(1), lens.cumsum(0)]).to(torch.int32)
+    cu_k = torch.cat([lens.new_zeros(1), (lens + more).cumsum(0)]).to(torch.int32)
+    q = randn(g, int(cu_q[-1]), 4, 64, dtype=torch.bfloat16)
+    k, v = randn(g, int(cu_k[-1]), 2, 64, dtype=torch.bfloat16), randn(g, int(cu_k[-1]), 2, 64, dtype=torch.bfloat16)
+    out = ops.window_attention(q, k, v, cu_q, 0.125, window=20, sinks=1, cu_seqlens_k=cu_k, out=torch.full_like(q, math.nan), variant=variant)
+    # Rounded outputs and one side's rounded weights: 3 2^-8 of the largest value.
+    other = ops.window_attention(q, k, v, cu_q, 0.125, window=20, sinks=1, cu_seqlens_k=cu_k, variant=2 - variant)
+    assert torch.isfinite(out).all() and (out.float() - other.float()).abs().max() <= 2.0**-6 * other.float().abs().max()
+    # A stretch of sequences against the definition.
+    for a in (0, seqs // 2 - 8, seqs - 16):
+        cq, ck = cu_q[a : a + 17].cpu(), cu_k[a : a + 17].cpu()
+        q0, q1, k0, k1 = int(cq[0]), int(cq[-1]), int(ck[0]), int(ck[-1])
+        check_window(out[q0:q1], q[q0:q1], k[k0:k1], v[k0:k1], cq - cq[0], ck - ck[0], 0.125, 20, 1, variant)
+
+
+def test_offsets_past_32_bits():
+    """A cache, rows and strides that reach past 2^32 bytes and 2^31 elements."""
+    g = gen(43)
+    page, h, d = 64, 2, 128
+    pages = 2**32 // (h * (page // 16) * 18 * d) + 9
+    cache = ops.kv4_cache(pages, page, h, d)
+    k, v = randn(g, 100, h, d, dtype=torch.bfloat16), randn(g, 100, h, d, dtype=torch.bfloat16)
+    slots = (pages - 2) * page + torch.arange(100, device="cuda", dtype=torch.int32)
+    ops.kv4_store(k, v, slots, cache)
+    assert ops.kernel_status() == (0, 0) and not cache[: 2].any() and not cache[pages - 3].any()
+    same(ops.kv4_load(cache, slots)[0], stored(k))
+    table, q = i32([[pages - 2, pages - 1]]), randn(g, 1, 8, d, dtype=torch.bfloat16)
+    out = ops.kv4_attention(q, cache, table, i32([100]), 0.1)
+    check_decode(out, q, serving.kv4_quantise(k), serving.kv4_quantise(v), page, i32([[0, 1]]), [100], 0.1, 0, 0)
+    del cache
+    far = 2**30  # elements from one token to the next
+    room = torch.empty(2 * far + 64 * 1024, device="cuda", dtype=torch.bfloat16)
+    view = lambda at, heads: room[at:].as_strided((3, heads, d), (far, d, 1))
+    fq, fk, fv, fo = view(0, 4), view(4096, 2), view(8192, 2), view(12288, 4)
+    fq.copy_(randn(g, 3, 4, d)), fk.copy_(randn(g, 3, 2, d)), fv.copy_(randn(g, 3, 2, d))
+    for variant in (0, 1, 2):
+        ops.window_attention(fq, fk, fv, i32([0, 3]), 0.1, out=fo, variant=variant)
+        check_window(fo, fq.contiguous(), fk.contiguous(), fv.contiguous(), cu([3]), cu([3]), 0.1, 0, 0, variant)
+    w, pos = torch.ones(d, device="cuda", dtype=torch.bfloat16), i32([5, 6, 2**31 - 1])
+    for variant in (1, 2):
+        a, b = ops.qk_norm_rope(fq, fk, w, w, pos, q_out=fo, variant=variant)
+        check_norm_rope(fq.contiguous(), fk.contiguous(), w, w, pos, (fo, b))
+    small = ops.kv4_cache(1, 16, 2, d)
+    ops.kv4_store(fk, fv, i32([0, 5, 9]), small)
+    kb, vb = ops.kv4_load(small, i32([0, 5, 9]), k_out=view(20000, 2), v_out=view(24000, 2))
+    same(kb, stored(fk.contiguous()))
+    same(vb, stored(fv.contiguous()))
