@@ -400,8 +400,9 @@ SF_API int sf_gemm_nn_noalloc(const void* A, const void* B, void* C, int64_t M, 
 
 /*
  * Read and clear the sticky status word of the tcgen05 kernels: code 0 = ok, 1 = a bounded
- * pipeline wait gave up (the launch's output is invalid); `where` names the wait.  Synchronises
- * `stream`.  Replaces the reference's launch watchdog verdict for device-side stalls
+ * pipeline wait gave up (the launch's output is invalid); `where` names the wait; 2 = a varlen sequence
+ * past its tensor, 3 = a slot, page or length outside the 4-bit cache or its table (skipped, the rest is
+ * valid).  Synchronises `stream`.  Replaces the reference's launch watchdog verdict for device-side stalls
  * (tcenv/evaluate.py:1029-1051) without trapping the GPU.
  */
 SF_API int sf_kernel_status(uint32_t* code, uint32_t* where, void* stream, char* err, uint64_t cap);
@@ -503,7 +504,7 @@ SF_API int32_t sf_op_nargs(int32_t op);
  *                   args = {q, cache, table, lens, o, workspace}
  *                   variant 1 deals every request's keys to all CTAs, 3 keeps a (request, head) to a CTA
  *   SF_OP_WINDOW_ATTENTION  dims = {Tq, Tk, seqs, Hq, Hk, D, window, sinks}  attrs = {scale}
- *                   args = {q, k, v, cu_q, cu_k, o}
+ *                   args = {q, k, v, cu_q, cu_k, o}; no workspace, so the keys are not split
  * (these five: contiguous tensors)
  * desc->variant: 0 = exact dispatch with fallback, 1 = force the specialised (tensor-core /
  * vectorised) kernel, 2 = force the general fallback kernel.
