@@ -31,7 +31,8 @@
 //    stretch for every CTA of one resident wave, whatever the lengths; each (request, head) counts
 //    ITEM_COST tiles more for its start and end.  One that spans CTAs leaves partial states in the
 //    workspace, joined by a second kernel in the order of the stretches (no atomics: the same call
-//    gives the same bits).  The first copies of a CTA's next (request, head) are issued before the
+//    gives the same bits).  A few requests of moderate length go to clusters instead, a (request, head) each:
+//    one launch, its CTAs' states joined through distributed shared memory.  The first copies of a CTA's next (request, head) are issued before the
 //    states of the one at hand are merged.
 #include "kv4.cuh"
 
@@ -55,6 +56,10 @@ constexpr int tiles_of_step(int nt) { return nt == 1 ? 2 : 1; }
 constexpr int MAX_SMEM = 227 * 1024;
 constexpr int LEAST = 4 * WARPS;  // tiles and costs a CTA has at least (one a warp: 13.3 against 11.6 us for one request of 4097 keys)
 constexpr int ITEM_COST = 24;  // what starting and merging a (request, head) costs, in tiles
+// CTAs a cluster, and tiles a CTA of one.  Against the line and its join, 32 heads on 8 of 128: one request of 1024
+// tokens 7.9 and 10.2 us, 4096 10.3 and 11.6, 8192 (32 tiles a CTA) 12.8 and 13.8, 16384 (64) 18.4 and 17.5; 8
+// requests of up to 2048 11.6 and 12.8, of 4096 (64 tiles a CTA) 16.7 and 14.9.
+constexpr int MAX_CLUSTER = 16, CLUSTER_LEAST = 8, CLUSTER_MOST = 32;
 constexpr float NO_MAX = -3e38f;  // the running max before any score
 // Smallest unit of a head's p s: p / unit stays finite for p up to 2^8.
 constexpr float UNIT_FLOOR = 0x1p-118f;
@@ -74,7 +79,8 @@ struct Args {
     int B, Hk, group, blocks;    // kv heads, query heads a kv head, head blocks a kv head
     int pages, tpp, width;       // pages in the cache, tiles a page, pages a table row
     float scale_log2;
-    bool split;
+    bool split;                  // all tiles in a line; else `cluster` CTAs a (request, head)
+    int cluster;
 };
 
 __device__ __forceinline__ void mma_f16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
@@ -104,6 +110,12 @@ __device__ __forceinline__ uint32_t f16x2(float a, float b) { return sf::Pair<__
 __device__ __forceinline__ uint32_t sub2(uint32_t a, uint32_t b) {
     const __half2 d = __hsub2(*reinterpret_cast<const __half2*>(&a), *reinterpret_cast<const __half2*>(&b));
     return *reinterpret_cast<const uint32_t*>(&d);
+}
+
+__device__ __forceinline__ float2 ld_cluster(uint32_t at) {
+    float2 v;
+    asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(at) : "memory");
+    return v;
 }
 
 // The largest over the warp's keys (lanes of one t).
@@ -159,7 +171,8 @@ struct Smem {
     static constexpr int AHEAD = BARS + (WARPS * STAGES + 2) * 8;  // [warp][64] record numbers of the next part
     static constexpr int LINE = AHEAD + WARPS * 64 * 4;            // [warp] Line
     static constexpr int SCAN = LINE + WARPS * 64;                 // prefix of the requests' costs
-    static constexpr int bytes(int B) { return SCAN + 4 * (B + 1); }
+    static constexpr int MERGED = SCAN;                            // or, in a cluster, [head][2] fp32: the CTA's own state
+    static constexpr int bytes(int B) { return SCAN + (4 * (B + 1) > HB * 8 ? 4 * (B + 1) : HB * 8); }
 };
 
 // What a request's (kv head, head block) counts in the line of tiles.
@@ -187,7 +200,8 @@ __device__ __forceinline__ void scan_costs(const Args& a, int* pre) {
     __syncwarp();
 }
 
-template <typename T, int NG, int NT>
+// JOINT: a cluster of a.cluster CTAs a (request, head), joined here.
+template <typename T, int NG, int NT, bool JOINT>
 __global__ void __launch_bounds__(THREADS, ctas_of(NT)) kv4_attention_kernel(const Args a) {
     using S = Smem<NG, NT>;
     using R = kv4::Record<NG>;
@@ -214,7 +228,7 @@ __global__ void __launch_bounds__(THREADS, ctas_of(NT)) kv4_attention_kernel(con
         const int64_t total = (int64_t)pre[a.B] * per_b;
         return max((int64_t)LEAST, (total + gridDim.x - 1) / gridDim.x);
     };
-    if (a.split) {
+    if (!JOINT && a.split) {
         scan_costs(a, pre);
         const int64_t total = (int64_t)pre[a.B] * per_b, share = share_of();
         Line x = {};
@@ -237,8 +251,9 @@ __global__ void __launch_bounds__(THREADS, ctas_of(NT)) kv4_attention_kernel(con
     } else if (lane == 0) {
         Line x = {};
         x.end = 1;  // the CTA's one item is still to come
-        x.b = blockIdx.x / per_b;
-        x.item = blockIdx.x - x.b * per_b;
+        const int i = JOINT ? blockIdx.x / a.cluster : blockIdx.x;
+        x.b = i / per_b;
+        x.item = i - x.b * per_b;
         *line = x;
     }
     __syncwarp();
@@ -248,10 +263,15 @@ __global__ void __launch_bounds__(THREADS, ctas_of(NT)) kv4_attention_kernel(con
             Line y = *line;
             Part& x = y.next;
             x.n = -1;
-            if (!a.split) {
+            if (JOINT || !a.split) {
                 if (y.at < y.end) {
                     const int n = Seen(a, y.b).n;
                     x = {y.b, y.item, 0, n, n};
+                    if constexpr (JOINT) {
+                        const int r = blockIdx.x % a.cluster;
+                        x.i0 = (int)((int64_t)n * r / a.cluster);
+                        x.n = (int)((int64_t)n * (r + 1) / a.cluster) - x.i0;
+                    }
                     y.at = y.end;
                 }
             } else {
@@ -351,7 +371,7 @@ __global__ void __launch_bounds__(THREADS, ctas_of(NT)) kv4_attention_kernel(con
     look_up(now);
     begin(now);
 
-    if (a.split) {  // requests that see nothing belong to no stretch
+    if (!JOINT && a.split) {  // requests that see nothing belong to no stretch
         for (int e = blockIdx.x; e < a.B; e += gridDim.x)
             if (pre[e + 1] == pre[e])
                 for (int i = threadIdx.x; i < a.Hk * a.group * D; i += THREADS)
@@ -737,7 +757,10 @@ __global__ void __launch_bounds__(THREADS, ctas_of(NT)) kv4_attention_kernel(con
                 acc.z = fmaf(f, y.z, acc.z);
                 acc.w = fmaf(f, y.w, acc.w);
             }
-            if (all_mine) {
+            if constexpr (JOINT) {
+                *reinterpret_cast<float4*>(out_s + head * S::PAD + d) = acc;  // warp 0's place, which no other thread reads
+                if (d == 0) *reinterpret_cast<float2*>(smem + S::MERGED + 8 * head) = make_float2(mx, sum);
+            } else if (all_mine) {
                 if (hb * HB + head < a.group) {
                     const float inv = sum == 0.f ? 0.f : 1.0f / sum;  // 0: every key was hidden
                     T* dst = (T*)a.o + (int64_t)done.b * a.ob + (int64_t)(kh * a.group + hb * HB + head) * a.oh + d;
@@ -750,13 +773,41 @@ __global__ void __launch_bounds__(THREADS, ctas_of(NT)) kv4_attention_kernel(con
             }
         }
         // An item that starts here and goes on in the CTAs behind is joined from here.
-        if (threadIdx.x == 0 && done.i0 == 0 && !all_mine) {
+        if (!JOINT && threadIdx.x == 0 && done.i0 == 0 && !all_mine) {
             const int64_t share = share_of();
             a.chain[2 * blockIdx.x] = done.b * per_b + done.item;
             a.chain[2 * blockIdx.x + 1] = (int)((now_end - done.n + done.whole - 1) / share) - blockIdx.x + 1;
         }
         __syncwarp();
         if (lane == 0) sm100::mbar_arrive(merged);
+    }
+
+    // ---- a cluster's states, each CTA a share of the elements ----
+    if constexpr (JOINT) {
+        __syncwarp();
+        sm100::cluster_sync();
+        const int i = blockIdx.x / a.cluster, b = i / per_b, kh = (i - b * per_b) / a.blocks, hb = i - b * per_b - kh * a.blocks;
+        const int rank = blockIdx.x % a.cluster;
+        for (int e = rank * THREADS + threadIdx.x; e < HB * D / 2; e += a.cluster * THREADS) {
+            const int head = e / (D / 2), d = 2 * (e % (D / 2));
+            if (hb * HB + head >= a.group) break;  // heads come in order
+            const uint32_t out_at = sm100::smem_u32(out_s + head * S::PAD + d), stat_at = sm100::smem_u32(smem + S::MERGED + 8 * head);
+            float mx = NO_MAX, sum = 0.f;
+            float2 acc = sf::f2(0.f);
+#pragma unroll 4
+            for (int r = 0; r < a.cluster; ++r) {
+                const float2 st = ld_cluster(sm100::mapa_shared(stat_at, r)), x = ld_cluster(sm100::mapa_shared(out_at, r));
+                const float mn = fmaxf(mx, st.x), f = exp2f(mx - mn), g2 = exp2f(st.x - mn);
+                mx = mn;
+                sum = sum * f + st.y * g2;
+                acc = make_float2(acc.x * f + x.x * g2, acc.y * f + x.y * g2);
+            }
+            const float inv = sum == 0.f ? 0.f : 1.0f / sum;
+            *reinterpret_cast<uint32_t*>((T*)a.o + (int64_t)b * a.ob + (int64_t)(kh * a.group + hb * HB + head) * a.oh + d) =
+                sf::Pair<T>::from_f2(make_float2(acc.x * inv, acc.y * inv));
+        }
+        __syncwarp();
+        sm100::cluster_sync();  // nobody leaves while its states are read
     }
 }
 
@@ -823,7 +874,7 @@ int64_t most_tiles(int64_t width, int64_t tpp, int64_t window, int64_t sinks) {
 struct Plan {
     int nt, blocks;
     bool split;
-    int grid;
+    int cluster, grid;
 };
 
 Plan plan_of(int64_t B, int64_t Hq, int64_t Hk, int64_t D, int64_t width, int64_t tpp, int64_t window, int64_t sinks, int32_t variant) {
@@ -834,14 +885,22 @@ Plan plan_of(int64_t B, int64_t Hq, int64_t Hk, int64_t D, int64_t width, int64_
     const int64_t items = B * Hk * p.blocks;
     const int64_t wave = (int64_t)sf::sm_count() * ctas_of(p.nt);
     const int64_t tiles = most_tiles(width, tpp, window, sinks);
-    // Whole items a CTA while an item is at most four tiles a warp: nothing to join, no second
-    // launch.  Longer items are cut so that every CTA gets the same number of tiles.  (Above 1024
-    // requests the items balance the CTAs by themselves, and the prefix of the costs would take the
-    // shared memory.)
+    // Whole items a CTA while an item is at most four tiles a warp: nothing to join.  Longer items of a small
+    // batch go to clusters of CTAs that join through each other's shared memory, without a second launch, as
+    // long as their stretches are short and the clusters, each of which one group of SMs has to hold, take
+    // up to three quarters of the places (16 clusters of 16 on 296 places ran in two rounds: 17.4 against
+    // 12.0 us).  Else items are cut so that every CTA gets the same number of tiles.  (Above 1024 requests
+    // the items balance the CTAs by themselves, and the prefix of the costs would take the shared memory.)
+    p.cluster = 1;
     p.split = tiles > LEAST && B <= 1024;
+    if (variant == 0 && p.split) {
+        int c = MAX_CLUSTER;
+        while (c > 1 && (4 * items * c > 3 * wave || tiles < c * CLUSTER_LEAST)) c /= 2;
+        if (c > 1 && tiles <= (int64_t)c * CLUSTER_MOST) p.cluster = c, p.split = false;
+    }
     if (variant == 3) p.split = false;
     if (variant == 1) p.split = true;
-    p.grid = (int)(p.split ? std::min(wave, std::max<int64_t>(1, (items * (tiles + ITEM_COST) + LEAST - 1) / LEAST)) : items);
+    p.grid = (int)(p.split ? std::min(wave, std::max<int64_t>(1, (items * (tiles + ITEM_COST) + LEAST - 1) / LEAST)) : items * p.cluster);
     return p;
 }
 
@@ -864,12 +923,30 @@ int launch_t(Args a, const Plan& p, cudaStream_t st, char* err, uint64_t cap) {
         cudaGetDevice(&dev);
         std::lock_guard<std::mutex> lock(mu);
         if (dev >= 64 || !(done >> dev & 1)) {
-            const cudaError_t e = cudaFuncSetAttribute(kv4_attention_kernel<T, NG, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, MAX_SMEM);
+            cudaError_t e = cudaFuncSetAttribute(kv4_attention_kernel<T, NG, NT, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, MAX_SMEM);
+            if (e == cudaSuccess) e = cudaFuncSetAttribute(kv4_attention_kernel<T, NG, NT, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, MAX_SMEM);
+            if (e == cudaSuccess) e = cudaFuncSetAttribute(kv4_attention_kernel<T, NG, NT, true>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
             if (e != cudaSuccess) return sf::fail(SF_EDEVICE, err, cap, "kv4_attention: %s", cudaGetErrorString(e));
             if (dev < 64) done |= 1ull << dev;
         }
     }
-    kv4_attention_kernel<T, NG, NT><<<p.grid, THREADS, smem, st>>>(a);
+    if (p.cluster > 1) {
+        cudaLaunchConfig_t cfg = {};
+        cfg.gridDim = dim3((unsigned)p.grid);
+        cfg.blockDim = dim3(THREADS);
+        cfg.dynamicSmemBytes = smem;
+        cfg.stream = st;
+        cudaLaunchAttribute attr[1];
+        attr[0].id = cudaLaunchAttributeClusterDimension;
+        attr[0].val.clusterDim.x = p.cluster;
+        attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+        cfg.attrs = attr;
+        cfg.numAttrs = 1;
+        const cudaError_t e = cudaLaunchKernelEx(&cfg, kv4_attention_kernel<T, NG, NT, true>, (const Args)a);
+        if (e != cudaSuccess) return sf::fail(SF_EDEVICE, err, cap, "kv4_attention launch: %s", cudaGetErrorString(e));
+        return SF_OK;
+    }
+    kv4_attention_kernel<T, NG, NT, false><<<p.grid, THREADS, smem, st>>>(a);
     int rc = sf::check_launch("kv4_attention launch", err, cap);
     if (rc || !p.split) return rc;
     // The join starts while the last CTAs of the first kernel run, and waits for all of it.
@@ -947,6 +1024,7 @@ extern "C" int sf_kv4_attention(const sf_kv4_attention_args* x, void* stream, ch
     a.pages = (int)pages, a.tpp = (int)tpp, a.width = (int)width;
     a.scale_log2 = scale * LOG2E;
     a.split = p.split;
+    a.cluster = p.cluster;
     const bool half = x->dtype == SF_DTYPE_F16;
     cudaStream_t st = (cudaStream_t)stream;
     if (D == 64) {

@@ -242,3 +242,10 @@ def test_numbers_that_are_no_sizes_are_refused():
 
 def test_above_1024_requests_a_cta_takes_a_whole_one():
     assert ops.kv4_attention_workspace_bytes(1024, 4, 2, 64, 16, 400) > 0 and ops.kv4_attention_workspace_bytes(1025, 4, 2, 64, 16, 400) == 0
+
+
+def test_a_few_requests_of_moderate_length_need_no_workspace():
+    size = ops.kv4_attention_workspace_bytes
+    assert size(1, 32, 8, 128, 64, 65) == 0 and size(4, 32, 8, 128, 64, 32) == 0
+    assert size(1, 32, 8, 128, 64, 256) > 0 and size(64, 32, 8, 128, 64, 128) > 0     # long, many
+    assert size(1, 32, 8, 128, 64, 65, variant=1) > 0 and size(1, 32, 8, 128, 64, 65, variant=3) == 0

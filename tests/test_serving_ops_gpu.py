@@ -332,6 +332,37 @@ def test_kv4_attention(case, dtype, variant):
     check_decode(out, q, kq, vq, page, table, lens, d**-0.5, window, sinks)
 
 
+CLUSTERS = [
+    # lengths, Hq, Hk, D, page, width, window, sinks: a few requests whose (request, head) pairs go to 16, 8, 4 and 2 CTAs each
+    ([1500], 8, 1, 128, 32, 60, 0, 0),
+    ([1, 17, 0, 640], 32, 8, 128, 16, 41, 0, 0),
+    ([700, 3, 0, 500, 111, 690, 16, 15], 64, 8, 128, 64, 11, 0, 0),
+    ([300, 0, 272, 299], 64, 32, 64, 16, 19, 0, 0),
+    ([2000, 90], 24, 2, 64, 16, 130, 0, 0),
+    ([900, 33], 40, 1, 128, 16, 60, 0, 0),
+    ([1500, 300], 16, 4, 128, 32, 60, 700, 20),
+    ([1024], 5, 1, 64, 1024, 1, 0, 0),
+]
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+@pytest.mark.parametrize("case", CLUSTERS, ids=[f"{len(c[0])}x{max(c[0])}-{'x'.join(map(str, c[1:]))}" for c in CLUSTERS])
+def test_kv4_attention_in_clusters(case, dtype):
+    """Small batches need no workspace; tiles that a cluster's last CTAs do not get, and empty requests, count nothing."""
+    lens, hq, h, d, page, width, window, sinks = case
+    g, dt, b = gen(44), TD[dtype], len(lens)
+    assert ops.kv4_attention_workspace_bytes(b, hq, h, d, page, width, window, sinks) == 0
+    assert ops.kv4_attention_workspace_bytes(b, hq, h, d, page, width, window, sinks, variant=1) > 0
+    cache, kq, vq = filled_cache(g, b * width, page, h, d, dt)
+    table = torch.randperm(b * width, device="cuda", generator=g).view(b, width).to(torch.int32)
+    q = randn(g, b, hq, d, dtype=dt)
+    out = torch.full((b, hq, d), math.nan, device="cuda", dtype=dt)
+    ops.kv4_attention(q, cache, table, i32(lens), d**-0.5, window=window, sinks=sinks, out=out)
+    check_decode(out, q, kq, vq, page, table, lens, d**-0.5, window, sinks)
+    for _ in range(3):
+        assert torch.equal(ops.kv4_attention(q, cache, table, i32(lens), d**-0.5, window=window, sinks=sinks), out)
+
+
 def test_kv4_attention_peaked_and_large_scores():
     """Scores far apart (one key takes nearly all), growing along the keys, and large queries."""
     g = gen(10)
@@ -427,15 +458,15 @@ def test_kv4_attention_strides_workspace_and_same_bits():
     q = packed[:, 8:16]
     out = torch.zeros(8, 2, 128, device="cuda", dtype=torch.bfloat16).transpose(0, 1)
     lens = [1100, 640]
-    need = ops.kv4_attention_workspace_bytes(2, 8, 2, 128, 64, 18)
+    need = ops.kv4_attention_workspace_bytes(2, 8, 2, 128, 64, 18, variant=1)
     ws = torch.full((need + 64,), 0xAB, dtype=torch.uint8, device="cuda")
-    ops.kv4_attention(q, cache, table, i32(lens), 0.1, out=out, workspace=ws[:need])
+    ops.kv4_attention(q, cache, table, i32(lens), 0.1, out=out, workspace=ws[:need], variant=1)
     check_decode(out, q, kq, vq, 64, table, lens, 0.1, 0, 0)
     assert (ws[need:] == 0xAB).all()
     with pytest.raises(_native.SfError):
-        ops.kv4_attention(q, cache, table, i32(lens), 0.1, workspace=ws[: need - 16])
+        ops.kv4_attention(q, cache, table, i32(lens), 0.1, workspace=ws[: need - 16], variant=1)
     for _ in range(3):
-        assert torch.equal(ops.kv4_attention(q, cache, table, i32(lens), 0.1), out)
+        assert torch.equal(ops.kv4_attention(q, cache, table, i32(lens), 0.1, variant=1), out)
 
 
 # ---- windowed attention of prompts --------------------------------------------------------------
