@@ -4,6 +4,9 @@
 // and head.  Four lanes hold a group of 64 elements, 16 each: the 16-byte pieces `quarter` and quarter
 // + 4, so that a warp's accesses to the values fill whole sectors; a thread keeps its (head, keys or
 // values, group, quarter) and walks the tokens, so everything but the slot is computed once.
+// 32768 tokens of 8 heads of 128 in bf16: store 41 us, 4.2 TB/s, bound by its instructions (issue slots 70 % busy:
+// extrema, exactly rounded quotients, packing); load 35 us, 4.9 TB/s, between DRAM and the expansion of the codes.
+// Pieces that fill no whole sectors took 55 and 38 us.
 #include "kv4.cuh"
 
 #include <initializer_list>

@@ -9,12 +9,14 @@
 // w_q, w_k [D], position [T] int32, fp16 / bf16 in and out, fp32 arithmetic, one rounding.  The
 // outputs may be the inputs' own buffers: the lanes that write a row have read all of it.
 //
-// HBM-bound: T (Hq + Hk) D elements in and out, each moved once.
+// HBM-bound: T (Hq + Hk) D elements in and out, each moved once.  16384 tokens of 32 + 8 heads of 128 in bf16:
+// 65 us, 5.1 TB/s (79 % of a copy); 64 tokens: 3.4 us, the launch and one round of loads.
 //  * A row of D elements is held by D/16 lanes, two 8-element chunks a lane; a lane's chunks are c
 //    and c + r/8, so both members of a rotated pair sit in one lane and only the sum of squares
 //    crosses lanes (2-4 shuffles).
 //  * The angle depends on (t, i) alone, so a warp stays with one token, takes sine and cosine of
-//    its 8 angles a lane once, and walks the token's heads, two row groups in flight.  Tokens are
+//    its 8 angles a lane once, and walks the token's heads, two row groups at work and the next two in
+//    flight (69 us without, and with the weights in registers instead of shared memory).  Tokens are
 //    split over heads only when there are too few of them to fill the GPU.
 //  * The angle is reduced in double precision (a position near 2^20 times a frequency leaves no
 //    fraction bits in fp32), in turns: frac(position * base^(-i/r) / 2 pi), |.| <= 1/2, then the

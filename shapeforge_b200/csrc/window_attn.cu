@@ -126,6 +126,11 @@ __global__ void __launch_bounds__(128) window_general_kernel(const Args a, int D
 // needs no alignment), and the sinks in front of it are a tile of their own; a tile of n keys costs
 // n rounded up to 16 in both products and 32 in the softmax.  Tiles that every row sees in full skip the
 // mask.  Running max and sum in fp32; the max follows a score only past 2^8, so O is rarely rescaled.
+// 16384 tokens, 16 heads on 2 of 128, window 4096, bf16: 381 us, 1264 TFLOP/s of seen scores (77 % of what a large
+// library product reaches; 65 % in loops of seconds under the power cap): a step of 128 keys for 256 rows takes
+// 1.40 us, its products 1.04 at the pipe's rate, and a CTA's start and end three steps.  1203 tokens in 9 prompts,
+// window 128: 21 us, two CTAs in turn on an SM, latency.  (CTAs that take their next piece from the hardware's
+// scheduler hide the start and end, but the registers that costs the softmax slowed every step: 411 us.)
 // P is rounded to the tensors' type (as the fp32 sum of the unrounded weights divides it, a weight is off
 // by half a step, which averages out over the keys).
 // A row that comes out NaN (or infinite) is computed again key by key: masked keys in its tiles may hold
