@@ -10,19 +10,20 @@
 // outputs may be the inputs' own buffers: the lanes that write a row have read all of it.
 //
 // HBM-bound: T (Hq + Hk) D elements in and out, each moved once.  16384 tokens of 32 + 8 heads of 128 in bf16:
-// 65 us, 5.1 TB/s (79 % of a copy); 64 tokens: 3.4 us, the launch and one round of loads.
+// 57 us, 5.9 TB/s (90 % of a copy); 64 tokens: 3.4 us, the launch and one round of loads.
 //  * A row of D elements is held by D/16 lanes, two 8-element chunks a lane; a lane's chunks are c
 //    and c + r/8, so both members of a rotated pair sit in one lane and only the sum of squares
 //    crosses lanes (2-4 shuffles).
 //  * The angle depends on (t, i) alone, so a warp stays with one token, takes sine and cosine of
-//    its 8 angles a lane once, and walks the token's heads, two row groups at work and the next two in
-//    flight (69 us without, and with the weights in registers instead of shared memory).  Tokens are
+//    its 8 angles a lane once, and walks the token's heads, two row groups at work and the next four in
+//    flight, the next token's among them (asynchronous copies into the lane's own places).  Tokens are
 //    split over heads only when there are too few of them to fill the GPU.
 //  * The angle is reduced in double precision (a position near 2^20 times a frequency leaves no
 //    fraction bits in fp32), in turns: frac(position * base^(-i/r) / 2 pi), |.| <= 1/2, then the
 //    special-function sine and cosine of at most pi (absolute error ~2^-21, far below half a step
 //    of a 16-bit output).
 #include "sf_common.cuh"
+#include "sm100.cuh"
 
 #include <cmath>
 #include <initializer_list>
@@ -55,13 +56,21 @@ __device__ __forceinline__ uint4 pack8(const float2 (&v)[4]) {
     return make_uint4(sf::Pair<T>::from_f2(v[0]), sf::Pair<T>::from_f2(v[1]), sf::Pair<T>::from_f2(v[2]), sf::Pair<T>::from_f2(v[3]));
 }
 
+// 16384 tokens of 40 heads of 128: 4 CTAs of 4 warps an SM 57 us, 3 58.7, 5 61.3, 6 60.7; 4 pairs of groups in the ring
+// 57.7; the next groups in registers instead (2 CTAs of 8 warps) 65.
+constexpr int WARPS = 4;  // a CTA
+constexpr int CTAS = 4;   // an SM
+constexpr int AHEAD = 3;  // pairs of row groups in a warp's ring
+
 // LPR lanes a row (a power of two >= D / 16); `items` = tokens x head parts, one warp an item.
 template <typename T, int LPR>
-__global__ void __launch_bounds__(256, 2) qk_norm_rope_kernel(const Side q, const Side k, const int32_t* __restrict__ position, int64_t tokens,
-                                                              int hq, int hk, int D, int r, double ratio, float eps, int parts) {
+__global__ void __launch_bounds__(32 * WARPS, CTAS) qk_norm_rope_kernel(const Side q, const Side k, const int32_t* __restrict__ position, int64_t tokens,
+                                                                     int hq, int hk, int D, int r, double ratio, float eps, int parts) {
     constexpr int RPW = 32 / LPR;  // rows a warp holds at once
     // Both weights, in the lanes' order: 16 bytes a chunk (in registers they would cost a third of the warps).
     __shared__ uint4 w_s[2][2][32];
+    // The rows in flight: a lane copies its own two chunks of each of a pair's groups and reads them back itself.
+    __shared__ uint4 ring_s[WARPS][AHEAD][2][2][32];
     const int lane = threadIdx.x & 31;
     const int p = lane % LPR, sub = lane / LPR;
     const bool live = p < D / 16;
@@ -95,31 +104,57 @@ __global__ void __launch_bounds__(256, 2) qk_norm_rope_kernel(const Side q, cons
     const int per = (groups + parts - 1) / parts;
     const int64_t items = tokens * parts;
     const int64_t step = (int64_t)gridDim.x * (blockDim.x >> 5);
-    for (int64_t item = (int64_t)blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5); item < items; item += step) {
-        const int64_t t = parts == 1 ? item : item / parts;
-        const int g0 = (int)(item - t * parts) * per, g1 = min(groups, g0 + per);
-        const T* xq = (const T*)q.x + t * q.xt;
-        const T* xk = (const T*)k.x + t * k.xt;
-        // Row of group g for this lane, -1: none.
-        auto row_of = [&](int g) {
-            const int row = g * RPW + sub;
-            return live && g < g1 && row < rows ? row : -1;
-        };
-        auto load = [&](int row, uint4& a, uint4& b) {
-            a = b = make_uint4(0, 0, 0, 0);
-            if (row >= 0) {
-                const T* x = row < hq ? xq + row * q.xh : xk + (row - hq) * k.xh;
-                a = *reinterpret_cast<const uint4*>(x + e0);
-                b = *reinterpret_cast<const uint4*>(x + e1);
-            }
-        };
-        uint4 na[2], nb[2];
+    const int64_t first = (int64_t)blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5);
+    uint4(*ring)[2][2][32] = ring_s[threadIdx.x >> 5];
+    // A place in the warp's rows, two groups at a time: token, next group, end of the item's groups.
+    struct Cursor {
+        int64_t item, t;
+        int g, g1;
+    };
+    auto enter = [&](Cursor& c) {
+        c.t = parts == 1 ? c.item : (int64_t)((uint32_t)c.item / (uint32_t)parts);  // items are few when tokens are split
+        c.g = (int)(c.item - c.t * parts) * per;
+        c.g1 = min(groups, c.g + per);
+    };
+    auto next = [&](Cursor& c) {
+        c.g += 2;
+        if (c.g >= c.g1) {
+            c.item += step;
+            if (c.item < items) enter(c);
+        }
+    };
+    auto row_of = [&](const Cursor& c, int u) {
+        const int row = (c.g + u) * RPW + sub;
+        return live && c.g + u < c.g1 && row < rows ? row : -1;
+    };
+    Cursor ahead = {first, 0, 0, 0};
+    if (first < items) enter(ahead);
+    Cursor at = ahead;
+    auto fetch = [&](int stage) {
+        if (ahead.item < items) {
 #pragma unroll
-        for (int u = 0; u < 2; ++u) load(row_of(g0 + u), na[u], nb[u]);
-        // Sines and cosines while the first rows are on their way.
-        const double pos = (double)__ldg(position + t);
-        float2 sn[4], cs[4];
-        {
+            for (int u = 0; u < 2; ++u) {
+                const int row = row_of(ahead, u);
+                if (row >= 0) {
+                    const T* x = row < hq ? (const T*)q.x + ahead.t * q.xt + row * q.xh : (const T*)k.x + ahead.t * k.xt + (row - hq) * k.xh;
+                    sm100::cp_async_16(sm100::smem_u32(&ring[stage][u][0][lane]), x + e0, 16);
+                    sm100::cp_async_16(sm100::smem_u32(&ring[stage][u][1][lane]), x + e1, 16);
+                }
+            }
+            next(ahead);
+        }
+        asm volatile("cp.async.commit_group;" ::: "memory");
+    };
+#pragma unroll
+    for (int i = 0; i < AHEAD - 1; ++i) fetch(i);
+    int stage = 0;
+    int64_t shown = -1;  // the token whose angles are held
+    float2 sn[4], cs[4];
+    while (at.item < items) {
+        const int64_t t = at.t;
+        if (t != shown) {
+            shown = t;
+            const double pos = (double)__ldg(position + t);
             double f = turn0;
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
@@ -133,49 +168,54 @@ __global__ void __launch_bounds__(256, 2) qk_norm_rope_kernel(const Side q, cons
                 }
             }
         }
-        for (int g = g0; g < g1; g += 2) {
-            uint4 a[2], b[2];
+        // Into the place that the last pair left, whose values have been used.
+        fetch(stage == 0 ? AHEAD - 1 : stage - 1);
+        asm volatile("cp.async.wait_group %0;" ::"n"(AHEAD - 1) : "memory");
+        uint4 a[2], b[2];
 #pragma unroll
-            for (int u = 0; u < 2; ++u) {
-                a[u] = na[u];
-                b[u] = nb[u];
-                load(row_of(g + 2 + u), na[u], nb[u]);
-            }
-#pragma unroll
-            for (int u = 0; u < 2; ++u) {
-                const int row = row_of(g + u);
-                float2 va[4], vb[4];
-                unpack8<T>(a[u], va);
-                unpack8<T>(b[u], vb);
-                float2 ss = sf::f2_mul(va[0], va[0]);
-#pragma unroll
-                for (int j = 1; j < 4; ++j) ss = sf::f2_fma(va[j], va[j], ss);
-#pragma unroll
-                for (int j = 0; j < 4; ++j) ss = sf::f2_fma(vb[j], vb[j], ss);
-                float sum = ss.x + ss.y;
-#pragma unroll
-                for (int o = LPR / 2; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-                if (row < 0) continue;
-                const float2 rs = sf::f2(rsqrtf(fmaf(sum, inv_d, eps)));
-                const bool isq = row < hq;
-                float2 w0[4], w1[4], o0[4], o1[4];
-                unpack8<T>(w_s[isq ? 0 : 1][0][p], w0);
-                unpack8<T>(w_s[isq ? 0 : 1][1][p], w1);
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    const float2 y0 = sf::f2_mul(sf::f2_mul(va[j], rs), w0[j]), y1 = sf::f2_mul(sf::f2_mul(vb[j], rs), w1[j]);
-                    o0[j] = y0;
-                    o1[j] = y1;
-                    if (turned) {  // where nothing turns an infinite partner would leave NaN
-                        o0[j] = make_float2(fmaf(-y1.x, sn[j].x, y0.x * cs[j].x), fmaf(-y1.y, sn[j].y, y0.y * cs[j].y));
-                        o1[j] = sf::f2_fma(y1, cs[j], sf::f2_mul(y0, sn[j]));
-                    }
-                }
-                T* y = isq ? (T*)q.y + t * q.yt + row * q.yh : (T*)k.y + t * k.yt + (row - hq) * k.yh;
-                *reinterpret_cast<uint4*>(y + e0) = pack8<T>(o0);
-                *reinterpret_cast<uint4*>(y + e1) = pack8<T>(o1);
+        for (int u = 0; u < 2; ++u) {
+            a[u] = b[u] = make_uint4(0, 0, 0, 0);
+            if (row_of(at, u) >= 0) {
+                a[u] = ring[stage][u][0][lane];
+                b[u] = ring[stage][u][1][lane];
             }
         }
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+            const int row = row_of(at, u);
+            float2 va[4], vb[4];
+            unpack8<T>(a[u], va);
+            unpack8<T>(b[u], vb);
+            float2 ss = sf::f2_mul(va[0], va[0]);
+#pragma unroll
+            for (int j = 1; j < 4; ++j) ss = sf::f2_fma(va[j], va[j], ss);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) ss = sf::f2_fma(vb[j], vb[j], ss);
+            float sum = ss.x + ss.y;
+#pragma unroll
+            for (int o = LPR / 2; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+            if (row < 0) continue;
+            const float2 rs = sf::f2(rsqrtf(fmaf(sum, inv_d, eps)));
+            const bool isq = row < hq;
+            float2 w0[4], w1[4], o0[4], o1[4];
+            unpack8<T>(w_s[isq ? 0 : 1][0][p], w0);
+            unpack8<T>(w_s[isq ? 0 : 1][1][p], w1);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const float2 y0 = sf::f2_mul(sf::f2_mul(va[j], rs), w0[j]), y1 = sf::f2_mul(sf::f2_mul(vb[j], rs), w1[j]);
+                o0[j] = y0;
+                o1[j] = y1;
+                if (turned) {  // where nothing turns an infinite partner would leave NaN
+                    o0[j] = make_float2(fmaf(-y1.x, sn[j].x, y0.x * cs[j].x), fmaf(-y1.y, sn[j].y, y0.y * cs[j].y));
+                    o1[j] = sf::f2_fma(y1, cs[j], sf::f2_mul(y0, sn[j]));
+                }
+            }
+            T* y = isq ? (T*)q.y + t * q.yt + row * q.yh : (T*)k.y + t * k.yt + (row - hq) * k.yh;
+            *reinterpret_cast<uint4*>(y + e0) = pack8<T>(o0);
+            *reinterpret_cast<uint4*>(y + e1) = pack8<T>(o1);
+        }
+        stage = stage + 1 == AHEAD ? 0 : stage + 1;
+        next(at);
     }
 }
 
@@ -218,18 +258,17 @@ template <typename T, int LPR>
 int launch_vec(const Side& q, const Side& k, const int32_t* pos, int64_t T_, int hq, int hk, int D, int r, double base, float eps,
                cudaStream_t st, char* err, uint64_t cap) {
     constexpr int RPW = 32 / LPR;
-    static const int resident = sf::resident_ctas(qk_norm_rope_kernel<T, LPR>, 256, 0);
-    const int64_t ctas = (int64_t)sf::sm_count() * resident;
+    const int64_t ctas = (int64_t)sf::sm_count() * CTAS;
     const int64_t groups = (hq + hk + RPW - 1) / RPW;
     // A warp takes a whole token (its angles once) while the tokens fill the GPU's warps; fewer
     // tokens are split over their heads so that every warp has work.
-    int64_t parts = ctas * 8 / T_;
+    int64_t parts = ctas * WARPS / T_;
     parts = parts < 1 ? 1 : (parts > groups ? groups : parts);
     const int64_t items = T_ * parts;
     // Small problems: two-warp CTAs spread over all SMs.
-    const int threads = items <= (int64_t)sf::sm_count() * 8 ? 64 : 256;
+    const int threads = items <= (int64_t)sf::sm_count() * 8 ? 64 : 32 * WARPS;
     int64_t blocks = (items + threads / 32 - 1) / (threads / 32);
-    if (blocks > ctas * (256 / threads)) blocks = ctas * (256 / threads);
+    if (blocks > ctas * (32 * WARPS / threads)) blocks = ctas * (32 * WARPS / threads);
     qk_norm_rope_kernel<T, LPR><<<(unsigned)blocks, threads, 0, st>>>(q, k, pos, T_, hq, hk, D, r, r ? std::pow(base, -1.0 / (double)r) : 1.0, eps,
                                                                       (int)parts);
     return sf::check_launch("qk_norm_rope launch", err, cap);
