@@ -30,7 +30,9 @@ struct Args {
     int seqs, group, heads;                  // sequences, query heads a kv head, query heads
     int window, sinks;
     float scale_log2;
-    int splits;          // CTAs that share a row tile's keys; above 1 each leaves its state for the join:
+    int slots;           // of tokens, a kv head
+    int splits;          // CTAs that share the keys of a pair of row tiles; above 1 each leaves its state for the join:
+    int whole;           // pairs of row tiles, in the grid's order, whose keys stay together all the same
     float *part, *stat;  // [splits][tq][heads][D] unnormalised outputs, [splits][tq][heads][2] running max, sum
 };
 
@@ -351,7 +353,8 @@ __device__ __forceinline__ float max32(const uint32_t* r, float m) {
     return max3_nan(a[0], a[1], a[1]);
 }
 
-template <typename T, int D>
+// LINE: a.whole pairs of row tiles keep their keys, the others are split, all in one line of CTAs.
+template <typename T, int D, bool LINE>
 __global__ void __launch_bounds__(TC_THREADS, 1)
     window_tc_kernel(const Args a, const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUtensorMap mk16,
                      const __grid_constant__ CUtensorMap mv, const __grid_constant__ CUtensorMap mv16, int tq_tile) {
@@ -363,7 +366,12 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
     Bars* bars = reinterpret_cast<Bars*>(smem + L::BARS);
     sm100::KernelStatus* status = &g_window_status;
     const int warp = uniform(threadIdx.x >> 5), lane = threadIdx.x & 31;
-    const int kvh = blockIdx.y;
+    // The whole pairs, then the others' first parts, their second parts and so on.
+    const int rest = LINE ? a.slots * (a.heads / a.group) - a.whole : 1;
+    const int part = !LINE ? blockIdx.z : (blockIdx.x < a.whole ? 0 : (blockIdx.x - a.whole) / rest);
+    const int parts = LINE && blockIdx.x < a.whole ? 1 : a.splits;
+    const int pair = LINE ? blockIdx.x - part * rest : 0;
+    const int kvh = LINE ? pair / a.slots : blockIdx.y;
 
     // Set-up that needs no lengths runs while the search below waits for them.
     if (threadIdx.x == 0) {
@@ -391,7 +399,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
     sm100::fence_proxy_async_smem();
 
     Where at;
-    const bool found = locate(a, 2 * tq_tile, gridDim.x - 1 - blockIdx.x, &at);
+    const bool found = locate(a, 2 * tq_tile, LINE ? a.slots - 1 - (pair - kvh * a.slots) : gridDim.x - 1 - blockIdx.x, &at);
     if (!found) return;  // a slot that rounding left over
     const int tok0 = at.tok0, kb = at.kb, ke = at.ke;
     const int rows_tok[2] = {min(tq_tile, at.qe - tok0), max(0, min(tq_tile, at.qe - tok0 - tq_tile))};
@@ -403,10 +411,10 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
     w.sink_tiles = (w.sink_end + 127) >> 7;
     w.n = w.high > 0 ? w.sink_tiles + ((w.high - w.low + 127) >> 7) : 0;
     w.base = 0;
-    if (a.splits > 1) {
+    if (parts > 1) {
         const int n = w.n;
-        w.base = (int)((int64_t)n * blockIdx.z / a.splits);
-        w.n = (int)((int64_t)n * (blockIdx.z + 1) / a.splits) - w.base;
+        w.base = (int)((int64_t)n * part / parts);
+        w.n = (int)((int64_t)n * (part + 1) / parts) - w.base;
     }
     const Span span0(a, w, pos0, uniform(rows_tok[0])), span1(a, w, pos0 + tq_tile, uniform(rows_tok[1]));
 
@@ -663,10 +671,10 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
         float2 nan = sf::f2(0.f);
         if (w.n > 0) ok = wait_soon(&bars->o_done[t], 0, status, 128) && ok;
         sm100::tc_fence_after();
-        if (a.splits > 1) {
+        if (parts > 1) {
             // The row's state for the join, O as it is: half its columns at a time through the Q buffer.
             const bool own = live && ok;
-            const int64_t row_at = ((int64_t)blockIdx.z * a.tq + tok0 + t * tq_tile + tok) * a.heads + kvh * a.group + row - tok * a.group;
+            const int64_t row_at = ((int64_t)part * a.tq + tok0 + t * tq_tile + tok) * a.heads + kvh * a.group + row - tok * a.group;
             if (own) *reinterpret_cast<float2*>(a.stat + 2 * row_at) = make_float2(turn ? s.m : -INFINITY, s.l);
             const uint32_t written = __ballot_sync(0xffffffffu, own);
             constexpr int PIECES = D / 8;  // 16-byte pieces of half a row
@@ -749,10 +757,16 @@ constexpr int JOIN_ROWS = 16;
 template <typename T, int D>
 __global__ void __launch_bounds__(256) window_join_kernel(const Args a, int tq_tile) {
     asm volatile("griddepcontrol.wait;" ::: "memory");
+    int slot = blockIdx.x, kvh = blockIdx.y;
+    if (a.whole) {
+        const int pair = a.whole + blockIdx.x;
+        kvh = pair / a.slots;
+        slot = a.slots - 1 - (pair - kvh * a.slots);
+    }
     Where at;
-    if (!locate(a, 2 * tq_tile, blockIdx.x, &at)) return;
+    if (!locate(a, 2 * tq_tile, slot, &at)) return;
     constexpr int ROWS = JOIN_ROWS / 8, E = D / 32;
-    const int lane = threadIdx.x & 31, kvh = blockIdx.y;
+    const int lane = threadIdx.x & 31;
     const int r0 = blockIdx.z * JOIN_ROWS + (threadIdx.x >> 5) * ROWS;
     const int rows = min(ROWS, min(2 * tq_tile, at.qe - at.tok0) * a.group - r0);
     if (rows <= 0) return;
@@ -819,25 +833,29 @@ __global__ void __launch_bounds__(256) window_join_kernel(const Args a, int tq_t
 // sequences of equal length.  bf16, 32 query heads on 8 key heads of 128, no window: 1 token x 32768 keys
 // 371 us unsplit, 37 us at the 16 chosen; 64 x 8192 104 and 27 (16); 4 x 16 x 4096 54 and 26 (4); 512 x 32768
 // 389 and 222 (2); 2048 x 16384 406 unsplit as chosen, 474 in two.
-int64_t splits_of(int64_t Tq, int64_t Tk, int64_t seqs, int64_t Hq, int64_t Hk, int64_t D, int64_t window, int64_t sinks) {
+// Where the pairs of row tiles are more than a round of CTAs, those of the whole rounds keep their keys and
+// only the last, partial round's are split: 1536 tokens in 3 prompts behind 8200, 28 heads on 4 (177 pairs),
+// 221 us unsplit, 197 all in 3, HYBRID.
+struct Split {
+    int64_t z, whole;
+};
+Split split_of(int64_t Tq, int64_t Tk, int64_t seqs, int64_t Hq, int64_t Hk, int64_t D, int64_t window, int64_t sinks) {
     const int64_t group = Hq / Hk;
-    if ((D != 64 && D != 128) || group > 128 || Tk == 0 || seqs == 0) return 1;
-    const int64_t tt = 2 * (128 / group), tokens = (Tq + seqs - 1) / seqs, ctas = std::min(seqs, Tq) * ((tokens + tt - 1) / tt) * Hk;
+    Split pick = {1, 0};
+    if ((D != 64 && D != 128) || group > 128 || Tk == 0 || seqs == 0) return pick;
+    const int64_t tt = 2 * (128 / group), tokens = (Tq + seqs - 1) / seqs, pairs = std::min(seqs, Tq) * ((tokens + tt - 1) / tt) * Hk;
     int64_t keys = Tk / seqs;
     if (window) keys = std::min(keys, window + tt + (sinks ? std::min<int64_t>(sinks, keys) : 0));
-    const int64_t tiles = (keys + 127) / 128;
-    const int64_t sms = sf::sm_count();
-    double best = 1e30;
-    int64_t pick = 1;
-    for (int64_t z : {1, 2, 3, 4, 6, 8, 12, 16, 24, 32}) {
-        if (z > 1 && tiles / z < 2) break;
-        const int64_t waves = (ctas * z + sms - 1) / sms;
-        double cost = (double)waves * ((tiles + z - 1) / z + 3);
-        if (z > 1) cost += 3 + (double)Tq * Hq * D * 8 * z / 9e6;  // 9 MB of states in a tile's time
-        if (cost < best) {
-            best = cost;
-            pick = z;
-        }
+    const int64_t tiles = (keys + 127) / 128, sms = sf::sm_count(), rounds = pairs / sms, rest = pairs % sms;
+    double best = (double)(rounds + (rest > 0)) * (tiles + 3);
+    for (int64_t z : {2, 3, 4, 6, 8, 12, 16, 24, 32}) {
+        if (tiles / z < 2) break;
+        const double part = (double)((tiles + z - 1) / z + 3), join = (double)Tq * Hq * D * 8 * z / 9e6;  // 9 MB of states in a tile's time
+        const double all = (double)((pairs * z + sms - 1) / sms) * part + 3 + join;
+        const double last = (double)rounds * (tiles + 3) + (double)((rest * z + sms - 1) / sms) * part + 3 + join * rest / pairs;
+        if (all < best) best = all, pick = {z, 0};
+        // The slots that rounding leaves over lie among the others.
+        if (rounds && rest && last < best) best = last, pick = {z, rounds * sms * (Tq / tt + seqs) * Hk / pairs};
     }
     return pick;
 }
@@ -866,18 +884,25 @@ int launch_tc(Args a, int64_t hk, bool* taken, cudaStream_t st, char* err, uint6
         cudaGetDevice(&dev);
         std::lock_guard<std::mutex> lock(mu);
         if (dev >= 64 || !(done >> dev & 1)) {
-            const cudaError_t e = cudaFuncSetAttribute(window_tc_kernel<T, D>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+            cudaError_t e = cudaFuncSetAttribute(window_tc_kernel<T, D, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+            if (e == cudaSuccess) e = cudaFuncSetAttribute(window_tc_kernel<T, D, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
             if (e != cudaSuccess) return sf::fail(SF_EDEVICE, err, cap, "window_attention: %s", cudaGetErrorString(e));
             if (dev < 64) done |= 1ull << dev;
         }
     }
     const int64_t slots = a.tq / (2 * tq_tile) + a.seqs;
     if (slots > 0x7fffffffLL) return sf::fail(SF_EINVAL, err, cap, "window_attention: grid too large");
-    window_tc_kernel<T, D><<<dim3((unsigned)slots, (unsigned)hk, (unsigned)a.splits), TC_THREADS, smem, st>>>(a, mq, mk, mk16, mv, mv16, tq_tile);
+    a.slots = (int)slots;
+    const int64_t rest = slots * hk - a.whole;  // pairs of row tiles that are split
+    if (a.whole && (rest <= 0 || a.whole + rest * a.splits > 0x7fffffffLL)) a.whole = 0;
+    const auto kernel = a.whole ? window_tc_kernel<T, D, true> : window_tc_kernel<T, D, false>;
+    const dim3 grid = a.whole ? dim3((unsigned)(a.whole + rest * a.splits)) : dim3((unsigned)slots, (unsigned)hk, (unsigned)a.splits);
+    kernel<<<grid, TC_THREADS, smem, st>>>(a, mq, mk, mk16, mv, mv16, tq_tile);
     int rc = sf::check_launch("window_attention launch", err, cap);
     if (rc || a.splits == 1) return rc;
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned)slots, (unsigned)hk, (unsigned)((2 * tq_tile * a.group + JOIN_ROWS - 1) / JOIN_ROWS));
+    const unsigned blocks = (unsigned)((2 * tq_tile * a.group + JOIN_ROWS - 1) / JOIN_ROWS);
+    cfg.gridDim = a.whole ? dim3((unsigned)rest, 1, blocks) : dim3((unsigned)slots, (unsigned)hk, blocks);
     cfg.blockDim = dim3(256);
     cfg.stream = st;
     cudaLaunchAttribute attr[1];
@@ -904,7 +929,7 @@ int launch_general(const Args& a, int64_t D, cudaStream_t st, char* err, uint64_
 extern "C" uint64_t sf_window_attention_workspace_bytes(int64_t Tq, int64_t Tk, int64_t seqs, int64_t Hq, int64_t Hk, int64_t D, int64_t window,
                                                         int64_t sinks) {
     if (Tq <= 0 || Tk <= 0 || seqs <= 0 || Hq <= 0 || Hk <= 0 || Hq % Hk || window < 0 || sinks < 0) return 0;
-    const int64_t z = splits_of(Tq, Tk, seqs, Hq, Hk, D, window, sinks);
+    const int64_t z = split_of(Tq, Tk, seqs, Hq, Hk, D, window, sinks).z;
     return z > 1 ? (uint64_t)(z * Tq * Hq * (D + 2) * 4) : 0;
 }
 
@@ -937,9 +962,11 @@ extern "C" int sf_window_attention(const sf_window_attention_args* x, void* stre
     a.scale_log2 = scale * LOG2E;
     a.splits = 1;
     if (x->variant != 4) {
-        const int64_t z = splits_of(Tq, Tk, seqs, Hq, Hk, D, x->window, x->sinks);
+        const Split split = split_of(Tq, Tk, seqs, Hq, Hk, D, x->window, x->sinks);
+        const int64_t z = split.z;
         if (z > 1 && x->workspace && sf::aligned16(x->workspace) && x->workspace_bytes >= (uint64_t)(z * Tq * Hq * (D + 2) * 4)) {
             a.splits = (int)z;
+            a.whole = (int)split.whole;
             a.part = (float*)x->workspace;
             a.stat = a.part + z * Tq * Hq * D;
         }

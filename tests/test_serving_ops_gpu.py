@@ -565,6 +565,43 @@ def test_window_attention_split_over_keys(case, dtype):
         check_window(whole, q, k, v, cu_q, cu_k, d**-0.5, window, sinks, 0, before)
 
 
+LAST_ROUND = [
+    # More pairs of row tiles than SMs by a few, many keys: only the last round's are split.
+    ([640], [1500], 64, 1, 64, 0, 0),
+    ([400, 300, 333], [900, 2000, 1500], 40, 2, 128, 900, 4),
+    ([560, 0, 760, 20], [1100, 50, 900, 3000], 28, 4, 128, 0, 0),
+    ([650, 3], [1300, 1400], 64, 1, 128, 0, 0),
+]
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+@pytest.mark.parametrize("case", LAST_ROUND, ids=[f"{'_'.join(map(str, c[0]))}-{'x'.join(map(str, c[2:]))}" for c in LAST_ROUND])
+def test_window_attention_split_in_the_last_round(case, dtype):
+    lq, ctx, hq, hk, d, window, sinks = case
+    g, dt = gen(45), TD[dtype]
+    lk = [max(0, a + b) for a, b in zip(lq, ctx)]
+    cu_q, cu_k = cu(lq), cu(lk)
+    q = randn(g, sum(lq) + 2, hq, d, dtype=dt)
+    k, v = randn(g, sum(lk), hk, d, dtype=dt), randn(g, sum(lk), hk, d, dtype=dt)
+    need = ops.window_attention_workspace_bytes(q.shape[0], k.shape[0], len(lq), hq, hk, d, window, sinks)
+    assert need > 0
+    ws = torch.full((need + 64,), 0xFF, dtype=torch.uint8, device="cuda")   # NaN everywhere it is not written
+    out = torch.full_like(q, 7.5)
+    before = out.clone()
+    ops.window_attention(q, k, v, cu_q.cuda(), d**-0.5, window=window, sinks=sinks, cu_seqlens_k=cu_k.cuda(), out=out, workspace=ws[:need])
+    check_window(out, q, k, v, cu_q, cu_k, d**-0.5, window, sinks, 0, before)
+    assert (ws[need:] == 0xFF).all()
+    v[-1, 0] = math.nan  # seen by the last query of the last sequence alone
+    again = ops.window_attention(q, k, v, cu_q.cuda(), d**-0.5, window=window, sinks=sinks, cu_seqlens_k=cu_k.cuda(), out=before.clone())
+    last = sum(lq) - 1
+    assert torch.isnan(again[last, : hq // hk]).all()
+    # Its tile's other rows are computed again key by key: not the same bits, the same bounds.
+    again[last], v[-1, 0] = out[last], 0
+    whole, clean = serving.window_attention(q, k, v, cu_q.tolist(), cu_k.tolist(), d**-0.5, window, sinks)
+    whole[last] = False
+    close(again[whole], clean.value[whole], attention_slack(clean, d, max(lk), U[dt], fp16_p=dt == torch.float16)[whole])
+
+
 def test_window_attention_split_masked_specials():
     """What a query does not see stays out of its result when its keys are split, and what it sees comes in."""
     g = gen(32)
