@@ -827,15 +827,15 @@ __global__ void __launch_bounds__(256) window_join_kernel(const Args a, int tq_t
     }
 }
 
-// CTAs that share a row tile's keys.  A tile of 128 keys takes a CTA about 1.5 us, a CTA's start and end
-// about three of them, and a row's state leaves and comes back through L2: the number of splits with the
-// least sum of waves x (tiles + 3) and the join.  The lengths are on the GPU, so CTAs and tiles are those of
-// sequences of equal length.  bf16, 32 query heads on 8 key heads of 128, no window: 1 token x 32768 keys
-// 371 us unsplit, 37 us at the 16 chosen; 64 x 8192 104 and 27 (16); 4 x 16 x 4096 54 and 26 (4); 512 x 32768
-// 389 and 222 (2); 2048 x 16384 406 unsplit as chosen, 474 in two.
-// Where the pairs of row tiles are more than a round of CTAs, those of the whole rounds keep their keys and
-// only the last, partial round's are split: 1536 tokens in 3 prompts behind 8200, 28 heads on 4 (177 pairs),
-// 221 us unsplit, 197 all in 3, HYBRID.
+// CTAs that share the keys of a pair of row tiles.  A tile of 128 keys takes a CTA about 1.4 us, a CTA's start
+// and end about three of them, and a row's state leaves and comes back through L2: the least estimate of
+// that over the SMs.  The lengths are on the GPU, so pairs and tiles are those of sequences of equal length.
+// bf16, 32 query heads on 8 key heads of 128, no window: 1 token x 32768 keys 371 us unsplit, 37 us at the 16
+// chosen; 64 x 8192 104 and 27 (16); 4 x 16 x 4096 54 and 26 (4); 512 x 32768 389 and 222 (2).
+// Where the pairs are more than a round of CTAs, those of the whole rounds keep their keys and only the last,
+// partial round's are split: 1536 tokens in 3 prompts behind 8200, 28 heads on 4 (177 pairs) 221 us unsplit,
+// 196 with all in 3, 169 so; 1280 x 8192 (160 pairs) 190 and 137; not for 3000 tokens without a context, whose
+// pairs differ and fill the last round by themselves (47 us, 55 if split).
 struct Split {
     int64_t z, whole;
 };
@@ -843,19 +843,24 @@ Split split_of(int64_t Tq, int64_t Tk, int64_t seqs, int64_t Hq, int64_t Hk, int
     const int64_t group = Hq / Hk;
     Split pick = {1, 0};
     if ((D != 64 && D != 128) || group > 128 || Tk == 0 || seqs == 0) return pick;
-    const int64_t tt = 2 * (128 / group), tokens = (Tq + seqs - 1) / seqs, pairs = std::min(seqs, Tq) * ((tokens + tt - 1) / tt) * Hk;
-    int64_t keys = Tk / seqs;
-    if (window) keys = std::min(keys, window + tt + (sinks ? std::min<int64_t>(sinks, keys) : 0));
-    const int64_t tiles = (keys + 127) / 128, sms = sf::sm_count(), rounds = pairs / sms, rest = pairs % sms;
-    double best = (double)(rounds + (rest > 0)) * (tiles + 3);
+    const int64_t tt = 2 * (128 / group), tokens = (Tq + seqs - 1) / seqs;
+    const double pairs = (double)(std::min(seqs, Tq) * ((tokens + tt - 1) / tt) * Hk);
+    // Key tiles of a pair: of the first tokens, which see the fewest, and on average (keys from a to b, at most w each).
+    const double b = (double)Tk / seqs, a = std::max(1.0, b - tokens);
+    const double w = window ? std::min(b, (double)window + tt + std::min<double>((double)sinks, b)) : b;
+    const double few = std::min(a, w) / 128 + 0.5, mean = (b <= w || a >= w ? (std::min(a, w) + std::min(b, w)) / 2 : ((w * w - a * a) / 2 + w * (b - w)) / (b - a)) / 128 + 0.5;
+    const double sms = sf::sm_count(), rounds = std::floor(pairs / sms), rest = pairs - rounds * sms;
+    // n CTAs of `tiles` tiles on average, the heaviest first: their sum over the SMs, and what the last round leaves idle.
+    auto time = [&](double n, double tiles, double least) { return n * (tiles + 3) / sms + (std::ceil(n / sms) - n / sms) * (least + 3); };
+    double best = time(pairs, mean, few);
     for (int64_t z : {2, 3, 4, 6, 8, 12, 16, 24, 32}) {
-        if (tiles / z < 2) break;
-        const double part = (double)((tiles + z - 1) / z + 3), join = (double)Tq * Hq * D * 8 * z / 9e6;  // 9 MB of states in a tile's time
-        const double all = (double)((pairs * z + sms - 1) / sms) * part + 3 + join;
-        const double last = (double)rounds * (tiles + 3) + (double)((rest * z + sms - 1) / sms) * part + 3 + join * rest / pairs;
+        if (mean < 2 * z) break;
+        const double join = (double)Tq * Hq * D * 8 * z / 9e6;  // 9 MB of states in a tile's time
+        const double all = time(pairs * z, mean / z, few / z) + 3 + join;
+        const double last = rounds * (mean + 3) + time(rest * z, mean / z, few / z) + 5 + join * rest / pairs;
         if (all < best) best = all, pick = {z, 0};
         // The slots that rounding leaves over lie among the others.
-        if (rounds && rest && last < best) best = last, pick = {z, rounds * sms * (Tq / tt + seqs) * Hk / pairs};
+        if (rounds > 0 && rest > 0 && last < best) best = last, pick = {z, (int64_t)(rounds * sms * (Tq / tt + seqs) * Hk / pairs)};
     }
     return pick;
 }
