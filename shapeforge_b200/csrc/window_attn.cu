@@ -971,7 +971,7 @@ extern "C" int sf_window_attention(const sf_window_attention_args* x, void* stre
         const int64_t z = split.z;
         if (z > 1 && x->workspace && sf::aligned16(x->workspace) && x->workspace_bytes >= (uint64_t)(z * Tq * Hq * (D + 2) * 4)) {
             a.splits = (int)z;
-            a.whole = (int)split.whole;
+            a.whole = split.whole <= 0x7fffffff ? (int)split.whole : 0;
             a.part = (float*)x->workspace;
             a.stat = a.part + z * Tq * Hq * D;
         }
