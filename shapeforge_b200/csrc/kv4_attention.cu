@@ -14,9 +14,11 @@
 //   o       = sum_j (p_j s_jG) (c_j - 8) + p_j (m_jG + 8 s_jG)  scales go into p, which is small.
 //
 //  * K: an fp16 whose low bits are a code is the subnormal c 2^-24, exactly, so one AND makes two
-//    operands.  The block's q are scaled by one power of two to at most 2^11 (an fp16 holds them exactly
-//    down to 2^-25 of the largest) and by 16 where the code sits in the lower nibble of its byte.  The
-//    minima's part is one bf16 MMA of its own: minima are bf16, sum(q_G) goes in as three bf16 parts.
+//    operands.  Each head's q are scaled by a power of two of its own to at most 2^11 (an fp16 holds them
+//    exactly down to 2^-25 of the head's largest; a head is a column of S^T, so nothing of it reaches another)
+//    and by 16 where the code sits in the lower nibble of its byte.  The minima's part is one bf16 MMA of its
+//    own: minima are bf16, sum(q_G) goes in as three bf16 parts.  S is held in units of 1024, which the
+//    exponential's FMA takes out: so every finite q has a finite factor.
 //  * V: with two keys' bytes side by side, 0x6400 | b is the fp16 1024 + b of a whole byte b = c + 16 c'
 //    (two neighbouring elements' codes) and clearing its low bits gives 1024 + 16 c'.  Both, less 1160
 //    and 1152, go through the MMA, and (c - 8) and (c' - 8) of the accumulators come from their
@@ -64,6 +66,7 @@ constexpr int ITEM_COST = 24;  // what starting and merging a (request, head) co
 // requests of up to 2048 11.6 and 12.8, of 4096 (64 tiles a CTA) 16.7 and 14.9.
 constexpr int MAX_CLUSTER = 16, CLUSTER_LEAST = 8, CLUSTER_MOST = 32;
 constexpr float NO_MAX = -3e38f;  // the running max before any score
+constexpr float S_UNIT = 1024.f;  // of the scores between the products and the exponential
 // Smallest unit of a head's p s: p / unit stays finite for p up to 2^8.
 constexpr float UNIT_FLOOR = 0x1p-118f;
 constexpr float LOG2E = 1.4426950408889634f;
@@ -395,12 +398,11 @@ __global__ void __launch_bounds__(THREADS, ctas_of(NT)) kv4_attention_kernel(con
 
         // ---- q as the B operand ----
         uint32_t qf[NT][8 * NG], qlow[NT];
-        float fac;
+        float2 fac[NT];  // of the lane's columns, heads 2t and 2t + 1
         {
-            float amax = 0.f;
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt) {
-                float sum[NG];
+                float amax = 0.f, sum[NG];
 #pragma unroll
                 for (int G = 0; G < NG; ++G) {
                     const uint32_t w[8] = {raw[nt][G][0].x, raw[nt][G][0].y, raw[nt][G][0].z, raw[nt][G][0].w,
@@ -410,12 +412,14 @@ __global__ void __launch_bounds__(THREADS, ctas_of(NT)) kv4_attention_kernel(con
                     for (int i = 0; i < 8; ++i) {
                         const float2 f = sf::Pair<T>::to_f2(w[i]);
                         amax = fmaxf(amax, fmaxf(fabsf(f.x), fabsf(f.y)));
-                        two = sf::f2_add(two, f);
+                        two = sf::f2_fma(f, sf::f2(1.0f / S_UNIT), two);
                     }
                     sum[G] = two.x + two.y;
 #pragma unroll
                     for (int o = 1; o <= 2; o <<= 1) sum[G] += __shfl_xor_sync(0xffffffffu, sum[G], o);
                 }
+#pragma unroll
+                for (int o = 1; o <= 2; o <<= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
                 // Of sum(q_G), G = 0, 1, the lane's t-th bf16 part: t = 0, 1, 2 make up 24 bits.
                 float part[2] = {sum[0] * a.scale_log2, NG == 2 ? sum[NG - 1] * a.scale_log2 : 0.f};
                 qlow[nt] = 0;
@@ -427,14 +431,12 @@ __global__ void __launch_bounds__(THREADS, ctas_of(NT)) kv4_attention_kernel(con
                     part[0] -= back.x;
                     part[1] -= back.y;
                 }
-            }
-            amax = sf::warp_max(amax);
-            // amax 2^(137 - ex) in [2^10, 2^11): times 16 it is still an fp16.
-            const uint32_t ex = min(max(__float_as_uint(amax) >> 23, 10u), 244u);
-            const float up = __uint_as_float((264u - ex) << 23);
-            fac = __uint_as_float((ex + 10u) << 23) * a.scale_log2;  // 2^(ex - 137) 2^20
-#pragma unroll
-            for (int nt = 0; nt < NT; ++nt)
+                // amax 2^(137 - ex) in [2^10, 2^11): times 16 it is still an fp16.  The least exponent keeps 16 up
+                // finite; an infinity takes the largest and turns its own head into NaN.
+                const uint32_t ex = min(max(__float_as_uint(amax) >> 23, 14u), 254u);
+                const float up = __uint_as_float((264u - ex) << 23), up16 = up * 16.f;
+                const float mine = __uint_as_float(ex << 23) * a.scale_log2;  // 2^(ex - 137) 2^20 / S_UNIT, head g's
+                fac[nt] = make_float2(__shfl_sync(0xffffffffu, mine, 8 * t), __shfl_sync(0xffffffffu, mine, 8 * t + 4));
 #pragma unroll
                 for (int G = 0; G < NG; ++G)
 #pragma unroll
@@ -443,12 +445,12 @@ __global__ void __launch_bounds__(THREADS, ctas_of(NT)) kv4_attention_kernel(con
                         const float2 e01 = sf::Pair<T>::to_f2(r4.x), e23 = sf::Pair<T>::to_f2(r4.y), e45 = sf::Pair<T>::to_f2(r4.z),
                                      e67 = sf::Pair<T>::to_f2(r4.w);
                         uint32_t* f = &qf[nt][(2 * G + h2) * 4];
-                        const float up16 = up * 16.f;
                         f[0] = f16x2(e01.x * up16, e45.x * up16);
                         f[1] = f16x2(e01.y * up, e45.y * up);
                         f[2] = f16x2(e23.x * up16, e67.x * up16);
                         f[3] = f16x2(e23.y * up, e67.y * up);
                     }
+            }
         }
 
         // O^T, heads 2t, 2t + 1, elements 64 G + 8 g + 4 i + 0..3 for i < 2: [4 G + i] whole bytes (rows g
@@ -520,6 +522,7 @@ __global__ void __launch_bounds__(THREADS, ctas_of(NT)) kv4_attention_kernel(con
                     }
                 }
                 // S^T = K q^T: the minima's part, then a group at a time.
+                float2 codes[NT][2];
 #pragma unroll
                 for (int nt = 0; nt < NT; ++nt)
                     mma_bf16_k8_first(s[u][nt], NG == 2 ? __byte_perm(kp[0][0], kp[0][NG - 1], 0x7632) : kp[0][0] >> 16,
@@ -542,14 +545,22 @@ __global__ void __launch_bounds__(THREADS, ctas_of(NT)) kv4_attention_kernel(con
                     }
 #pragma unroll
                     for (int r = 0; r < 2; ++r) {
-                        const float kf = __uint_as_float(kp[r][G] << 16) * fac;
+                        const float2 ks = sf::f2(__uint_as_float(kp[r][G] << 16));
 #pragma unroll
                         for (int nt = 0; nt < NT; ++nt) {
-                            s[u][nt][2 * r] = fmaf(acc[nt][2 * r], kf, s[u][nt][2 * r]);
-                            s[u][nt][2 * r + 1] = fmaf(acc[nt][2 * r + 1], kf, s[u][nt][2 * r + 1]);
+                            const float2 x = make_float2(acc[nt][2 * r], acc[nt][2 * r + 1]);
+                            codes[nt][r] = G == 0 ? sf::f2_mul(x, ks) : sf::f2_fma(x, ks, codes[nt][r]);
                         }
                     }
                 }
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                    for (int r = 0; r < 2; ++r) {
+                        const float2 x = sf::f2_fma(codes[nt][r], fac[nt], make_float2(s[u][nt][2 * r], s[u][nt][2 * r + 1]));
+                        s[u][nt][2 * r] = x.x;
+                        s[u][nt][2 * r + 1] = x.y;
+                    }
                 const int at_tile = warp + WARPS * (TS * k + u);
                 if (at_tile == edge0 || at_tile == edge1 || at_tile == edge2 || (none >> u & 1u)) {
                     const int j = seen.tile(now.i0 + at_tile) * 16 + row;
@@ -572,7 +583,7 @@ __global__ void __launch_bounds__(THREADS, ctas_of(NT)) kv4_attention_kernel(con
                 for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
                     for (int r = 0; r < 2; ++r)
-                        over = fmaxf(over, fmaxf(s[u][nt][2 * r] + nm[nt].x, s[u][nt][2 * r + 1] + nm[nt].y));
+                        over = fmaxf(over, fmaxf(fmaf(s[u][nt][2 * r], S_UNIT, nm[nt].x), fmaf(s[u][nt][2 * r + 1], S_UNIT, nm[nt].y)));
             if (__any_sync(0xffffffffu, over > 8.f)) {
 #pragma unroll
                 for (int nt = 0; nt < NT; ++nt) {
@@ -580,7 +591,7 @@ __global__ void __launch_bounds__(THREADS, ctas_of(NT)) kv4_attention_kernel(con
                     if constexpr (TS == 2)
                         mx = make_float2(fmaxf(mx.x, fmaxf(s[TS - 1][nt][0], s[TS - 1][nt][2])), fmaxf(mx.y, fmaxf(s[TS - 1][nt][1], s[TS - 1][nt][3])));
                     mx = over_keys(mx);
-                    mx = make_float2(fmaxf(mx.x, -nm[nt].x), fmaxf(mx.y, -nm[nt].y));
+                    mx = make_float2(fmaxf(mx.x * S_UNIT, -nm[nt].x), fmaxf(mx.y * S_UNIT, -nm[nt].y));
                     const float2 f = make_float2(exp2f(-nm[nt].x - mx.x), exp2f(-nm[nt].y - mx.y));
                     nm[nt] = make_float2(-mx.x, -mx.y);
                     l[nt] = sf::f2_mul(l[nt], f);
@@ -607,7 +618,7 @@ __global__ void __launch_bounds__(THREADS, ctas_of(NT)) kv4_attention_kernel(con
                     const float top = NG == 2 ? fmaxf(vs[0], vs[NG - 1]) : vs[0];
 #pragma unroll
                     for (int nt = 0; nt < NT; ++nt) {
-                        float2 p = sf::f2_add(make_float2(s[u][nt][2 * r], s[u][nt][2 * r + 1]), nm[nt]);
+                        float2 p = sf::f2_fma(make_float2(s[u][nt][2 * r], s[u][nt][2 * r + 1]), sf::f2(S_UNIT), nm[nt]);
                         p = make_float2(sf::ex2_ftz(p.x), sf::ex2_ftz(p.y));
                         l[nt] = sf::f2_add(l[nt], p);
 #pragma unroll

@@ -1,0 +1,101 @@
+"""The serving operators on the B200 at the edges of what a call may hold: heads whose queries differ by
+orders of magnitude, infinite and zero queries (64-bit definitions: oracle/serving.py; tolerances: see
+tests/test_serving_ops_gpu.py, whose helpers are used)."""
+
+from __future__ import annotations
+
+import math
+
+import pytest
+import torch
+
+from oracle import serving
+from shapeforge_b200 import ops
+from tests.test_serving_ops_gpu import TD, _status, check_decode, filled_cache, gen, i32, randn  # noqa: F401
+
+pytestmark = pytest.mark.gpu
+
+
+# ---- every query head of kv4_attention stands alone ------------------------------------------------
+
+
+HEADS = [(8, 2, 64), (16, 2, 128), (12, 1, 128), (40, 1, 64)]  # 4 and 8 heads a block of 8, 12 and 40 in blocks of 16
+
+
+def decode_case(g, hq, h, d, dt, n=500, page=32):
+    width = -(-n // page)
+    cache, kq, vq = filled_cache(g, width + 1, page, h, d, dt)
+    table = torch.randperm(width + 1, device="cuda", generator=g)[:width].view(1, width).to(torch.int32)
+    return cache, kq, vq, table, randn(g, 1, hq, d, dtype=dt)
+
+
+@pytest.mark.parametrize("variant", [0, 1, 3])
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+@pytest.mark.parametrize("shape", HEADS, ids=["x".join(map(str, s)) for s in HEADS])
+def test_an_infinite_query_spoils_its_own_head_alone(shape, dtype, variant):
+    hq, h, d = shape
+    cache, kq, vq, table, q = decode_case(gen(60), hq, h, d, TD[dtype])
+    want = ops.kv4_attention(q, cache, table, i32([500]), d**-0.5, variant=variant)
+    check_decode(want, q, kq, vq, 32, table, [500], d**-0.5, 0, 0)
+    for value in (math.inf, -math.inf, math.nan):
+        bad = q.clone()
+        bad[0, 1, 5] = bad[0, hq - 1, d - 1] = value
+        out = ops.kv4_attention(bad, cache, table, i32([500]), d**-0.5, variant=variant)
+        assert torch.isnan(out[0, 1]).all() and torch.isnan(out[0, hq - 1]).all()
+        out[0, [1, hq - 1]] = want[0, [1, hq - 1]]
+        check_decode(out, q, kq, vq, 32, table, [500], d**-0.5, 0, 0)
+
+
+@pytest.mark.parametrize("dtype, small", [("bf16", 2.0**-30), ("bf16", 2.0**-70), ("fp16", 2.0**-14)])
+@pytest.mark.parametrize("shape", HEADS, ids=["x".join(map(str, s)) for s in HEADS])
+def test_heads_of_very_different_size_keep_their_precision(shape, dtype, small):
+    """Head 0 a multiple of the others (2^30, 2^70, or what fp16 has room for): each within its own bound."""
+    hq, h, d = shape
+    cache, kq, vq, table, q = decode_case(gen(61), hq, h, d, TD[dtype])
+    scale = 1.0 / (math.sqrt(d) * small)
+    lone = q * small
+    want = ops.kv4_attention(lone, cache, table, i32([500]), scale)
+    check_decode(want, lone, kq, vq, 32, table, [500], scale, 0, 0)
+    both = lone.clone()
+    both[0, 0] = q[0, 0] * 4
+    out = ops.kv4_attention(both, cache, table, i32([500]), scale)
+    first = out[0, 0].clone()
+    out[0, 0] = want[0, 0]
+    check_decode(out, lone, kq, vq, 32, table, [500], scale, 0, 0)
+    # One key has nearly all of head 0's weight, where it leads by more than a score's error (four times its
+    # D products' in fp32) and 2^30 in weight.
+    kv, vv = serving.kv4_values(*kq), serving.kv4_values(*vq)
+    at = torch.arange(500, device="cuda")
+    rows = table[0].long()[at // 32] * 32 + at % 32
+    scores = both[0, 0].double() @ kv[rows, 0].T * scale
+    error = 4 * (d + 16) * 2.0**-23 * (both[0, 0].double().abs() @ kv[rows, 0].abs().T * scale).max()
+    top = scores.topk(2)
+    if top.values[0] - top.values[1] > 2 * error + 21:
+        best = vv[rows[top.indices[0]], 0]
+        # Half a step of the type and of the weight, at most 2^-8 of the value each.
+        assert (first.double() - best).abs().max() <= 2.0**-7 * best.abs().max()
+
+
+@pytest.mark.parametrize("shape", HEADS, ids=["x".join(map(str, s)) for s in HEADS])
+def test_zero_tiny_and_huge_queries(shape):
+    """Queries of zero (a padded request) weigh all keys alike; bf16 queries at both ends of the type's range, with a
+    scale that brings the scores back (or keys that do), are as precise as any."""
+    hq, h, d = shape
+    g = gen(62)
+    cache, kq, vq, table, q = decode_case(g, hq, h, d, torch.bfloat16)
+    zero = torch.zeros_like(q)
+    out = ops.kv4_attention(zero, cache, table, i32([500]), 0.1)
+    assert torch.isfinite(out).all()
+    check_decode(out, zero, kq, vq, 32, table, [500], 0.1, 0, 0)
+    for power in (-110, -60, 60, 110, 120):
+        x = (q.float() * 2.0**power).bfloat16()
+        out = ops.kv4_attention(x, cache, table, i32([500]), d**-0.5 * 2.0**-power)
+        check_decode(out, x, kq, vq, 32, table, [500], d**-0.5 * 2.0**-power, 0, 0)
+    # Small keys against large queries at an ordinary scale.
+    small = ops.kv4_cache(cache.shape[0], 32, h, d)
+    n = cache.shape[0] * 32
+    k, v = (randn(g, n, h, d) * 2.0**-119).bfloat16(), randn(g, n, h, d, dtype=torch.bfloat16)
+    ops.kv4_store(k, v, torch.arange(n, device="cuda", dtype=torch.int32), small)
+    x = (q.float() * 2.0**119).bfloat16()
+    out = ops.kv4_attention(x, small, table, i32([500]), d**-0.5)
+    check_decode(out, x, serving.kv4_quantise(k), serving.kv4_quantise(v), 32, table, [500], d**-0.5, 0, 0)
