@@ -881,7 +881,7 @@ __global__ void __launch_bounds__(32 * JOIN_HEADS * JOIN) kv4_join_kernel(const 
 // Most tiles a request can see, from the table's width, window and sinks alone.
 int64_t most_tiles(int64_t width, int64_t tpp, int64_t window, int64_t sinks) {
     const int64_t all = width * tpp;
-    if (!window) return all;
+    if (!window || window >= 16 * all || sinks >= 16 * all) return all;
     return std::min(all, (window + 15) / 16 + 1 + (sinks + 15) / 16);
 }
 

@@ -41,7 +41,7 @@ struct Keys {
     int sinks, low, high;
     __device__ __forceinline__ Keys(const Args& a, int p) {
         high = max(0, p + 1);
-        low = a.window ? max(0, p - a.window + 1) : 0;
+        low = a.window ? max(0, max(0, p) - a.window + 1) : 0;  // a position far below 0 less a large window wraps
         sinks = min(a.sinks, low);
     }
 };
@@ -187,7 +187,7 @@ struct Span {
         last = tokens > 0 ? first_ + tokens - 1 : -1;
         end = min(w.high, last + 1);
         front = a.window ? last - a.window + 1 : 0;
-        skip = a.window && last >= 0 && w.low + 128 <= first - a.window + 1 && w.low >= a.sinks ? 1 : 0;
+        skip = a.window && last >= 0 && w.low + 128 <= max(0, first) - a.window + 1 && w.low >= a.sinks ? 1 : 0;
     }
     // Keys [0, count) of tile j can be seen.
     __device__ __forceinline__ int count(const Walk& w, int j) const { return max(0, min(128, (w.in_sinks(j) ? w.sink_end : end) - w.start(j))); }
@@ -406,7 +406,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
     const int pos0 = uniform(at.pos0);
     Walk w;
     w.high = max(0, pos0 + uniform(rows_tok[0] + rows_tok[1]));
-    w.low = uniform(a.window ? max(0, pos0 - a.window + 1) : 0);
+    w.low = uniform(a.window ? max(0, max(0, pos0) - a.window + 1) : 0);
     w.sink_end = min(a.sinks, w.low);
     w.sink_tiles = (w.sink_end + 127) >> 7;
     w.n = w.high > 0 ? w.sink_tiles + ((w.high - w.low + 127) >> 7) : 0;
@@ -934,7 +934,7 @@ int launch_general(const Args& a, int64_t D, cudaStream_t st, char* err, uint64_
 extern "C" uint64_t sf_window_attention_workspace_bytes(int64_t Tq, int64_t Tk, int64_t seqs, int64_t Hq, int64_t Hk, int64_t D, int64_t window,
                                                         int64_t sinks) {
     if (Tq <= 0 || Tk <= 0 || seqs <= 0 || Hq <= 0 || Hk <= 0 || Hq % Hk || window < 0 || sinks < 0) return 0;
-    const int64_t z = split_of(Tq, Tk, seqs, Hq, Hk, D, window, sinks).z;
+    const int64_t z = split_of(Tq, Tk, seqs, Hq, Hk, D, window < Tk ? window : 0, sinks).z;
     return z > 1 ? (uint64_t)(z * Tq * Hq * (D + 2) * 4) : 0;
 }
 
@@ -962,12 +962,14 @@ extern "C" int sf_window_attention(const sf_window_attention_args* x, void* stre
     a.vt = x->v_rows.token, a.vh = x->v_rows.head, a.ot = x->o_rows.token, a.oh = x->o_rows.head;
     a.tq = Tq, a.tk = Tk;
     a.seqs = (int)seqs, a.group = (int)(Hq / Hk), a.heads = (int)Hq;
-    a.window = (int)std::min<int64_t>(x->window, 0x7fffffff);
-    a.sinks = x->window ? (int)std::min<int64_t>(x->sinks, 0x7fffffff) : 0;
+    // Positions are below Tk, so a window of Tk keys leaves none out: below, position - window stays within 32 bits.
+    const int64_t window = x->window < Tk ? x->window : 0;
+    a.window = (int)window;
+    a.sinks = window ? (int)std::min<int64_t>(x->sinks, 0x7fffffff) : 0;
     a.scale_log2 = scale * LOG2E;
     a.splits = 1;
     if (x->variant != 4) {
-        const Split split = split_of(Tq, Tk, seqs, Hq, Hk, D, x->window, x->sinks);
+        const Split split = split_of(Tq, Tk, seqs, Hq, Hk, D, window, x->sinks);
         const int64_t z = split.z;
         if (z > 1 && x->workspace && sf::aligned16(x->workspace) && x->workspace_bytes >= (uint64_t)(z * Tq * Hq * (D + 2) * 4)) {
             a.splits = (int)z;

@@ -11,7 +11,7 @@ import torch
 
 from oracle import serving
 from shapeforge_b200 import ops
-from tests.test_serving_ops_gpu import TD, _status, check_decode, filled_cache, gen, i32, randn  # noqa: F401
+from tests.test_serving_ops_gpu import TD, _status, check_decode, check_window, cu, filled_cache, gen, i32, randn  # noqa: F401
 
 pytestmark = pytest.mark.gpu
 
@@ -99,3 +99,30 @@ def test_zero_tiny_and_huge_queries(shape):
     x = (q.float() * 2.0**119).bfloat16()
     out = ops.kv4_attention(x, small, table, i32([500]), d**-0.5)
     check_decode(out, x, serving.kv4_quantise(k), serving.kv4_quantise(v), 32, table, [500], d**-0.5, 0, 0)
+
+
+# ---- windows that leave nothing out ----------------------------------------------------------------
+
+
+@pytest.mark.parametrize("variant", [0, 2])
+@pytest.mark.parametrize("window", [200, 2**31 - 2, 2**31 - 1, 2**31, 2**63 - 1])
+@pytest.mark.parametrize("sinks", [0, 4, 2**31 - 1, 2**63 - 1])
+def test_windows_past_every_key_are_no_window(window, sinks, variant):
+    """A window that says "unlimited", with queries in front of the first key: the same bits as no window."""
+    g = gen(63)
+    lq, lk = [70, 40, 5], [40, 49, 0]
+    cu_q, cu_k = cu(lq), cu(lk)
+    q, k, v = randn(g, 115, 4, 64, dtype=torch.bfloat16), randn(g, 89, 2, 64, dtype=torch.bfloat16), randn(g, 89, 2, 64, dtype=torch.bfloat16)
+    run = lambda **kw: ops.window_attention(q, k, v, cu_q.cuda(), 0.125, cu_seqlens_k=cu_k.cuda(), variant=variant, **kw)
+    out = run(window=window, sinks=sinks)
+    check_window(out, q, k, v, cu_q, cu_k, 0.125, 0, 0, variant)
+    assert not out[:30].any() and not out[110:].any() and torch.equal(out, run())
+
+
+@pytest.mark.parametrize("window", [2**31 - 1, 2**63 - 1])
+def test_decoding_with_a_window_past_every_key(window):
+    cache, kq, vq, table, q = decode_case(gen(64), 8, 2, 64, torch.bfloat16)
+    for sinks in (0, 2**63 - 1):
+        for variant in (0, 1, 3):
+            out = ops.kv4_attention(q, cache, table, i32([500]), 0.125, window=window, sinks=sinks, variant=variant)
+            check_decode(out, q, kq, vq, 32, table, [500], 0.125, 0, 0)
