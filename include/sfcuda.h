@@ -330,7 +330,8 @@ SF_API int sf_kv4_attention(const sf_kv4_attention_args* args, void* stream, cha
  * Sequence s has queries cu_q[s]..cu_q[s+1] and keys cu_k[s]..cu_k[s+1] (both [seqs + 1], not decreasing);
  * its query i sits at position p = i + nk - nq and sees keys j <= p with j > p - window or j < sinks
  * (window 0: all j <= p).  A query that sees nothing gives zeros; rows of no sequence are left as they
- * were.  D <= 256; tcgen05 kernel for D in {64, 128}, 16-byte aligned tensors, strides that are
+ * were.  Scores, softmax sums and accumulation in fp32; a weight enters its product as a 16-bit value and its 16-bit
+ * residual (some 16 bits in bf16, 22 in fp16).  D <= 256; tcgen05 kernel for D in {64, 128}, 16-byte aligned tensors, strides that are
  * multiples of 8 elements and at most 128 query heads a key head (variant 1 forces it), general kernel
  * otherwise (variant 2).  With a workspace (16-byte aligned, sf_window_attention_workspace_bytes bytes, no
  * initial content; two calls that overlap on the GPU need one each) few queries with many keys are split

@@ -5,7 +5,7 @@
 //   keys j <= p with j > p - window or j < sinks (window 0: all j <= p)
 //
 // q, o [Tq, Hq, D] and k, v [Tk, Hk, D] with any token and head strides, g = Hq / Hk, sequences packed
-// by cu_seqlens; fp16 / bf16, softmax statistics in fp32.  A query that sees nothing gives zeros; rows
+// by cu_seqlens; fp16 / bf16, softmax statistics in fp32, weights in some 16 (bf16) or 22 (fp16) bits.  A query that sees nothing gives zeros; rows
 // of no sequence are left as they were.
 #include "sf_common.cuh"
 #include "sm100.cuh"
@@ -119,7 +119,7 @@ __global__ void __launch_bounds__(128) window_general_kernel(const Args a, int D
 //   warp 1        MMA issuer, in the order P0.V(j-1), S0(j), P1.V(j-1), S1(j): one tile's products run
 //                 under the other's softmax; S (then P over it) and O of both tiles fill TMEM.  (An
 //                 issuer a tile let both tiles wait, then compute, at the same time: 498 against 402 us
-//                 at 16384 tokens, window 4096, 16 heads on 2.)  Its operands are kept uniform over the
+//                 at 16384 tokens, window 4096, 16 heads on 2, without P's residual.)  Its operands are kept uniform over the
 //                 warp: issued from one divergent lane a product cost ~130 cycles against the pipe's 64;
 //   warp 2        zeroes the value rows behind a sequence's last key (0 times another sequence's NaN or
 //                 infinity would be NaN) and hands the tile on;
@@ -128,13 +128,14 @@ __global__ void __launch_bounds__(128) window_general_kernel(const Args a, int D
 // needs no alignment), and the sinks in front of it are a tile of their own; a tile of n keys costs
 // n rounded up to 16 in both products and 32 in the softmax.  Tiles that every row sees in full skip the
 // mask.  Running max and sum in fp32; the max follows a score only past 2^8, so O is rarely rescaled.
-// 16384 tokens, 16 heads on 2 of 128, window 4096, bf16: 381 us, 1264 TFLOP/s of seen scores (77 % of what a large
-// library product reaches; 65 % in loops of seconds under the power cap): a step of 128 keys for 256 rows takes
-// 1.40 us, its products 1.04 at the pipe's rate, and a CTA's start and end three steps.  1203 tokens in 9 prompts,
-// window 128: 21 us, two CTAs in turn on an SM, latency.  (CTAs that take their next piece from the hardware's
-// scheduler hide the start and end, but the registers that costs the softmax slowed every step: 411 us.)
-// P is rounded to the tensors' type (as the fp32 sum of the unrounded weights divides it, a weight is off
-// by half a step, which averages out over the keys).
+// P goes into its product twice, as a 16-bit high part and the 16-bit residual, over the columns that its scores
+// leave, as in this library's other attention: rounded once to bf16, it moved results by half a step of the type
+// (and took 381 us where the two take 522).
+// 16384 tokens, 16 heads on 2 of 128, window 4096, bf16: 522 us, 922 TFLOP/s of seen scores (56 % of what a large
+// library product reaches; 84 % with P . V counted twice): a step of 128 keys for 256 rows takes 1.9 us, its products
+// 1.56 at the pipe's rate.  P's first hand-over at 32, 64 or 96 keys: 527, 523, 522.  1203 tokens in 9 prompts, window
+// 128: 22 us, two CTAs in turn on an SM, latency.  (Without the residual, CTAs that take their next piece from the
+// hardware's scheduler hid the start and end, but the registers that cost the softmax slowed every step: 411 us.)
 // A row that comes out NaN (or infinite) is computed again key by key: masked keys in its tiles may hold
 // infinities or NaN that their zero weights do not silence.
 
@@ -269,16 +270,18 @@ __device__ __forceinline__ void issue_qk(uint32_t d, uint64_t a, uint64_t b, uin
                      : "memory");
     }
 }
-// O += P . V over 32 keys (P of 32 keys lies in 16 columns of every 32, 16 keys of V are 128 on) or over 16.
+// O += P . V over 32 keys or over 16.  P of 32 keys lies in 32 columns: the high parts in the first 16, the
+// residuals behind them; 16 keys of V are 128 on.
 #define SF_PV_STEP(col, off, acc) "add.u32 y, %1, " col ";\n" SF_DESC("db", "%2", "%3", off) "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [y], db, %4, " acc ";\n"
 __device__ __forceinline__ void issue_pv32(uint32_t d, uint32_t p, uint64_t v, uint32_t idesc, uint32_t accumulate, uint32_t lead) {
     asm volatile("{\n.reg .pred p, f, q;\n.reg .b32 x, y;\n.reg .b64 db;\nsetp.ne.b32 q, %6, 0;\nsetp.eq.b32 p, %6, %6;\nsetp.ne.b32 f, %5, 0;\n" SF_PV_STEP(
-                     "0", "0", "f") SF_PV_STEP("8", "128", "p") "}\n" ::"r"(d),
+                     "0", "0", "f") SF_PV_STEP("8", "128", "p") SF_PV_STEP("16", "0", "p") SF_PV_STEP("24", "128", "p") "}\n" ::"r"(d),
                  "r"(p), "r"((uint32_t)v), "r"((uint32_t)(v >> 32)), "r"(idesc), "r"(accumulate), "r"(lead)
                  : "memory");
 }
 __device__ __forceinline__ void issue_pv16(uint32_t d, uint32_t p, uint64_t v, uint32_t idesc, uint32_t accumulate, uint32_t lead) {
-    asm volatile("{\n.reg .pred f, q;\n.reg .b32 x, y;\n.reg .b64 db;\nsetp.ne.b32 q, %6, 0;\nsetp.ne.b32 f, %5, 0;\n" SF_PV_STEP("0", "0", "f") "}\n" ::"r"(d),
+    asm volatile("{\n.reg .pred p, f, q;\n.reg .b32 x, y;\n.reg .b64 db;\nsetp.ne.b32 q, %6, 0;\nsetp.eq.b32 p, %6, %6;\nsetp.ne.b32 f, %5, 0;\n" SF_PV_STEP(
+                     "0", "0", "f") SF_PV_STEP("16", "0", "p") "}\n" ::"r"(d),
                  "r"(p), "r"((uint32_t)v), "r"((uint32_t)(v >> 32)), "r"(idesc), "r"(accumulate), "r"(lead)
                  : "memory");
 }
@@ -303,10 +306,14 @@ __device__ __forceinline__ bool wait_soon(uint64_t* bar, uint32_t parity, sm100:
 }
 
 // Running state of a row: `m` the max that weights are relative to (log2 units), `l` their sum.
+// An fp16 weight is held times 2^7: at most 2^15, and 2^-32 of the running max is still a half step of its
+// smallest residual; `l` and O carry the same factor, which the division takes out.
+template <typename T>
+constexpr float LIFT = std::is_same<T, __half>::value ? 7.f : 0.f;
 struct RowState {
     float m, l;
     // Take in a tile's row max; O (in TMEM) is rescaled when the max has grown by more than 2^8.
-    template <int D>
+    template <typename T, int D>
     __device__ __forceinline__ float raise(float rmax, float scale_log2, uint32_t tmem_o, bool some) {
         const float m_new = max3_nan(m, rmax * scale_log2, m);
         const bool need = !(m_new <= m + 8.0f);
@@ -326,20 +333,31 @@ struct RowState {
             }
         }
         if (need) m = m_new;
-        return m == -INFINITY ? 0.f : m;
+        return m == -INFINITY ? 0.f : m - LIFT<T>;
     }
 };
 
-// 32 scores to weights (16 packed words), adding them up.
+// 32 scores to weights, adding them up: 16 words of high parts, then 16 of what they leave out, so that P . V is a
+// product with P to some 16 (bf16) or 22 (fp16) bits.  A bf16 high part is the upper half of the fp32 word
+// (one byte permute for two weights); the residual is exact before its own rounding.
 template <typename T>
-__device__ __forceinline__ void weights32(const uint32_t* r, float scale_log2, float m, float2 (&acc)[2], uint32_t (&w)[16]) {
-    const float2 sc = sf::f2(scale_log2), nm = sf::f2(-m);
+__device__ __forceinline__ void weights32(const uint32_t* r, float scale_log2, float m, float2 (&acc)[2], uint32_t (&w)[32]) {
+    const float2 sc = sf::f2(scale_log2), nm = sf::f2(-m), minus = sf::f2(-1.f);
 #pragma unroll
     for (int i = 0; i < 16; ++i) {
         const float2 x = sf::f2_fma(make_float2(__uint_as_float(r[2 * i]), __uint_as_float(r[2 * i + 1])), sc, nm);
         const float2 p = make_float2(sf::ex2_ftz(x.x), sf::ex2_ftz(x.y));
         acc[i & 1] = sf::f2_add(acc[i & 1], p);
-        w[i] = sf::Pair<T>::from_f2(p);
+        float2 high;
+        if constexpr (std::is_same<T, __nv_bfloat16>::value) {
+            const uint32_t a = __float_as_uint(p.x), b = __float_as_uint(p.y);
+            w[i] = __byte_perm(a, b, 0x7632);
+            high = make_float2(__uint_as_float(a & 0xFFFF0000u), __uint_as_float(b & 0xFFFF0000u));
+        } else {
+            w[i] = sf::Pair<T>::from_f2(p);
+            high = sf::Pair<T>::to_f2(w[i]);
+        }
+        w[16 + i] = sf::Pair<T>::from_f2(sf::f2_fma(high, minus, p));
     }
 }
 
@@ -614,12 +632,12 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
                 float mx = -INFINITY;
 #pragma unroll
                 for (int c = 0; c < 4; ++c) mx = max32(r + 32 * c, mx);
-                const float m = s.raise<D>(mx, a.scale_log2, to, turn > 0);
+                const float m = s.raise<T, D>(mx, a.scale_log2, to, turn > 0);
 #pragma unroll
                 for (int c = 0; c < 4; ++c) {
-                    uint32_t pw[16];
+                    uint32_t pw[32];
                     weights32<T>(r + 32 * c, a.scale_log2, m, acc, pw);
-                    sm100::tmem_st_32x32b_x16(ts + 32u * c, pw);
+                    sm100::tmem_st_32x32b_x32(ts + 32u * c, pw);
                     if (c == FIRST_KEYS / 32 - 1 || c == 3) {
                         sm100::tmem_st_wait();
                         sm100::tc_fence_before();
@@ -649,13 +667,13 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
                         if (!(seen >> i & 1u)) r[32 * c + i] = 0xff800000u;
                     mx = max32(r + 32 * c, mx);
                 }
-                const float m = s.raise<D>(mx, a.scale_log2, to, turn > 0);
+                const float m = s.raise<T, D>(mx, a.scale_log2, to, turn > 0);
 #pragma unroll
                 for (int c = 0; c < 4; ++c) {
                     if (c >= chunks) continue;
-                    uint32_t pw[16];
+                    uint32_t pw[32];
                     weights32<T>(r + 32 * c, a.scale_log2, m, acc, pw);
-                    sm100::tmem_st_32x32b_x16(ts + 32u * c, pw);
+                    sm100::tmem_st_32x32b_x32(ts + 32u * c, pw);
                 }
                 sm100::tmem_st_wait();
                 sm100::tc_fence_before();

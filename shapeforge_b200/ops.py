@@ -730,8 +730,8 @@ def window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqle
     rows).  Query ``i`` of a sequence with nq queries and nk keys sits at ``p = i + nk - nq`` and sees the
     keys ``j <= p`` with ``j > p - window`` or ``j < sinks`` (``window`` 0: all ``j <= p``), so a prompt's next
     chunk comes with its whole context as keys.  A query that sees nothing gives zeros; rows of ``out``
-    that belong to no sequence are left as they were.  ``out`` must not overlap the inputs.  D up to 256; D 64 and 128 with 16-byte aligned
-    rows and at most 128 query heads a key head run on the tensor cores, where few queries with many keys
+    that belong to no sequence are left as they were.  ``out`` must not overlap the inputs.  Softmax in fp32, its
+    weights to some 16 (bf16) or 22 (fp16) bits in their product.  D up to 256; D 64 and 128 with 16-byte aligned rows and at most 128 query heads a key head run on the tensor cores, where few queries with many keys
     are split over the keys by way of ``workspace`` (uint8, :func:`window_attention_workspace_bytes`,
     allocated here when not given; calls that overlap on the GPU need one each).  ``variant``: 0 = by
     shape, 1 = tensor cores (refused where they do not apply), 2 = general kernel, 4 = unsplit."""

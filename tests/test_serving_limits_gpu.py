@@ -11,7 +11,8 @@ import torch
 
 from oracle import serving
 from shapeforge_b200 import ops
-from tests.test_serving_ops_gpu import TD, _status, check_decode, check_window, cu, filled_cache, gen, i32, randn  # noqa: F401
+from tests.test_serving_ops_gpu import (  # noqa: F401
+    LAST_ROUND, SPLIT, TD, WINDOW, _status, attention_slack, check_decode, check_window, close, cu, filled_cache, gen, i32, randn)
 
 pytestmark = pytest.mark.gpu
 
@@ -126,3 +127,47 @@ def test_decoding_with_a_window_past_every_key(window):
         for variant in (0, 1, 3):
             out = ops.kv4_attention(q, cache, table, i32([500]), 0.125, window=window, sinks=sinks, variant=variant)
             check_decode(out, q, kq, vq, 32, table, [500], 0.125, 0, 0)
+
+
+# ---- the weights' precision ------------------------------------------------------------------------
+
+
+def check_precise(out, q, k, v, cu_q, cu_k, scale, window, sinks):
+    """As check_window, with the weights held in two 16-bit parts: a bf16 high part leaves less than 2^-7 of the weight,
+    whose own half step is 2^-8 of that; fp16 2^-11 and 2^-11, and 2^-25 of 2^-7 of the largest at the least."""
+    inside, r = serving.window_attention(q, k, v, cu_q.tolist(), cu_k.tolist(), scale, window, sinks)
+    half = q.dtype == torch.float16
+    n = int((cu_k[1:] - cu_k[:-1]).max())
+    slack = attention_slack(r, q.shape[2], n, 2.0**-22 if half else 2.0**-15) + (n * 2.0**-32 * r.peak if half else 0)
+    close(out[inside], r.value[inside], slack[inside])
+
+
+PRECISE = WINDOW + SPLIT + LAST_ROUND
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+@pytest.mark.parametrize("case", PRECISE, ids=[f"{'_'.join(map(str, c[0]))}+{'_'.join(map(str, c[1]))}-{'x'.join(map(str, c[2:]))}" for c in PRECISE])
+def test_window_attention_keeps_the_weights_precision(case, dtype):
+    """The result is the definition's to its own rounding, in one piece and split over the keys."""
+    lq, ctx, hq, hk, d, window, sinks = case
+    g, dt = gen(65), TD[dtype]
+    lk = [max(0, a + b) for a, b in zip(lq, ctx)]
+    cu_q, cu_k = cu(lq), cu(lk)
+    q, k, v = randn(g, sum(lq), hq, d, dtype=dt), randn(g, sum(lk), hk, d, dtype=dt), randn(g, sum(lk), hk, d, dtype=dt)
+    for variant in (0, 4):
+        out = ops.window_attention(q, k, v, cu_q.cuda(), d**-0.5, window=window, sinks=sinks, cu_seqlens_k=cu_k.cuda(), variant=variant)
+        check_precise(out, q, k, v, cu_q, cu_k, d**-0.5, window, sinks)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+def test_window_attention_keeps_small_weights_precision(dtype):
+    """Many keys of little weight each (2^-14 of the largest and less), all on one side: their sum keeps its bits."""
+    g, dt = gen(66), TD[dtype]
+    n, d = 3000, 64
+    q, k = torch.zeros(4, 2, d, device="cuda", dtype=dt), torch.zeros(n, 1, d, device="cuda", dtype=dt)
+    q[:, :, 0], k[:, 0, 0] = 1, -10 - torch.rand(n, device="cuda", generator=g) * 4
+    k[7, 0, 0] = 0
+    v = (1 + randn(g, n, 1, d).abs()).to(dt)
+    v[7] = 0
+    out = ops.window_attention(q, k, v, cu([4]).cuda(), 1.0, cu_seqlens_k=cu([n]).cuda())
+    check_precise(out, q, k, v, cu([4]), cu([n]), 1.0, 0, 0)
