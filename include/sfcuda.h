@@ -308,8 +308,9 @@ SF_API int sf_kv4_load(const sf_kv4_cache_args* args, void* stream, char* err, u
  * outside the cache hides its tokens, both reported through sf_kernel_status (code 3); zeros where every
  * token is hidden.  q and o 16-byte aligned, strides multiples of 8 elements.  workspace: 16-byte aligned,
  * sf_kv4_attention_workspace_bytes bytes (0: may be NULL), no initial content; two calls that overlap
- * on the GPU need one each.  variant 1 deals every request's keys to all CTAs, 3 keeps a (request,
- * head) to a CTA, 0 decides by size.
+ * on the GPU need one each.  Scores, softmax sums and accumulation in fp32; a weight times its value's scale enters
+ * its product as an fp16 (bf16 tensors) or an fp16 and its residual (fp16 tensors).  variant 1 deals every request's
+ * keys to all CTAs, 3 keeps a (request, head) to a CTA, 0 decides by size.
  */
 typedef struct sf_kv4_attention_args {
     const void *q, *cache, *table, *lens;

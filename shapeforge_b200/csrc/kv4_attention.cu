@@ -24,8 +24,8 @@
 //    and 1152, go through the MMA, and (c - 8) and (c' - 8) of the accumulators come from their
 //    difference and a factor 1/16 at the end: two integer operations a pair of codes.  Codes taken off
 //    their centre keep the fp32 accumulator from growing one-sided.  p s is an fp16 in a unit of each
-//    head's own that its largest p s so far sets, so what matters of it has 11 bits (flash attention's p
-//    has 8 or 11) whatever the values' range.
+//    head's own that its largest p s so far sets, so what matters of it has 11 bits (22 with the residual that
+//    fp16 outputs take) whatever the values' range.
 //  * S^T = K q^T and O^T = V^T p^T (mma.sync m16n8k16, keys / elements in the 16 rows, 8 query heads
 //    in the columns): a group of up to 8 heads wastes no rows, the cache is the A operand straight
 //    from shared memory, and p becomes the next B operand by a transposing matrix move.  tcgen05
@@ -69,6 +69,9 @@ constexpr float NO_MAX = -3e38f;  // the running max before any score
 constexpr float S_UNIT = 1024.f;  // of the scores between the products and the exponential
 // Smallest unit of a head's p s: p / unit stays finite for p up to 2^8.
 constexpr float UNIT_FLOOR = 0x1p-118f;
+// The largest p s of a head in O's unit: UNITS_NEW where it sets the unit, up to UNITS_MOST before the next does, an
+// fp16 still; 2^-32 of it is a half step of the smallest.
+constexpr float UNITS_NEW = 128.f, UNITS_MOST = 32768.f;
 constexpr float LOG2E = 1.4426950408889634f;
 
 struct Args {
@@ -212,6 +215,11 @@ __global__ void __launch_bounds__(THREADS, ctas_of(NT)) kv4_attention_kernel(con
     using S = Smem<NG, NT>;
     using R = kv4::Record<NG>;
     constexpr int D = 64 * NG, HB = S::HB, ST = S::STAGES, TS = S::TS;
+    // p s goes into its product as one fp16 for bf16 outputs, an eighth of whose step that is, and with its residual
+    // for fp16 outputs.  Relative error over 32 requests of up to 16384 tokens, 64 heads on 8 of 128: bf16 1.67e-3 with
+    // one part (1.66e-3 is the output's own rounding), fp16 2.9e-4 with one, 2.15e-4 with two (2.06e-4); 80 us with one
+    // part, 89 with two.
+    constexpr int PARTS = std::is_same<T, __half>::value ? 2 : 1;
     extern __shared__ __align__(128) uint8_t smem[];
     float* out_s = reinterpret_cast<float*>(smem + S::OUT);
     float* stat_s = reinterpret_cast<float*>(smem + S::STAT);
@@ -457,7 +465,7 @@ __global__ void __launch_bounds__(THREADS, ctas_of(NT)) kv4_attention_kernel(con
         // and g + 8 are the lower and upper pair of elements), [4 G + 2 + i] their upper codes times 16.
         float o[NT][4 * NG][4];
         float2 nm[NT], l[NT], pm[NT][NG];  // minus the max that weights are relative to, their sum, sum p (minimum + 8 scale)
-        float2 unit[NT], per_unit[NT];     // O is in this unit, a head each; the largest p s is at most 2^8 of it
+        float2 unit[NT], per_unit[NT];     // O is in this unit, a head each; the largest p s is at most UNITS_MOST of it
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
@@ -629,7 +637,7 @@ __global__ void __launch_bounds__(THREADS, ctas_of(NT)) kv4_attention_kernel(con
                         s[u][nt][2 * r + 1] = p.y;
                     }
                 }
-            if (__any_sync(0xffffffffu, over > 256.f)) {
+            if (__any_sync(0xffffffffu, over > UNITS_MOST)) {
 #pragma unroll
                 for (int nt = 0; nt < NT; ++nt) {
                     float2 top = sf::f2(0.f);  // the head's largest p s
@@ -644,8 +652,8 @@ __global__ void __launch_bounds__(THREADS, ctas_of(NT)) kv4_attention_kernel(con
                             }
                     top = over_keys(top);
                     // Where this head's own weights fit, its unit stays.
-                    const float2 un = make_float2(top.x > 256.f * unit[nt].x ? fmaxf(top.x, UNIT_FLOOR) : unit[nt].x,
-                                                  top.y > 256.f * unit[nt].y ? fmaxf(top.y, UNIT_FLOOR) : unit[nt].y);
+                    const float2 un = make_float2(top.x > UNITS_MOST * unit[nt].x ? fmaxf(top.x * (1.0f / UNITS_NEW), UNIT_FLOOR) : unit[nt].x,
+                                                  top.y > UNITS_MOST * unit[nt].y ? fmaxf(top.y * (1.0f / UNITS_NEW), UNIT_FLOOR) : unit[nt].y);
                     per_unit[nt] = make_float2(1.0f / un.x, 1.0f / un.y);
                     const float2 f = sf::f2_mul(unit[nt], per_unit[nt]);
                     unit[nt] = un;
@@ -661,7 +669,7 @@ __global__ void __launch_bounds__(THREADS, ctas_of(NT)) kv4_attention_kernel(con
 #pragma unroll
             for (int u = 0; u < TS; ++u) {
                 const uint8_t* tile = rec + u * R::BYTES;
-                uint32_t pf[NT][NG][2];  // p s in O's unit, the B operand of O^T = V^T p^T
+                uint32_t pf[NT][NG][PARTS][2];  // p s in O's unit, the B operand of O^T = V^T p^T
 #pragma unroll
                 for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -670,7 +678,13 @@ __global__ void __launch_bounds__(THREADS, ctas_of(NT)) kv4_attention_kernel(con
 #pragma unroll
                         for (int G = 0; G < NG; ++G) {
                             const float vs = __uint_as_float(vp[u][r][G] << 16);
-                            pf[nt][G][r] = transpose8(f16x2(pu.x * vs, pu.y * vs));
+                            const float2 ps = sf::f2_mul(pu, sf::f2(vs));
+                            const uint32_t high = f16x2(ps.x, ps.y);
+                            pf[nt][G][0][r] = transpose8(high);
+                            if constexpr (PARTS == 2) {
+                                const float2 rest = sf::f2_fma(sf::Pair<__half>::to_f2(high), sf::f2(-1.f), ps);
+                                pf[nt][G][PARTS - 1][r] = transpose8(f16x2(rest.x, rest.y));
+                            }
                         }
                     }
                 // O^T += V^T p^T: the lane reads its 8 elements a group of keys t, 7 - t, 8 + t, 15 - t.
@@ -700,10 +714,12 @@ __global__ void __launch_bounds__(THREADS, ctas_of(NT)) kv4_attention_kernel(con
                             up[c] = sub2(b[c] & 0xFFF0FFF0u, 0x64806480u);    // 1024 + 16 code - 1152
                         }
 #pragma unroll
-                        for (int nt = 0; nt < NT; ++nt) {
-                            mma_f16(o[nt][4 * G + i], all, pf[nt][G][0], pf[nt][G][1]);
-                            mma_f16(o[nt][4 * G + 2 + i], up, pf[nt][G][0], pf[nt][G][1]);
-                        }
+                        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                            for (int part = 0; part < PARTS; ++part) {
+                                mma_f16(o[nt][4 * G + i], all, pf[nt][G][part][0], pf[nt][G][part][1]);
+                                mma_f16(o[nt][4 * G + 2 + i], up, pf[nt][G][part][0], pf[nt][G][part][1]);
+                            }
                     }
             }
         }

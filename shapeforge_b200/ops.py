@@ -674,7 +674,8 @@ def kv4_attention(q: torch.Tensor, cache: torch.Tensor, block_table: torch.Tenso
     in the cache, the query's own last.  Token ``j`` is seen when ``j >= seq_len - window`` or ``j <
     sinks`` (``window`` 0: all).  A length of 0 gives zeros; a length past the table is cut to it and a
     page id outside the cache hides its tokens, both reported by :func:`kernel_status` (code 3); a request
-    with every token hidden gives zeros.  q and ``out`` need 16-byte aligned rows and must not overlap.
+    with every token hidden gives zeros.  Softmax in fp32, its weights to 11 (bf16) or 22 (fp16) bits in their
+    product.  q and ``out`` need 16-byte aligned rows and must not overlap.
     ``workspace`` (uint8, :func:`kv4_attention_workspace_bytes`) is allocated here when not given;
     calls that overlap on the GPU need one each.  ``variant``: 0 = by size, 1 = all requests' keys
     dealt evenly to all CTAs, 3 = a CTA a (request, head)."""

@@ -171,3 +171,28 @@ def test_window_attention_keeps_small_weights_precision(dtype):
     v[7] = 0
     out = ops.window_attention(q, k, v, cu([4]).cuda(), 1.0, cu_seqlens_k=cu([n]).cuda())
     check_precise(out, q, k, v, cu([4]), cu([n]), 1.0, 0, 0)
+
+
+@pytest.mark.parametrize("variant", [0, 1, 3])
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+@pytest.mark.parametrize("shape", [(8, 2, 64), (32, 4, 128), (24, 2, 64), (40, 2, 128)], ids=["8x2x64", "32x4x128", "24x2x64", "40x2x128"])
+def test_kv4_attention_keeps_the_weights_precision(shape, dtype, variant):
+    """The error's mean square is that of the output's own rounding.  What else there is, is some 2^-18 of a result (sums
+    in fp32 of whole bytes, 17 times a code, in steps of 2^-24) and the weights' rounding: 2^-22 (fp16) or 2^-11 of a
+    bf16 step of 2^-8, at most 1/64 of its square.  Weights of 11 bits would double it in fp16."""
+    hq, h, d = shape
+    g, dt, n, page, b = gen(67), TD[dtype], 900, 32, 3
+    cache = ops.kv4_cache(30 * b, page, h, d)
+    # Values about zero, so that results are as small as the weights' errors can make them.
+    kx, vx = randn(g, 30 * b * page, h, d, dtype=dt), randn(g, 30 * b * page, h, d, dtype=dt)
+    ops.kv4_store(kx, vx, torch.arange(30 * b * page, device="cuda", dtype=torch.int32), cache)
+    table = torch.randperm(30 * b, device="cuda", generator=g).view(b, 30).to(torch.int32)
+    q = randn(g, b, hq, d, dtype=dt)
+    out = ops.kv4_attention(q, cache, table, i32([n] * b), d**-0.5, variant=variant)
+    kv, vv = serving.kv4_values(*serving.kv4_quantise(kx)), serving.kv4_values(*serving.kv4_quantise(vx))
+    at = torch.arange(n, device="cuda")
+    rows = table.long()[:, at // page] * page + at % page
+    k, v = (x[rows].transpose(1, 2).repeat_interleave(hq // h, 1) for x in (kv, vv))
+    want = (torch.softmax(torch.einsum("bhd,bhnd->bhn", q.double(), k) * d**-0.5, -1)[:, :, None] @ v)[:, :, 0]
+    own, error = ((x.double() - want).square().mean() for x in (want.to(dt), out))
+    assert error <= 1.1 * own
