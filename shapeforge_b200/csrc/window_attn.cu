@@ -33,7 +33,9 @@ struct Args {
     int slots;           // of tokens, a kv head
     int splits;          // CTAs that share the keys of a pair of row tiles; above 1 each leaves its state for the join:
     int whole;           // pairs of row tiles, in the grid's order, whose keys stay together all the same
-    float *part, *stat;  // [splits][tq][heads][D] unnormalised outputs, [splits][tq][heads][2] running max, sum
+    // [splits][rows][D] unnormalised outputs, [splits][rows][2] running max, sum; the rows are the tensor's [tq][heads],
+    // or with whole > 0 only those of the other pairs, in the grid's order.
+    float *part, *stat;
 };
 
 // Keys [0, sinks) and [low, high) of a query at position p.
@@ -692,7 +694,8 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
         if (parts > 1) {
             // The row's state for the join, O as it is: half its columns at a time through the Q buffer.
             const bool own = live && ok;
-            const int64_t row_at = ((int64_t)part * a.tq + tok0 + t * tq_tile + tok) * a.heads + kvh * a.group + row - tok * a.group;
+            const int64_t row_at = LINE ? ((int64_t)part * rest + pair - a.whole) * (2 * qrows) + t * qrows + row
+                                        : ((int64_t)part * a.tq + tok0 + t * tq_tile + tok) * a.heads + kvh * a.group + row - tok * a.group;
             if (own) *reinterpret_cast<float2*>(a.stat + 2 * row_at) = make_float2(turn ? s.m : -INFINITY, s.l);
             const uint32_t written = __ballot_sync(0xffffffffu, own);
             constexpr int PIECES = D / 8;  // 16-byte pieces of half a row
@@ -788,13 +791,13 @@ __global__ void __launch_bounds__(256) window_join_kernel(const Args a, int tq_t
     const int r0 = blockIdx.z * JOIN_ROWS + (threadIdx.x >> 5) * ROWS;
     const int rows = min(ROWS, min(2 * tq_tile, at.qe - at.tok0) * a.group - r0);
     if (rows <= 0) return;
-    const int64_t all = a.tq * a.heads;
+    const int64_t all = a.whole ? (int64_t)gridDim.x * (2 * tq_tile * a.group) : a.tq * a.heads;
     int64_t row_at[ROWS];
     float m[ROWS], l[ROWS], acc[ROWS][E];
 #pragma unroll
     for (int i = 0; i < ROWS; ++i) {
         const int r = r0 + min(i, rows - 1), tok = r / a.group;
-        row_at[i] = (int64_t)(at.tok0 + tok) * a.heads + kvh * a.group + r - tok * a.group;
+        row_at[i] = a.whole ? (int64_t)blockIdx.x * (2 * tq_tile * a.group) + r : (int64_t)(at.tok0 + tok) * a.heads + kvh * a.group + r - tok * a.group;
         m[i] = -INFINITY;
         l[i] = 0.f;
 #pragma unroll
@@ -845,21 +848,26 @@ __global__ void __launch_bounds__(256) window_join_kernel(const Args a, int tq_t
     }
 }
 
-// CTAs that share the keys of a pair of row tiles.  A tile of 128 keys takes a CTA about 1.4 us, a CTA's start
-// and end about three of them, and a row's state leaves and comes back through L2: the least estimate of
-// that over the SMs.  The lengths are on the GPU, so pairs and tiles are those of sequences of equal length.
-// bf16, 32 query heads on 8 key heads of 128, no window: 1 token x 32768 keys 371 us unsplit, 37 us at the 16
-// chosen; 64 x 8192 104 and 27 (16); 4 x 16 x 4096 54 and 26 (4); 512 x 32768 389 and 222 (2).
+// CTAs that share the keys of a pair of row tiles.  A tile of 128 keys takes a CTA about 1.9 us, a CTA's start
+// and end some 4, and a row's state leaves and comes back through L2: the least estimate of that over the SMs, if
+// it is a twentieth below the unsplit one's.  The lengths are on the GPU, so pairs and tiles are those of sequences of
+// equal length.
+// bf16, 32 query heads on 8 key heads of 128, no window: 1 token x 32768 keys 514 us unsplit, 51 us at the 16
+// chosen; 64 x 8192 138 and 33 (16); 64 x 32768 527 and 61 (16); 512 x 32768 544 and 306 (2).
 // Where the pairs are more than a round of CTAs, those of the whole rounds keep their keys and only the last,
-// partial round's are split: 1536 tokens in 3 prompts behind 8200, 28 heads on 4 (177 pairs) 221 us unsplit,
-// 196 with all in 3, 169 so; 1280 x 8192 (160 pairs) 190 and 137; not for 3000 tokens without a context, whose
-// pairs differ and fill the last round by themselves (47 us, 55 if split).
+// partial round's are split, and only their states are in the workspace: 1536 tokens in 3 prompts behind 8200, 28
+// heads on 4 (177 pairs) 317 us unsplit, 226 so, 17 MB; 1280 x 8192 (160 pairs) 279 and 199, 21 MB; not for 16384
+// tokens behind 65536, where a percent would have to be gained.
 struct Split {
     int64_t z, whole;
+    int64_t rows;  // whose states a part leaves in the workspace
+    uint64_t bytes(int64_t D) const { return z > 1 ? (uint64_t)(z * rows * (D + 2) * 4) : 0; }
 };
+// The states stay in L2 (126 MB) until they are joined; 1000 tokens behind 500000 would else have 32 parts and 470 MB.
+constexpr double MOST_STATES = 96e6;
 Split split_of(int64_t Tq, int64_t Tk, int64_t seqs, int64_t Hq, int64_t Hk, int64_t D, int64_t window, int64_t sinks) {
     const int64_t group = Hq / Hk;
-    Split pick = {1, 0};
+    Split pick = {1, 0, 0};
     if ((D != 64 && D != 128) || group > 128 || Tk == 0 || seqs == 0) return pick;
     const int64_t tt = 2 * (128 / group), tokens = (Tq + seqs - 1) / seqs;
     const double pairs = (double)(std::min(seqs, Tq) * ((tokens + tt - 1) / tt) * Hk);
@@ -868,17 +876,21 @@ Split split_of(int64_t Tq, int64_t Tk, int64_t seqs, int64_t Hq, int64_t Hk, int
     const double w = window ? std::min(b, (double)window + tt + std::min<double>((double)sinks, b)) : b;
     const double few = std::min(a, w) / 128 + 0.5, mean = (b <= w || a >= w ? (std::min(a, w) + std::min(b, w)) / 2 : ((w * w - a * a) / 2 + w * (b - w)) / (b - a)) / 128 + 0.5;
     const double sms = sf::sm_count(), rounds = std::floor(pairs / sms), rest = pairs - rounds * sms;
+    constexpr double ENDS = 2.2;  // a CTA's start and end, in tiles; so is the join's launch
     // n CTAs of `tiles` tiles on average, the heaviest first: their sum over the SMs, and what the last round leaves idle.
-    auto time = [&](double n, double tiles, double least) { return n * (tiles + 3) / sms + (std::ceil(n / sms) - n / sms) * (least + 3); };
-    double best = time(pairs, mean, few);
+    auto time = [&](double n, double tiles, double least) { return n * (tiles + ENDS) / sms + (std::ceil(n / sms) - n / sms) * (least + ENDS); };
+    // Of the pairs in the grid, those of the whole rounds; the slots that rounding leaves over lie among the others.
+    const double slots = (double)(Tq / tt + seqs) * Hk, whole = std::floor(rounds * sms * slots / pairs), split = slots - whole;
+    double best = 0.95 * time(pairs, mean, few);
     for (int64_t z : {2, 3, 4, 6, 8, 12, 16, 24, 32}) {
         if (mean < 2 * z) break;
-        const double join = (double)Tq * Hq * D * 8 * z / 9e6;  // 9 MB of states in a tile's time
-        const double all = time(pairs * z, mean / z, few / z) + 3 + join;
-        const double last = rounds * (mean + 3) + time(rest * z, mean / z, few / z) + 5 + join * rest / pairs;
-        if (all < best) best = all, pick = {z, 0};
-        // The slots that rounding leaves over lie among the others.
-        if (rounds > 0 && rest > 0 && last < best) best = last, pick = {z, (int64_t)(rounds * sms * (Tq / tt + seqs) * Hk / pairs)};
+        const double join = (double)Tq * Hq * D * 8 * z / 12e6;  // 12 MB of states in a tile's time
+        const double all = time(pairs * z, mean / z, few / z) + ENDS + join;
+        const double last = rounds * (mean + ENDS) + time(rest * z, mean / z, few / z) + 1.7 * ENDS + join * rest / pairs;
+        auto fits = [&](double rows) { return z * rows * (D + 2) * 4 <= MOST_STATES; };
+        if (all < best && fits((double)Tq * Hq)) best = all, pick = {z, 0, Tq * Hq};
+        if (rounds > 0 && rest > 0 && split > 0 && last < best && whole + split * z <= 0x7fffffff && fits(split * tt * group))
+            best = last, pick = {z, (int64_t)whole, (int64_t)split * tt * group};
     }
     return pick;
 }
@@ -917,7 +929,6 @@ int launch_tc(Args a, int64_t hk, bool* taken, cudaStream_t st, char* err, uint6
     if (slots > 0x7fffffffLL) return sf::fail(SF_EINVAL, err, cap, "window_attention: grid too large");
     a.slots = (int)slots;
     const int64_t rest = slots * hk - a.whole;  // pairs of row tiles that are split
-    if (a.whole && (rest <= 0 || a.whole + rest * a.splits > 0x7fffffffLL)) a.whole = 0;
     const auto kernel = a.whole ? window_tc_kernel<T, D, true> : window_tc_kernel<T, D, false>;
     const dim3 grid = a.whole ? dim3((unsigned)(a.whole + rest * a.splits)) : dim3((unsigned)slots, (unsigned)hk, (unsigned)a.splits);
     kernel<<<grid, TC_THREADS, smem, st>>>(a, mq, mk, mk16, mv, mv16, tq_tile);
@@ -952,8 +963,7 @@ int launch_general(const Args& a, int64_t D, cudaStream_t st, char* err, uint64_
 extern "C" uint64_t sf_window_attention_workspace_bytes(int64_t Tq, int64_t Tk, int64_t seqs, int64_t Hq, int64_t Hk, int64_t D, int64_t window,
                                                         int64_t sinks) {
     if (Tq <= 0 || Tk <= 0 || seqs <= 0 || Hq <= 0 || Hk <= 0 || Hq % Hk || window < 0 || sinks < 0) return 0;
-    const int64_t z = split_of(Tq, Tk, seqs, Hq, Hk, D, window < Tk ? window : 0, sinks).z;
-    return z > 1 ? (uint64_t)(z * Tq * Hq * (D + 2) * 4) : 0;
+    return split_of(Tq, Tk, seqs, Hq, Hk, D, window < Tk ? window : 0, sinks).bytes(D);
 }
 
 extern "C" int sf_window_attention(const sf_window_attention_args* x, void* stream, char* err, uint64_t cap) {
@@ -988,12 +998,11 @@ extern "C" int sf_window_attention(const sf_window_attention_args* x, void* stre
     a.splits = 1;
     if (x->variant != 4) {
         const Split split = split_of(Tq, Tk, seqs, Hq, Hk, D, window, x->sinks);
-        const int64_t z = split.z;
-        if (z > 1 && x->workspace && sf::aligned16(x->workspace) && x->workspace_bytes >= (uint64_t)(z * Tq * Hq * (D + 2) * 4)) {
-            a.splits = (int)z;
-            a.whole = split.whole <= 0x7fffffff ? (int)split.whole : 0;
+        if (split.z > 1 && x->workspace && sf::aligned16(x->workspace) && x->workspace_bytes >= split.bytes(D)) {
+            a.splits = (int)split.z;
+            a.whole = (int)split.whole;
             a.part = (float*)x->workspace;
-            a.stat = a.part + z * Tq * Hq * D;
+            a.stat = a.part + split.z * split.rows * D;
         }
     }
     cudaStream_t st = (cudaStream_t)stream;

@@ -18,3 +18,18 @@ def test_windows_past_every_key_are_no_window(far):
     wide = ops.window_attention_workspace_bytes
     for shape in ((1, 32768, 1, 32, 8, 128), (1536, 26136, 3, 28, 4, 128), (4, 70, 1, 8, 2, 64)):
         assert wide(*shape, window=far) == wide(*shape) == wide(*shape, window=far, sinks=far)
+
+
+def test_window_workspace_stays_small():
+    """The states of a split are those of the rows that are split, and only where that is worth it: 100 MB at most."""
+    size = ops.window_attention_workspace_bytes
+    for chunk, context, hq, hk in ((8192, 57344, 128, 8), (16384, 65536, 64, 8), (16384, 131072, 64, 8), (11264, 16384, 64, 8)):
+        assert size(chunk, chunk + context, 1, hq, hk, 128) == 0    # below a twentieth of the time
+    assert 0 < size(1536, 26136, 3, 28, 4, 128) < 20e6
+    for d in (64, 128):
+        for hq, hk in ((8, 8), (32, 8), (28, 4), (64, 8), (128, 8), (64, 1), (96, 96)):
+            for chunk in (1, 7, 64, 500, 1000, 1536, 2048, 4096, 11264, 16384, 65536):
+                for context in (0, 4096, 65536, 131072, 500000):
+                    for seqs in (1, 3, 32):
+                        for window in (0, 1024, 30000):
+                            assert size(chunk, chunk + context * seqs, seqs, hq, hk, d, window=window, sinks=4) <= 100e6

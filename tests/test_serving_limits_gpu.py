@@ -196,3 +196,24 @@ def test_kv4_attention_keeps_the_weights_precision(shape, dtype, variant):
     want = (torch.softmax(torch.einsum("bhd,bhnd->bhn", q.double(), k) * d**-0.5, -1)[:, :, None] @ v)[:, :, 0]
     own, error = ((x.double() - want).square().mean() for x in (want.to(dt), out))
     assert error <= 1.1 * own
+
+
+# ---- the workspace of a split ----------------------------------------------------------------------
+
+
+def test_a_chunk_split_in_its_last_round_writes_what_it_asked_for():
+    """2100 tokens behind 3000 and a short neighbour, 32 heads on 8: the workspace holds the last round's rows alone, all
+    of them, and nothing behind it is touched."""
+    g, hq, hk, d = gen(68), 32, 8, 128
+    cu_q, cu_k = cu([1200, 37]), cu([4200, 3037])
+    q, k, v = randn(g, 1240, hq, d, dtype=torch.bfloat16), randn(g, 7237, hk, d, dtype=torch.bfloat16), randn(g, 7237, hk, d, dtype=torch.bfloat16)
+    need = ops.window_attention_workspace_bytes(1240, 7237, 2, hq, hk, d)
+    assert 0 < need < 1240 * hq * (d + 2) * 4
+    ws = torch.full((need + 4096,), 0xFF, dtype=torch.uint8, device="cuda")
+    before = torch.full_like(q, 7.5)
+    out = ops.window_attention(q, k, v, cu_q.cuda(), 0.09, cu_seqlens_k=cu_k.cuda(), workspace=ws[:need], out=before.clone())
+    assert (ws[need:] == 0xFF).all() and torch.equal(out[1237:], before[1237:])
+    check_precise(out[:1237], q[:1237], k, v, cu_q, cu_k, 0.09, 0, 0)
+    for small in (ws[: need - 16], ws[:0]):
+        whole = ops.window_attention(q, k, v, cu_q.cuda(), 0.09, cu_seqlens_k=cu_k.cuda(), workspace=small, out=before.clone())
+        check_precise(whole[:1237], q[:1237], k, v, cu_q, cu_k, 0.09, 0, 0)
