@@ -138,8 +138,12 @@ __global__ void __launch_bounds__(128) window_general_kernel(const Args a, int D
 // 1.56 at the pipe's rate.  P's first hand-over at 32, 64 or 96 keys: 527, 523, 522.  1203 tokens in 9 prompts, window
 // 128: 22 us, two CTAs in turn on an SM, latency.  (Without the residual, CTAs that take their next piece from the
 // hardware's scheduler hid the start and end, but the registers that cost the softmax slowed every step: 411 us.)
-// A row that comes out NaN (or infinite) is computed again key by key: masked keys in its tiles may hold
-// infinities or NaN that their zero weights do not silence.
+// A row that comes out NaN or infinite may have that from values that it does not see, which share its tiles and which
+// a weight of zero does not silence.  If its softmax sum is not finite the scores it sees are not, and all of it is NaN;
+// else `settle` looks through the values that the warp's rows see, once for all of them: a column that sees a NaN or an
+// infinity is that, and a row with some other column of that kind is computed again key by key.  So only rows within a
+// tile or two of a bad value that they do not see are (16384 causal tokens of 16 heads on 2: 1.1 ms, 5.6 with
+// the first value infinite, 1.1 with the first key NaN).
 
 constexpr int BOX = 128 * 128;       // 128 rows of 64 16-bit elements
 constexpr int TC_THREADS = 384;
@@ -373,10 +377,75 @@ __device__ __forceinline__ float max32(const uint32_t* r, float m) {
     return max3_nan(a[0], a[1], a[1]);
 }
 
+// The rows of a warp whose output (written, at `out`) is not finite although their softmax sum is: lanes with `again`,
+// each with its row's position and query row.  Values in 16-byte aligned rows, as the kernel below takes them.
+template <typename T, int D>
+__device__ __forceinline__ void settle(const Args& a, bool again, int p, int64_t kbegin, int64_t qrow, int head, T* out) {
+    constexpr int E = D / 32, W = E / 2;  // the lane's columns E lane .. E lane + E - 1, two a word
+    constexpr uint32_t EXP = std::is_same<T, __half>::value ? 0x7C00u : 0x7F80u;
+    const int lane = threadIdx.x & 31;
+    uint32_t todo = __ballot_sync(0xffffffffu, again);
+    if (!todo) return;
+    const int kvh = __shfl_sync(0xffffffffu, head, __ffs(todo) - 1) / a.group;
+    const T* v = (const T*)a.v + kbegin * a.vt + (int64_t)kvh * a.vh + E * lane;
+    const Keys mine(a, again ? p : -1);
+    const Keys all(a, -__reduce_max_sync(0xffffffffu, again ? -p : -0x7fffffff));  // of the first of them, but up to
+    const int high = __reduce_max_sync(0xffffffffu, mine.high);                    // what the last sees
+    const int n = all.sinks + high - all.low;
+    // What the lane's row sees in column E l + e: bit l of [e].
+    uint32_t nan[E] = {}, pos[E] = {}, neg[E] = {};
+    constexpr int AHEAD = 8;
+#pragma unroll 1
+    for (int i0 = 0; i0 < n; i0 += AHEAD) {
+        uint32_t x[AHEAD][W];
+#pragma unroll
+        for (int u = 0; u < AHEAD; ++u) {
+            const int i = min(i0 + u, n - 1);
+            const T* row = v + (int64_t)(i < all.sinks ? i : all.low + (i - all.sinks)) * a.vt;
+            if constexpr (W == 2) *reinterpret_cast<uint2*>(x[u]) = *reinterpret_cast<const uint2*>(row);
+            else x[u][0] = *reinterpret_cast<const uint32_t*>(row);
+        }
+#pragma unroll
+        for (int u = 0; u < AHEAD; ++u) {
+            bool bad = false;
+#pragma unroll
+            for (int k = 0; k < W; ++k) bad |= (x[u][k] & EXP) == EXP || (x[u][k] >> 16 & EXP) == EXP;
+            if (!__any_sync(0xffffffffu, bad)) continue;
+            const int i = min(i0 + u, n - 1), j = i < all.sinks ? i : all.low + (i - all.sinks);
+            const bool sees = j < mine.sinks || (j >= mine.low && j < mine.high);
+#pragma unroll
+            for (int e = 0; e < E; ++e) {
+                const uint32_t y = x[u][e / 2] >> (16 * (e & 1)) & 0xFFFFu;
+                const bool special = (y & EXP) == EXP, is_nan = (y & 0x7FFFu) > EXP;
+                const uint32_t b_nan = __ballot_sync(0xffffffffu, is_nan), b_pos = __ballot_sync(0xffffffffu, special && !is_nan && !(y >> 15)),
+                               b_neg = __ballot_sync(0xffffffffu, special && !is_nan && y >> 15);
+                if (sees) nan[e] |= b_nan, pos[e] |= b_pos, neg[e] |= b_neg;
+            }
+        }
+    }
+    for (; todo; todo &= todo - 1) {
+        const int src = __ffs(todo) - 1;
+        T* o = reinterpret_cast<T*>(__shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(out), src)) + E * lane;
+        bool left = false;
+#pragma unroll
+        for (int e = 0; e < E; ++e) {
+            const uint32_t here = __shfl_sync(0xffffffffu, nan[e], src) >> lane & 1u, up = __shfl_sync(0xffffffffu, pos[e], src) >> lane & 1u,
+                           down = __shfl_sync(0xffffffffu, neg[e], src) >> lane & 1u;
+            if (here | up | down) o[e] = sf::Dt<T>::from_f(here || (up && down) ? NAN : (up ? INFINITY : -INFINITY));
+            else left |= !(fabsf(sf::Dt<T>::to_f(o[e])) < INFINITY);
+        }
+        if (__any_sync(0xffffffffu, left)) {
+            __syncwarp();
+            row_by_warp<T>(a, D, __shfl_sync(0xffffffffu, (long long)qrow, src), __shfl_sync(0xffffffffu, head, src), kbegin,
+                           __shfl_sync(0xffffffffu, p, src), o - E * lane);
+        }
+    }
+}
+
 // LINE: a.whole pairs of row tiles keep their keys, the others are split, all in one line of CTAs.
 template <typename T, int D, bool LINE>
 __global__ void __launch_bounds__(TC_THREADS, 1)
-    window_tc_kernel(const Args a, const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUtensorMap mk16,
+    window_tc_kernel(const __grid_constant__ Args a, const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUtensorMap mk16,
                      const __grid_constant__ CUtensorMap mv, const __grid_constant__ CUtensorMap mv16, int tq_tile) {
     using L = Layout<D>;
     constexpr int DB = L::DB;
@@ -743,7 +812,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
                     stage[lane * PIECES + ((4 * c + i) ^ (lane & 7))] = make_uint4(o4[0], o4[1], o4[2], o4[3]);
                 }
             }
-            const bool again = live && ok && !(nan.x + nan.y == 0.f);
+            const bool again = live && ok && !(nan.x + nan.y == 0.f) && s.l < INFINITY;
             const int64_t mine = (int64_t)(tok0 + t * tq_tile + tok) * a.ot + (int64_t)(kvh * a.group + row - tok * a.group) * a.oh;
             __syncwarp();
             const uint32_t written = __ballot_sync(0xffffffffu, live && ok);
@@ -755,13 +824,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
                 if (written >> rl & 1u) *reinterpret_cast<uint4*>((T*)a.o + at + 8 * piece) = x;
             }
             __syncwarp();
-            for (uint32_t todo = __ballot_sync(0xffffffffu, again); todo; todo &= todo - 1) {
-                const int src = __ffs(todo) - 1;
-                const int rw = (warp & 3) * 32 + src;
-                const int tk = rw / a.group, hd = kvh * a.group + rw - tk * a.group;
-                const int64_t qrow = (int64_t)tok0 + t * tq_tile + tk;
-                row_by_warp<T>(a, D, qrow, hd, kb, first + tk, (T*)a.o + qrow * a.ot + (int64_t)hd * a.oh);
-            }
+            settle<T, D>(a, again, p, kb, (int64_t)tok0 + t * tq_tile + tok, kvh * a.group + row - tok * a.group, (T*)a.o + mine);
         }
     }
     sm100::tc_fence_before();
@@ -776,7 +839,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
 // time behind its max, 197 so, 198 and 200 in blocks of 32 and 64 rows.
 constexpr int JOIN_ROWS = 16;
 template <typename T, int D>
-__global__ void __launch_bounds__(256) window_join_kernel(const Args a, int tq_tile) {
+__global__ void __launch_bounds__(256) window_join_kernel(const __grid_constant__ Args a, int tq_tile) {
     asm volatile("griddepcontrol.wait;" ::: "memory");
     int slot = blockIdx.x, kvh = blockIdx.y;
     if (a.whole) {
@@ -789,21 +852,23 @@ __global__ void __launch_bounds__(256) window_join_kernel(const Args a, int tq_t
     constexpr int ROWS = JOIN_ROWS / 8, E = D / 32;
     const int lane = threadIdx.x & 31;
     const int r0 = blockIdx.z * JOIN_ROWS + (threadIdx.x >> 5) * ROWS;
-    const int rows = min(ROWS, min(2 * tq_tile, at.qe - at.tok0) * a.group - r0);
-    if (rows <= 0) return;
+    const int rows = max(0, min(ROWS, min(2 * tq_tile, at.qe - at.tok0) * a.group - r0));
+    __shared__ uint32_t again_s;  // of the block's rows, those that have to be settled
+    if (threadIdx.x == 0) again_s = 0;
+    __syncthreads();
     const int64_t all = a.whole ? (int64_t)gridDim.x * (2 * tq_tile * a.group) : a.tq * a.heads;
     int64_t row_at[ROWS];
     float m[ROWS], l[ROWS], acc[ROWS][E];
 #pragma unroll
     for (int i = 0; i < ROWS; ++i) {
-        const int r = r0 + min(i, rows - 1), tok = r / a.group;
+        const int r = r0 + min(i, max(0, rows - 1)), tok = r / a.group;
         row_at[i] = a.whole ? (int64_t)blockIdx.x * (2 * tq_tile * a.group) + r : (int64_t)(at.tok0 + tok) * a.heads + kvh * a.group + r - tok * a.group;
         m[i] = -INFINITY;
         l[i] = 0.f;
 #pragma unroll
         for (int e = 0; e < E; ++e) acc[i][e] = 0.f;
     }
-    for (int z = 0; z < a.splits; ++z) {
+    for (int z = 0; z < (rows ? a.splits : 0); ++z) {
         float2 st[ROWS];
         float x[ROWS][E];
 #pragma unroll
@@ -824,7 +889,6 @@ __global__ void __launch_bounds__(256) window_join_kernel(const Args a, int tq_t
             for (int e = 0; e < E; ++e) acc[i][e] = acc[i][e] * f + x[i][e] * g;
         }
     }
-    uint32_t todo = 0;  // rows to compute key by key
 #pragma unroll
     for (int i = 0; i < ROWS; ++i) {
         if (i >= rows) break;
@@ -839,12 +903,13 @@ __global__ void __launch_bounds__(256) window_join_kernel(const Args a, int tq_t
             again |= !(v.x * 0.f + v.y * 0.f == 0.f);
             *reinterpret_cast<uint32_t*>(out + E * lane + e) = sf::Pair<T>::from_f2(v);
         }
-        if (__any_sync(0xffffffffu, again)) todo |= 1u << i;
+        if (__any_sync(0xffffffffu, again) && l[i] < INFINITY && lane == 0) atomicOr(&again_s, 1u << (ROWS * (threadIdx.x >> 5) + i));
     }
-    for (; todo; todo &= todo - 1) {
-        const int r = r0 + __ffs(todo) - 1, tok = r / a.group, head = kvh * a.group + r - tok * a.group;
-        __syncwarp();
-        row_by_warp<T>(a, D, at.tok0 + tok, head, at.kb, at.pos0 + tok, (T*)a.o + (int64_t)(at.tok0 + tok) * a.ot + (int64_t)head * a.oh);
+    __syncthreads();
+    if (again_s && threadIdx.x < 32) {  // one warp for the block's rows, a lane each
+        const int r = blockIdx.z * JOIN_ROWS + lane, tok = r / a.group, head = kvh * a.group + r - tok * a.group;
+        settle<T, D>(a, again_s >> lane & 1u, at.pos0 + tok, at.kb, (int64_t)at.tok0 + tok, head,
+                     (T*)a.o + (int64_t)(at.tok0 + tok) * a.ot + (int64_t)head * a.oh);
     }
 }
 

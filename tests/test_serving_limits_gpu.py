@@ -217,3 +217,70 @@ def test_a_chunk_split_in_its_last_round_writes_what_it_asked_for():
     for small in (ws[: need - 16], ws[:0]):
         whole = ops.window_attention(q, k, v, cu_q.cuda(), 0.09, cu_seqlens_k=cu_k.cuda(), workspace=small, out=before.clone())
         check_precise(whole[:1237], q[:1237], k, v, cu_q, cu_k, 0.09, 0, 0)
+
+
+# ---- values that are not finite --------------------------------------------------------------------
+
+
+SPECIAL = [
+    # query lengths, contexts in front, Hq, Hk, D, window, sinks
+    ([300, 40], [0, 33], 4, 2, 128, 0, 0),
+    ([300, 150], [20, 0], 8, 1, 64, 90, 0),
+    ([260], [100], 5, 1, 128, 70, 6),
+    ([400], [0], 2, 2, 64, 40, 150),
+    ([3], [2000], 4, 2, 128, 0, 0),             # split over the keys
+    ([9, 2], [3333, 2500], 3, 1, 64, 1500, 4),
+    ([650, 3], [1300, 1400], 64, 1, 64, 0, 0),  # in the last round
+]
+
+
+@pytest.mark.parametrize("variant", [0, 2, 4])
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+@pytest.mark.parametrize("case", SPECIAL, ids=[f"{'_'.join(map(str, c[0]))}-{'x'.join(map(str, c[2:]))}" for c in SPECIAL])
+def test_infinite_values_come_out_as_the_definition_has_them(case, dtype, variant):
+    """An element of the result whose column holds infinities among the values seen is that infinity (NaN with both signs
+    or a NaN); every other element is as ever, in the same row and beside values that the row does not see."""
+    lq, ctx, hq, hk, d, window, sinks = case
+    g, dt = gen(69), TD[dtype]
+    lk = [a + b for a, b in zip(lq, ctx)]
+    cu_q, cu_k = cu(lq), cu(lk)
+    q, k, v = randn(g, sum(lq), hq, d, dtype=dt), randn(g, sum(lk), hk, d, dtype=dt), randn(g, sum(lk) + 1, hk, d, dtype=dt)
+    n = lk[0]
+    for row, col, value in ((0, 3, math.inf), (n // 2, 3, math.inf), (n // 3, 5, -math.inf), (n - 1, 5, math.inf), (n - 2, 7, math.nan), (n // 2 + 1, 8, -math.inf),
+                            (n - 3, d - 1, math.inf), (n // 4, slice(40, 44), math.inf), (n, 9, math.nan)):
+        v[row, 0, col] = value
+    v[n // 5, hk - 1, 1] = math.nan
+    out = ops.window_attention(q, k, v[: sum(lk)], cu_q.cuda(), d**-0.5, window=window, sinks=sinks, cu_seqlens_k=cu_k.cuda(), variant=variant)
+    inside, r = serving.window_attention(q, k, v[: sum(lk)], cu_q.tolist(), cu_k.tolist(), d**-0.5, window, sinks)
+    assert torch.isinf(r.value).any() and torch.isnan(r.value).any()
+    half = dt == torch.float16
+    close(out, r.value, attention_slack(r, d, max(lk), 2.0**-22 if half else 2.0**-15) + (max(lk) * 2.0**-32 * r.peak if half else 0))
+
+
+def test_one_bad_token_does_not_slow_the_whole_prompt_down():
+    """A NaN key and value, or an infinite value alone, that every query sees: what comes out is known without going over
+    each row's keys again (hundreds of times the work)."""
+    g = gen(70)
+    n = 6144
+    q, k, v = (randn(g, n, h, 128, dtype=torch.bfloat16) for h in (8, 1, 1))
+    table = cu([n]).cuda()
+
+    def time():
+        best = math.inf
+        for _ in range(3):
+            start, end = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+            start.record()
+            out = ops.window_attention(q, k, v, table, 0.09)
+            end.record()
+            torch.cuda.synchronize()
+            best = min(best, start.elapsed_time(end))
+        return out, best
+
+    _, clean = time()
+    v[0] = math.inf
+    out, infinite = time()
+    assert torch.isposinf(out).all()
+    k[0], v[0] = math.nan, math.nan
+    out, bad = time()
+    assert torch.isnan(out).all()
+    assert infinite < 20 * clean and bad < 5 * clean, (clean, infinite, bad)
