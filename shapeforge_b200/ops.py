@@ -661,8 +661,10 @@ def kv4_attention_workspace_bytes(batch: int, q_heads: int, kv_heads: int, dim: 
 
 @functools.lru_cache(maxsize=512)
 def _kv4_attention_need(dev: int, *sizes: int) -> int:
-    """The sizes' workspace bytes on GPU ``dev``: a decode loop asks for the same ones again and again."""
-    return kv4_attention_workspace_bytes(*sizes)
+    """The sizes' workspace bytes on GPU ``dev`` (the plan goes by its SMs, so it is asked for with that GPU current):
+    a decode loop asks for the same ones again and again."""
+    with torch.cuda.device(dev):
+        return kv4_attention_workspace_bytes(*sizes)
 
 
 def kv4_attention(q: torch.Tensor, cache: torch.Tensor, block_table: torch.Tensor, seq_lens: torch.Tensor, scale: float, window: int = 0,
@@ -718,7 +720,8 @@ def window_attention_workspace_bytes(q_tokens: int, k_tokens: int, sequences: in
 
 @functools.lru_cache(maxsize=512)
 def _window_attention_need(dev: int, *sizes: int) -> int:
-    return window_attention_workspace_bytes(*sizes)
+    with torch.cuda.device(dev):  # as above
+        return window_attention_workspace_bytes(*sizes)
 
 
 def window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqlens: torch.Tensor, scale: float, window: int = 0, sinks: int = 0,

@@ -33,3 +33,25 @@ def test_window_workspace_stays_small():
                     for seqs in (1, 3, 32):
                         for window in (0, 1024, 30000):
                             assert size(chunk, chunk + context * seqs, seqs, hq, hk, d, window=window, sinks=4) <= 100e6
+
+
+def test_workspace_sizes_are_those_of_the_tensors_gpu(monkeypatch):
+    """GPUs may have different numbers of SMs, which the plans go by."""
+    current = [0]
+
+    class Device:
+        def __init__(self, index):
+            self.index = index
+
+        def __enter__(self):
+            self.before, current[0] = current[0], self.index
+
+        def __exit__(self, *_):
+            current[0] = self.before
+
+    monkeypatch.setattr(torch.cuda, "device", Device)
+    for need, query in (("_kv4_attention_need", "kv4_attention_workspace_bytes"), ("_window_attention_need", "window_attention_workspace_bytes")):
+        monkeypatch.setattr(ops, query, lambda *sizes: 1000 * current[0] + sizes[0])
+        getattr(ops, need).cache_clear()
+        assert [getattr(ops, need)(dev, 7) for dev in (0, 2, 1, 2)] == [7, 2007, 1007, 2007] and current == [0]
+        getattr(ops, need).cache_clear()
