@@ -901,6 +901,15 @@ int64_t most_tiles(int64_t width, int64_t tpp, int64_t window, int64_t sinks) {
     return std::min(all, (window + 15) / 16 + 1 + (sinks + 15) / 16);
 }
 
+// CTAs of the line kernel an SM holds: the prefix of the requests' costs is part of its shared memory, and above some 740
+// requests (D 128, one head tile) a third CTA no longer fits into the SM's 228 KB (1 KB a CTA is the system's): 800 requests of up
+// to 2048 tokens 445 us with three an SM in the grid, 335 with two.
+int64_t resident(int nt, int64_t D, int64_t B) {
+    const int b = (int)std::min<int64_t>(B, 1 << 20);
+    const int smem = D == 64 ? (nt == 1 ? Smem<1, 1>::bytes(b) : Smem<1, 2>::bytes(b)) : (nt == 1 ? Smem<2, 1>::bytes(b) : Smem<2, 2>::bytes(b));
+    return std::max(1, std::min(ctas_of(nt), 228 * 1024 / (smem + 1024)));
+}
+
 struct Plan {
     int nt, blocks;
     bool split;
@@ -913,7 +922,7 @@ Plan plan_of(int64_t B, int64_t Hq, int64_t Hk, int64_t D, int64_t width, int64_
     p.nt = group > 8 ? 2 : 1;
     p.blocks = (int)((group + 8 * p.nt - 1) / (8 * p.nt));
     const int64_t items = B * Hk * p.blocks;
-    const int64_t wave = (int64_t)sf::sm_count() * ctas_of(p.nt);
+    const int64_t sms = sf::sm_count(), wave = sms * ctas_of(p.nt);
     const int64_t tiles = most_tiles(width, tpp, window, sinks);
     // Whole items a CTA while an item is at most four tiles a warp: nothing to join.  Longer items of a small
     // batch go to clusters of CTAs that join through each other's shared memory, without a second launch, as
@@ -930,7 +939,7 @@ Plan plan_of(int64_t B, int64_t Hq, int64_t Hk, int64_t D, int64_t width, int64_
     }
     if (variant == 3) p.split = false;
     if (variant == 1) p.split = true;
-    p.grid = (int)(p.split ? std::min(wave, std::max<int64_t>(1, (items * (tiles + ITEM_COST) + LEAST - 1) / LEAST)) : items * p.cluster);
+    p.grid = (int)(p.split ? std::min(sms * resident(p.nt, D, B), std::max<int64_t>(1, (items * (tiles + ITEM_COST) + LEAST - 1) / LEAST)) : items * p.cluster);
     return p;
 }
 

@@ -55,3 +55,12 @@ def test_workspace_sizes_are_those_of_the_tensors_gpu(monkeypatch):
         getattr(ops, need).cache_clear()
         assert [getattr(ops, need)(dev, 7) for dev in (0, 2, 1, 2)] == [7, 2007, 1007, 2007] and current == [0]
         getattr(ops, need).cache_clear()
+
+
+def test_the_line_is_one_resident_wave():
+    """Its grid, and so its workspace, is what the SMs hold at once: three CTAs each, two where the prefix of the
+    requests' costs leaves room for no more (74 KB and 4 bytes a request of 228 KB)."""
+    size = ops.kv4_attention_workspace_bytes
+    full, less = (size(b, 32, 8, 128, 64, 200) for b in (700, 800))
+    assert full % 3 == 0 and less == full // 3 * 2 == size(1024, 32, 8, 128, 64, 200)
+    assert size(700, 32, 8, 64, 64, 200) == size(1024, 32, 8, 64, 64, 200)
