@@ -284,3 +284,90 @@ def test_one_bad_token_does_not_slow_the_whole_prompt_down():
     out, bad = time()
     assert torch.isnan(out).all()
     assert infinite < 20 * clean and bad < 5 * clean, (clean, infinite, bad)
+
+
+# ---- workspaces of calls that overlap --------------------------------------------------------------
+
+
+def overlap_calls(g):
+    """(call(i, **keywords) of two inputs each, workspace bytes): the line of kv4_attention in one shape that takes it by
+    itself and one that is told to, window_attention split in all its row tiles and in the last round's."""
+    cache, _, _ = filled_cache(g, 128, 64, 2, 128, torch.bfloat16)
+    small = torch.randperm(128, device="cuda", generator=g).to(torch.int32).view(2, 64)
+    many = torch.randint(128, (24, 64), device="cuda", generator=g).to(torch.int32)
+    q2, q24 = ([randn(g, b, 8, 128, dtype=torch.bfloat16) for _ in range(2)] for b in (2, 24))
+    n2, n24 = i32([4000, 3333]), torch.randint(1, 4097, (24,), device="cuda", generator=g).to(torch.int32)
+    size = ops.kv4_attention_workspace_bytes
+    yield lambda i, **kw: ops.kv4_attention(q2[i], cache, small, n2, 0.09, variant=1, **kw), size(2, 8, 2, 128, 64, 64, variant=1)
+    yield lambda i, **kw: ops.kv4_attention(q24[i], cache, many, n24, 0.09, **kw), size(24, 8, 2, 128, 64, 64)
+    for lq, n, hq, hk in ((7, 3000, 8, 2), (650, 1950, 64, 1)):
+        q = [randn(g, lq, hq, 64, dtype=torch.bfloat16) for _ in range(2)]
+        k, v = randn(g, n, hk, 64, dtype=torch.bfloat16), randn(g, n, hk, 64, dtype=torch.bfloat16)
+        a, b = cu([lq]).cuda(), cu([n]).cuda()
+        yield (lambda i, q=q, k=k, v=v, a=a, b=b, **kw: ops.window_attention(q[i], k, v, a, 0.1, cu_seqlens_k=b, **kw),
+               ops.window_attention_workspace_bytes(lq, n, 1, hq, hk, 64))
+
+
+@pytest.mark.parametrize("which", range(4))
+def test_overlapping_calls_have_workspaces_of_their_own(which):
+    """Two streams at once, allocating or given a workspace each: what they give alone."""
+    call, need = list(overlap_calls(gen(71)))[which]
+    assert need > 0
+    want = [call(i) for i in range(2)]
+    assert not torch.equal(*want)
+    spaces = [torch.full((need,), 0xFF, dtype=torch.uint8, device="cuda") for _ in range(2)]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    outs = [[], []]
+    for turn in range(10):
+        for i, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                outs[i].append(call(i, **(dict(workspace=spaces[i]) if turn % 2 else {})))
+    torch.cuda.synchronize()
+    for i in range(2):
+        assert all(torch.equal(o, want[i]) for o in outs[i])
+
+
+@pytest.mark.parametrize("which", range(4))
+def test_graphs_have_workspaces_of_their_own(which):
+    """Two graphs captured one after the other and replayed at once on two streams, beside eager calls."""
+    call, need = list(overlap_calls(gen(72)))[which]
+    assert need > 0
+    want = [call(i) for i in range(2)]
+    torch.cuda.synchronize()
+    graphs = []
+    for i in range(2):
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = [call(i) for _ in range(3)]
+        graphs.append((graph, out))
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    for _ in range(3):
+        for graph, out in graphs:
+            for o in out:
+                o.zero_()
+        torch.cuda.synchronize()
+        for (graph, _), s in zip(graphs, streams):
+            with torch.cuda.stream(s):
+                graph.replay()
+        eager = [call(i) for i in range(2)]
+        torch.cuda.synchronize()
+        for i, (_, out) in enumerate(graphs):
+            assert all(torch.equal(o, want[i]) for o in (*out, eager[i]))
+
+
+# ---- the quantiser's arithmetic --------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("sign", [1, -1])
+def test_codes_are_those_of_fp32_arithmetic(sign):
+    """x - minimum and its quotient are IEEE fp32 operations: an element a little past a tie that fp32 does not tell from
+    the tie goes where the tie goes, to the even code."""
+    x = torch.zeros(1, 1, 64, device="cuda", dtype=torch.bfloat16)
+    x[0, 0, 0], x[0, 0, 1], x[0, 0, 2] = -6.5, 8.5, sign * 2.0**-30   # scale 1; 6.5 +- 2^-30 is 6.5 in fp32
+    cache = ops.kv4_cache(1, 16, 1, 64)
+    ops.kv4_store(x, x, i32([0]), cache)
+    k, v = ops.kv4_load(cache, i32([0]))
+    assert torch.equal(k, v) and k[0, 0, :3].tolist() == [-6.5, 8.5, -0.5]
+    codes, scale, low = serving.kv4_quantise(x)
+    assert codes[0, 0, 0, :3].tolist() == [0, 15, 6] and scale.item() == 1 and low.item() == -6.5
