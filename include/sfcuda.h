@@ -281,7 +281,8 @@ SF_API int sf_qk_norm_rope(const sf_qk_norm_rope_args* args, void* stream, char*
  * multiple of 16, D 64 or 128), one record for 16 tokens of a head (csrc/kv4.cuh gives its layout).
  * Token slot s is row s % page_size of page s / page_size.  Every 64 elements of a token's head hold a
  * bf16 minimum and scale = (max - min) / 15 and codes clamp(rint((x - minimum) / scale), 0, 15); a code
- * q stands for minimum + scale q.  A group with a value or a range that is not finite is stored as NaN.
+ * q stands for minimum + scale q.  The differences and quotients are IEEE fp32 operations, each rounded; a value is
+ * rounded once to its type (past the type's range, near fp16's largest, to an infinity).  A group with a value or a range that is not finite is stored as NaN.
  *
  * kv4_store writes tokens k, v [T, H, D] at slots[T]; kv4_load reads them back.  A negative slot is
  * padding (nothing written; zeros read); one past the cache is treated the same and reported through

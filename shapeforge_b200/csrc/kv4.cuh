@@ -18,7 +18,8 @@
 // Quantisation of a group of 64: minimum = bf16(min x), scale = bf16((max x - min x) / 15),
 // q = rint((x - minimum) / scale) clamped to 0..15 (0 when the scale is 0).  bf16 keeps the range of
 // both 16-bit types; the codes are taken against the rounded pair, so its rounding costs at most
-// the clamped ends.  A group whose values or range are not finite is stored with minimum NaN.
+// the clamped ends.  Differences and quotients are IEEE fp32 operations, each rounded: an element that fp32 does
+// not tell from a tie between two codes goes where the tie goes.  A group whose values or range are not finite is stored with minimum NaN.
 #pragma once
 
 #include "sf_common.cuh"

@@ -614,8 +614,8 @@ def _check_cache(cache: torch.Tensor, dev: int | None = None) -> tuple[int, int,
 def kv4_store(k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor, cache: torch.Tensor) -> torch.Tensor:
     """Quantise the tokens ``k, v [T, H, D]`` (unit stride along D) to 4 bits and write them at ``slots
     [T]`` (int32) of ``cache`` (:func:`kv4_cache`); returns ``cache``.  Every 64 elements of a token's
-    head get a bf16 minimum and scale = (max - min) / 15 and codes rint((x - minimum) / scale) in 0..15; a
-    group that is not finite reads back as NaN.  A negative slot is padding and skipped, one past the
+    head get a bf16 minimum and scale = (max - min) / 15 and codes rint((x - minimum) / scale) in 0..15, in
+    fp32 operations; a group that is not finite reads back as NaN.  A negative slot is padding and skipped, one past the
     cache is skipped and reported by :func:`kernel_status` (code 3).  The slots must differ."""
     dev = _gpu(k, "k")
     pages, heads, page, d = _check_cache(cache, dev)
@@ -630,7 +630,8 @@ def kv4_store(k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor, cache: torc
 def kv4_load(cache: torch.Tensor, slots: torch.Tensor, dtype: torch.dtype = torch.bfloat16, k_out: torch.Tensor | None = None,
              v_out: torch.Tensor | None = None) -> tuple[torch.Tensor, torch.Tensor]:
     """Read the tokens at ``slots [T]`` (int32, in any order, repeated or not) of a 4-bit cache back as
-    ``(k, v)``, each ``[T, H, D]`` in ``dtype`` (minimum + scale * code, rounded once), e.g. as the
+    ``(k, v)``, each ``[T, H, D]`` in ``dtype`` (minimum + scale * code, rounded once; the minimum is a bf16, so fp16
+    values within 2^8 of the type's largest may come back infinite), e.g. as the
     context of a prompt's next chunk for :func:`window_attention`.  Negative slots (and, reported by
     :func:`kernel_status`, slots past the cache) read as zeros.  ``k_out`` / ``v_out`` set the type when
     given."""
@@ -734,7 +735,8 @@ def window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqle
     rows).  Query ``i`` of a sequence with nq queries and nk keys sits at ``p = i + nk - nq`` and sees the
     keys ``j <= p`` with ``j > p - window`` or ``j < sinks`` (``window`` 0: all ``j <= p``), so a prompt's next
     chunk comes with its whole context as keys.  A query that sees nothing gives zeros; rows of ``out``
-    that belong to no sequence are left as they were.  ``out`` must not overlap the inputs.  Softmax in fp32, its
+    that belong to no sequence are left as they were (with no ``out`` given: not initialised).  ``out`` must not
+    overlap the inputs.  Softmax in fp32, its
     weights to some 16 (bf16) or 22 (fp16) bits in their product.  D up to 256; D 64 and 128 with 16-byte aligned rows and at most 128 query heads a key head run on the tensor cores, where few queries with many keys
     are split over the keys by way of ``workspace`` (uint8, :func:`window_attention_workspace_bytes`,
     allocated here when not given; calls that overlap on the GPU need one each).  ``variant``: 0 = by
