@@ -3,8 +3,8 @@
 //   o[b, h, :] = sum_j softmax_j(scale q[b, h, :] . k_j) v_j
 //   over keys j < n_b with j >= n_b - window or j < sinks (window 0: all), k, v = minimum + scale * code
 //
-// 32 requests of up to 16384 tokens, 64 heads on 8 of 128: 80 us, 4.2 TB/s, 64 % of the floor; issue slots are 58 %
-// busy with three warps a scheduler at 340 instructions a tile.  One request of 4097 tokens: 10 us, latency.
+// 32 requests of up to 16384 tokens, 64 heads on 8 of 128: 80 us, 4.2 TB/s, 64 % of the floor; issue slots are 57 %
+// busy with three warps a scheduler at 335 instructions a tile.  One request of 4097 tokens: 10 us, latency.
 //
 // HBM-bound by its bytes: every record (16 keys of one head, 18 D bytes) is read once for all query heads of its
 // group, ~4.5 bits a value.  What has to be kept up with is turning 4-bit codes into MMA operands,
