@@ -202,7 +202,7 @@ def test_kv4_attention_keeps_the_weights_precision(shape, dtype, variant):
 
 
 def test_a_chunk_split_in_its_last_round_writes_what_it_asked_for():
-    """2100 tokens behind 3000 and a short neighbour, 32 heads on 8: the workspace holds the last round's rows alone, all
+    """1200 tokens behind 3000 and a short neighbour, 32 heads on 8: the workspace holds the last round's rows alone, all
     of them, and nothing behind it is touched."""
     g, hq, hk, d = gen(68), 32, 8, 128
     cu_q, cu_k = cu([1200, 37]), cu([4200, 3037])
